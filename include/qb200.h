@@ -374,6 +374,62 @@ QB200_API int qb200_rope_kv_append_seqs(qb200_tensor* q, int dims, float base, f
                                         const qb200_tensor* dense_v, const int64_t* offsets, int num_seqs, int bits, int group_size,
                                         qb200_stream s);
 
+/* ==== The paged key-value cache.  No counterpart in the reference, whose slots own one capacity buffer per layer (src/scheduler.zig:463-480):
+ * sequences hold pages of a common pool, so that answers of one prompt share its pages and a cache grows without moving.
+ *   pool    codes [pages, heads, page, D*bits/32] uint32 with scales and biases [pages, heads, page, D/64] bf16 at 4 and 8 bits; rows
+ *           [pages, heads, page, D] bf16 at 16 bits, scales and biases empty then.  Any strides with the last axis contiguous and
+ *           code rows on 16 bytes; page = tokens of a page, a power of two from 16 on; groups of 64, D a multiple of 64;
+ *   table   [sequences, M] int32: page numbers of a sequence in order, below 0 where there is none;
+ *   lens    [sequences] int32: tokens of a sequence;
+ *   refs    [pages] int32: how many table entries name a page (0: free).  One table serves the pools of all layers.
+ * All of them live on the device and are changed there, in stream order; nothing is read back.  Entries of lists that name no
+ * sequence of the table are skipped, page numbers outside the pool are no page. ==== */
+
+/* New rows of K and V into the pages of their sequences, quantised as qb200_quantize does (16 bits: as they are).
+ * dense_k / dense_v [N, heads, S, D] bf16; token i of entry n goes to position positions[n] + i of sequence rows[n] (rows empty: n),
+ * for i < counts[n] (counts empty: S).  Tokens whose position has no page are dropped; all other rows of the pool stay as they are.
+ * Two tokens for one position: either one is kept. */
+QB200_API int qb200_kv_pages_append(qb200_tensor* k_q, qb200_tensor* k_scales, qb200_tensor* k_biases, qb200_tensor* v_q, qb200_tensor* v_scales,
+                                    qb200_tensor* v_biases, const qb200_tensor* dense_k, const qb200_tensor* dense_v, const qb200_tensor* table,
+                                    const qb200_tensor* rows, const qb200_tensor* positions, const qb200_tensor* counts, int bits, int group_size,
+                                    qb200_stream s);
+/* Frees the pages of sequences rows[n] that lie wholly in tokens [begin[n], end[n]) (empty: from 0, to the sequence's end): their
+ * entries become -1, their references one fewer.  An end at or behind the sequence's length shortens the sequence to begin[n] tokens;
+ * an end before it leaves the length (a window that moved on: begin = sinks, end = length - window).  A sequence listed again is
+ * skipped. */
+QB200_API int qb200_kv_pages_free(qb200_tensor* table, qb200_tensor* lens, qb200_tensor* refs, int page, const qb200_tensor* rows, const qb200_tensor* begin,
+                                  const qb200_tensor* end, qb200_stream s);
+/* Sequence dst[n], which must hold no tokens, begins with the first tokens[n] tokens (empty: all) of sequence src[n]: it shares their
+ * pages, the last one in part.  shared[n] = tokens shared, or -1 where the entry was refused (no such sequence, src == dst, dst holds
+ * tokens, or an earlier entry has the same dst); sources are taken as they were before the call.  At most 2048 entries. */
+QB200_API int qb200_kv_pages_fork(qb200_tensor* shared, qb200_tensor* table, qb200_tensor* lens, qb200_tensor* refs, int page, const qb200_tensor* src,
+                                  const qb200_tensor* dst, const qb200_tensor* tokens, qb200_stream s);
+/* Room for counts[n] more tokens in sequence rows[n]: positions[n] = its length before, which grows by counts[n]; missing pages are
+ * the free pages of the pool in ascending order, handed out in the order of the list.  A half-filled last page that others read too
+ * is replaced by a fresh one: copies[n] = (old, new), else (-1, -1), for qb200_kv_pages_copy before the next change of the table.
+ * positions[n] = -1 and nothing changed where an entry is refused: no such sequence, a count below 0, listed before, beyond the table's
+ * M pages, or the pool ran out (then also for all later entries that need pages).  At most 2048 entries and 2^19 pages. */
+QB200_API int qb200_kv_pages_reserve(qb200_tensor* positions, qb200_tensor* copies, qb200_tensor* table, qb200_tensor* lens, qb200_tensor* refs, int page,
+                                     const qb200_tensor* rows, const qb200_tensor* counts, qb200_stream s);
+/* Moves the live pages (refs > 0) to the front of the pool: of n live pages the k-th one with a number >= n goes to the k-th free number
+ * below n.  remap [pages] = the new number of every page (-1: free), moves [at least pages / 2, 2] = (old, new) pairs in ascending
+ * order and -1 behind them, count [1] = how many; table and refs are rewritten.  The rows themselves move with qb200_kv_pages_copy. */
+QB200_API int qb200_kv_pages_compact(qb200_tensor* remap, qb200_tensor* moves, qb200_tensor* count, qb200_tensor* table, qb200_tensor* refs, qb200_stream s);
+/* Copies page pairs[n][0] to page pairs[n][1] in each of the pools (tensors whose first axis is the page: codes, scales and biases of
+ * all layers).  Pairs outside the pool say nothing; count (empty: all) limits them to the first count[0].  No page may be the target
+ * of two pairs, nor the target of one and the source of another; the lists of the two entries above hold no such pairs. */
+QB200_API int qb200_kv_pages_copy(qb200_tensor* const* pools, int num_pools, const qb200_tensor* pairs, const qb200_tensor* count, qb200_stream s);
+/* Attention of one new token per sequence (already in the cache) over its pages: qb200_kv_decode_attention through a table.
+ * q, res [B, Hq, 1, D] bf16, D 64 or 128; query b reads sequence rows[b] (empty: b), of lens[rows[b]] tokens.  window > 0: it sees the last
+ * `window` tokens and the first `sinks`; 0: all.  Tokens without a page are not seen; a query that sees nothing gives zeros.
+ * At most 1024 sequences.  workspace: device scratch of the size below, on 16 bytes, whatever it holds; two calls that overlap on the
+ * GPU need one each. */
+QB200_API int qb200_kv_pages_decode_attention(qb200_tensor* res, const qb200_tensor* q, const qb200_tensor* k_q, const qb200_tensor* k_scales,
+                                              const qb200_tensor* k_biases, const qb200_tensor* v_q, const qb200_tensor* v_scales, const qb200_tensor* v_biases,
+                                              const qb200_tensor* table, const qb200_tensor* rows, const qb200_tensor* lens, int bits, int group_size, float scale,
+                                              int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes, qb200_stream s);
+QB200_API size_t qb200_kv_pages_decode_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
+
 /* ==== checkpoint -> device loader: MLX-format quantized safetensors (host side; the device layout is the file's) ==== */
 
 /* One opened .safetensors file (memory-mapped).  Quantized linears are stored as <name>.weight (uint32 packed codes),

@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -148,6 +149,22 @@ PyObject* wrap(at::Tensor t) { return THPVariable_Wrap(std::move(t)); }
 PyObject* ret(PyObject* o) { Py_INCREF(o); return o; }
 using Shape = c10::SmallVector<int64_t, 8>;
 Shape lead(const at::Tensor& t, int drop) { const auto s = t.sizes(); return Shape(s.begin(), s.end() - std::min<size_t>(drop, s.size())); }
+
+// The device that a call's tensors share, made current for the call; tensors of the host or of different devices are refused.
+struct OnDevice {
+  c10::cuda::OptionalCUDAGuard guard;
+  int index = -1;
+  void add(const at::Tensor& t) {
+    if (!t.is_cuda()) throw std::invalid_argument("qb200: a CUDA tensor was expected");
+    if (index >= 0 && t.get_device() != index) throw std::invalid_argument("qb200: tensors on different devices");
+    index = (int)t.get_device();
+  }
+  void add(PyObject* o) { if (o != Py_None) add(tensor(o)); }
+  void* stream() {
+    guard.set_index((c10::DeviceIndex)index);
+    return (void*)c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)index).stream();
+  }
+};
 
 // A list or tuple's items without a copy.
 struct Seq {
@@ -569,6 +586,135 @@ PyObject* kv_append_seqs(Args a) {
   return ret(Py_None);
 }
 
+// A cache pool's (codes, scales, biases); at 16 bits (rows, None, None).
+struct PagePool {
+  T d[3];
+  const at::Tensor* codes;
+  PagePool(PyObject* o, long bits, OnDevice& dev) {
+    Seq s(o);
+    if (s.size() != 3) { PyErr_SetString(PyExc_ValueError, "qb200: (codes, scales, biases) were expected"); throw PyFail(); }
+    for (int i = 0; i < 3; ++i) {
+      dev.add(s[i]);
+      d[i] = i == 0 && bits != 16 ? packed(s[i]) : plain(s[i]);
+    }
+    codes = &tensor(s[0]);
+  }
+};
+
+// k_pool, v_pool, dense_k, dense_v, table, positions, bits, group_size, rows, counts
+PyObject* kv_pages_append(Args a) {
+  OnDevice dev;
+  const int nb = (int)as_long(a[6]), gs = (int)as_long(a[7]);
+  PagePool k(a[0], nb, dev), v(a[1], nb, dev);
+  for (int i : {2, 3, 4, 5, 8, 9}) dev.add(a[i]);
+  T dk = plain(a[2]), dv = plain(a[3]), t = plain(a[4]), p = plain(a[5]), r = plain(a[8]), c = plain(a[9]);
+  void* st = dev.stream();
+  call([&] {
+    return qb200_kv_pages_append(&k.d[0].d, &k.d[1].d, &k.d[2].d, &v.d[0].d, &v.d[1].d, &v.d[2].d, &dk.d, &dv.d, &t.d, &r.d, &p.d, &c.d, nb, gs, st);
+  });
+  return ret(Py_None);
+}
+
+// table, lens, refs, page, rows, begin, end
+PyObject* kv_pages_free(Args a) {
+  OnDevice dev;
+  for (int i : {0, 1, 2, 4, 5, 6}) dev.add(a[i]);
+  T t = plain(a[0]), l = plain(a[1]), f = plain(a[2]), r = plain(a[4]), b = plain(a[5]), e = plain(a[6]);
+  const int page = (int)as_long(a[3]);
+  void* st = dev.stream();
+  call([&] { return qb200_kv_pages_free(&t.d, &l.d, &f.d, page, &r.d, &b.d, &e.d, st); });
+  return ret(Py_None);
+}
+
+// table, lens, refs, page, src, dst, tokens
+PyObject* kv_pages_fork(Args a) {
+  OnDevice dev;
+  for (int i : {0, 1, 2, 4, 5, 6}) dev.add(a[i]);
+  T t = plain(a[0]), l = plain(a[1]), f = plain(a[2]), s = plain(a[4]), d = plain(a[5]), n = plain(a[6]);
+  const int page = (int)as_long(a[3]);
+  void* st = dev.stream();
+  at::Tensor shared = empty(tensor(a[4]).sizes(), tensor(a[4]), at::kInt);
+  T o = plain(shared);
+  call([&] { return qb200_kv_pages_fork(&o.d, &t.d, &l.d, &f.d, page, &s.d, &d.d, &n.d, st); });
+  return wrap(std::move(shared));
+}
+
+// table, lens, refs, page, rows, counts
+PyObject* kv_pages_reserve(Args a) {
+  OnDevice dev;
+  for (int i : {0, 1, 2, 4, 5}) dev.add(a[i]);
+  T t = plain(a[0]), l = plain(a[1]), f = plain(a[2]), r = plain(a[4]), c = plain(a[5]);
+  const int page = (int)as_long(a[3]);
+  void* st = dev.stream();
+  const at::Tensor& rows = tensor(a[4]);
+  at::Tensor pos = empty(rows.sizes(), rows, at::kInt), copies = empty({rows.numel(), 2}, rows, at::kInt);
+  T p = plain(pos), o = plain(copies);
+  call([&] { return qb200_kv_pages_reserve(&p.d, &o.d, &t.d, &l.d, &f.d, page, &r.d, &c.d, st); });
+  return pack({wrap(std::move(pos)), wrap(std::move(copies))});
+}
+
+// table, refs
+PyObject* kv_pages_compact(Args a) {
+  OnDevice dev;
+  for (int i : {0, 1}) dev.add(a[i]);
+  T t = plain(a[0]), f = plain(a[1]);
+  void* st = dev.stream();
+  const at::Tensor& refs = tensor(a[1]);
+  at::Tensor remap = empty(refs.sizes(), refs, at::kInt), moves = empty({refs.numel() / 2, 2}, refs, at::kInt), count = empty({1}, refs, at::kInt);
+  T r = plain(remap), m = plain(moves), c = plain(count);
+  call([&] { return qb200_kv_pages_compact(&r.d, &m.d, &c.d, &t.d, &f.d, st); });
+  return pack({wrap(std::move(remap)), wrap(std::move(moves)), wrap(std::move(count))});
+}
+
+// pools, pairs, count
+PyObject* kv_pages_copy(Args a) {
+  OnDevice dev;
+  Seq list(a[0]);
+  const Py_ssize_t n = list.size();
+  std::vector<T> d((size_t)n);
+  std::vector<qb200_tensor*> p((size_t)n);
+  dev.add(a[1]);
+  dev.add(a[2]);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    dev.add(tensor(list[i]));
+    d[i] = plain(list[i]);
+    p[i] = &d[i].d;
+  }
+  T pr = plain(a[1]), c = plain(a[2]);
+  void* st = dev.stream();
+  call([&] { return qb200_kv_pages_copy(p.data(), (int)n, &pr.d, &c.d, st); });
+  return ret(Py_None);
+}
+
+// q, k_pool, v_pool, table, lens, bits, group_size, scale, window, sinks, rows, workspace, out
+PyObject* kv_pages_decode_attention(Args a) {
+  OnDevice dev;
+  const int nb = (int)as_long(a[5]), gs = (int)as_long(a[6]);
+  PagePool k(a[1], nb, dev), v(a[2], nb, dev);
+  for (int i : {0, 3, 4, 10, 11, 12}) dev.add(a[i]);
+  const at::Tensor& q = tensor(a[0]);
+  const float scale = (float)as_double(a[7]);
+  const int64_t window = as_index(a[8]), sinks = as_index(a[9]);
+  void* st = dev.stream();
+  at::Tensor out = a[12] == Py_None ? at::empty(q.sizes(), q.options().requires_grad(false)) : tensor(a[12]), ws;
+  if (a[11] == Py_None) {
+    const bool known = q.dim() == 4 && k.codes->dim() == 4;
+    const size_t need = known ? qb200_kv_pages_decode_attention_workspace_size(q.size(0), q.size(1), k.codes->size(1), q.size(3)) : 0;
+    ws = empty({(int64_t)(need > 16 ? need : 16)}, q, at::kByte);
+  } else {
+    ws = tensor(a[11]);
+    if (!ws.is_contiguous()) throw std::invalid_argument("qb200: the workspace must be contiguous");
+  }
+  T y = plain(out), dq = plain(q), t = plain(a[3]), l = plain(a[4]), r = plain(a[10]);
+  void* wp = ws.data_ptr();
+  const size_t wn = (size_t)ws.nbytes();
+  call([&] {
+    return qb200_kv_pages_decode_attention(&y.d, &dq.d, &k.d[0].d, &k.d[1].d, &k.d[2].d, &v.d[0].d, &v.d[1].d, &v.d[2].d, &t.d, &r.d, &l.d, nb, gs, scale, window,
+                                           sinks, wp, wn, st);
+  });
+  return a[12] == Py_None ? wrap(std::move(out)) : ret(a[12]);
+}
+
 PyObject* set_error_class(Args a) {
   Py_INCREF(a[0]);
   Py_XDECREF(g_error_class);
@@ -583,6 +729,8 @@ PyMethodDef methods[] = {
     QB_ENTRY(dequantize, 8), QB_ENTRY(quantize, 4), QB_ENTRY(kv_append, 7), QB_ENTRY(kv_decode_attention, 11),
     QB_ENTRY(kv_decode_attention_noalloc, 10), QB_ENTRY(kv_decode_attention_ptrs, 11), QB_ENTRY(add_rms_norm, 7), QB_ENTRY(rms_norm, 4),
     QB_ENTRY(rope, 6), QB_ENTRY(turbo_rotate, 3), QB_ENTRY(swiglu, 3), QB_ENTRY(kv_append_seqs, 11), QB_ENTRY(set_error_class, 1),
+    QB_ENTRY(kv_pages_append, 10), QB_ENTRY(kv_pages_free, 7), QB_ENTRY(kv_pages_fork, 7), QB_ENTRY(kv_pages_reserve, 6), QB_ENTRY(kv_pages_compact, 2),
+    QB_ENTRY(kv_pages_copy, 3), QB_ENTRY(kv_pages_decode_attention, 13),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native half of the qb200 Python binding", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -7,6 +7,7 @@
 // (src/kv_quant.zig:126-162); the scale/bias rule is the one restated in
 // tests/dsv4_imatrix.py:169-183 and the codes follow :264.
 #include "kernels.h"
+#include "quant_rows.cuh"
 
 namespace qb {
 
@@ -161,7 +162,6 @@ cudaError_t quant_dispatch_x(const QuantArgs& a, cudaStream_t st) {
 // HBM-bound: 16 values per thread, 16-byte accesses on the dense side, the row's offsets from a (block, row) pair instead of
 // 64-bit divisions per element.  K and V of 2 x 8 x 4096 tokens at head dim 128, 8 bits, appended and read back as bf16 (87 MB):
 // 168 us with the element-wise kernels above, which stay for other dtypes, 2 bits and unaligned rows.
-constexpr int kRowVals = 16;    // values per thread: the group's parameters (four divisions) are worked out once per 16
 
 // Rows as z x y x inner; each tensor's element strides along the three.
 struct RowAxis { int64_t z, y, inner; };
@@ -172,17 +172,6 @@ struct RowGrid {
 __device__ __forceinline__ int64_t row_base(const RowAxis& m, int row) { return blockIdx.z * m.z + blockIdx.y * m.y + row * m.inner; }
 __device__ __forceinline__ int row_of(const RowGrid& rg, int i) { return rg.shift >= 0 ? i >> rg.shift : (int)((uint32_t)i / (uint32_t)rg.per_row); }
 
-// rint(x / s) clamped to [0, bins], exactly as the division rounds: away from the ties the product with 1 / s decides, near
-// them (within 2^-10, far more than its error for quotients up to 256) and where anything is not finite the division does.
-__device__ __forceinline__ uint32_t code_of(float x, float bias, float s, float rs, float bins) {
-  const float n = __fsub_rn(x, bias);
-  const float t = fmaf(n, rs, 12582912.f);          // 1.5 * 2^23 + rint(n / s): the low bits are the integer
-  const float r = fmaf(n, rs, 12582912.f - t);      // what the rounding left
-  float c = t - 12582912.f;
-  if (!(fabsf(r) < 0.5f - 9.765625e-4f)) c = rintf(__fdiv_rn(n, s));
-  return (uint32_t)fminf(fmaxf(c, 0.0f), bins);
-}
-
 template <int BITS>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const uint16_t* x, uint32_t* qo, uint16_t* so, uint16_t* bo, RowAxis ax, RowAxis aq, RowAxis as,
                                                          RowGrid rg, int gs) {
@@ -192,32 +181,11 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const uint16_t* x, uint
   const uint16_t* xp = x + row_base(ax, row) + c * kRowVals;
   float v[kRowVals];
 #pragma unroll
-  for (int k = 0; k < kRowVals / 8; ++k) {
-    const uint4 raw = ((const uint4*)xp)[k];
-    const uint32_t q[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) { v[8 * k + 2 * j] = bf16lo(q[j]); v[8 * k + 2 * j + 1] = bf16hi(q[j]); }
-  }
-  float xmin = v[0], xmax = v[0];
-#pragma unroll
-  for (int k = 1; k < kRowVals; ++k) { xmin = fminf(xmin, v[k]); xmax = fmaxf(xmax, v[k]); }
+  for (int k = 0; k < kRowVals / 8; ++k) unpack8_bf16(((const uint4*)xp)[k], v + 8 * k);
   const int tpg = gs / kRowVals;   // neighbouring lanes share a group: 2, 4 or 8
-  for (int off = tpg >> 1; off > 0; off >>= 1) {
-    xmin = fminf(xmin, __shfl_xor_sync(0xffffffffu, xmin, off));
-    xmax = fmaxf(xmax, __shfl_xor_sync(0xffffffffu, xmax, off));
-  }
-  const float n_bins = (float)((1 << BITS) - 1);
-  const bool mask = fabsf(xmin) > fabsf(xmax);
-  float scale = fmaxf(__fdiv_rn(__fsub_rn(xmax, xmin), n_bins), 1e-7f);
-  scale = mask ? scale : -scale;
-  const float edge = mask ? xmin : xmax;
-  const float q0 = rintf(__fdiv_rn(edge, scale));
-  float bias = 0.0f;
-  if (q0 != 0.0f) { scale = __fdiv_rn(edge, q0); bias = edge; }
-  const float rs = __fdiv_rn(1.0f, scale);
-  uint32_t w[BITS / 2] = {};
-#pragma unroll
-  for (int k = 0; k < kRowVals; ++k) w[k * BITS / 32] |= code_of(v[k], bias, scale, rs, n_bins) << (k * BITS % 32);
+  float scale, bias;
+  uint32_t w[BITS / 2];
+  quantize16<BITS>(v, tpg, w, scale, bias);
   if (!live) return;
   uint32_t* qp = qo + row_base(aq, row) + c * (BITS / 2);
   if constexpr (BITS == 4) *(uint2*)qp = make_uint2(w[0], w[1]); else *(uint4*)qp = make_uint4(w[0], w[1], w[BITS / 2 - 2], w[BITS / 2 - 1]);

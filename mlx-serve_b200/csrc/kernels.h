@@ -271,4 +271,69 @@ bool kv_fast_supported(const KvAttnArgs& a, const KvSeqTable* seqs = nullptr);  
 bool kv_f16_supported(const KvAttnArgs& a, const KvSeqTable* seqs = nullptr);    // kv_attn_f16.cu: fp16 MMA, D = 64 / 128, GQA <= 8, T_q <= 8
 cudaError_t launch_kv_attn(const KvAttnArgs& a, cudaStream_t st, const KvSeqTable* seqs = nullptr);  // seqs: a.B <= kMaxSeqPtrs views, a.T their longest
 
+// ---- kv_pages.cu: the paged cache ----
+// One side (K or V) of a pool: codes (or bf16 rows at 16 bits) with (page, head, token) strides in elements, and at 4 and 8 bits the
+// scales and biases of groups of 64.
+struct KvPoolView {
+  const void* q; const void* s; const void* b;
+  int64_t q_str[3], sb_str[3];
+};
+struct KvPagesAppendArgs {
+  KvPoolView pool[2];
+  const uint16_t* dense[2]; int64_t dense_str[2][3];   // (sequence, head, token) strides
+  const int32_t* table; int64_t table_str;
+  const int32_t* rows; const int32_t* positions; const int32_t* counts;   // rows, counts may be null
+  int64_t M, seqs, P;
+  int page_shift, N, H, S, per_row, bits, dense_vec;
+};
+cudaError_t launch_pages_append(const KvPagesAppendArgs& a, cudaStream_t st);
+struct PageState {
+  int32_t* table; int64_t table_str;     // [S, M]
+  int32_t* lens; int32_t* refs;
+  int S, M, P, page_shift;
+};
+constexpr int kMaxPageList = 2048;       // sequences listed in one fork or reserve
+constexpr int kMaxPages = 1 << 19;       // pages whose bits one block can hold
+constexpr int kPageSmem = kMaxPages / 32 * 8 + kMaxPageList * 20;
+cudaError_t launch_pages_free(const PageState& s, const int32_t* rows, const int32_t* begin, const int32_t* end, int n, cudaStream_t st);
+cudaError_t launch_pages_fork(const PageState& s, const int32_t* src, const int32_t* dst, const int32_t* tokens, int n, int32_t* shared, cudaStream_t st);
+cudaError_t launch_pages_reserve(const PageState& s, const int32_t* rows, const int32_t* counts, int n, int32_t* positions, int32_t* copies, cudaStream_t st);
+cudaError_t launch_pages_compact(const PageState& s, int32_t* remap, int32_t* moves, int64_t cap, int32_t* count, cudaStream_t st);
+// A page of a pool: `bytes` in runs of `run`, `inner` runs inner_str bytes apart, then outer_str.
+struct PagesCopyPool {
+  char* base; int64_t page_str, outer_str, inner_str;
+  uint32_t bytes, run, inner;
+  int first_piece;
+};
+constexpr int kMaxCopyPools = 96;        // pools per launch
+struct PagesCopyArgs {
+  const int32_t* pairs; const int32_t* count;   // count may be null
+  int64_t n, P;
+  int pools, pieces;
+  PagesCopyPool pool[kMaxCopyPools];
+};
+cudaError_t launch_pages_copy(const PagesCopyArgs& a, int vec, cudaStream_t st);   // vec: bytes every offset and length is a multiple of (16, 4, 2, 1)
+int pages_copy_piece();
+
+// ---- kv_pages_attn.cu: attention of one new token over pages ----
+constexpr int kMaxPageSeqs = 1024;       // sequences per launch
+constexpr int kPagesCtas = 4;            // CTAs an SM at most (the workspace holds the parts of so many)
+struct KvPagesAttnArgs {
+  const void* q; void* out; int64_t q_str[2], o_str[2];   // (sequence, head) strides
+  KvPoolView pool[2];
+  int64_t q_head[2];                     // bytes from head to head of the codes
+  uint32_t page_bytes[2], tok_bytes[2];  // bytes from page to page and from token to token of the codes
+  const int32_t* table; int64_t table_str;
+  const int32_t* rows; const int32_t* lens;   // rows may be null
+  int64_t seqs;
+  int B, Hq, Hkv, gqa, M, P, page_shift, window, sinks, bits;
+  int sb_vec, q_vec;                     // scale rows packed and 16-byte aligned; query rows aligned
+  float scale;
+  // by the launcher
+  int qtiles, tiles, min_units;
+  int4* joins; float2* part_ml; float* part_o;
+};
+size_t kv_pages_workspace_bytes(int64_t D);
+cudaError_t launch_kv_pages_attn(KvPagesAttnArgs a, int D, void* workspace, cudaStream_t st);
+
 }  // namespace qb

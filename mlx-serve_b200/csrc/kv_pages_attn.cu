@@ -1,0 +1,763 @@
+// Attention of one new token over a paged key-value cache, 4- or 8-bit codes or bf16 rows, head dim 64 or 128, with an optional
+// window and a few first tokens that stay visible.
+//
+// o = sum_j p_j v_j, p = softmax_j(scale * q . k_j) over the cached tokens j < len that the newest token sees: all of them, or
+// j < sinks and j >= len - window.  The codes are read once, straight from their pages; with q*s + b the weight terms stay in
+// fp32: s scales sums of codes, b meets the group sums of q (keys) or is summed with p (values).
+//
+//  * Work.  A unit is a block of 64 tokens of one (sequence, cache head, tile of 8 query heads).  The grid is what the device holds
+//    at once; every CTA works out all lengths' units from `lens` and takes an even share of their total, so that ragged batches stay
+//    balanced with lengths that only the device knows.  A share cuts at most two sequences; their parts go to the workspace and a
+//    second kernel joins them, whole sequences are stored directly.
+//  * A warp walks blocks of 64 tokens with its own softmax (running maximum and sum per query in fp32) and its own cp.async ring.
+//    Page numbers are read a block ahead; rows that the query does not see are not read, their place is zeroed.
+//  * Codes are the A operand of the fp16 tensor cores: 16 tokens x 16 dims for the scores, 16 dims x 16 tokens for the values, the
+//    8 queries the B operand, so that a matrix instruction takes 256 codes (as the B operand it would take 128).  A code in the low
+//    bits of a 16-bit word IS the fp16 subnormal c * 2^-24: one AND makes an operand register; the next nibble is 16 times that.
+//    The value operand comes out of ldmatrix.m16n16.trans.b8, four tokens of a byte column a lane.
+//  * Queries are scaled by a power of two into fp16's range (exact for bf16 down to 2^-38 of the row's largest), the probabilities
+//    times the value scale are rounded once to fp16 (2^-11 relative, against 2^-8 of the bf16 result) with the softmax's reference
+//    kept low enough by the block's largest value scale; at 16 bits they stay a sum of two bf16 (16 bits).  The score tile's
+//    layout becomes the B operand of the next product by movmatrix.
+#include <mutex>
+
+#include "kernels.h"
+#include "stream_ptx.cuh"
+
+namespace qb {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kBlk = 64;              // tokens per unit
+constexpr int kRows = 8;              // queries per tile
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegBig = -1e30f;
+constexpr int kMergeWarps = 16;
+
+template <int BITS, int D> struct Geo {
+  static constexpr int G = BITS == 16 ? 1 : D / 64;       // scale groups per token
+  static constexpr int ROWB = D * BITS / 8;               // bytes per token
+  static constexpr int CH = ROWB / 16;                    // 16-byte chunks per token
+  static constexpr int TOK = ROWB >= 256 ? 16 : 32;       // tokens per ring stage
+  static constexpr int STAGE = TOK * ROWB;
+  static constexpr int STAGES = 4;
+  static constexpr int ITEMS = 2 * kBlk / TOK;            // stages per block: K, then V
+  static constexpr int SB = BITS == 16 ? 0 : kBlk * G * 2;    // bytes of one of {ks, kb, vs, vb} for a block
+  static constexpr int RING = STAGES * STAGE;
+  static constexpr int NT = D / 16;                       // 16-dim tiles of the output
+  static constexpr int SMEM_MAIN = kWarps * (RING + 2 * 4 * SB);
+  static constexpr int SMEM_MERGE = kWarps * kRows * (D + 2) * 4;
+  static constexpr int SMEM = SMEM_MAIN > SMEM_MERGE ? SMEM_MAIN : SMEM_MERGE;
+};
+
+template <int BITS, int CH> __device__ __forceinline__ int swz(int row) {
+  if (BITS == 16) return row & 7;
+  int f = (row >> 3) & 1;
+  if (CH >= 4) f |= ((row >> 1) & 1) << 1;
+  if (CH >= 8) f |= (row & 1) << 2;
+  return f;
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <bool TRANS> __device__ __forceinline__ void ldmatrix_b16_x4(uint32_t (&r)[4], uint32_t addr) {
+  if constexpr (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+
+// What the newest token of a sequence sees, in blocks of 64 tokens.
+struct Seen {
+  int len, w0, sinks;       // tokens; start of the window
+  int front, skip;          // blocks [0, front) and, from there on, block i + skip
+  int blocks;
+};
+__device__ __forceinline__ Seen seen_of(const KvPagesAttnArgs& a, int64_t b) {
+  Seen s;
+  const int64_t row = a.rows ? a.rows[b] : b;
+  int64_t len = row >= 0 && row < a.seqs ? a.lens[row] : 0;
+  const int64_t cap = (int64_t)a.M << a.page_shift;
+  len = len < 0 ? 0 : (len > cap ? cap : len);
+  s.len = (int)len;
+  const int nb = (int)((len + kBlk - 1) / kBlk);
+  s.w0 = a.window > 0 && a.window < len ? (int)(len - a.window) : 0;
+  s.sinks = a.sinks < s.len ? a.sinks : s.len;
+  s.front = (int)(((int64_t)s.sinks + kBlk - 1) / kBlk);
+  s.skip = s.w0 / kBlk - s.front;
+  if (s.skip < 0) s.skip = 0;
+  s.blocks = nb - s.skip;
+  return s;
+}
+
+// units[b] = units before sequence b, units[B] = all.
+__device__ __forceinline__ void plan_units(const KvPagesAttnArgs& a, int* units, int* warp_sums) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int each = (a.B + kWarps * 32 - 1) / (kWarps * 32), b0 = tid * each;
+  int mine = 0;
+  for (int i = 0; i < each && b0 + i < a.B; ++i) {
+    const int n = seen_of(a, b0 + i).blocks * a.tiles;
+    units[b0 + i] = mine;
+    mine += n;
+  }
+  int v = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  if (lane == 31) warp_sums[warp] = v;
+  __syncthreads();
+  int before = v - mine;
+  for (int w = 0; w < warp; ++w) before += warp_sums[w];
+  for (int i = 0; i < each && b0 + i < a.B; ++i) units[b0 + i] += before;
+  if (tid == 0) units[a.B] = warp_sums[0] + warp_sums[1] + warp_sums[2] + warp_sums[3];
+  __syncthreads();
+}
+
+template <int BITS, int D>
+__global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kernel(const __grid_constant__ KvPagesAttnArgs a) {
+  using GE = Geo<BITS, D>;
+  constexpr int G = GE::G, CH = GE::CH, TOK = GE::TOK, ITEMS = GE::ITEMS, STAGES = GE::STAGES;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int units[kMaxPageSeqs + 1];
+  __shared__ int warp_sums[kWarps];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  asm volatile("griddepcontrol.launch_dependents;");
+  plan_units(a, units, warp_sums);
+  // sequences that see nothing: zeros
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+    if (units[b + 1] == units[b])
+      for (int i = tid; i < a.Hq * D; i += kWarps * 32) ((uint16_t*)a.out)[(int64_t)b * a.o_str[0] + (int64_t)(i / D) * a.o_str[1] + i % D] = 0;
+
+  const int U = units[a.B];
+  int per = (U + (int)gridDim.x - 1) / (int)gridDim.x;
+  per = per < a.min_units ? a.min_units : per;
+  const int64_t u_from = (int64_t)blockIdx.x * per;
+  const int u_to = u_from + per < U ? (int)(u_from + per) : U;
+  if (tid == 0 && a.joins) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (u_from >= U) return;
+
+  const uint32_t my_ring = (uint32_t)__cvta_generic_to_shared(smem + (size_t)warp * GE::RING);
+  const unsigned char* my_ring_p = smem + (size_t)warp * GE::RING;
+  unsigned char* my_sb_p = smem + (size_t)kWarps * GE::RING + (size_t)warp * 2 * 4 * GE::SB;
+  const uint32_t my_sb = (uint32_t)__cvta_generic_to_shared(my_sb_p);
+
+  int b = 0;
+  {
+    int hi = a.B - 1;
+    while (b < hi) {
+      const int mid = (b + hi + 1) >> 1;
+      if (units[mid] <= (int)u_from) b = mid; else hi = mid - 1;
+    }
+  }
+  for (int u = (int)u_from; u < u_to;) {
+    while (units[b + 1] <= u) ++b;
+    const Seen sn = seen_of(a, b);
+    const int tile = (u - units[b]) / sn.blocks, blk0 = u - units[b] - tile * sn.blocks;
+    const int left = sn.blocks - blk0, todo = left < u_to - u ? left : u_to - u;
+    const int hk = tile / a.qtiles, qt = tile - hk * a.qtiles;
+    const int row = a.rows ? a.rows[b] : b;
+    const int32_t* tab = a.table + (int64_t)row * a.table_str;
+    const int my_blocks = warp < todo ? (todo - warp + kWarps - 1) / kWarps : 0;
+    const int my_items = my_blocks * ITEMS;
+    const unsigned char* kv_base[2] = {(const unsigned char*)a.pool[0].q + (int64_t)hk * a.q_head[0], (const unsigned char*)a.pool[1].q + (int64_t)hk * a.q_head[1]};
+    const int pmask = (1 << a.page_shift) - 1;
+    auto first_token = [&](int j) { const int i = blk0 + warp + j * kWarps; return (i < sn.front ? i : i + sn.skip) * kBlk; };
+    auto visible = [&](int tok) { return tok < sn.len && (tok >= sn.w0 || tok < sn.sinks); };
+
+    // ---- producer ----
+    // lane l holds the page of the 16 tokens from 16 * (l & 3) on, -1 where there is none
+    auto page_at = [&](int j) {
+      int pid = -1;
+      if (j < my_blocks) {
+        const int tok = first_token(j) + 16 * (lane & 3);
+        if (tok < sn.len) pid = tab[tok >> a.page_shift];
+        if (pid >= a.P) pid = -1;
+      }
+      return pid;
+    };
+    int pid_next = page_at(0), pid_cur = -1, blk_tok = 0;
+    uint32_t valid = 0;                                   // four bits a block, the newest lowest
+    constexpr int RPI = 32 / CH;                          // token rows of one copy instruction
+    const int cc = lane % CH, r0 = lane / CH;
+    auto issue = [&](int item, int stage) {
+      const int part = item % ITEMS;
+      if (part == 0) {
+        const int j = item / ITEMS;
+        pid_cur = pid_next;
+        blk_tok = first_token(j);
+        valid = (valid << 4) | (__ballot_sync(0xffffffffu, pid_cur >= 0) & 15u);
+        pid_next = page_at(j + 1);
+        if constexpr (BITS != 16) {
+          const uint32_t dst0 = my_sb + (j & 1) * 4 * GE::SB;
+          const uint16_t* const sbase[4] = {(const uint16_t*)a.pool[0].s, (const uint16_t*)a.pool[0].b, (const uint16_t*)a.pool[1].s, (const uint16_t*)a.pool[1].b};
+          if (a.sb_vec) {
+            constexpr int PC = GE::SB / 16, TP = 8 / G;   // 16-byte pieces per array, tokens per piece
+#pragma unroll
+            for (int i = lane; i < 4 * PC; i += 32) {
+              const int arr = i / PC, pc = i - arr * PC, tk = pc * TP, kv = arr >> 1;
+              const int pid = __shfl_sync(0xffffffffu, pid_cur, tk >> 4);
+              const uint16_t* base = arr == 0 ? sbase[0] : (arr == 1 ? sbase[1] : (arr == 2 ? sbase[2] : sbase[3]));
+              const uint16_t* src = base + (int64_t)(pid < 0 ? 0 : pid) * (kv ? a.pool[1].sb_str[0] : a.pool[0].sb_str[0]) +
+                                    (int64_t)hk * (kv ? a.pool[1].sb_str[1] : a.pool[0].sb_str[1]) + ((blk_tok + tk) & pmask) * G;
+              cp_async16_z(dst0 + arr * GE::SB + pc * 16, src, pid >= 0 && blk_tok + tk < sn.len ? 16u : 0u);
+            }
+          } else {
+            uint16_t* dst = (uint16_t*)(my_sb_p + (j & 1) * 4 * GE::SB);
+#pragma unroll
+            for (int arr = 0; arr < 4; ++arr) {
+              const KvPoolView& pl = a.pool[arr >> 1];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int tk = h * 32 + lane;
+                const int pid = __shfl_sync(0xffffffffu, pid_cur, tk >> 4);
+#pragma unroll
+                for (int c = 0; c < G; ++c)
+                  dst[arr * (GE::SB / 2) + tk * G + c] = pid >= 0 && blk_tok + tk < sn.len
+                      ? sbase[arr][(int64_t)pid * pl.sb_str[0] + (int64_t)hk * pl.sb_str[1] + (int64_t)((blk_tok + tk) & pmask) * pl.sb_str[2] + c] : (uint16_t)0;
+              }
+            }
+          }
+        }
+      }
+      const int kv = part >= ITEMS / 2 ? 1 : 0, tk0 = (part - kv * (ITEMS / 2)) * TOK;
+      const unsigned char* base = kv ? kv_base[1] : kv_base[0];
+      const uint32_t page_b = kv ? a.page_bytes[1] : a.page_bytes[0], tok_b = kv ? a.tok_bytes[1] : a.tok_bytes[0];
+      const uint32_t st = my_ring + stage * GE::STAGE;
+#pragma unroll
+      for (int r = 0; r < TOK / RPI; ++r) {
+        const int rw = r0 + r * RPI, tok = blk_tok + tk0 + rw;
+        const int pid = __shfl_sync(0xffffffffu, pid_cur, (tk0 + r * RPI) >> 4);
+        const bool ok = pid >= 0 && visible(tok);
+        const unsigned char* src = base + (uint64_t)(uint32_t)(ok ? pid : 0) * page_b + (uint64_t)(uint32_t)(tok & pmask) * tok_b + cc * 16;
+        cp_async16_z(st + rw * GE::ROWB + ((cc ^ swz<BITS, CH>(rw)) << 4), src, ok ? 16u : 0u);
+      }
+    };
+    int issued = 0;
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) {
+      if (issued < my_items) issue(issued, issued % STAGES);
+      cp_async_commit();
+      ++issued;
+    }
+
+    // ---- queries: row g of the tile as the B operand ----
+    uint32_t qf[D / 16][2];
+    uint32_t qb = 0;                 // bias product: this lane's part of the group sums of query g
+    float C0, C1;                    // factor of the scores of queries 2t and 2t + 1
+    {
+      const int r = qt * kRows + g;
+      const bool live = r < a.gqa && my_blocks > 0;
+      const uint16_t* qp = (const uint16_t*)a.q + (int64_t)b * a.q_str[0] + (int64_t)(hk * a.gqa + (live ? r : 0)) * a.q_str[1];
+      if constexpr (BITS == 16) {
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint16_t* p = qp + 16 * s + 2 * t + 8 * h;
+            qf[s][h] = live ? (uint32_t)p[0] | ((uint32_t)p[1] << 16) : 0u;
+          }
+        C0 = C1 = a.scale * kLog2e;
+      } else {
+        float f[G][16], sum[G], mx = 0.f;
+#pragma unroll
+        for (int grp = 0; grp < G; ++grp) {
+          const uint16_t* p = qp + grp * 64 + 16 * t;
+          uint4 raw[2];
+          if (a.q_vec) {
+            raw[0] = ((const uint4*)p)[0]; raw[1] = ((const uint4*)p)[1];
+          } else {
+            uint32_t e[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) e[k] = (uint32_t)p[2 * k] | ((uint32_t)p[2 * k + 1] << 16);
+            raw[0] = make_uint4(e[0], e[1], e[2], e[3]); raw[1] = make_uint4(e[4], e[5], e[6], e[7]);
+          }
+          const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+          sum[grp] = 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            f[grp][2 * k] = live ? bf16lo(w[k]) : 0.f; f[grp][2 * k + 1] = live ? bf16hi(w[k]) : 0.f;
+            mx = fmax_nan(mx, fmax_nan(fabsf(f[grp][2 * k]), fabsf(f[grp][2 * k + 1])));
+            sum[grp] += f[grp][2 * k] + f[grp][2 * k + 1];
+          }
+          sum[grp] += __shfl_xor_sync(0xffffffffu, sum[grp], 1);
+          sum[grp] += __shfl_xor_sync(0xffffffffu, sum[grp], 2);
+        }
+        mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        int e = (int)((__float_as_uint(mx) >> 23) & 0xFF) - 127;    // mx < 2^(e + 1)
+        e = e < -100 ? -100 : (e > 110 ? 110 : e);
+        const float up = pow2i(14 - e);
+        const float qc = poison_if(nonfinite(mx), pow2i(24 - 14 + e) * (a.scale * kLog2e));
+        C0 = __shfl_sync(0xffffffffu, qc, 8 * t);
+        C1 = __shfl_sync(0xffffffffu, qc, 8 * t + 4);
+        // s = qc * (scale * sum q~ c 2^-24 + bias * sum q~ 2^-24): the sum in three bf16 parts, one a lane
+#pragma unroll
+        for (int grp = 0; grp < G; ++grp) {
+          float v = sum[grp] * up * 5.9604644775390625e-8f;
+          uint16_t part = 0;
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            const uint16_t pi = f32_to_bf16_bits(v);
+            v -= bf16_bits_to_f32(pi);
+            part = t == i ? pi : part;
+          }
+          qb |= (uint32_t)part << (16 * grp);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const float* x = BITS == 4 ? &f[grp][8 * (s >> 1) + 2 * (s & 1)] : &f[grp][4 * s];
+            if constexpr (BITS == 4) {   // codes j and j + 4 of a word, then 16 times codes j + 1 and j + 5
+              qf[grp * 4 + s][0] = pack_f16x2(x[0] * up, x[4] * up);
+              qf[grp * 4 + s][1] = pack_f16x2(x[1] * up * 0.0625f, x[5] * up * 0.0625f);
+            } else {                     // codes 0 and 2 of a word, then 1 and 3
+              qf[grp * 4 + s][0] = pack_f16x2(x[0] * up, x[2] * up);
+              qf[grp * 4 + s][1] = pack_f16x2(x[1] * up, x[3] * up);
+            }
+          }
+        }
+      }
+    }
+
+    int consumed = 0;
+    auto acquire = [&]() -> const unsigned char* {
+      if (issued < my_items) issue(issued, issued % STAGES);
+      cp_async_commit();
+      ++issued;
+      cp_async_wait<STAGES - 1>();
+      __syncwarp();
+      const unsigned char* st = my_ring_p + (consumed % STAGES) * GE::STAGE;
+      ++consumed;
+      return st;
+    };
+
+    float r_run[2] = {kNegBig, kNegBig}, l_part[2] = {0.f, 0.f};
+    float O[GE::NT][4];
+    float ob[G][2];
+#pragma unroll
+    for (int i = 0; i < GE::NT; ++i) O[i][0] = O[i][1] = O[i][2] = O[i][3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < G; ++i) ob[i][0] = ob[i][1] = 0.f;
+
+    for (int j = 0; j < my_blocks; ++j) {
+      const int tok_blk = first_token(j);
+      unsigned char* sbb = my_sb_p + (j & 1) * 4 * GE::SB;
+      float sc[4][4];     // [16 tokens][token g | g + 8][query 2t | 2t + 1]
+      bool whole = false;
+      uint32_t vm = 0;
+      // ---------------- scores ----------------
+#pragma unroll
+      for (int it = 0; it < ITEMS / 2; ++it) {
+        const unsigned char* st = acquire();
+        if (it == 0) {
+          const int newest = (issued - 1 < my_items ? issued - 1 : my_items - 1) / ITEMS;   // the block whose pages were read last
+          vm = (valid >> (4 * (newest - j))) & 15u;
+          whole = vm == 15u && tok_blk + kBlk <= sn.len && (tok_blk >= sn.w0 || tok_blk + kBlk <= sn.sinks);
+          if constexpr (BITS != 16) {
+            if (!whole) {             // parameters of rows that were not read: zero, whatever lies there
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int tk = h * 32 + lane;
+                if (!(visible(tok_blk + tk) && ((vm >> (tk >> 4)) & 1u)))
+#pragma unroll
+                  for (int i = 0; i < 4 * G; ++i) ((uint16_t*)(sbb + (i / G) * GE::SB))[tk * G + i % G] = 0;
+              }
+              __syncwarp();
+            }
+          }
+        }
+#pragma unroll
+        for (int s2 = 0; s2 < TOK / 16; ++s2) {
+          const int sub = it * (TOK / 16) + s2;
+          if constexpr (BITS == 16) {
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            const int rw = s2 * 16 + (lane & 15);
+            const uint32_t addr = (uint32_t)__cvta_generic_to_shared(st) + rw * GE::ROWB;
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s) {
+              uint32_t k4[4];
+              ldmatrix_b16_x4<false>(k4, addr + (((2 * s + (lane >> 4)) ^ swz<BITS, CH>(rw)) << 4));
+              mma_bf16_16816(d, k4, qf[s][0], qf[s][1]);
+            }
+            sc[sub][0] = d[0] * C0; sc[sub][1] = d[1] * C1; sc[sub][2] = d[2] * C0; sc[sub][3] = d[3] * C1;
+          } else {
+            float d[G][4];
+            const int ra = s2 * 16 + g, rb = ra + 8;
+#pragma unroll
+            for (int grp = 0; grp < G; ++grp) {
+              d[grp][0] = d[grp][1] = d[grp][2] = d[grp][3] = 0.f;
+              uint32_t wa[4], wb[4];
+              if constexpr (BITS == 4) {
+                const int c = 2 * grp + (t >> 1), o = (t & 1) * 8;
+                const uint2 x = *(const uint2*)(st + ra * GE::ROWB + ((c ^ swz<BITS, CH>(ra)) << 4) + o);
+                const uint2 y = *(const uint2*)(st + rb * GE::ROWB + ((c ^ swz<BITS, CH>(rb)) << 4) + o);
+                wa[0] = x.x; wa[1] = x.y; wb[0] = y.x; wb[1] = y.y;
+              } else {
+                const int c = 4 * grp + t;
+                const uint4 x = *(const uint4*)(st + ra * GE::ROWB + ((c ^ swz<BITS, CH>(ra)) << 4));
+                const uint4 y = *(const uint4*)(st + rb * GE::ROWB + ((c ^ swz<BITS, CH>(rb)) << 4));
+                wa[0] = x.x; wa[1] = x.y; wa[2] = x.z; wa[3] = x.w;
+                wb[0] = y.x; wb[1] = y.y; wb[2] = y.z; wb[3] = y.w;
+              }
+#pragma unroll
+              for (int s = 0; s < 4; ++s) {
+                uint32_t a0, a1, a2, a3;
+                if constexpr (BITS == 4) {
+                  const uint32_t x = (s & 1) ? wa[s >> 1] >> 8 : wa[s >> 1], y = (s & 1) ? wb[s >> 1] >> 8 : wb[s >> 1];
+                  a0 = x & 0x000F000Fu; a1 = y & 0x000F000Fu; a2 = x & 0x00F000F0u; a3 = y & 0x00F000F0u;
+                } else {
+                  a0 = wa[s] & 0x00FF00FFu; a1 = wb[s] & 0x00FF00FFu; a2 = (wa[s] >> 8) & 0x00FF00FFu; a3 = (wb[s] >> 8) & 0x00FF00FFu;
+                }
+                mma_f16_16816(d[grp], a0, a1, a2, a3, qf[grp * 4 + s][0], qf[grp * 4 + s][1]);
+              }
+            }
+            const int tk = sub * 16 + g;
+            float e[4] = {0.f, 0.f, 0.f, 0.f};
+            float s0[G], s1[G];
+            if constexpr (G == 2) {
+              mma_bf16_1688(e, *(const uint32_t*)(sbb + GE::SB + tk * 4), *(const uint32_t*)(sbb + GE::SB + (tk + 8) * 4), qb);
+              const uint32_t x = *(const uint32_t*)(sbb + tk * 4), y = *(const uint32_t*)(sbb + (tk + 8) * 4);
+              s0[0] = bf16lo(x); s0[1] = bf16hi(x); s1[0] = bf16lo(y); s1[1] = bf16hi(y);
+            } else {
+              mma_bf16_1688(e, (uint32_t) * (const uint16_t*)(sbb + GE::SB + tk * 2), (uint32_t) * (const uint16_t*)(sbb + GE::SB + (tk + 8) * 2), qb);
+              s0[0] = bf16_bits_to_f32(*(const uint16_t*)(sbb + tk * 2)); s1[0] = bf16_bits_to_f32(*(const uint16_t*)(sbb + (tk + 8) * 2));
+            }
+#pragma unroll
+            for (int grp = 0; grp < G; ++grp) {
+              e[0] = fmaf(s0[grp], d[grp][0], e[0]); e[1] = fmaf(s0[grp], d[grp][1], e[1]);
+              e[2] = fmaf(s1[grp], d[grp][2], e[2]); e[3] = fmaf(s1[grp], d[grp][3], e[3]);
+            }
+            sc[sub][0] = e[0] * C0; sc[sub][1] = e[1] * C1; sc[sub][2] = e[2] * C0; sc[sub][3] = e[3] * C1;
+          }
+        }
+        __syncwarp();
+      }
+      if (!whole) {
+#pragma unroll
+        for (int sub = 0; sub < 4; ++sub)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int tk = sub * 16 + h * 8 + g;
+            if (!(visible(tok_blk + tk) && ((vm >> sub) & 1u))) sc[sub][2 * h] = sc[sub][2 * h + 1] = kNegBig;
+          }
+      }
+      // ---------------- the block's softmax ----------------
+      int ex = 141;
+      if constexpr (BITS != 16) {      // exponent of the block's largest |v_scale|
+        uint32_t m;
+        if constexpr (G == 2) {
+          const uint2 v = *(const uint2*)(sbb + 2 * GE::SB + lane * 8);
+          m = __vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu);
+        } else {
+          m = *(const uint32_t*)(sbb + 2 * GE::SB + lane * 4) & 0x7FFF7FFFu;
+        }
+        ex = (int)(__reduce_max_sync(0xffffffffu, max(m >> 16, m & 0xFFFFu)) >> 7);
+        ex = ex < 60 ? 60 : ex;          // (p <= 2^81: its sum stays finite over any length)
+      }
+      float mb[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float m = fmaxf(sc[0][c], sc[0][2 + c]);
+#pragma unroll
+        for (int sub = 1; sub < 4; ++sub) m = fmaxf(m, fmaxf(sc[sub][c], sc[sub][2 + c]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        mb[c] = fmaxf(r_run[c], m + (float)(ex - 141));   // p = 2^(s - r), r >= max s + ex - 141: p * v_scale stays below 2^15
+      }
+      if (__any_sync(0xffffffffu, mb[0] > r_run[0] || mb[1] > r_run[1])) {
+        const float al0 = ex2(r_run[0] - mb[0]), al1 = ex2(r_run[1] - mb[1]);
+#pragma unroll
+        for (int i = 0; i < GE::NT; ++i) { O[i][0] *= al0; O[i][1] *= al1; O[i][2] *= al0; O[i][3] *= al1; }
+#pragma unroll
+        for (int i = 0; i < G; ++i) { ob[i][0] *= al0; ob[i][1] *= al1; }
+        l_part[0] *= al0; l_part[1] *= al1;
+        r_run[0] = mb[0]; r_run[1] = mb[1];
+      }
+#pragma unroll
+      for (int sub = 0; sub < 4; ++sub)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = sc[sub][i] <= kNegBig ? 0.f : ex2(sc[sub][i] - r_run[i & 1]);
+          l_part[i & 1] += p;
+          sc[sub][i] = p;
+        }
+      // ---------------- values ----------------
+#pragma unroll
+      for (int it = 0; it < ITEMS / 2; ++it) {
+        const uint32_t stv = (uint32_t)__cvta_generic_to_shared(acquire());
+#pragma unroll
+        for (int s2 = 0; s2 < TOK / 16; ++s2) {
+          const int sub = it * (TOK / 16) + s2;
+          if constexpr (BITS == 16) {
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float p0 = sc[sub][2 * h], p1 = sc[sub][2 * h + 1];
+              const uint32_t u = pack2(p0, p1);
+              hi[h] = transpose8x8(u);
+              lo[h] = transpose8x8(pack2(p0 - bf16lo(u), p1 - bf16hi(u)));
+            }
+            const int rw = s2 * 16 + (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+            for (int n = 0; n < GE::NT; ++n) {
+              uint32_t v4[4];
+              ldmatrix_b16_x4<true>(v4, stv + rw * GE::ROWB + (((2 * n + ((lane >> 3) & 1)) ^ swz<BITS, CH>(rw)) << 4));
+              mma_bf16_16816(O[n], v4, hi[0], hi[1]);
+              mma_bf16_16816(O[n], v4, lo[0], lo[1]);
+            }
+          } else {
+            uint32_t pb[G][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int tk = sub * 16 + h * 8 + g;
+              const float p0 = sc[sub][2 * h], p1 = sc[sub][2 * h + 1];
+              float vs[G], vb[G];
+              if constexpr (G == 2) {
+                const uint32_t x = *(const uint32_t*)(sbb + 2 * GE::SB + tk * 4), y = *(const uint32_t*)(sbb + 3 * GE::SB + tk * 4);
+                vs[0] = bf16lo(x); vs[1] = bf16hi(x); vb[0] = bf16lo(y); vb[1] = bf16hi(y);
+              } else {
+                vs[0] = bf16_bits_to_f32(*(const uint16_t*)(sbb + 2 * GE::SB + tk * 2)); vb[0] = bf16_bits_to_f32(*(const uint16_t*)(sbb + 3 * GE::SB + tk * 2));
+              }
+#pragma unroll
+              for (int grp = 0; grp < G; ++grp) {
+                pb[grp][h] = transpose8x8(pack_f16x2(p0 * vs[grp], p1 * vs[grp]));
+                ob[grp][0] = fmaf(p0, vb[grp], ob[grp][0]);
+                ob[grp][1] = fmaf(p1, vb[grp], ob[grp][1]);
+              }
+            }
+            // matrix row 4u + i of ldmatrix = token {2u, 8 + 2u, 2u + 1, 9 + 2u}[i]
+            const int mr = lane & 15, half_m = lane >> 4;
+            const int tokrow = s2 * 16 + 2 * (mr >> 2) + ((mr >> 1) & 1) + 8 * (mr & 1);
+#pragma unroll
+            for (int kb = 0; kb < CH; kb += 2) {
+              uint32_t r[4];
+              ldmatrix_b8_trans_x2(r, stv + tokrow * GE::ROWB + (((kb + half_m) ^ swz<BITS, CH>(tokrow)) << 4));
+#pragma unroll
+              for (int m = 0; m < 2; ++m) {   // chunk kb + m: byte columns g (row g of the tile) and g + 8
+                const uint32_t x = r[2 * m], y = r[2 * m + 1], xh = x >> 8, yh = y >> 8;
+                if constexpr (BITS == 4) {
+                  const int grp = (kb + m) >> 1, n = 2 * (kb + m);
+                  mma_f16_16816(O[n], x & 0x000F000Fu, y & 0x000F000Fu, xh & 0x000F000Fu, yh & 0x000F000Fu, pb[grp][0], pb[grp][1]);
+                  mma_f16_16816(O[n + 1], x & 0x00F000F0u, y & 0x00F000F0u, xh & 0x00F000F0u, yh & 0x00F000F0u, pb[grp][0], pb[grp][1]);
+                } else {
+                  const int grp = (kb + m) >> 2, n = kb + m;
+                  mma_f16_16816(O[n], x & 0x00FF00FFu, y & 0x00FF00FFu, xh & 0x00FF00FFu, yh & 0x00FF00FFu, pb[grp][0], pb[grp][1]);
+                }
+              }
+            }
+          }
+        }
+        __syncwarp();
+      }
+    }
+    cp_async_wait<0>();
+
+    // ---- join the warps: sums are partial over the 8 lanes that share a query ----
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        l_part[c] += __shfl_xor_sync(0xffffffffu, l_part[c], o);
+#pragma unroll
+        for (int grp = 0; grp < G; ++grp) ob[grp][c] += __shfl_xor_sync(0xffffffffu, ob[grp][c], o);
+      }
+    }
+    __syncthreads();      // every warp is done with its ring
+    float* wm = (float*)smem;                     // [warp][8]
+    float* wl = wm + kWarps * kRows;
+    float* wo = wl + kWarps * kRows;              // [warp][8][D]
+    if (g == 0) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) { wm[warp * kRows + 2 * t + c] = r_run[c]; wl[warp * kRows + 2 * t + c] = l_part[c]; }
+    }
+#pragma unroll
+    for (int n = 0; n < GE::NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int m = g + 8 * (i >> 1), c = i & 1;
+        int dim; float v = O[n][i];
+        if constexpr (BITS == 4) {      // codes came in as c * 2^-24 (even dims) or 16 c * 2^-24 (odd)
+          dim = 32 * (n >> 1) + 2 * m + (n & 1);
+          v = fmaf(v, (n & 1) ? 1048576.f : 16777216.f, ob[(n >> 2) % G][c]);
+        } else if constexpr (BITS == 8) {
+          dim = 16 * n + m;
+          v = fmaf(v, 16777216.f, ob[(n >> 2) % G][c]);
+        } else dim = 16 * n + m;
+        wo[(size_t)(warp * kRows + 2 * t + c) * D + dim] = v;
+      }
+    __syncthreads();
+    const int rows = a.gqa - qt * kRows < kRows ? a.gqa - qt * kRows : kRows;
+    const bool all = blk0 == 0 && todo == sn.blocks;
+    const int slot = 2 * blockIdx.x + (blk0 == 0 ? 1 : 0);
+    if (!all && blk0 == 0 && tid == 0) {          // the first of the blocks that share this sequence
+      const int more = (units[b] + (tile + 1) * sn.blocks - 1) / per - (int)blockIdx.x;
+      a.joins[blockIdx.x] = make_int4(b, hk * a.gqa + qt * kRows, rows, more);
+    }
+    for (int i = tid; i < rows * D; i += kWarps * 32) {
+      const int h = i / D, e = i - h * D;
+      float M = kNegBig;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, wm[w * kRows + h]);
+      float L = 0.f, Ov = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = ex2(wm[w * kRows + h] - M);
+        L += wl[w * kRows + h] * f;
+        Ov += wo[(size_t)(w * kRows + h) * D + e] * f;
+      }
+      if (all) {
+        const float v = Ov * (L > 0.f ? 1.f / L : (L == L ? 0.f : L));
+        ((uint16_t*)a.out)[(int64_t)b * a.o_str[0] + (int64_t)(hk * a.gqa + qt * kRows + h) * a.o_str[1] + e] = f32_to_bf16_bits(v);
+      } else {
+        a.part_o[((int64_t)slot * kRows + h) * D + e] = Ov;
+        if (e == 0) { a.part_ml[slot * kRows + h] = make_float2(M, L); }
+      }
+    }
+    __syncthreads();      // the ring may be filled again
+    u += todo;
+  }
+}
+
+// ---- the parts of a sequence that several blocks share: out = (sum_r o_r w_r) / (sum_r l_r w_r), w_r = 2^(m_r - max m) ----
+// Block c joins the sequence that begins in block c's share and ends behind it: its own part (slot 2c + 1) and those of the next
+// blocks (slots 2(c + k)).  A warp takes one query's every parts-th part.
+template <int D>
+__global__ void __launch_bounds__(kMergeWarps * 32) kv_pages_join_kernel(const __grid_constant__ KvPagesAttnArgs a) {
+  __shared__ float red[kMergeWarps][D + 2];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 jn = a.joins[blockIdx.x];
+  if (jn.x < 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = jn.z, n = jn.w + 1;
+  const int parts = kMergeWarps / rows, h = warp % rows, part = warp / rows;
+  constexpr int V = D / 32;
+  auto slot = [&](int k) { return k == 0 ? 2 * (int)blockIdx.x + 1 : 2 * ((int)blockIdx.x + k); };
+  float M = kNegBig, L = 0.f, o[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) o[i] = 0.f;
+  if (part < parts) {
+    for (int k0 = part; k0 < n; k0 += parts * 32) {
+      const int k = k0 + lane * parts;
+      float2 ml = make_float2(kNegBig, 0.f);
+      if (k < n) ml = __ldcg(a.part_ml + slot(k) * kRows + h);
+      float m = ml.x;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+      const float Mn = fmaxf(M, m), f = ex2(M - Mn), w = ex2(ml.x - Mn);
+      L = L * f + w * ml.y;          // a lane's own parts
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] *= f;
+      M = Mn;
+      const int cnt = (n - k0 + parts - 1) / parts < 32 ? (n - k0 + parts - 1) / parts : 32;
+#pragma unroll 8
+      for (int q = 0; q < cnt; ++q) {
+        const float wq = __shfl_sync(0xffffffffu, w, q);
+        const float* src = a.part_o + ((int64_t)slot(k0 + q * parts) * kRows + h) * D + lane * V;
+        if constexpr (V == 4) {
+          const float4 x = __ldcg((const float4*)src);
+          o[0] = fmaf(wq, x.x, o[0]); o[1] = fmaf(wq, x.y, o[1]); o[2] = fmaf(wq, x.z, o[2]); o[3] = fmaf(wq, x.w, o[3]);
+        } else {
+          const float2 x = __ldcg((const float2*)src);
+          o[0] = fmaf(wq, x.x, o[0]); o[1] = fmaf(wq, x.y, o[1]);
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+#pragma unroll
+    for (int i = 0; i < V; ++i) red[warp][lane * V + i] = o[i];
+    if (lane == 0) { red[warp][D] = M; red[warp][D + 1] = L; }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * D; i += kMergeWarps * 32) {
+    const int r = i / D, e = i - r * D;
+    float Mx = kNegBig;
+    for (int p = 0; p < parts; ++p) Mx = fmaxf(Mx, red[p * rows + r][D]);
+    float Ls = 0.f, Os = 0.f;
+    for (int p = 0; p < parts; ++p) {
+      const float f = ex2(red[p * rows + r][D] - Mx);
+      Ls += red[p * rows + r][D + 1] * f;
+      Os += red[p * rows + r][e] * f;
+    }
+    const float v = Os * (Ls > 0.f ? 1.f / Ls : (Ls == Ls ? 0.f : Ls));
+    ((uint16_t*)a.out)[(int64_t)jn.x * a.o_str[0] + (int64_t)(jn.y + r) * a.o_str[1] + e] = f32_to_bf16_bits(v);
+  }
+}
+
+// CTAs of an instance that the device holds at once.
+template <int BITS, int D> cudaError_t resident(int* n) {
+  auto kern = kv_pages_kernel<BITS, D>;
+  static int cached[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> setup_lk(setup_mutex());   // first use on a device, from any thread
+  if (dev < 0 || dev >= 64 || cached[dev] == 0) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<BITS, D>::SMEM);
+    if (e != cudaSuccess) return e;
+    int per = 0;
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, kWarps * 32, Geo<BITS, D>::SMEM);
+    if (e != cudaSuccess) return e;
+    const int all = (per < 1 ? 1 : (per > kPagesCtas ? kPagesCtas : per)) * sm_count();
+    if (dev < 0 || dev >= 64) { *n = all; return cudaSuccess; }
+    cached[dev] = all;
+  }
+  *n = cached[dev];
+  return cudaSuccess;
+}
+
+template <int BITS, int D> cudaError_t launch_inst(KvPagesAttnArgs a, int64_t most_units, cudaStream_t st) {
+  int n = 0;
+  cudaError_t e = resident<BITS, D>(&n);
+  if (e != cudaSuccess) return e;
+  const unsigned grid = (unsigned)(most_units < n ? (most_units < 1 ? 1 : most_units) : n);
+  e = launch_kernel(kv_pages_kernel<BITS, D>, dim3(grid), dim3(kWarps * 32), Geo<BITS, D>::SMEM, st, a);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kMergeWarps * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv_pages_join_kernel<D>, a);
+}
+}  // namespace
+
+// [joins: int4 per CTA][m, l: float2 per slot and row][o: D floats per slot and row], two slots a CTA
+size_t kv_pages_workspace_bytes(int64_t D) {
+  const size_t ctas = (size_t)kPagesCtas * sm_count();
+  return ctas * 16 + ctas * 2 * kRows * 8 + ctas * 2 * kRows * (size_t)D * 4;
+}
+
+cudaError_t launch_kv_pages_attn(KvPagesAttnArgs a, int D, void* workspace, cudaStream_t st) {
+  const size_t ctas = (size_t)kPagesCtas * sm_count();
+  a.joins = (int4*)workspace;
+  a.part_ml = (float2*)((char*)workspace + ctas * 16);
+  a.part_o = (float*)((char*)workspace + ctas * 16 + ctas * 2 * kRows * 8);
+  a.qtiles = (a.gqa + kRows - 1) / kRows;
+  a.tiles = a.Hkv * a.qtiles;
+  a.min_units = kWarps;
+  // the most blocks that a sequence can see
+  int64_t most = (((int64_t)a.M << a.page_shift) + kBlk - 1) / kBlk;
+  if (a.window > 0) {
+    const int64_t w = ((int64_t)a.window + kBlk - 1) / kBlk + 1 + ((int64_t)a.sinks + kBlk - 1) / kBlk;
+    most = most < w ? most : w;
+  }
+  const int64_t units = most * a.tiles * a.B;
+  switch (a.bits * 1000 + D) {
+    case 4064: return launch_inst<4, 64>(a, units, st);
+    case 4128: return launch_inst<4, 128>(a, units, st);
+    case 8064: return launch_inst<8, 64>(a, units, st);
+    case 8128: return launch_inst<8, 128>(a, units, st);
+    case 16064: return launch_inst<16, 64>(a, units, st);
+    case 16128: return launch_inst<16, 128>(a, units, st);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace qb

@@ -148,6 +148,17 @@ def lib():
         L.qb200_kv_append_seqs.argtypes = [C.POINTER(TP)] * 6 + [TP, TP, C.POINTER(C.c_int64), C.c_int, C.c_int, C.c_int, C.c_void_p]
         L.qb200_rope_kv_append_seqs.argtypes = [TP, C.c_int, C.c_float, C.c_float] + L.qb200_kv_append_seqs.argtypes
         L.qb200_rope_kv_append_seqs.restype = C.c_int
+        L.qb200_kv_pages_append.argtypes = [TP] * 12 + [C.c_int, C.c_int, C.c_void_p]
+        L.qb200_kv_pages_free.argtypes = [TP] * 3 + [C.c_int] + [TP] * 3 + [C.c_void_p]
+        L.qb200_kv_pages_fork.argtypes = [TP] * 4 + [C.c_int] + [TP] * 3 + [C.c_void_p]
+        L.qb200_kv_pages_reserve.argtypes = [TP] * 5 + [C.c_int] + [TP] * 2 + [C.c_void_p]
+        L.qb200_kv_pages_compact.argtypes = [TP] * 5 + [C.c_void_p]
+        L.qb200_kv_pages_copy.argtypes = [C.POINTER(TP), C.c_int, TP, TP, C.c_void_p]
+        L.qb200_kv_pages_decode_attention.argtypes = [TP] * 11 + [C.c_int, C.c_int, C.c_float, C.c_int64, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]
+        L.qb200_kv_pages_decode_attention_workspace_size.argtypes = [C.c_int64] * 4
+        L.qb200_kv_pages_decode_attention_workspace_size.restype = C.c_size_t
+        for name in ("append", "free", "fork", "reserve", "compact", "copy", "decode_attention"):
+            getattr(L, "qb200_kv_pages_" + name).restype = C.c_int
         for name in ("qb200_rms_norm", "qb200_add_rms_norm", "qb200_rope", "qb200_swiglu", "qb200_kv_append_seqs"):
             getattr(L, name).restype = C.c_int
         L.qb200_kv_decode_attention_noalloc.argtypes = [TP, TP, TP, TP, TP, TP, TP, TP, C.c_int, C.c_int, C.c_float,
@@ -333,6 +344,54 @@ def kv_append_seqs(k_triples, v_triples, dense_k, dense_v, offsets, bits, group_
     src/transformer.zig:9738-9756): k_triples[n] / v_triples[n] are the capacity buffers [1, Hkv, cap_n, .].
     With ``rope_q`` the same launch rotates the queries in place and the keys on their way into the cache."""
     _native.kv_append_seqs(k_triples, v_triples, dense_k, dense_v, offsets, bits, group_size, rope_q, rope_dims, rope_base, rope_scale)
+
+
+# ---- the paged cache: a pool is (codes, scales, biases) of [pages, heads, page, cols], at 16 bits (rows, None, None); table [sequences, M],
+# lens [sequences] and refs [pages] are int32 tensors on the device that the calls change in place ----
+
+def kv_pages_append(k_pool, v_pool, dense_k, dense_v, table, positions, bits, group_size=64, rows=None, counts=None):
+    """New rows dense_k / dense_v [N, heads, S, D] into pages: token i of entry n at position positions[n] + i of sequence rows[n]
+    (default n), for i < counts[n] (default S)."""
+    _native.kv_pages_append(k_pool, v_pool, dense_k, dense_v, table, positions, bits, group_size, rows, counts)
+
+
+def kv_pages_free(table, lens, refs, page, rows, begin=None, end=None):
+    """Frees the pages of the listed sequences that lie wholly in tokens [begin, end) (default: all); an end at the sequence's
+    length or behind it shortens the sequence to ``begin`` tokens."""
+    _native.kv_pages_free(table, lens, refs, page, rows, begin, end)
+
+
+def kv_pages_fork(table, lens, refs, page, src, dst, tokens=None):
+    """Sequence dst[n], which is empty, begins with the first tokens[n] tokens (default: all) of sequence src[n] and shares their pages.
+    Returns the tokens shared, -1 for a refused entry."""
+    return _native.kv_pages_fork(table, lens, refs, page, src, dst, tokens)
+
+
+def kv_pages_reserve(table, lens, refs, page, rows, counts):
+    """Room for counts[n] more tokens in sequence rows[n].  Returns (positions, copies): the length before (-1: refused) and, where a
+    half-filled shared page was replaced, the pair (old, new) for ``kv_pages_copy``, else (-1, -1)."""
+    return _native.kv_pages_reserve(table, lens, refs, page, rows, counts)
+
+
+def kv_pages_compact(table, refs):
+    """Moves the live pages to the front of the pool.  Returns (remap, moves, count): the new number of every page (-1: free), the
+    (old, new) pairs with -1 behind them, and how many; the rows move with ``kv_pages_copy(pools, moves, count)``."""
+    return _native.kv_pages_compact(table, refs)
+
+
+def kv_pages_copy(pools, pairs, count=None):
+    """Copies page pairs[n, 0] to page pairs[n, 1] in every tensor of the list ``pools`` (first axis: pages)."""
+    _native.kv_pages_copy(pools, pairs, count)
+
+
+def kv_pages_decode_attention_workspace_size(B, Hq, Hkv, D) -> int:
+    return int(lib().qb200_kv_pages_decode_attention_workspace_size(B, Hq, Hkv, D))
+
+
+def kv_pages_decode_attention(q, k_pool, v_pool, table, lens, bits, group_size, scale, window=0, sinks=0, rows=None, workspace=None, out=None):
+    """Attention of one new token per sequence over its pages; q [B, Hq, 1, D] bf16, query b of sequence rows[b] (default b).  With a
+    window the query sees the last ``window`` tokens and the first ``sinks``."""
+    return _native.kv_pages_decode_attention(q, k_pool, v_pool, table, lens, bits, group_size, scale, window, sinks, rows, workspace, out)
 
 
 _Q2TORCH = {v: k for k, v in _TORCH2Q.items()}
