@@ -430,6 +430,16 @@ QB200_API int qb200_kv_pages_decode_attention(qb200_tensor* res, const qb200_ten
                                               int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes, qb200_stream s);
 QB200_API size_t qb200_kv_pages_decode_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
 
+/* ---- causal attention of a prompt, or of a chunk behind cached tokens, with a sliding window and sinks ----
+ * The dense attention of the reference's prefill (mlx_fast_scaled_dot_product_attention, src/mlx.zig:325; its window as the mask of the
+ * sliding layers).  q, res [B, Hq, Tq, D], k, v [B, Hkv, Tk, D], all bf16, D 64 or 128, rows of q, k and v on 16 bytes.  Sequence b has
+ * kv_lens[b] keys (int32 on the device; empty: Tk, which must be at least Tq then); its query i stands at position p = kv_lens[b] - Tq + i
+ * and sees the keys j <= p with j > p - window or j < sinks (window 0: all j <= p).  A query before position 0 sees nothing and gives
+ * zeros.  scale must be positive.  Keys and values that no query sees may hold anything; a query that sees a value which is not finite
+ * gives results that are not. */
+QB200_API int qb200_window_attention(qb200_tensor* res, const qb200_tensor* q, const qb200_tensor* k, const qb200_tensor* v, float scale, int64_t window,
+                                     int64_t sinks, const qb200_tensor* kv_lens, qb200_stream s);
+
 /* ==== checkpoint -> device loader: MLX-format quantized safetensors (host side; the device layout is the file's) ==== */
 
 /* One opened .safetensors file (memory-mapped).  Quantized linears are stored as <name>.weight (uint32 packed codes),

@@ -715,6 +715,20 @@ PyObject* kv_pages_decode_attention(Args a) {
   return a[12] == Py_None ? wrap(std::move(out)) : ret(a[12]);
 }
 
+// q, k, v, scale, window, sinks, kv_lens, out
+PyObject* window_attention(Args a) {
+  OnDevice dev;
+  for (int i : {0, 1, 2, 6, 7}) dev.add(a[i]);
+  const at::Tensor& q = tensor(a[0]);
+  const float scale = (float)as_double(a[3]);
+  const int64_t window = as_index(a[4]), sinks = as_index(a[5]);
+  void* st = dev.stream();
+  at::Tensor out = a[7] == Py_None ? at::empty(q.sizes(), q.options().requires_grad(false)) : tensor(a[7]);
+  T y = plain(out), dq = plain(q), k = plain(a[1]), v = plain(a[2]), l = plain(a[6]);
+  call([&] { return qb200_window_attention(&y.d, &dq.d, &k.d, &v.d, scale, window, sinks, &l.d, st); });
+  return a[7] == Py_None ? wrap(std::move(out)) : ret(a[7]);
+}
+
 PyObject* set_error_class(Args a) {
   Py_INCREF(a[0]);
   Py_XDECREF(g_error_class);
@@ -730,7 +744,7 @@ PyMethodDef methods[] = {
     QB_ENTRY(kv_decode_attention_noalloc, 10), QB_ENTRY(kv_decode_attention_ptrs, 11), QB_ENTRY(add_rms_norm, 7), QB_ENTRY(rms_norm, 4),
     QB_ENTRY(rope, 6), QB_ENTRY(turbo_rotate, 3), QB_ENTRY(swiglu, 3), QB_ENTRY(kv_append_seqs, 11), QB_ENTRY(set_error_class, 1),
     QB_ENTRY(kv_pages_append, 10), QB_ENTRY(kv_pages_free, 7), QB_ENTRY(kv_pages_fork, 7), QB_ENTRY(kv_pages_reserve, 6), QB_ENTRY(kv_pages_compact, 2),
-    QB_ENTRY(kv_pages_copy, 3), QB_ENTRY(kv_pages_decode_attention, 13),
+    QB_ENTRY(kv_pages_copy, 3), QB_ENTRY(kv_pages_decode_attention, 13), QB_ENTRY(window_attention, 8),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native half of the qb200 Python binding", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

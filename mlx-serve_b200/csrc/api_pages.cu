@@ -45,6 +45,8 @@ int expect_list(const qb200_tensor* t, const char* who, const char* name, int64_
 }
 // Rows that a kernel writes: no two of them may be the same memory.
 bool rows_distinct(const qb200_tensor* t) {
+  for (int d = 0; d < t->ndim; ++d)
+    if (t->shape[d] == 0) return true;
   for (int d = 0; d + 1 < t->ndim; ++d)
     if (t->shape[d] > 1 && t->stride[d] < t->shape[t->ndim - 1]) return false;
   return true;
@@ -405,6 +407,61 @@ QB200_API int qb200_kv_pages_decode_attention(qb200_tensor* res, const qb200_ten
   a.sinks = (int)(sinks < INT32_MAX ? sinks : INT32_MAX);
   a.bits = bits; a.scale = scale; a.sb_vec = vec[0] && vec[1];
   const cudaError_t e = launch_kv_pages_attn(a, (int)D, workspace, (cudaStream_t)s);
+  return e == cudaSuccess ? QB200_OK : pg_cuda(e, who);
+}
+
+QB200_API int qb200_window_attention(qb200_tensor* res, const qb200_tensor* q, const qb200_tensor* k, const qb200_tensor* v, float scale, int64_t window,
+                                     int64_t sinks, const qb200_tensor* kv_lens, qb200_stream s) {
+  const char* who = "window_attention";
+  int st;
+  const qb200_tensor* const ts[4] = {q, k, v, res};
+  const char* const names[4] = {"q", "k", "v", "res"};
+  for (int i = 0; i < 4; ++i) {
+    if (ts[i] != nullptr && ts[i]->dtype != QB200_BFLOAT16) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: %s must be bf16", who, names[i]);
+    if ((st = expect(ts[i], who, names[i], 4, QB200_BFLOAT16))) return st;
+  }
+  const int64_t B = q->shape[0], Hq = q->shape[1], Tq = q->shape[2], D = q->shape[3], Hkv = k->shape[1], Tk = k->shape[2];
+  if (k->shape[0] != B || k->shape[3] != D) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: k must be [B, Hkv, Tk, D] with q's B and D", who);
+  for (int d = 0; d < 4; ++d) {
+    if (v->shape[d] != k->shape[d]) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: v must have k's shape", who);
+    if (res->shape[d] != q->shape[d]) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: res must have q's shape", who);
+  }
+  if (Hkv <= 0 || Hq % Hkv != 0) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: Hq %lld not a multiple of Hkv %lld", who, (long long)Hq, (long long)Hkv);
+  if (D != 64 && D != 128) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: head dim %lld is not served (64, 128)", who, (long long)D);
+  if (window < 0 || sinks < 0) return pg_fail(QB200_ERR_BAD_ARG, "%s: window and sinks must not be negative", who);
+  if (!(scale > 0.f) || !(scale <= 3.0e38f)) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: scale must be positive and finite", who);
+  if (!empty(kv_lens)) {
+    if ((st = expect_list(kv_lens, who, "kv_lens", B))) return st;
+  } else if (Tk < Tq) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: %lld queries need as many keys (%lld given)", who, (long long)Tq, (long long)Tk);
+  if (!rows_distinct(res)) return pg_fail(QB200_ERR_BAD_STRIDE, "%s: rows of res overlap", who);
+  if (B == 0 || Hq == 0 || Tq == 0) return QB200_OK;
+  if (Tk == 0) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: no keys", who);
+  const int64_t lim = (int64_t)1 << 30;
+  if (Tq > lim || Tk > lim || B > lim || Hq > lim || B * Hq > lim || ((Tq + 127) / 128) * B * Hq > INT32_MAX)
+    return pg_fail(QB200_ERR_UNSUPPORTED, "%s: %lld x %lld heads of %lld queries are too many for one call", who, (long long)B, (long long)Hq, (long long)Tq);
+  WindowArgs a;
+  std::memset(&a, 0, sizeof(a));
+  for (int i = 0; i < 3; ++i) {
+    bool ok = ((uintptr_t)ts[i]->data & 15) == 0;
+    for (int d = 0; d < 3; ++d) {
+      a.str[i][d] = ts[i]->stride[d];
+      if (ts[i]->shape[d] > 1) ok = ok && ts[i]->stride[d] % 8 == 0 && ts[i]->stride[d] < ((int64_t)1 << 38);
+    }
+    if (!ok) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: the rows of %s must start on 16 bytes", who, names[i]);
+    if (ts[i]->shape[2] > 1 && ts[i]->stride[2] == 0) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: %s repeats one token", who, names[i]);
+  }
+  a.o_vec = ((uintptr_t)res->data & 15) == 0;
+  for (int d = 0; d < 3; ++d) {
+    a.o_str[d] = res->stride[d];
+    if (res->shape[d] > 1 && res->stride[d] % 8 != 0) a.o_vec = 0;
+  }
+  a.q = q->data; a.k = k->data; a.v = v->data; a.out = res->data;
+  a.kv_lens = empty(kv_lens) ? nullptr : (const int32_t*)kv_lens->data;
+  a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.Tq = Tq; a.Tk = Tk; a.D = D;
+  a.window = window >= Tk ? 0 : (int)window;            // (no query has that many keys before it)
+  a.sinks = (int)(sinks < Tk ? sinks : Tk);
+  a.scale = scale;
+  const cudaError_t e = launch_window_attn(a, (cudaStream_t)s);
   return e == cudaSuccess ? QB200_OK : pg_cuda(e, who);
 }
 

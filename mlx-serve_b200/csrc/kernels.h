@@ -336,4 +336,17 @@ struct KvPagesAttnArgs {
 size_t kv_pages_workspace_bytes(int64_t D);
 cudaError_t launch_kv_pages_attn(KvPagesAttnArgs a, int D, void* workspace, cudaStream_t st);
 
+// ---- window_attn.cu: causal attention of a prompt, sliding window and sinks ----
+struct WindowArgs {
+  const void* q; const void* k; const void* v; void* out;
+  int64_t str[3][3], o_str[3];           // (sequence, head, token) strides of q, k, v; of the result
+  const int32_t* kv_lens;                // may be null
+  int64_t B, Hq, Hkv, Tq, Tk, D;
+  int window, sinks, o_vec;
+  float scale;
+};
+cudaError_t launch_window_attn(const WindowArgs& a, cudaStream_t st);
+void window_attn_error_reset();
+int window_attn_error_code();  // 0, or the code of a bounded wait that expired in it
+
 }  // namespace qb

@@ -1,0 +1,494 @@
+// Causal attention of a prompt (or a chunk of one behind cached tokens) with an optional sliding window and a few first tokens that
+// stay visible: bf16, head dim 64 or 128, on the tensor cores (tcgen05) with the scores and results in tensor memory.
+//
+// Query i stands at position p = kv_len - Tq + i and sees the keys j <= p with j > p - window or j < sinks.
+//   o = sum_j P_j v_j / sum_j P_j,  P_j = 2^(c s_j - c r),  s = q . k, c = scale * log2(e), r a running reference of the row.
+//
+// One CTA of 12 warps takes two tiles of 128 queries that read the same keys: two heads of a group where the group is even, else
+// two neighbouring tiles of one head.
+//   warps 0-3, 4-7 : the softmax of a tile, a thread a row.  Scores come from tensor memory, the probabilities go back in their place as
+//                    bf16, the A operand of the second product.  r follows the row's maximum only when it has fallen 2^8 behind, so the
+//                    result is rescaled in the first steps of a row and hardly ever after.
+//   warp 8         : copies (TMA): both query tiles once, then keys and values of 128 tokens in a ring.
+//   warp 9         : issues the matrix products, S = Q K^T of the next step behind P V of this one, the tiles in turn: while one
+//                    tile's softmax runs, the tensor cores work for the other.
+//   warps 10, 11   : make the values fit for a product with masked probabilities (0 * NaN is NaN): where a block is masked for
+//                    some query, rows that no query of the CTA sees are zeroed, and rows with anything not finite are zeroed and
+//                    noted; the queries that see such a row give NaN.
+// Blocks of 128 keys that no query of a tile sees are left out; only those cut by a border of the mask are masked element by element.
+#include <mutex>
+
+#include "tc_ptx.cuh"
+
+namespace qb {
+namespace {
+
+__device__ int g_window_error = 0;   // 0 = ok; otherwise the code of the wait that expired
+
+constexpr int kThreads = 384;
+constexpr int kTile = 128;           // queries of a tile, keys of a block
+constexpr uint32_t kPolls = 1u << 18;
+constexpr float kSlack = 8.f;        // exponents that the reference may lie below the maximum
+
+template <int D> struct Shape {
+  static constexpr int BYTES = kTile * D * 2;              // a tile of queries, keys or values
+  static constexpr int STAGES = D == 128 ? 5 : 8;
+  static constexpr int SMEM = (2 + STAGES) * BYTES + 1024;
+  static constexpr int HALVES = D / 64;                    // blocks of 64 columns (128 bytes) side by side
+};
+
+struct WindowK {
+  uint16_t* out; int64_t o_str[3];     // (sequence, head, token)
+  const int32_t* kv_lens;
+  int B, Hq, gqa, Tq, Tk, window, sinks;
+  int qblocks, heads2;                 // 1: the two tiles are two heads; 0: two tiles of one head
+  int mul[3][2];                       // coordinates along (head, sequence) of q, k, v: 0 where the tensor is broadcast
+  float c;
+  int o_vec;                           // result rows can be stored 16 bytes at a time
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+               ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accum) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(accum) : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bd, uint32_t idesc, uint32_t accum) {   // A in tensor memory
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(bd), "r"(idesc), "r"(accum) : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The key blocks of a CTA and what its tiles see of them; every role works this out for itself.
+struct Plan {
+  int p_lo[2], p_hi[2];     // positions of a tile's first and last query (p_lo may be below 0; p_hi < 0: it sees nothing)
+  int lo, hi;               // keys [lo, hi] and the sinks are all that the CTA sees
+  int window, sinks;
+  int front, skip, blocks;  // blocks [0, front), then i + skip
+  __device__ __forceinline__ int block(int i) const { return i < front ? i : i + skip; }
+  __device__ __forceinline__ bool needs(int t, int blk) const {       // some query of tile t sees some key of the block
+    const int k0 = blk * kTile, lo_t = t ? p_lo[1] : p_lo[0], hi_t = t ? p_hi[1] : p_hi[0];
+    const int first = lo_t > 0 ? lo_t : 0;
+    return k0 <= hi_t && (window == 0 || k0 + kTile - 1 > first - window || k0 < sinks);
+  }
+  __device__ __forceinline__ bool whole(int t, int blk) const {       // every query of tile t sees every key of the block
+    const int k0 = blk * kTile, lo_t = t ? p_lo[1] : p_lo[0], hi_t = t ? p_hi[1] : p_hi[0];
+    return k0 + kTile - 1 <= lo_t && (window == 0 || k0 > hi_t - window || k0 + kTile <= sinks);
+  }
+  __device__ __forceinline__ bool masked(int blk) const { return (needs(0, blk) && !whole(0, blk)) || (needs(1, blk) && !whole(1, blk)); }
+};
+
+__device__ __forceinline__ Plan make_plan(const WindowK& a, int b, int row0) {
+  Plan p;
+  int len = a.kv_lens ? a.kv_lens[b] : a.Tk;
+  len = len < 0 ? 0 : (len > a.Tk ? a.Tk : len);
+  const int base = len - a.Tq;
+  const int r1 = a.heads2 ? row0 : row0 + kTile;
+  const int rows[2] = {row0, r1};
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int last = rows[t] + kTile - 1 < a.Tq - 1 ? rows[t] + kTile - 1 : a.Tq - 1;
+    p.p_lo[t] = base + rows[t];
+    p.p_hi[t] = rows[t] < a.Tq ? base + last : -1;
+  }
+  p.window = a.window;
+  p.hi = p.p_hi[0] > p.p_hi[1] ? p.p_hi[0] : p.p_hi[1];
+  const int first = p.p_lo[0] > 0 ? p.p_lo[0] : 0;
+  p.lo = a.window > 0 && first - a.window + 1 > 0 ? first - a.window + 1 : 0;
+  p.sinks = a.sinks < p.hi + 1 ? a.sinks : p.hi + 1;
+  if (p.sinks < 0) p.sinks = 0;
+  const int nb = p.hi >= 0 ? p.hi / kTile + 1 : 0;
+  p.front = (p.sinks + kTile - 1) / kTile;
+  p.skip = p.lo / kTile - p.front;
+  if (p.skip < 0) p.skip = 0;
+  p.blocks = nb - p.skip;
+  return p;
+}
+
+// V as the B operand with its columns contiguous (rows of 128 bytes, swizzled): atoms of 8 tokens 1024 bytes apart, blocks of 64
+// columns a tile of 128 tokens apart.
+__device__ __forceinline__ uint64_t make_desc_mn(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+  d |= (uint64_t)((kTile * 128) >> 4) << 16;     // from 64 columns to the next 64
+  d |= (uint64_t)(1024 >> 4) << 32;              // from 8 tokens to the next 8
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+constexpr int kNotes = 48;    // groups of 32 keys of masked blocks: at most 3 blocks at the diagonal, 3 at the window's start, 2 where the sinks end
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                                                                  const __grid_constant__ CUtensorMap mv, const __grid_constant__ WindowK a) {
+  using SH = Shape<D>;
+  constexpr int ST = SH::STAGES;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t q_full, kv_full[ST], kv_empty[ST], v_ok[ST], s_full[2], p_ready[2], o_done[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int s_fail, noted;
+  __shared__ int note_key[kNotes];
+  __shared__ uint32_t note_bits[kNotes];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  // ---- which tiles: the longest rows of the prompt first ----
+  const int per_q = (a.heads2 ? a.Hq / 2 : a.Hq) * a.B;
+  const int qb = a.qblocks - 1 - (int)blockIdx.x / per_q;
+  int rem = (int)blockIdx.x % per_q;
+  const int b = rem / (per_q / a.B), hu = rem % (per_q / a.B);
+  const int head0 = a.heads2 ? 2 * hu : hu, head1 = a.heads2 ? head0 + 1 : head0, hk = head0 / a.gqa;
+  const int row0 = qb * (a.heads2 ? kTile : 2 * kTile), row1 = a.heads2 ? row0 : row0 + kTile;
+  const Plan plan = make_plan(a, b, row0);
+
+  if (tid >= 32 && tid < 32 + kNotes) note_bits[tid - 32] = 0u;
+  if (tid == 0) {
+    s_fail = 0; noted = 0;
+    mbar_init(&q_full, 1);
+    for (int i = 0; i < ST; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); mbar_init(&v_ok[i], 2); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&o_done[i], 1); }
+    asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t ring = smem_u32(smem) + 2 * SH::BYTES;
+  auto failed = [&](int code) { s_fail = code; atomicCAS(&g_window_error, 0, code); };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 8) {
+      // ---- copies ----
+      if (elect_one() && plan.blocks > 0) {
+        mbar_expect_tx(&q_full, 2 * SH::BYTES);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int h = 0; h < SH::HALVES; ++h)
+            tma_load_4d(smem_u32(smem) + t * SH::BYTES + h * kTile * 128, &mq, &q_full, 64 * h, t ? row1 : row0, (t ? head1 : head0) * a.mul[0][0], b * a.mul[0][1]);
+        bool ok = true;
+        for (int it = 0; it < 2 * plan.blocks; ++it) {
+          const int st = it % ST, round = it / ST;
+          if (round > 0 && !wait_cta(&kv_empty[st], (uint32_t)(round - 1) & 1, kPolls)) { failed(501); ok = false; break; }
+          const int blk = plan.block(it >> 1), kv = 1 + (it & 1);
+          mbar_expect_tx(&kv_full[st], SH::BYTES);
+#pragma unroll
+          for (int h = 0; h < SH::HALVES; ++h)
+            tma_load_4d(ring + st * SH::BYTES + h * kTile * 128, kv == 1 ? &mk : &mv, &kv_full[st], 64 * h, blk * kTile, hk * a.mul[kv][0], b * a.mul[kv][1]);
+        }
+        if (!ok)
+          for (int i = 0; i < 1000; ++i) __nanosleep(1000);    // (copies may still be on their way)
+      }
+    } else if (warp == 9) {
+      // ---- products ----
+      constexpr uint32_t idesc0 = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);   // f32 += bf16 x bf16, M = 128
+      constexpr uint32_t idesc_s = idesc0 | ((uint32_t)(kTile >> 3) << 17), idesc_o = idesc0 | ((uint32_t)(D >> 3) << 17) | (1u << 16);
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int phase) { if (ok) ok = __all_sync(0xffffffffu, wait_cta(bar, (uint32_t)phase & 1, kPolls)); };
+      int done[2] = {0, 0};
+      auto scores = [&](int t, int it) {        // S of tile t with the keys in ring slot it
+        if (ok && elect_one()) {
+          const uint64_t ad = make_desc(smem_u32(smem) + t * SH::BYTES), bd = make_desc(ring + (it % ST) * SH::BYTES);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t o = (k >> 2) * ((kTile * 128) >> 4) + (k & 3) * 2;
+            umma_ss(tmem + t * 128, ad + o, bd + o, idesc_s, k > 0);
+          }
+          commit(&s_full[t]);
+        }
+        __syncwarp();
+      };
+      if (plan.blocks > 0) {
+        wait(&q_full, 0);
+        wait(&kv_full[0], 0);
+        for (int t = 0; t < 2; ++t)
+          if (plan.needs(t, plan.block(0))) scores(t, 0);
+        if (ok && elect_one()) commit(&kv_empty[0]);
+        __syncwarp();
+        for (int n = 0; n < plan.blocks; ++n) {
+          const int iv = 2 * n + 1, ik = 2 * n + 2;
+          const bool more = n + 1 < plan.blocks;
+          const int blk = plan.block(n), next = more ? plan.block(n + 1) : 0;
+          wait(&kv_full[iv % ST], iv / ST);
+          wait(&v_ok[iv % ST], (ST & 1) ? (iv / ST) >> 1 : iv / ST);   // (a slot of an odd ring holds values every other round)
+          if (more) wait(&kv_full[ik % ST], ik / ST);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (plan.needs(t, blk)) {
+              wait(&p_ready[t], done[t]);
+              fence_after();
+              if (ok && elect_one()) {
+                const uint64_t bd = make_desc_mn(ring + (iv % ST) * SH::BYTES);
+#pragma unroll
+                for (int k = 0; k < kTile / 16; ++k)
+                  umma_ts(tmem + 256 + t * D, tmem + t * 128 + k * 8, bd + k * (2048 >> 4), idesc_o, done[t] > 0 || k > 0);
+                commit(&o_done[t]);
+              }
+              __syncwarp();
+              ++done[t];
+            }
+            if (more && plan.needs(t, next)) scores(t, ik);
+          }
+          if (ok && elect_one()) {
+            commit(&kv_empty[iv % ST]);
+            if (more) commit(&kv_empty[ik % ST]);
+          }
+          __syncwarp();
+        }
+        // every product is complete before tensor memory and the ring go
+        for (int t = 0; t < 2; ++t)
+          if (done[t] > 0) wait(&o_done[t], done[t] - 1);
+      }
+      if (!ok) {
+        if (lane == 0 && !s_fail) failed(502);
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);    // (products may still be on their way)
+      }
+    } else {
+      // ---- values of masked blocks ----
+      bool ok = true;
+      const int me = tid - 320;
+      for (int n = 0; n < plan.blocks && ok; ++n) {
+        const int iv = 2 * n + 1, blk = plan.block(n);
+        ok = __all_sync(0xffffffffu, wait_cta(&kv_full[iv % ST], (uint32_t)(iv / ST) & 1, kPolls));
+        if (ok && plan.masked(blk)) {
+          unsigned char* v = smem + (2 + iv % ST) * SH::BYTES;
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            const int r = half * 64 + me, key = blk * kTile + r;
+            const bool seen = key <= plan.hi && (key >= plan.lo || key < plan.sinks);
+            bool bad = false;
+            if (seen) {
+              uint32_t acc = 0;
+#pragma unroll
+              for (int c = 0; c < D / 8; ++c) {
+                const uint4 x = *(const uint4*)(v + (c >> 3) * kTile * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                acc |= ((x.x & 0x7F807F80u) + 0x00800080u) | ((x.y & 0x7F807F80u) + 0x00800080u) | ((x.z & 0x7F807F80u) + 0x00800080u) | ((x.w & 0x7F807F80u) + 0x00800080u);
+              }
+              bad = (acc & 0x80008000u) != 0;      // an exponent of all ones
+            }
+            if (!seen || bad)
+#pragma unroll
+              for (int c = 0; c < D / 8; ++c) *(uint4*)(v + (c >> 3) * kTile * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t m = __ballot_sync(0xffffffffu, bad);
+            if (m && lane == 0) {
+              const int at = atomicAdd(&noted, 1);
+              if (at < kNotes) {
+                note_key[at] = blk * kTile + half * 64 + (warp - 10) * 32;
+                __threadfence_block();           // (the bits, zero until now, make the note count)
+                *(volatile uint32_t*)&note_bits[at] = m;
+              }
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(&v_ok[iv % ST]);
+      }
+      if (!ok && lane == 0 && !s_fail) failed(503);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    // ---- softmax: a thread a row ----
+    const int t = warp >> 2, in_tile = tid & 127, row = (t ? row1 : row0) + in_tile, pos = (t ? plan.p_lo[1] : plan.p_lo[0]) + in_tile;
+    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21), s_at = lanes + (uint32_t)t * 128, o_at = lanes + 256 + (uint32_t)t * D;
+    float ref = -INFINITY, l = 0.f;
+    int done = 0;
+    bool ok = true;
+    for (int n = 0; n < plan.blocks; ++n) {
+      const int blk = plan.block(n);
+      if (!plan.needs(t, blk)) continue;
+      ok = __all_sync(0xffffffffu, wait_cta(&s_full[t], (uint32_t)done & 1, kPolls));
+      if (!ok) break;
+      fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) tmem_ld32(s_at + 32 * q, s[q]);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      const bool whole = plan.whole(t, blk);
+      if (!whole) {
+        // key k0 + i is seen where i <= hi and (i > lo or i < sk)
+        const int k0 = blk * kTile, hi = pos - k0, lo = plan.window > 0 ? pos - plan.window - k0 : -1, sk = plan.sinks - k0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          auto below = [&](int x) { const int y = x - 32 * q; return y <= 0 ? 0u : (y >= 32 ? 0xffffffffu : (1u << y) - 1u); };   // keys < x
+          const uint32_t m = below(hi + 1) & (~below(lo + 1) | below(sk));
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!((m >> i) & 1u)) s[q][i] = 0xff800000u;
+        }
+      }
+      float mx = __uint_as_float(s[0][0]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(s[q][i]));
+      mx *= a.c;
+      const bool grow = mx > ref + kSlack;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float f = grow ? ex2f(ref - mx) : 1.f;      // (0 for a row that saw nothing before)
+        if (grow) ref = mx;
+        l *= f;
+        if (done > 0) {
+          ok = __all_sync(0xffffffffu, wait_cta(&o_done[t], (uint32_t)(done - 1) & 1, kPolls));
+          if (!ok) break;
+          fence_after();
+#pragma unroll 1
+          for (int q = 0; q < D / 32; ++q) {
+            uint32_t o[32];
+            tmem_ld32(o_at + 32 * q, o);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st32(o_at + 32 * q, o);
+          }
+        }
+      }
+      const float r = ref == -INFINITY ? 0.f : ref;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t p[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float x0 = ex2f(fmaf(__uint_as_float(s[2 * h + (i >> 4)][2 * (i & 15)]), a.c, -r));
+          const float x1 = ex2f(fmaf(__uint_as_float(s[2 * h + (i >> 4)][2 * (i & 15) + 1]), a.c, -r));
+          sum[2 * (i & 1)] += x0;
+          sum[2 * (i & 1) + 1] += x1;
+          p[i] = pack2(x0, x1);
+        }
+        tmem_st32(s_at + 32 * h, p);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_ready[t]);
+      ++done;
+    }
+    if (ok && done > 0) ok = __all_sync(0xffffffffu, wait_cta(&o_done[t], (uint32_t)(done - 1) & 1, kPolls));
+    fence_after();
+    if (!ok && lane == 0 && !s_fail) failed(504);
+    float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+    const int notes = *(volatile int*)&noted;
+    for (int i = 0; i < notes && i < kNotes; ++i)
+      for (uint32_t m = *(volatile uint32_t*)&note_bits[i]; m; m &= m - 1) {
+        const int key = *(volatile int*)&note_key[i] + __ffs(m) - 1;
+        if (key <= pos && (plan.window == 0 || key > pos - plan.window || key < plan.sinks)) inv = __uint_as_float(0x7fc00000u);
+      }
+    const bool live = row < a.Tq;
+    uint16_t* out = a.out + (int64_t)b * a.o_str[0] + (int64_t)(t ? head1 : head0) * a.o_str[1] + (int64_t)row * a.o_str[2];
+#pragma unroll 1
+    for (int q = 0; q < D / 32; ++q) {
+      uint32_t o[32];
+      if (done > 0) {
+        tmem_ld32(o_at + 32 * q, o);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0u;
+      }
+      uint32_t w[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = pack2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+      if (live) {
+        if (a.o_vec) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *(uint4*)(out + 32 * q + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) { out[32 * q + 2 * i] = (uint16_t)w[i]; out[32 * q + 2 * i + 1] = (uint16_t)(w[i] >> 16); }
+        }
+      }
+    }
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+}
+
+// [T, H, B] rows of D values as boxes of 64 x 128; broadcast axes as one entry at coordinate 0.
+bool rows_map(CUtensorMap* m, const void* base, int64_t D, const int64_t (&shape)[3], const int64_t (&str)[3], int* mul) {
+  const EncodeFn enc = get_encode();
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)shape[2], 1, 1}, strides[3] = {(cuuint64_t)str[2] * 2, (cuuint64_t)D * 2, (cuuint64_t)D * 2};
+  if (shape[2] == 1) strides[0] = (cuuint64_t)D * 2;
+  for (int d = 0; d < 2; ++d) {            // head, sequence
+    mul[d] = shape[1 - d] > 1 && str[1 - d] > 0 ? 1 : 0;
+    if (mul[d]) { dims[2 + d] = (cuuint64_t)shape[1 - d]; strides[1 + d] = (cuuint64_t)str[1 - d] * 2; }
+  }
+  const cuuint32_t box[4] = {64, kTile, 1, 1}, es[4] = {1, 1, 1, 1};
+  return enc && enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void*)base, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D> cudaError_t launch_d(const WindowArgs& w, cudaStream_t st) {
+  WindowK a;
+  a.out = (uint16_t*)w.out; a.kv_lens = w.kv_lens;
+  for (int i = 0; i < 3; ++i) a.o_str[i] = w.o_str[i];
+  a.o_vec = w.o_vec;
+  a.B = (int)w.B; a.Hq = (int)w.Hq; a.gqa = (int)(w.Hq / w.Hkv); a.Tq = (int)w.Tq; a.Tk = (int)w.Tk;
+  a.window = w.window; a.sinks = w.sinks;
+  a.c = w.scale * 1.4426950408889634f;
+  a.heads2 = a.gqa % 2 == 0;
+  a.qblocks = (a.Tq + (a.heads2 ? 1 : 2) * kTile - 1) / ((a.heads2 ? 1 : 2) * kTile);
+  CUtensorMap m[3];
+  const int64_t qs[3] = {w.B, w.Hq, w.Tq}, ks[3] = {w.B, w.Hkv, w.Tk};
+  if (!rows_map(&m[0], w.q, D, qs, w.str[0], a.mul[0]) || !rows_map(&m[1], w.k, D, ks, w.str[1], a.mul[1]) || !rows_map(&m[2], w.v, D, ks, w.str[2], a.mul[2]))
+    return cudaErrorInvalidValue;
+  auto kern = window_attn_kernel<D>;
+  static bool done[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  {
+    std::lock_guard<std::mutex> setup_lk(setup_mutex());   // first use on a device, from any thread
+    if (dev < 0 || dev >= 64 || !done[dev]) {
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::SMEM);
+      if (e != cudaSuccess) return e;
+      if (dev >= 0 && dev < 64) done[dev] = true;
+    }
+  }
+  const int64_t ctas = (int64_t)a.qblocks * (a.heads2 ? a.Hq / 2 : a.Hq) * a.B;
+  return launch_kernel(kern, dim3((unsigned)ctas), dim3(kThreads), Shape<D>::SMEM, st, m[0], m[1], m[2], a);
+}
+}  // namespace
+
+cudaError_t launch_window_attn(const WindowArgs& w, cudaStream_t st) { return w.D == 64 ? launch_d<64>(w, st) : launch_d<128>(w, st); }
+
+void window_attn_error_reset() {
+  const int zero = 0;
+  cudaMemcpyToSymbol(g_window_error, &zero, sizeof(int));
+}
+int window_attn_error_code() {
+  int v = 0;
+  cudaMemcpyFromSymbol(&v, g_window_error, sizeof(int));
+  return v;
+}
+
+}  // namespace qb

@@ -157,6 +157,8 @@ def lib():
         L.qb200_kv_pages_decode_attention.argtypes = [TP] * 11 + [C.c_int, C.c_int, C.c_float, C.c_int64, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]
         L.qb200_kv_pages_decode_attention_workspace_size.argtypes = [C.c_int64] * 4
         L.qb200_kv_pages_decode_attention_workspace_size.restype = C.c_size_t
+        L.qb200_window_attention.argtypes = [TP] * 4 + [C.c_float, C.c_int64, C.c_int64, TP, C.c_void_p]
+        L.qb200_window_attention.restype = C.c_int
         for name in ("append", "free", "fork", "reserve", "compact", "copy", "decode_attention"):
             getattr(L, "qb200_kv_pages_" + name).restype = C.c_int
         for name in ("qb200_rms_norm", "qb200_add_rms_norm", "qb200_rope", "qb200_swiglu", "qb200_kv_append_seqs"):
@@ -392,6 +394,12 @@ def kv_pages_decode_attention(q, k_pool, v_pool, table, lens, bits, group_size, 
     """Attention of one new token per sequence over its pages; q [B, Hq, 1, D] bf16, query b of sequence rows[b] (default b).  With a
     window the query sees the last ``window`` tokens and the first ``sinks``."""
     return _native.kv_pages_decode_attention(q, k_pool, v_pool, table, lens, bits, group_size, scale, window, sinks, rows, workspace, out)
+
+
+def window_attention(q, k, v, scale, window=0, sinks=0, kv_lens=None, out=None):
+    """Causal attention of a prompt or of a chunk behind cached tokens: q [B, Hq, Tq, D], k / v [B, Hkv, Tk, D] bf16, query i at position
+    kv_lens[b] - Tq + i (default Tk - Tq + i).  With a window it sees the last ``window`` keys and the first ``sinks``."""
+    return _native.window_attention(q, k, v, scale, window, sinks, kv_lens, out)
 
 
 _Q2TORCH = {v: k for k, v in _TORCH2Q.items()}
