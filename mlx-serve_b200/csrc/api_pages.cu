@@ -375,6 +375,7 @@ QB200_API int qb200_kv_pages_decode_attention(qb200_tensor* res, const qb200_ten
     if ((st = expect_list(rows, who, "rows", B))) return st;
     a.rows = (const int32_t*)rows->data;
   } else if (ps.S != B) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: %lld queries for a table of %d sequences (pass rows)", who, (long long)B, ps.S);
+  if (!(scale >= -3.0e38f && scale <= 3.0e38f)) return pg_fail(QB200_ERR_BAD_ARG, "%s: scale must be finite", who);
   if (window < 0 || sinks < 0) return pg_fail(QB200_ERR_BAD_ARG, "%s: window and sinks must not be negative", who);
   if (!rows_distinct(res)) return pg_fail(QB200_ERR_BAD_STRIDE, "%s: rows of res overlap", who);
   if (B == 0 || Hq == 0) return QB200_OK;

@@ -20,6 +20,7 @@
 //    kept low enough by the block's largest value scale; at 16 bits they stay a sum of two bf16 (16 bits).  The score tile's
 //    layout becomes the B operand of the next product by movmatrix.
 #include <mutex>
+#include <type_traits>
 
 #include "kernels.h"
 #include "stream_ptx.cuh"
@@ -57,10 +58,34 @@ template <int BITS, int CH> __device__ __forceinline__ int swz(int row) {
   if (CH >= 8) f |= (row & 1) << 2;
   return f;
 }
+// Where a stage's token lies in shared memory: at 4 and 8 bits the four tokens 4g .. 4g + 3 of its 32 are rows g, g + 8, g + 16, g + 24, so
+// that the tokens whose scores a lane holds have their scales side by side.
+template <int BITS> __device__ __forceinline__ int place(int tok) { return BITS == 16 ? tok : (tok & 3) * 8 + (tok >> 2); }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
+}
+// D = A B (+ D unless the sum begins): no registers to clear first
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, bool first) {
+  if (first)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  else mma_f16_16816(d, a0, a1, a2, a3, b0, b1);
+}
+__device__ __forceinline__ void mma_bf16_1688_z(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(b), "f"(0.f));
+}
+// bf16 parameters of four consecutive tokens, G a token, each token's in one register (at G = 1 in its low half)
+template <int G> __device__ __forceinline__ void load4(uint32_t (&r)[4], const unsigned char* p) {
+  if constexpr (G == 2) {
+    const uint4 v = *(const uint4*)p;
+    r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
+  } else {
+    const uint2 v = *(const uint2*)p;
+    r[0] = v.x & 0xFFFFu; r[1] = v.x >> 16; r[2] = v.y & 0xFFFFu; r[3] = v.y >> 16;
+  }
 }
 template <bool TRANS> __device__ __forceinline__ void ldmatrix_b16_x4(uint32_t (&r)[4], uint32_t addr) {
   if constexpr (TRANS)
@@ -118,7 +143,7 @@ __device__ __forceinline__ void plan_units(const KvPagesAttnArgs& a, int* units,
 }
 
 template <int BITS, int D>
-__global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kernel(const __grid_constant__ KvPagesAttnArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_constant__ KvPagesAttnArgs a) {
   using GE = Geo<BITS, D>;
   constexpr int G = GE::G, CH = GE::CH, TOK = GE::TOK, ITEMS = GE::ITEMS, STAGES = GE::STAGES;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -162,8 +187,6 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kerne
     const int row = a.rows ? a.rows[b] : b;
     const int32_t* tab = a.table + (int64_t)row * a.table_str;
     const int my_blocks = warp < todo ? (todo - warp + kWarps - 1) / kWarps : 0;
-    const int my_items = my_blocks * ITEMS;
-    const unsigned char* kv_base[2] = {(const unsigned char*)a.pool[0].q + (int64_t)hk * a.q_head[0], (const unsigned char*)a.pool[1].q + (int64_t)hk * a.q_head[1]};
     const int pmask = (1 << a.page_shift) - 1;
     auto first_token = [&](int j) { const int i = blk0 + warp + j * kWarps; return (i < sn.front ? i : i + sn.skip) * kBlk; };
     auto visible = [&](int tok) { return tok < sn.len && (tok >= sn.w0 || tok < sn.sinks); };
@@ -179,37 +202,52 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kerne
       }
       return pid;
     };
-    int pid_next = page_at(0), pid_cur = -1, blk_tok = 0;
-    uint32_t valid = 0;                                   // four bits a block, the newest lowest
     constexpr int RPI = 32 / CH;                          // token rows of one copy instruction
     const int cc = lane % CH, r0 = lane / CH;
-    auto issue = [&](int item, int stage) {
-      const int part = item % ITEMS;
-      if (part == 0) {
-        const int j = item / ITEMS;
+    const unsigned char* const base_k = (const unsigned char*)a.pool[0].q + (int64_t)hk * a.q_head[0] + (int64_t)r0 * a.tok_bytes[0] + cc * 16;
+    const unsigned char* const base_v = (const unsigned char*)a.pool[1].q + (int64_t)hk * a.q_head[1] + (int64_t)r0 * a.tok_bytes[1] + cc * 16;
+    // scales and biases of a block, [ks, kb, vs, vb][64 tokens][G]: 16-byte pieces, G of them a lane (ks or kb, then vs or vb; at G = 1 one of the four)
+    constexpr int TP = 8 / G;                             // tokens per piece
+    const int sb_tok = lane % (kBlk / TP) * TP;
+    const uint16_t* sb_at[G];
+    if constexpr (BITS != 16) {
+#pragma unroll
+      for (int k = 0; k < G; ++k) {
+        const int arr = (lane + 32 * k) / (kBlk / TP), kv = arr >> 1;
+        const uint16_t* const p = (const uint16_t*)(arr == 0 ? a.pool[0].s : (arr == 1 ? a.pool[0].b : (arr == 2 ? a.pool[1].s : a.pool[1].b)));
+        sb_at[k] = p + (int64_t)hk * (kv ? a.pool[1].sb_str[1] : a.pool[0].sb_str[1]);
+      }
+    }
+    // what the block whose copies are being issued is: its first token, its pages, which 16 tokens have one, whether the query sees it all
+    int pid_next = page_at(0), pid_cur = -1, blk_tok = 0;
+    uint32_t vm_next = 0;
+    bool whole_next = false;
+    auto issue = [&](auto part_c, int j) {                // the copies of stage `part` of block j
+      constexpr int part = decltype(part_c)::value, stage = part % STAGES;
+      if constexpr (part == 0) {
         pid_cur = pid_next;
         blk_tok = first_token(j);
-        valid = (valid << 4) | (__ballot_sync(0xffffffffu, pid_cur >= 0) & 15u);
+        vm_next = __ballot_sync(0xffffffffu, pid_cur >= 0) & 15u;
+        whole_next = vm_next == 15u && blk_tok + kBlk <= sn.len && (blk_tok >= sn.w0 || blk_tok + kBlk <= sn.sinks);
         pid_next = page_at(j + 1);
         if constexpr (BITS != 16) {
           const uint32_t dst0 = my_sb + (j & 1) * 4 * GE::SB;
-          const uint16_t* const sbase[4] = {(const uint16_t*)a.pool[0].s, (const uint16_t*)a.pool[0].b, (const uint16_t*)a.pool[1].s, (const uint16_t*)a.pool[1].b};
           if (a.sb_vec) {
-            constexpr int PC = GE::SB / 16, TP = 8 / G;   // 16-byte pieces per array, tokens per piece
+            const int pid = __shfl_sync(0xffffffffu, pid_cur, sb_tok >> 4);
+            const bool ok = pid >= 0 && blk_tok + sb_tok < sn.len;
+            const int slot = ((blk_tok + sb_tok) & pmask) * G;
 #pragma unroll
-            for (int i = lane; i < 4 * PC; i += 32) {
-              const int arr = i / PC, pc = i - arr * PC, tk = pc * TP, kv = arr >> 1;
-              const int pid = __shfl_sync(0xffffffffu, pid_cur, tk >> 4);
-              const uint16_t* base = arr == 0 ? sbase[0] : (arr == 1 ? sbase[1] : (arr == 2 ? sbase[2] : sbase[3]));
-              const uint16_t* src = base + (int64_t)(pid < 0 ? 0 : pid) * (kv ? a.pool[1].sb_str[0] : a.pool[0].sb_str[0]) +
-                                    (int64_t)hk * (kv ? a.pool[1].sb_str[1] : a.pool[0].sb_str[1]) + ((blk_tok + tk) & pmask) * G;
-              cp_async16_z(dst0 + arr * GE::SB + pc * 16, src, pid >= 0 && blk_tok + tk < sn.len ? 16u : 0u);
+            for (int k = 0; k < G; ++k) {
+              const bool v = G == 2 ? k == 1 : lane >= 16;
+              const uint16_t* src = sb_at[k] + (int64_t)(ok ? pid : 0) * (v ? a.pool[1].sb_str[0] : a.pool[0].sb_str[0]) + slot;
+              cp_async16_z(dst0 + (lane + 32 * k) * 16, src, ok ? 16u : 0u);
             }
           } else {
             uint16_t* dst = (uint16_t*)(my_sb_p + (j & 1) * 4 * GE::SB);
 #pragma unroll
             for (int arr = 0; arr < 4; ++arr) {
               const KvPoolView& pl = a.pool[arr >> 1];
+              const uint16_t* src = (const uint16_t*)((arr & 1) ? pl.b : pl.s) + (int64_t)hk * pl.sb_str[1];
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const int tk = h * 32 + lane;
@@ -217,32 +255,40 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kerne
 #pragma unroll
                 for (int c = 0; c < G; ++c)
                   dst[arr * (GE::SB / 2) + tk * G + c] = pid >= 0 && blk_tok + tk < sn.len
-                      ? sbase[arr][(int64_t)pid * pl.sb_str[0] + (int64_t)hk * pl.sb_str[1] + (int64_t)((blk_tok + tk) & pmask) * pl.sb_str[2] + c] : (uint16_t)0;
+                      ? src[(int64_t)pid * pl.sb_str[0] + (int64_t)((blk_tok + tk) & pmask) * pl.sb_str[2] + c] : (uint16_t)0;
               }
             }
           }
         }
       }
-      const int kv = part >= ITEMS / 2 ? 1 : 0, tk0 = (part - kv * (ITEMS / 2)) * TOK;
-      const unsigned char* base = kv ? kv_base[1] : kv_base[0];
-      const uint32_t page_b = kv ? a.page_bytes[1] : a.page_bytes[0], tok_b = kv ? a.tok_bytes[1] : a.tok_bytes[0];
-      const uint32_t st = my_ring + stage * GE::STAGE;
+      constexpr bool V = part >= ITEMS / 2;
+      constexpr int tk0 = (part % (ITEMS / 2)) * TOK;
+      const uint32_t page_b = a.page_bytes[V], tok_b = a.tok_bytes[V], st = my_ring + stage * GE::STAGE;
+      auto copy = [&](auto all_c) {
 #pragma unroll
-      for (int r = 0; r < TOK / RPI; ++r) {
-        const int rw = r0 + r * RPI, tok = blk_tok + tk0 + rw;
-        const int pid = __shfl_sync(0xffffffffu, pid_cur, (tk0 + r * RPI) >> 4);
-        const bool ok = pid >= 0 && visible(tok);
-        const unsigned char* src = base + (uint64_t)(uint32_t)(ok ? pid : 0) * page_b + (uint64_t)(uint32_t)(tok & pmask) * tok_b + cc * 16;
-        cp_async16_z(st + rw * GE::ROWB + ((cc ^ swz<BITS, CH>(rw)) << 4), src, ok ? 16u : 0u);
-      }
+        for (int s16 = 0; s16 < TOK / 16; ++s16) {        // 16 tokens lie in one page
+          const int pid = __shfl_sync(0xffffffffu, pid_cur, tk0 / 16 + s16);
+          const int tok = blk_tok + tk0 + s16 * 16;
+          const unsigned char* src = (V ? base_v : base_k) + (uint64_t)(uint32_t)(pid < 0 ? 0 : pid) * page_b + (uint64_t)(uint32_t)(tok & pmask) * tok_b;
+#pragma unroll
+          for (int r = 0; r < 16 / RPI; ++r) {
+            const int in = s16 * 16 + r * RPI + r0, rw = place<BITS>(in);
+            const uint32_t dst = st + rw * GE::ROWB + ((cc ^ swz<BITS, CH>(rw)) << 4);
+            if (decltype(all_c)::value) cp_async16(dst, src);
+            else cp_async16_z(dst, src, pid >= 0 && visible(tok + r * RPI + r0) ? 16u : 0u);
+            src += (uint64_t)tok_b * RPI;
+          }
+        }
+      };
+      if (whole_next) copy(std::true_type{}); else copy(std::false_type{});
     };
-    int issued = 0;
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-      if (issued < my_items) issue(issued, issued % STAGES);
-      cp_async_commit();
-      ++issued;
-    }
+#define QB_PART(n) std::integral_constant<int, (n)>{}
+    if (my_blocks > 0) issue(QB_PART(0), 0);
+    cp_async_commit();
+    if (my_blocks > 0) issue(QB_PART(1), 0);
+    cp_async_commit();
+    if (my_blocks > 0) issue(QB_PART(2), 0);
+    cp_async_commit();
 
     // ---- queries: row g of the tile as the B operand ----
     uint32_t qf[D / 16][2];
@@ -252,15 +298,17 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kerne
       const int r = qt * kRows + g;
       const bool live = r < a.gqa && my_blocks > 0;
       const uint16_t* qp = (const uint16_t*)a.q + (int64_t)b * a.q_str[0] + (int64_t)(hk * a.gqa + (live ? r : 0)) * a.q_str[1];
+      // (the sign of the scale goes to the queries, so that the largest score is the largest sum; a factor of 0 would meet scores of -inf)
+      const float factor = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
       if constexpr (BITS == 16) {
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint16_t* p = qp + 16 * s + 2 * t + 8 * h;
-            qf[s][h] = live ? (uint32_t)p[0] | ((uint32_t)p[1] << 16) : 0u;
+            qf[s][h] = live ? ((uint32_t)p[0] | ((uint32_t)p[1] << 16)) ^ (a.scale < 0.f ? 0x80008000u : 0u) : 0u;
           }
-        C0 = C1 = a.scale * kLog2e;
+        C0 = C1 = factor;
       } else {
         float f[G][16], sum[G], mx = 0.f;
 #pragma unroll
@@ -290,8 +338,8 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kerne
         mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         int e = (int)((__float_as_uint(mx) >> 23) & 0xFF) - 127;    // mx < 2^(e + 1)
         e = e < -100 ? -100 : (e > 110 ? 110 : e);
-        const float up = pow2i(14 - e);
-        const float qc = poison_if(nonfinite(mx), pow2i(24 - 14 + e) * (a.scale * kLog2e));
+        const float up = a.scale < 0.f ? -pow2i(14 - e) : pow2i(14 - e);
+        const float least = 1e-37f, qf2 = pow2i(24 - 14 + e) * factor, qc = poison_if(nonfinite(mx), qf2 < least ? least : qf2);
         C0 = __shfl_sync(0xffffffffu, qc, 8 * t);
         C1 = __shfl_sync(0xffffffffu, qc, 8 * t + 4);
         // s = qc * (scale * sum q~ c 2^-24 + bias * sum q~ 2^-24): the sum in three bf16 parts, one a lane
@@ -321,16 +369,15 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kerne
       }
     }
 
-    int consumed = 0;
-    auto acquire = [&]() -> const unsigned char* {
-      if (issued < my_items) issue(issued, issued % STAGES);
+    // the next stage of block j: what it takes to stay three stages ahead is issued, and its own copies are complete
+    auto acquire = [&](auto it_c, int j) -> const unsigned char* {
+      constexpr int it = decltype(it_c)::value, ahead = it + STAGES - 1;
+      if constexpr (ahead < ITEMS) issue(QB_PART(ahead), j);
+      else if (j + 1 < my_blocks) issue(QB_PART(ahead - ITEMS), j + 1);
       cp_async_commit();
-      ++issued;
       cp_async_wait<STAGES - 1>();
       __syncwarp();
-      const unsigned char* st = my_ring_p + (consumed % STAGES) * GE::STAGE;
-      ++consumed;
-      return st;
+      return my_ring_p + (it % STAGES) * GE::STAGE;
     };
 
     float r_run[2] = {kNegBig, kNegBig}, l_part[2] = {0.f, 0.f};
@@ -345,16 +392,13 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kerne
       const int tok_blk = first_token(j);
       unsigned char* sbb = my_sb_p + (j & 1) * 4 * GE::SB;
       float sc[4][4];     // [16 tokens][token g | g + 8][query 2t | 2t + 1]
-      bool whole = false;
-      uint32_t vm = 0;
+      const bool whole = whole_next;
+      const uint32_t vm = vm_next;
       // ---------------- scores ----------------
-#pragma unroll
-      for (int it = 0; it < ITEMS / 2; ++it) {
-        const unsigned char* st = acquire();
-        if (it == 0) {
-          const int newest = (issued - 1 < my_items ? issued - 1 : my_items - 1) / ITEMS;   // the block whose pages were read last
-          vm = (valid >> (4 * (newest - j))) & 15u;
-          whole = vm == 15u && tok_blk + kBlk <= sn.len && (tok_blk >= sn.w0 || tok_blk + kBlk <= sn.sinks);
+      auto score_stage = [&](auto it_c) {
+        constexpr int it = decltype(it_c)::value;
+        const unsigned char* st = acquire(it_c, j);
+        if constexpr (it == 0) {
           if constexpr (BITS != 16) {
             if (!whole) {             // parameters of rows that were not read: zero, whatever lies there
 #pragma unroll
@@ -367,6 +411,11 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kerne
               __syncwarp();
             }
           }
+        }
+        uint32_t ks[4], kb[4];            // of the lane's four tokens 4g + i: sub s2 has i = 2 s2 (row g of the tile) and 2 s2 + 1 (row g + 8)
+        if constexpr (BITS != 16) {
+          load4<G>(ks, sbb + (it * TOK + 4 * g) * G * 2);
+          load4<G>(kb, sbb + GE::SB + (it * TOK + 4 * g) * G * 2);
         }
 #pragma unroll
         for (int s2 = 0; s2 < TOK / 16; ++s2) {
@@ -381,13 +430,12 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kerne
               ldmatrix_b16_x4<false>(k4, addr + (((2 * s + (lane >> 4)) ^ swz<BITS, CH>(rw)) << 4));
               mma_bf16_16816(d, k4, qf[s][0], qf[s][1]);
             }
-            sc[sub][0] = d[0] * C0; sc[sub][1] = d[1] * C1; sc[sub][2] = d[2] * C0; sc[sub][3] = d[3] * C1;
+            sc[sub][0] = d[0]; sc[sub][1] = d[1]; sc[sub][2] = d[2]; sc[sub][3] = d[3];
           } else {
             float d[G][4];
             const int ra = s2 * 16 + g, rb = ra + 8;
 #pragma unroll
             for (int grp = 0; grp < G; ++grp) {
-              d[grp][0] = d[grp][1] = d[grp][2] = d[grp][3] = 0.f;
               uint32_t wa[4], wb[4];
               if constexpr (BITS == 4) {
                 const int c = 2 * grp + (t >> 1), o = (t & 1) * 8;
@@ -410,37 +458,32 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kerne
                 } else {
                   a0 = wa[s] & 0x00FF00FFu; a1 = wb[s] & 0x00FF00FFu; a2 = (wa[s] >> 8) & 0x00FF00FFu; a3 = (wb[s] >> 8) & 0x00FF00FFu;
                 }
-                mma_f16_16816(d[grp], a0, a1, a2, a3, qf[grp * 4 + s][0], qf[grp * 4 + s][1]);
+                mma_f16_first(d[grp], a0, a1, a2, a3, qf[grp * 4 + s][0], qf[grp * 4 + s][1], s == 0);
               }
             }
-            const int tk = sub * 16 + g;
-            float e[4] = {0.f, 0.f, 0.f, 0.f};
-            float s0[G], s1[G];
-            if constexpr (G == 2) {
-              mma_bf16_1688(e, *(const uint32_t*)(sbb + GE::SB + tk * 4), *(const uint32_t*)(sbb + GE::SB + (tk + 8) * 4), qb);
-              const uint32_t x = *(const uint32_t*)(sbb + tk * 4), y = *(const uint32_t*)(sbb + (tk + 8) * 4);
-              s0[0] = bf16lo(x); s0[1] = bf16hi(x); s1[0] = bf16lo(y); s1[1] = bf16hi(y);
-            } else {
-              mma_bf16_1688(e, (uint32_t) * (const uint16_t*)(sbb + GE::SB + tk * 2), (uint32_t) * (const uint16_t*)(sbb + GE::SB + (tk + 8) * 2), qb);
-              s0[0] = bf16_bits_to_f32(*(const uint16_t*)(sbb + tk * 2)); s1[0] = bf16_bits_to_f32(*(const uint16_t*)(sbb + (tk + 8) * 2));
-            }
+            float e[4], s0[G], s1[G];
+            mma_bf16_1688_z(e, kb[2 * s2], kb[2 * s2 + 1], qb);
+            s0[0] = bf16lo(ks[2 * s2]); s1[0] = bf16lo(ks[2 * s2 + 1]);
+            if constexpr (G == 2) { s0[G - 1] = bf16hi(ks[2 * s2]); s1[G - 1] = bf16hi(ks[2 * s2 + 1]); }
 #pragma unroll
             for (int grp = 0; grp < G; ++grp) {
               e[0] = fmaf(s0[grp], d[grp][0], e[0]); e[1] = fmaf(s0[grp], d[grp][1], e[1]);
               e[2] = fmaf(s1[grp], d[grp][2], e[2]); e[3] = fmaf(s1[grp], d[grp][3], e[3]);
             }
-            sc[sub][0] = e[0] * C0; sc[sub][1] = e[1] * C1; sc[sub][2] = e[2] * C0; sc[sub][3] = e[3] * C1;
+            sc[sub][0] = e[0]; sc[sub][1] = e[1]; sc[sub][2] = e[2]; sc[sub][3] = e[3];
           }
         }
         __syncwarp();
-      }
+      };
+      score_stage(QB_PART(0)); score_stage(QB_PART(1));
+      if constexpr (ITEMS == 8) { score_stage(QB_PART(2)); score_stage(QB_PART(3)); }
       if (!whole) {
 #pragma unroll
         for (int sub = 0; sub < 4; ++sub)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int tk = sub * 16 + h * 8 + g;
-            if (!(visible(tok_blk + tk) && ((vm >> sub) & 1u))) sc[sub][2 * h] = sc[sub][2 * h + 1] = kNegBig;
+            const int tk = BITS == 16 ? sub * 16 + h * 8 + g : (sub >> 1) * 32 + 4 * g + 2 * (sub & 1) + h;
+            if (!(visible(tok_blk + tk) && ((vm >> (tk >> 4)) & 1u))) sc[sub][2 * h] = sc[sub][2 * h + 1] = -INFINITY;
           }
       }
       // ---------------- the block's softmax ----------------
@@ -456,7 +499,7 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kerne
         ex = (int)(__reduce_max_sync(0xffffffffu, max(m >> 16, m & 0xFFFFu)) >> 7);
         ex = ex < 60 ? 60 : ex;          // (p <= 2^81: its sum stays finite over any length)
       }
-      float mb[2];
+      float mb[2];     // the least reference that this block allows: p = 2^(s - r), r >= max s + ex - 141 keeps p * v_scale below 2^15
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float m = fmaxf(sc[0][c], sc[0][2 + c]);
@@ -465,29 +508,36 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kerne
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        mb[c] = fmaxf(r_run[c], m + (float)(ex - 141));   // p = 2^(s - r), r >= max s + ex - 141: p * v_scale stays below 2^15
+        mb[c] = fmaf(m, c ? C1 : C0, (float)(ex - 141));
       }
+      // a reference that has to move moves 6 further, so that few blocks have to rescale (from 12 of 21 blocks of a warp to 2)
       if (__any_sync(0xffffffffu, mb[0] > r_run[0] || mb[1] > r_run[1])) {
-        const float al0 = ex2(r_run[0] - mb[0]), al1 = ex2(r_run[1] - mb[1]);
+        const float n0 = mb[0] > r_run[0] ? mb[0] + 6.f : r_run[0], n1 = mb[1] > r_run[1] ? mb[1] + 6.f : r_run[1];
+        const float al0 = ex2(r_run[0] - n0), al1 = ex2(r_run[1] - n1);
 #pragma unroll
         for (int i = 0; i < GE::NT; ++i) { O[i][0] *= al0; O[i][1] *= al1; O[i][2] *= al0; O[i][3] *= al1; }
 #pragma unroll
         for (int i = 0; i < G; ++i) { ob[i][0] *= al0; ob[i][1] *= al1; }
         l_part[0] *= al0; l_part[1] *= al1;
-        r_run[0] = mb[0]; r_run[1] = mb[1];
+        r_run[0] = n0; r_run[1] = n1;
       }
 #pragma unroll
       for (int sub = 0; sub < 4; ++sub)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float p = sc[sub][i] <= kNegBig ? 0.f : ex2(sc[sub][i] - r_run[i & 1]);
+          const float p = ex2(fmaf(sc[sub][i], (i & 1) ? C1 : C0, -r_run[i & 1]));   // (0 where the score is -inf: r is finite)
           l_part[i & 1] += p;
           sc[sub][i] = p;
         }
       // ---------------- values ----------------
-#pragma unroll
-      for (int it = 0; it < ITEMS / 2; ++it) {
-        const uint32_t stv = (uint32_t)__cvta_generic_to_shared(acquire());
+      auto value_stage = [&](auto it_c) {
+        constexpr int it = decltype(it_c)::value - ITEMS / 2;
+        const uint32_t stv = (uint32_t)__cvta_generic_to_shared(acquire(it_c, j));
+        uint32_t vs4[4], vb4[4];
+        if constexpr (BITS != 16) {
+          load4<G>(vs4, sbb + 2 * GE::SB + (it * TOK + 4 * g) * G * 2);
+          load4<G>(vb4, sbb + 3 * GE::SB + (it * TOK + 4 * g) * G * 2);
+        }
 #pragma unroll
         for (int s2 = 0; s2 < TOK / 16; ++s2) {
           const int sub = it * (TOK / 16) + s2;
@@ -512,15 +562,10 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kerne
             uint32_t pb[G][2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const int tk = sub * 16 + h * 8 + g;
               const float p0 = sc[sub][2 * h], p1 = sc[sub][2 * h + 1];
               float vs[G], vb[G];
-              if constexpr (G == 2) {
-                const uint32_t x = *(const uint32_t*)(sbb + 2 * GE::SB + tk * 4), y = *(const uint32_t*)(sbb + 3 * GE::SB + tk * 4);
-                vs[0] = bf16lo(x); vs[1] = bf16hi(x); vb[0] = bf16lo(y); vb[1] = bf16hi(y);
-              } else {
-                vs[0] = bf16_bits_to_f32(*(const uint16_t*)(sbb + 2 * GE::SB + tk * 2)); vb[0] = bf16_bits_to_f32(*(const uint16_t*)(sbb + 3 * GE::SB + tk * 2));
-              }
+              vs[0] = bf16lo(vs4[2 * s2 + h]); vb[0] = bf16lo(vb4[2 * s2 + h]);
+              if constexpr (G == 2) { vs[G - 1] = bf16hi(vs4[2 * s2 + h]); vb[G - 1] = bf16hi(vb4[2 * s2 + h]); }
 #pragma unroll
               for (int grp = 0; grp < G; ++grp) {
                 pb[grp][h] = transpose8x8(pack_f16x2(p0 * vs[grp], p1 * vs[grp]));
@@ -528,7 +573,7 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kerne
                 ob[grp][1] = fmaf(p1, vb[grp], ob[grp][1]);
               }
             }
-            // matrix row 4u + i of ldmatrix = token {2u, 8 + 2u, 2u + 1, 9 + 2u}[i]
+            // matrix row 4u + i of ldmatrix = row {2u, 8 + 2u, 2u + 1, 9 + 2u}[i] of the tile, which is row 16 s2 + that of the stage
             const int mr = lane & 15, half_m = lane >> 4;
             const int tokrow = s2 * 16 + 2 * (mr >> 2) + ((mr >> 1) & 1) + 8 * (mr & 1);
 #pragma unroll
@@ -551,9 +596,13 @@ __global__ void __launch_bounds__(kWarps * 32, BITS == 4 ? 4 : 3) kv_pages_kerne
           }
         }
         __syncwarp();
-      }
+      };
+      if constexpr (ITEMS == 8) { value_stage(QB_PART(4)); value_stage(QB_PART(5)); value_stage(QB_PART(6)); value_stage(QB_PART(7)); }
+      else { value_stage(QB_PART(2)); value_stage(QB_PART(3)); }
     }
     cp_async_wait<0>();
+
+#undef QB_PART
 
     // ---- join the warps: sums are partial over the 8 lanes that share a query ----
 #pragma unroll

@@ -61,7 +61,7 @@ def check(out, q, kp, vp, table, lens, page, bits, scale, window=0, sinks=0, row
             if not keep:
                 assert (got[b, h, 0] == 0).all()
                 continue
-            S = float((scale * (np.abs(g[0][:, hk]) + np.abs(g[1][:, hk])) @ np.abs(qs[b, h, 0])).max())
+            S = float((abs(scale) * (np.abs(g[0][:, hk]) + np.abs(g[1][:, hk])) @ np.abs(qs[b, h, 0])).max())
             tol = 2.0 ** -8 * np.abs(o) + half * (p @ a) + (10 * 2.0 ** -24 * S + 2.0 ** -21) * (p @ (a + np.abs(g[3][:, hk]))) + 1e-30
             err = np.abs(got[b, h, 0] - o)
             assert (err <= tol * 1.01).all(), f"b {b} h {h}: worst {float((err / tol).max()):.2f} of the tolerance"
@@ -181,6 +181,18 @@ def test_magnitudes(bits, kstd, vstd, qstd):
     q = (torch.randn(2, 8, 1, D, device="cuda") * qstd).to(BF16)
     out = qb200.kv_pages_decode_attention(q, kp, vp, ints(table), ints(lens), bits, 64, D ** -0.5)
     check(out, q, kp, vp, table, lens, page, bits, D ** -0.5)
+
+
+@pytest.mark.parametrize("bits", [4, 8, 16])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30])
+def test_scales_of_either_sign(bits, scale):
+    torch.manual_seed(11)
+    page, D, H, lens = 32, 64, 2, [300, 90]
+    kp, vp = make_pool(40, H, page, D, bits), make_pool(40, H, page, D, bits)
+    table = make_table(lens, page, 16, 40)
+    q = torch.randn(2, 8, 1, D, device="cuda").to(BF16)
+    out = qb200.kv_pages_decode_attention(q, kp, vp, ints(table), ints(lens), bits, 64, scale, window=100, sinks=5)
+    check(out, q, kp, vp, table, lens, page, bits, scale, 100, 5)
 
 
 def test_constant_values_without_scale():

@@ -122,9 +122,9 @@ def test_copy_of_nothing_is_nothing():
     assert copy([t(BF16, [6, 4])]) == 0 and copy([]) == 0 and copy([t(BF16, [6, 0, 4])], t(I32, [2, 2])) == 0
 
 
-def attend(res=None, qq=None, k=None, v=None, table=None, rows=NONE, lens=None, bits=4, gs=64, window=0, sinks=0, ws=0x100000, n=1 << 30):
+def attend(res=None, qq=None, k=None, v=None, table=None, rows=NONE, lens=None, bits=4, gs=64, window=0, sinks=0, ws=0x100000, n=1 << 30, scale=0.1):
     qq = qq or t(BF16, [3, 4, 1, 128])
-    return q.lib().qb200_kv_pages_decode_attention(*ref(res or qq, qq, *(k or pool()), *(v or pool()), table or t(I32, [3, 4]), rows, lens or t(I32, [3])), bits, gs, 0.1,
+    return q.lib().qb200_kv_pages_decode_attention(*ref(res or qq, qq, *(k or pool()), *(v or pool()), table or t(I32, [3, 4]), rows, lens or t(I32, [3])), bits, gs, scale,
                                                    window, sinks, ws, n, None)
 
 
@@ -132,7 +132,7 @@ def attend(res=None, qq=None, k=None, v=None, table=None, rows=NONE, lens=None, 
     (1, dict(qq=t(q.FLOAT32, [3, 4, 1, 128]))), (2, dict(qq=t(BF16, [3, 4, 128]))), (1, dict(qq=t(BF16, [3, 4, 2, 128]))), (2, dict(res=t(BF16, [3, 4, 1, 64]))),
     (4, dict(res=t(q.FLOAT32, [3, 4, 1, 128]))), (1, dict(bits=2)), (1, dict(gs=128)), (2, dict(qq=t(BF16, [3, 5, 1, 128]))), (2, dict(k=pool(D=64))),
     (1, dict(qq=t(BF16, [3, 4, 1, 192]), k=pool(D=192), v=pool(D=192))), (2, dict(lens=t(I32, [2]))), (2, dict(table=t(I32, [4, 4]), lens=t(I32, [4]))),
-    (2, dict(rows=t(I32, [2]))), (5, dict(window=-1)), (5, dict(sinks=-1)), (7, dict(ws=None)), (7, dict(n=1024)), (7, dict(ws=0x100008)),
+    (2, dict(rows=t(I32, [2]))), (5, dict(scale=float("nan"))), (5, dict(scale=float("-inf"))), (5, dict(window=-1)), (5, dict(sinks=-1)), (7, dict(ws=None)), (7, dict(n=1024)), (7, dict(ws=0x100008)),
     (2, dict(k=pool(P=0), v=pool(P=0))), (1, dict(qq=t(BF16, [1025, 4, 1, 128]), table=t(I32, [1025, 4]), lens=t(I32, [1025]))),
     (3, dict(res=t(BF16, [3, 4, 1, 128], stride=[512, 64, 128, 1]))), (1, dict(k=pool(ptr=0x1008))), (4, dict(bits=16)),
 ])
