@@ -17,6 +17,7 @@
 //                    noted; the queries that see such a row give NaN.
 // Blocks of 128 keys that no query of a tile sees are left out; only those cut by a border of the mask are masked element by element.
 #include <mutex>
+#include <type_traits>
 
 #include "tc_ptx.cuh"
 
@@ -27,7 +28,9 @@ __device__ int g_window_error = 0;   // 0 = ok; otherwise the code of the wait t
 
 constexpr int kThreads = 384;
 constexpr int kTile = 128;           // queries of a tile, keys of a block
-constexpr uint32_t kPolls = 1u << 18;
+constexpr uint32_t kPolls = 1u << 18, kSpins = 1u << 23;
+constexpr int kPolyOf8 = 2;          // pairs of 8 whose exponentials the fp32 units work out
+constexpr float kMostSum = 16777216.f;   // of a block's probabilities, with the reference as it was
 constexpr float kSlack = 8.f;        // exponents that the reference may lie below the maximum
 
 template <int D> struct Shape {
@@ -77,6 +80,62 @@ __device__ __forceinline__ float ex2f(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two fp32 in a 64-bit register: one instruction does both.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void untwo(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float clamp126(float x) {
+  asm("max.NaN.f32 %0, %0, %1;\n\tmin.NaN.f32 %0, %0, %2;" : "+f"(x) : "f"(-126.f), "f"(126.f));
+  return x;
+}
+// 2^x for a pair without the special-function unit, which the softmax would otherwise wait for: x = n + f with n the nearest
+// integer (from the low bits of x + 1.5 * 2^23), 2^f on [-1/2, 1/2] by the cubic of least relative error (7.5e-5, a fiftieth of what
+// rounding to bf16 takes; Lawson's iteration), n added to the exponent.  x counts as -126 below that, as 126 above, a NaN gives
+// 3.4e38: what the sum over the row then shows.
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+  const uint64_t magic = two(12582912.f, 12582912.f), unmagic = two(-12582912.f, -12582912.f), minus = two(-1.f, -1.f);
+  float a, b, p, q, u, v;
+  untwo(x, a, b);
+  x = two(clamp126(a), clamp126(b));
+  const uint64_t t = add2(x, magic), f = fma2(add2(t, unmagic), minus, x);
+  uint64_t y = fma2(f, two(0.0551716685f, 0.0551716685f), two(0.2426111251f, 0.2426111251f));
+  y = fma2(y, f, two(0.6932609677f, 0.6932609677f));
+  y = fma2(y, f, two(0.9999280572f, 0.9999280572f));
+  untwo(y, p, q);
+  untwo(t, u, v);
+  return two(__int_as_float(__float_as_int(p) + (__float_as_int(u) << 23)), __int_as_float(__float_as_int(q) + (__float_as_int(v) << 23)));
+}
+
+// A bounded wait that polls without sleeping.
+__device__ __forceinline__ bool spin_cta(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  for (uint32_t it = 0; it < kSpins; ++it) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(addr), "r"(parity) : "memory");
+    if (done) return true;
+  }
+  return false;
 }
 
 // The key blocks of a CTA and what its tiles see of them; every role works this out for itself.
@@ -146,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
   constexpr int ST = SH::STAGES;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t q_full, kv_full[ST], kv_empty[ST], v_ok[ST], s_full[2], p_ready[2], o_done[2];
+  __shared__ uint64_t q_full, kv_full[ST], kv_empty[ST], s_full[2], p_ready[2], o_done[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int s_fail, noted;
   __shared__ int note_key[kNotes];
@@ -166,8 +225,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
   if (tid == 0) {
     s_fail = 0; noted = 0;
     mbar_init(&q_full, 1);
-    for (int i = 0; i < ST; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); mbar_init(&v_ok[i], 2); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&o_done[i], 1); }
+    for (int i = 0; i < ST; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 6); mbar_init(&o_done[i], 1); }
     asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 9) {
@@ -207,65 +266,80 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       }
     } else if (warp == 9) {
       // ---- products ----
+      // What the instructions take is made uniform over the warp, and one lane is elected where the compiler sees that it is one: an
+      // MMA issues in 9 - 16 cycles then, in about 73 otherwise, which is more than it takes.
       constexpr uint32_t idesc0 = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);   // f32 += bf16 x bf16, M = 128
       constexpr uint32_t idesc_s = idesc0 | ((uint32_t)(kTile >> 3) << 17), idesc_o = idesc0 | ((uint32_t)(D >> 3) << 17) | (1u << 16);
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, int phase) { if (ok) ok = __all_sync(0xffffffffu, wait_cta(bar, (uint32_t)phase & 1, kPolls)); };
-      int done[2] = {0, 0};
-      auto scores = [&](int t, int it) {        // S of tile t with the keys in ring slot it
-        if (ok && elect_one()) {
-          const uint64_t ad = make_desc(smem_u32(smem) + t * SH::BYTES), bd = make_desc(ring + (it % ST) * SH::BYTES);
+      auto U = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+      Plan pl;
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t o = (k >> 2) * ((kTile * 128) >> 4) + (k & 3) * 2;
-            umma_ss(tmem + t * 128, ad + o, bd + o, idesc_s, k > 0);
-          }
-          commit(&s_full[t]);
+      for (int t = 0; t < 2; ++t) { pl.p_lo[t] = U(plan.p_lo[t]); pl.p_hi[t] = U(plan.p_hi[t]); }
+      pl.window = U(plan.window); pl.sinks = U(plan.sinks); pl.front = U(plan.front); pl.skip = U(plan.skip); pl.blocks = U(plan.blocks);
+      const uint32_t tm = (uint32_t)U((int)tmem), slot = SH::BYTES >> 4;
+      const uint64_t hi_k = make_desc(0) & 0xFFFFFFFF00000000ull, hi_v = make_desc_mn(0) & 0xFFFFFFFF00000000ull;
+      const uint32_t q_d = (uint32_t)U((int)(uint32_t)make_desc(smem_u32(smem))), k_d = (uint32_t)U((int)(uint32_t)make_desc(ring)),
+                     v_d = (uint32_t)U((int)(uint32_t)make_desc_mn(ring));
+      auto wait = [&](uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, spin_cta(bar, phase & 1)); };
+      auto scores = [&](int t, uint32_t st) {                // S of tile t with the keys in ring slot st (by the elected lane)
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t o = (k >> 2) * ((kTile * 128) >> 4) + (k & 3) * 2;
+          umma_ss(tm + t * 128, hi_k | (q_d + t * slot + o), hi_k | (k_d + st * slot + o), idesc_s, k > 0);
+        }
+        commit(&s_full[t]);
+      };
+      auto products = [&]() -> bool {
+        if (!wait(&q_full, 0) || !wait(&kv_full[0], 0)) return false;
+        uint32_t done[2] = {0, 0};
+        bool now[2] = {pl.needs(0, pl.block(0)), pl.needs(1, pl.block(0))};
+        if (elect_one()) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (now[t]) scores(t, 0);
+          commit(&kv_empty[0]);
         }
         __syncwarp();
-      };
-      if (plan.blocks > 0) {
-        wait(&q_full, 0);
-        wait(&kv_full[0], 0);
-        for (int t = 0; t < 2; ++t)
-          if (plan.needs(t, plan.block(0))) scores(t, 0);
-        if (ok && elect_one()) commit(&kv_empty[0]);
-        __syncwarp();
-        for (int n = 0; n < plan.blocks; ++n) {
-          const int iv = 2 * n + 1, ik = 2 * n + 2;
-          const bool more = n + 1 < plan.blocks;
-          const int blk = plan.block(n), next = more ? plan.block(n + 1) : 0;
-          wait(&kv_full[iv % ST], iv / ST);
-          wait(&v_ok[iv % ST], (ST & 1) ? (iv / ST) >> 1 : iv / ST);   // (a slot of an odd ring holds values every other round)
-          if (more) wait(&kv_full[ik % ST], ik / ST);
+        // A wait takes the issuer some 160 cycles even where there is nothing to wait for, and the tensor cores take few products in
+        // advance.  So it waits for p_ready alone: the warps that look after the values arrive there too, once this block's values
+        // and the next one's keys are in place.
+        uint32_t sv = 1, sk = 2, rk = 0;                     // slots of this block's values and of the next one's keys, the latter's round
+        for (int n = 0; n < pl.blocks; ++n) {
+          const bool more = n + 1 < pl.blocks;
+          const int next = pl.block(n + 1);
+          const bool then[2] = {more && pl.needs(0, next), more && pl.needs(1, next)};
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (plan.needs(t, blk)) {
-              wait(&p_ready[t], done[t]);
+            if (now[t]) {
+              if (!wait(&p_ready[t], done[t])) return false;
               fence_after();
-              if (ok && elect_one()) {
-                const uint64_t bd = make_desc_mn(ring + (iv % ST) * SH::BYTES);
+            } else if (then[t] && !wait(&kv_full[sk], rk)) return false;
+            if (elect_one()) {
+              if (now[t]) {
 #pragma unroll
                 for (int k = 0; k < kTile / 16; ++k)
-                  umma_ts(tmem + 256 + t * D, tmem + t * 128 + k * 8, bd + k * (2048 >> 4), idesc_o, done[t] > 0 || k > 0);
+                  umma_ts(tm + 256 + t * D, tm + t * 128 + k * 8, hi_v | (v_d + sv * slot + k * (2048 >> 4)), idesc_o, k > 0 ? 1u : (done[t] > 0 ? 1u : 0u));
                 commit(&o_done[t]);
               }
-              __syncwarp();
-              ++done[t];
+              if (t == 1) commit(&kv_empty[sv]);
+              if (then[t]) scores(t, sk);
+              if (t == 1 && more) commit(&kv_empty[sk]);
             }
-            if (more && plan.needs(t, next)) scores(t, ik);
+            __syncwarp();
+            if (now[t]) ++done[t];
           }
-          if (ok && elect_one()) {
-            commit(&kv_empty[iv % ST]);
-            if (more) commit(&kv_empty[ik % ST]);
-          }
-          __syncwarp();
+          now[0] = then[0]; now[1] = then[1];
+          sv = sk + 1;
+          if (sv == ST) { sv = 0; ++rk; }
+          sk = sv + 1;
+          if (sk == ST) { sk = 0; ++rk; }
         }
         // every product is complete before tensor memory and the ring go
+#pragma unroll
         for (int t = 0; t < 2; ++t)
-          if (done[t] > 0) wait(&o_done[t], done[t] - 1);
-      }
-      if (!ok) {
+          if (done[t] > 0 && !wait(&o_done[t], done[t] - 1)) return false;
+        return true;
+      };
+      if (pl.blocks > 0 && !products()) {
         if (lane == 0 && !s_fail) failed(502);
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);    // (products may still be on their way)
       }
@@ -273,6 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       // ---- values of masked blocks ----
       bool ok = true;
       const int me = tid - 320;
+      int cnt[2] = {0, 0};
       for (int n = 0; n < plan.blocks && ok; ++n) {
         const int iv = 2 * n + 1, blk = plan.block(n);
         ok = __all_sync(0xffffffffu, wait_cta(&kv_full[iv % ST], (uint32_t)(iv / ST) & 1, kPolls));
@@ -307,8 +382,16 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        __syncwarp();
-        if (ok && lane == 0) mbar_arrive(&v_ok[iv % ST]);
+        if (ok && n + 1 < plan.blocks) ok = __all_sync(0xffffffffu, wait_cta(&kv_full[(iv + 1) % ST], (uint32_t)((iv + 1) / ST) & 1, kPolls));
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (plan.needs(t, blk)) {
+            // (the phase before is complete, so that this arrival is not taken for one of its own)
+            if (ok && cnt[t] > 0) ok = __all_sync(0xffffffffu, wait_cta(&p_ready[t], (uint32_t)(cnt[t] - 1) & 1, kPolls));
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(&p_ready[t]);
+            ++cnt[t];
+          }
       }
       if (!ok && lane == 0 && !s_fail) failed(503);
     }
@@ -320,78 +403,118 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
     float ref = -INFINITY, l = 0.f;
     int done = 0;
     bool ok = true;
+    const uint64_t c2 = two(a.c, a.c);
     for (int n = 0; n < plan.blocks; ++n) {
       const int blk = plan.block(n);
       if (!plan.needs(t, blk)) continue;
       ok = __all_sync(0xffffffffu, wait_cta(&s_full[t], (uint32_t)done & 1, kPolls));
       if (!ok) break;
       fence_after();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) tmem_ld32(s_at + 32 * q, s[q]);
-      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      // A block that all queries see whole is taken with the reference as it is, scores and all in one pass: the sum tells afterwards
+      // whether that was right (a maximum of more than 2^24 would be among it, and what is not finite shows).
+      uint32_t p[64];
+      float sum = 0.f;
+      bool again = true;
       const bool whole = plan.whole(t, blk);
-      if (!whole) {
-        // key k0 + i is seen where i <= hi and (i > lo or i < sk)
-        const int k0 = blk * kTile, hi = pos - k0, lo = plan.window > 0 ? pos - plan.window - k0 : -1, sk = plan.sinks - k0;
+      if (whole && __all_sync(0xffffffffu, ref > -INFINITY)) {
+        const uint64_t r2 = two(-ref, -ref);
+        uint64_t sums[2] = {0ull, 0ull};
+        uint32_t s[2][32];
+        tmem_ld32(s_at, s[0]);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          auto below = [&](int x) { const int y = x - 32 * q; return y <= 0 ? 0u : (y >= 32 ? 0xffffffffu : (1u << y) - 1u); };   // keys < x
-          const uint32_t m = below(hi + 1) & (~below(lo + 1) | below(sk));
+          if (q < 3) tmem_ld32(s_at + 32 * (q + 1), s[(q + 1) & 1]);
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!((m >> i) & 1u)) s[q][i] = 0xff800000u;
+          for (int i = 0; i < 16; ++i) {
+            const uint64_t x = fma2(two(__uint_as_float(s[q & 1][2 * i]), __uint_as_float(s[q & 1][2 * i + 1])), c2, r2);
+            float x0, x1;
+            if ((i & 7) < kPolyOf8) untwo(exp2_pair(x), x0, x1);
+            else {
+              untwo(x, x0, x1);
+              x0 = ex2f(x0); x1 = ex2f(x1);
+            }
+            sums[i & 1] = add2(sums[i & 1], two(x0, x1));
+            p[16 * q + i] = pack2(x0, x1);
+          }
+          if (q < 3) asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         }
+        float u, v;
+        untwo(add2(sums[0], sums[1]), u, v);
+        sum = u + v;
+        again = __any_sync(0xffffffffu, !(sum <= kMostSum));
       }
-      float mx = __uint_as_float(s[0][0]);
+      if (again) {
+        uint32_t s[4][32];
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < 4; ++q) tmem_ld32(s_at + 32 * q, s[q]);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (!whole) {
+          // key k0 + i is seen where i <= hi and (i > lo or i < sk)
+          const int k0 = blk * kTile, hi = pos - k0, lo = plan.window > 0 ? pos - plan.window - k0 : -1, sk = plan.sinks - k0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(s[q][i]));
-      mx *= a.c;
-      const bool grow = mx > ref + kSlack;
-      if (__any_sync(0xffffffffu, grow)) {
-        const float f = grow ? ex2f(ref - mx) : 1.f;      // (0 for a row that saw nothing before)
-        if (grow) ref = mx;
-        l *= f;
-        if (done > 0) {
-          ok = __all_sync(0xffffffffu, wait_cta(&o_done[t], (uint32_t)(done - 1) & 1, kPolls));
-          if (!ok) break;
-          fence_after();
-#pragma unroll 1
-          for (int q = 0; q < D / 32; ++q) {
-            uint32_t o[32];
-            tmem_ld32(o_at + 32 * q, o);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          for (int q = 0; q < 4; ++q) {
+            auto below = [&](int x) { const int y = x - 32 * q; return y <= 0 ? 0u : (y >= 32 ? 0xffffffffu : (1u << y) - 1u); };   // keys < x
+            const uint32_t m = below(hi + 1) & (~below(lo + 1) | below(sk));
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st32(o_at + 32 * q, o);
+            for (int i = 0; i < 32; ++i)
+              if (!((m >> i) & 1u)) s[q][i] = 0xff800000u;
           }
         }
-      }
-      const float r = ref == -INFINITY ? 0.f : ref;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        // the row's maximum, NaN if anything is NaN or +inf: the whole row is then
+        float mx;
+        {
+          float m8[8];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t p[32];
+          for (int i = 0; i < 8; ++i) m8[i] = __uint_as_float(s[0][i]);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float x0 = ex2f(fmaf(__uint_as_float(s[2 * h + (i >> 4)][2 * (i & 15)]), a.c, -r));
-          const float x1 = ex2f(fmaf(__uint_as_float(s[2 * h + (i >> 4)][2 * (i & 15) + 1]), a.c, -r));
-          sum[2 * (i & 1)] += x0;
-          sum[2 * (i & 1) + 1] += x1;
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = q ? 0 : 8; i < 32; i += 2) m8[(i >> 1) & 7] = max3_nan(m8[(i >> 1) & 7], __uint_as_float(s[q][i]), __uint_as_float(s[q][i + 1]));
+          mx = max3_nan(max3_nan(m8[0], m8[1], m8[2]), max3_nan(m8[3], m8[4], m8[5]), max3_nan(m8[6], m8[6], m8[7]));
+        }
+        mx = mx < INFINITY ? mx * a.c : __uint_as_float(0x7fc00000u);
+        const bool grow = !(mx <= ref + kSlack) && mx != -INFINITY;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float f = grow ? ex2f(ref - mx) : 1.f;      // (0 for a row that saw nothing before)
+          if (grow) ref = mx;
+          l *= f;
+          if (done > 0) {
+            ok = __all_sync(0xffffffffu, wait_cta(&o_done[t], (uint32_t)(done - 1) & 1, kPolls));
+            if (!ok) break;
+            fence_after();
+#pragma unroll 1
+            for (int q = 0; q < D / 32; ++q) {
+              uint32_t o[32];
+              tmem_ld32(o_at + 32 * q, o);
+              asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st32(o_at + 32 * q, o);
+            }
+          }
+        }
+        const float r = ref == -INFINITY ? 0.f : ref;
+        float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 64; ++i) {                       // (scores of -inf give 0)
+          const float x0 = ex2f(fmaf(__uint_as_float(s[i >> 4][2 * (i & 15)]), a.c, -r)), x1 = ex2f(fmaf(__uint_as_float(s[i >> 4][2 * (i & 15) + 1]), a.c, -r));
+          sums[2 * (i & 1)] += x0;
+          sums[2 * (i & 1) + 1] += x1;
           p[i] = pack2(x0, x1);
         }
-        tmem_st32(s_at + 32 * h, p);
+        sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st32(s_at, *(const uint32_t(*)[32])&p[0]);
+      tmem_st32(s_at + 32, *(const uint32_t(*)[32])&p[32]);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_ready[t]);
+      l += sum;
       ++done;
     }
-    if (ok && done > 0) ok = __all_sync(0xffffffffu, wait_cta(&o_done[t], (uint32_t)(done - 1) & 1, kPolls));
+    if (ok && done > 0) ok = __all_sync(0xffffffffu, spin_cta(&o_done[t], (uint32_t)(done - 1) & 1));
     fence_after();
     if (!ok && lane == 0 && !s_fail) failed(504);
     float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
@@ -401,8 +524,10 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
         const int key = *(volatile int*)&note_key[i] + __ffs(m) - 1;
         if (key <= pos && (plan.window == 0 || key > pos - plan.window || key < plan.sinks)) inv = __uint_as_float(0x7fc00000u);
       }
-    const bool live = row < a.Tq;
-    uint16_t* out = a.out + (int64_t)b * a.o_str[0] + (int64_t)(t ? head1 : head0) * a.o_str[1] + (int64_t)row * a.o_str[2];
+    // The results go through shared memory, in the place of the warp's own queries, so that a store covers whole rows (a thread a
+    // row, 32 rows a store, took 5000 cycles); 16-byte chunks swizzled by the row.
+    unsigned char* const stage = smem + t * SH::BYTES + (warp & 3) * (32 * D * 2);
+    constexpr int CH = D / 8;
 #pragma unroll 1
     for (int q = 0; q < D / 32; ++q) {
       uint32_t o[32];
@@ -413,17 +538,28 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = 0u;
       }
-      uint32_t w[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = pack2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-      if (live) {
-        if (a.o_vec) {
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) *(uint4*)(out + 32 * q + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-        } else {
+        for (int i = 0; i < 4; ++i) w[i] = pack2(__uint_as_float(o[8 * c + 2 * i]) * inv, __uint_as_float(o[8 * c + 2 * i + 1]) * inv);
+        *(uint4*)(stage + lane * (D * 2) + (((4 * q + c) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    __syncwarp();
+    uint16_t* out = a.out + (int64_t)b * a.o_str[0] + (int64_t)(t ? head1 : head0) * a.o_str[1];
+    const int first = row - lane;
+#pragma unroll 4
+    for (int i = lane; i < 32 * CH; i += 32) {
+      const int r = i / CH, c = i % CH;
+      if (first + r >= a.Tq) break;
+      const uint4 v = *(const uint4*)(stage + r * (D * 2) + ((c ^ (r & 7)) << 4));
+      uint16_t* p = out + (int64_t)(first + r) * a.o_str[2] + 8 * c;
+      if (a.o_vec) *(uint4*)p = v;
+      else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-          for (int i = 0; i < 16; ++i) { out[32 * q + 2 * i] = (uint16_t)w[i]; out[32 * q + 2 * i + 1] = (uint16_t)(w[i] >> 16); }
-        }
+        for (int k = 0; k < 4; ++k) { p[2 * k] = (uint16_t)w[k]; p[2 * k + 1] = (uint16_t)(w[k] >> 16); }
       }
     }
   }
