@@ -34,6 +34,7 @@ constexpr int kRows = 8;              // queries per tile
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegBig = -1e30f;
 constexpr int kMergeWarps = 16;
+constexpr int kPiece = 3;             // what a piece of a sequence takes beside its blocks, in blocks of a warp
 
 template <int BITS, int D> struct Geo {
   static constexpr int G = BITS == 16 ? 1 : D / 64;       // scale groups per token
@@ -47,7 +48,8 @@ template <int BITS, int D> struct Geo {
   static constexpr int RING = STAGES * STAGE;
   static constexpr int NT = D / 16;                       // 16-dim tiles of the output
   static constexpr int SMEM_MAIN = kWarps * (RING + 2 * 4 * SB);
-  static constexpr int SMEM_MERGE = kWarps * kRows * (D + 2) * 4;
+  static constexpr int WROW = D + 4;                      // a query's row of a warp's result, padded against bank conflicts
+  static constexpr int SMEM_MERGE = kWarps * kRows * (WROW + 2) * 4;
   static constexpr int SMEM = SMEM_MAIN > SMEM_MERGE ? SMEM_MAIN : SMEM_MERGE;
 };
 
@@ -117,29 +119,63 @@ __device__ __forceinline__ Seen seen_of(const KvPagesAttnArgs& a, int64_t b) {
   return s;
 }
 
-// units[b] = units before sequence b, units[B] = all.
-__device__ __forceinline__ void plan_units(const KvPagesAttnArgs& a, int* units, int* warp_sums) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int each = (a.B + kWarps * 32 - 1) / (kWarps * 32), b0 = tid * each;
-  int mine = 0;
-  for (int i = 0; i < each && b0 + i < a.B; ++i) {
-    const int n = seen_of(a, b0 + i).blocks * a.tiles;
-    units[b0 + i] = mine;
-    mine += n;
-  }
-  int v = mine;
+// All lengths, as every CTA reads them: the units before each sequence, and what the cut is decided by.  Up to 32 sequences a warp keeps
+// them in registers, one a lane (no barrier, no second look at memory); above, they lie in shared memory.
+struct Lengths {
+  Seen mine; int before;      // of sequence `lane` (B <= 32)
+  int all, longest;           // units; blocks of the longest sequence
+};
+__device__ __forceinline__ int warp_scan(int v) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += u;
   }
-  if (lane == 31) warp_sums[warp] = v;
+  return v;
+}
+__device__ __forceinline__ Lengths read_lengths(const KvPagesAttnArgs& a, int* units, int* warp_sums) {
+  Lengths L;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (a.B <= 32) {
+    if (lane < a.B) L.mine = seen_of(a, lane);
+    else { L.mine.len = L.mine.w0 = L.mine.sinks = L.mine.front = L.mine.skip = L.mine.blocks = 0; }
+    const int n = L.mine.blocks * a.tiles, upto = warp_scan(n);
+    L.before = upto - n;
+    L.all = __shfl_sync(0xffffffffu, upto, 31);
+    L.longest = __reduce_max_sync(0xffffffffu, L.mine.blocks);
+    return L;
+  }
+  const int each = (a.B + kWarps * 32 - 1) / (kWarps * 32), b0 = tid * each;
+  int mine = 0, longest = 0;
+  for (int i = 0; i < each && b0 + i < a.B; ++i) {
+    const int n = seen_of(a, b0 + i).blocks;
+    units[b0 + i] = mine;
+    mine += n * a.tiles;
+    longest = n > longest ? n : longest;
+  }
+  const int upto = warp_scan(mine);
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (lane == 31) { warp_sums[warp] = upto; warp_sums[kWarps + warp] = longest; }
   __syncthreads();
-  int before = v - mine;
-  for (int w = 0; w < warp; ++w) before += warp_sums[w];
+  int before = upto - mine;
+  L.all = 0; L.longest = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += warp_sums[w];
+    L.all += warp_sums[w];
+    L.longest = warp_sums[kWarps + w] > L.longest ? warp_sums[kWarps + w] : L.longest;
+  }
   for (int i = 0; i < each && b0 + i < a.B; ++i) units[b0 + i] += before;
-  if (tid == 0) units[a.B] = warp_sums[0] + warp_sums[1] + warp_sums[2] + warp_sums[3];
+  if (tid == 0) units[a.B] = L.all;
   __syncthreads();
+  return L;
+}
+__device__ __forceinline__ Seen seen_from(const Lengths& L, int b) {
+  Seen s;
+  s.len = __shfl_sync(0xffffffffu, L.mine.len, b); s.w0 = __shfl_sync(0xffffffffu, L.mine.w0, b); s.sinks = __shfl_sync(0xffffffffu, L.mine.sinks, b);
+  s.front = __shfl_sync(0xffffffffu, L.mine.front, b); s.skip = __shfl_sync(0xffffffffu, L.mine.skip, b); s.blocks = __shfl_sync(0xffffffffu, L.mine.blocks, b);
+  return s;
 }
 
 template <int BITS, int D>
@@ -147,23 +183,33 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
   using GE = Geo<BITS, D>;
   constexpr int G = GE::G, CH = GE::CH, TOK = GE::TOK, ITEMS = GE::ITEMS, STAGES = GE::STAGES;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int units[kMaxPageSeqs + 1];
-  __shared__ int warp_sums[kWarps];
+  int* const units = (int*)(smem + GE::SMEM);      // [B + 1], above 32 sequences
+  __shared__ int warp_sums[2 * kWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   asm volatile("griddepcontrol.launch_dependents;");
-  plan_units(a, units, warp_sums);
+  const bool few = a.B <= 32;
+  const Lengths L = read_lengths(a, units, warp_sums);
   // sequences that see nothing: zeros
   for (int b = blockIdx.x; b < a.B; b += gridDim.x)
-    if (units[b + 1] == units[b])
+    if ((few ? __shfl_sync(0xffffffffu, L.mine.blocks, b) : units[b + 1] - units[b]) == 0)
       for (int i = tid; i < a.Hq * D; i += kWarps * 32) ((uint16_t*)a.out)[(int64_t)b * a.o_str[0] + (int64_t)(i / D) * a.o_str[1] + i % D] = 0;
 
-  const int U = units[a.B];
-  int per = (U + (int)gridDim.x - 1) / (int)gridDim.x;
+  // The cut: an even share of all units for every CTA, or every sequence in the same number of parts, whichever ends first by blocks a
+  // warp walks and what a piece takes beside them (about kPiece blocks' time): even shares cut long ragged batches best, parts keep a
+  // CTA from working on the ends of two short sequences.
+  const int U = L.all, ctas = (int)gridDim.x, seqs = a.B * a.tiles;
+  int per = (U + ctas - 1) / ctas;
   per = per < a.min_units ? a.min_units : per;
-  const int64_t u_from = (int64_t)blockIdx.x * per;
-  const int u_to = u_from + per < U ? (int)(u_from + per) : U;
-  if (tid == 0 && a.joins) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
-  if (u_from >= U) return;
+  int parts = ctas / seqs;                              // 0: even shares
+  if (parts > 0) {
+    const int most = (L.longest + a.min_units - 1) / a.min_units;
+    parts = parts > most ? (most < 1 ? 1 : most) : parts;
+    const int pieces = 1 + (int)(((int64_t)per * seqs + U - 1) / (U > 0 ? U : 1));
+    if ((L.longest + parts - 1) / parts + kPiece * kWarps > per + pieces * kPiece * kWarps) parts = 0;
+  }
+  int64_t u_from = (int64_t)blockIdx.x * per;
+  int u_to = u_from + per < U ? (int)(u_from + per) : U;
+  if (tid == 0) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
 
   const uint32_t my_ring = (uint32_t)__cvta_generic_to_shared(smem + (size_t)warp * GE::RING);
   const unsigned char* my_ring_p = smem + (size_t)warp * GE::RING;
@@ -171,18 +217,44 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
   const uint32_t my_sb = (uint32_t)__cvta_generic_to_shared(my_sb_p);
 
   int b = 0;
-  {
-    int hi = a.B - 1;
-    while (b < hi) {
-      const int mid = (b + hi + 1) >> 1;
-      if (units[mid] <= (int)u_from) b = mid; else hi = mid - 1;
+  bool next = parts > 0 ? (int)blockIdx.x < seqs * parts : u_from < U;
+  for (int u = (int)u_from; next;) {
+    Seen sn;
+    int tile, blk0, todo, more;                      // blocks [blk0, blk0 + todo) of the tile; how many CTAs behind this one share it
+    if (parts > 0) {
+      const int seq = (int)blockIdx.x / parts, part = (int)blockIdx.x - seq * parts;
+      b = seq / a.tiles;
+      tile = seq - b * a.tiles;
+      sn = few ? seen_from(L, b) : seen_of(a, b);
+      const int mine = parts < sn.blocks ? parts : sn.blocks;
+      if (part >= mine) return;
+      blk0 = (int)((int64_t)sn.blocks * part / mine);
+      todo = (int)((int64_t)sn.blocks * (part + 1) / mine) - blk0;
+      more = mine - 1;
+      next = false;
+    } else {
+      int before;
+      if (few) {
+        b = 31 - __clz(__ballot_sync(0xffffffffu, L.before <= u && L.mine.blocks > 0));
+        before = __shfl_sync(0xffffffffu, L.before, b);
+        sn = seen_from(L, b);
+      } else {
+        int hi = a.B - 1;                            // (the last one that begins at u or before: empty ones share their begin with the next)
+        while (b < hi) {
+          const int mid = (b + hi + 1) >> 1;
+          if (units[mid] <= u) b = mid; else hi = mid - 1;
+        }
+        before = units[b];
+        sn = seen_of(a, b);
+      }
+      tile = (u - before) / sn.blocks;
+      blk0 = u - before - tile * sn.blocks;
+      const int left = sn.blocks - blk0;
+      todo = left < u_to - u ? left : u_to - u;
+      more = (before + (tile + 1) * sn.blocks - 1) / per - (int)blockIdx.x;
+      u += todo;
+      next = u < u_to;
     }
-  }
-  for (int u = (int)u_from; u < u_to;) {
-    while (units[b + 1] <= u) ++b;
-    const Seen sn = seen_of(a, b);
-    const int tile = (u - units[b]) / sn.blocks, blk0 = u - units[b] - tile * sn.blocks;
-    const int left = sn.blocks - blk0, todo = left < u_to - u ? left : u_to - u;
     const int hk = tile / a.qtiles, qt = tile - hk * a.qtiles;
     const int row = a.rows ? a.rows[b] : b;
     const int32_t* tab = a.table + (int64_t)row * a.table_str;
@@ -190,6 +262,33 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
     const int pmask = (1 << a.page_shift) - 1;
     auto first_token = [&](int j) { const int i = blk0 + warp + j * kWarps; return (i < sn.front ? i : i + sn.skip) * kBlk; };
     auto visible = [&](int tok) { return tok < sn.len && (tok >= sn.w0 || tok < sn.sinks); };
+
+    // ---- queries: row g of the tile, asked for before anything else ----
+    const bool q_live = qt * kRows + g < a.gqa;
+    const uint16_t* const qp = (const uint16_t*)a.q + (int64_t)b * a.q_str[0] + (int64_t)(hk * a.gqa + (q_live ? qt * kRows + g : 0)) * a.q_str[1];
+    uint32_t qraw[D / 16][2];        // at 16 bits the operand, else dims 16 t .. 16 t + 15 of a group in eight registers
+    if constexpr (BITS == 16) {
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint16_t* p = qp + 16 * s + 2 * t + 8 * h;
+          qraw[s][h] = (uint32_t)p[0] | ((uint32_t)p[1] << 16);
+        }
+    } else {
+#pragma unroll
+      for (int grp = 0; grp < G; ++grp) {
+        const uint16_t* p = qp + grp * 64 + 16 * t;
+        if (a.q_vec) {
+          const uint4 x = ((const uint4*)p)[0], y = ((const uint4*)p)[1];
+          qraw[4 * grp][0] = x.x; qraw[4 * grp][1] = x.y; qraw[4 * grp + 1][0] = x.z; qraw[4 * grp + 1][1] = x.w;
+          qraw[4 * grp + 2][0] = y.x; qraw[4 * grp + 2][1] = y.y; qraw[4 * grp + 3][0] = y.z; qraw[4 * grp + 3][1] = y.w;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) qraw[4 * grp + (k >> 1)][k & 1] = (uint32_t)p[2 * k] | ((uint32_t)p[2 * k + 1] << 16);
+        }
+      }
+    }
 
     // ---- producer ----
     // lane l holds the page of the 16 tokens from 16 * (l & 3) on, -1 where there is none
@@ -290,14 +389,11 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
     if (my_blocks > 0) issue(QB_PART(2), 0);
     cp_async_commit();
 
-    // ---- queries: row g of the tile as the B operand ----
+    // ---- the queries as the B operand ----
     uint32_t qf[D / 16][2];
     uint32_t qb = 0;                 // bias product: this lane's part of the group sums of query g
     float C0, C1;                    // factor of the scores of queries 2t and 2t + 1
     {
-      const int r = qt * kRows + g;
-      const bool live = r < a.gqa && my_blocks > 0;
-      const uint16_t* qp = (const uint16_t*)a.q + (int64_t)b * a.q_str[0] + (int64_t)(hk * a.gqa + (live ? r : 0)) * a.q_str[1];
       // (the sign of the scale goes to the queries, so that the largest score is the largest sum; a factor of 0 would meet scores of -inf)
       const float factor = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
       if constexpr (BITS == 16) {
@@ -305,29 +401,17 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
         for (int s = 0; s < D / 16; ++s)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint16_t* p = qp + 16 * s + 2 * t + 8 * h;
-            qf[s][h] = live ? ((uint32_t)p[0] | ((uint32_t)p[1] << 16)) ^ (a.scale < 0.f ? 0x80008000u : 0u) : 0u;
+            qf[s][h] = q_live ? qraw[s][h] ^ (a.scale < 0.f ? 0x80008000u : 0u) : 0u;
           }
         C0 = C1 = factor;
       } else {
         float f[G][16], sum[G], mx = 0.f;
 #pragma unroll
         for (int grp = 0; grp < G; ++grp) {
-          const uint16_t* p = qp + grp * 64 + 16 * t;
-          uint4 raw[2];
-          if (a.q_vec) {
-            raw[0] = ((const uint4*)p)[0]; raw[1] = ((const uint4*)p)[1];
-          } else {
-            uint32_t e[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) e[k] = (uint32_t)p[2 * k] | ((uint32_t)p[2 * k + 1] << 16);
-            raw[0] = make_uint4(e[0], e[1], e[2], e[3]); raw[1] = make_uint4(e[4], e[5], e[6], e[7]);
-          }
-          const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
           sum[grp] = 0.f;
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            f[grp][2 * k] = live ? bf16lo(w[k]) : 0.f; f[grp][2 * k + 1] = live ? bf16hi(w[k]) : 0.f;
+            f[grp][2 * k] = q_live ? bf16lo(qraw[4 * grp + (k >> 1)][k & 1]) : 0.f; f[grp][2 * k + 1] = q_live ? bf16hi(qraw[4 * grp + (k >> 1)][k & 1]) : 0.f;
             mx = fmax_nan(mx, fmax_nan(fabsf(f[grp][2 * k]), fabsf(f[grp][2 * k + 1])));
             sum[grp] += f[grp][2 * k] + f[grp][2 * k + 1];
           }
@@ -617,7 +701,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
     __syncthreads();      // every warp is done with its ring
     float* wm = (float*)smem;                     // [warp][8]
     float* wl = wm + kWarps * kRows;
-    float* wo = wl + kWarps * kRows;              // [warp][8][D]
+    float* wo = wl + kWarps * kRows;              // [warp][8][WROW]
     if (g == 0) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) { wm[warp * kRows + 2 * t + c] = r_run[c]; wl[warp * kRows + 2 * t + c] = l_part[c]; }
@@ -635,14 +719,13 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
           dim = 16 * n + m;
           v = fmaf(v, 16777216.f, ob[(n >> 2) % G][c]);
         } else dim = 16 * n + m;
-        wo[(size_t)(warp * kRows + 2 * t + c) * D + dim] = v;
+        wo[(warp * kRows + 2 * t + c) * GE::WROW + dim] = v;
       }
     __syncthreads();
     const int rows = a.gqa - qt * kRows < kRows ? a.gqa - qt * kRows : kRows;
     const bool all = blk0 == 0 && todo == sn.blocks;
     const int slot = 2 * blockIdx.x + (blk0 == 0 ? 1 : 0);
     if (!all && blk0 == 0 && tid == 0) {          // the first of the blocks that share this sequence
-      const int more = (units[b] + (tile + 1) * sn.blocks - 1) / per - (int)blockIdx.x;
       a.joins[blockIdx.x] = make_int4(b, hk * a.gqa + qt * kRows, rows, more);
     }
     for (int i = tid; i < rows * D; i += kWarps * 32) {
@@ -655,7 +738,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
       for (int w = 0; w < kWarps; ++w) {
         const float f = ex2(wm[w * kRows + h] - M);
         L += wl[w * kRows + h] * f;
-        Ov += wo[(size_t)(w * kRows + h) * D + e] * f;
+        Ov += wo[(w * kRows + h) * GE::WROW + e] * f;
       }
       if (all) {
         const float v = Ov * (L > 0.f ? 1.f / L : (L == L ? 0.f : L));
@@ -666,7 +749,6 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
       }
     }
     __syncthreads();      // the ring may be filled again
-    u += todo;
   }
 }
 
@@ -735,34 +817,34 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv_pages_join_kernel(const _
   }
 }
 
-// CTAs of an instance that the device holds at once.
-template <int BITS, int D> cudaError_t resident(int* n) {
+// CTAs of an instance that the device holds at once, with the lengths of up to 32, 512 or more sequences in shared memory.
+constexpr int kSeqSteps[3] = {32, 512, kMaxPageSeqs};
+template <int BITS, int D> constexpr int smem_of(int step) { return Geo<BITS, D>::SMEM + (step == 0 ? 0 : (kSeqSteps[step] + 1) * 4); }
+template <int BITS, int D> cudaError_t resident(int step, int* n) {
   auto kern = kv_pages_kernel<BITS, D>;
-  static int cached[64] = {};
+  static int cached[64][3] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   std::lock_guard<std::mutex> setup_lk(setup_mutex());   // first use on a device, from any thread
-  if (dev < 0 || dev >= 64 || cached[dev] == 0) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<BITS, D>::SMEM);
-    if (e != cudaSuccess) return e;
-    int per = 0;
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, kWarps * 32, Geo<BITS, D>::SMEM);
-    if (e != cudaSuccess) return e;
-    const int all = (per < 1 ? 1 : (per > kPagesCtas ? kPagesCtas : per)) * sm_count();
-    if (dev < 0 || dev >= 64) { *n = all; return cudaSuccess; }
-    cached[dev] = all;
-  }
-  *n = cached[dev];
+  if (dev >= 0 && dev < 64 && cached[dev][step] != 0) { *n = cached[dev][step]; return cudaSuccess; }
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_of<BITS, D>(2));
+  if (e != cudaSuccess) return e;
+  int per = 0;
+  e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, kWarps * 32, smem_of<BITS, D>(step));
+  if (e != cudaSuccess) return e;
+  *n = (per < 1 ? 1 : (per > kPagesCtas ? kPagesCtas : per)) * sm_count();
+  if (dev >= 0 && dev < 64) cached[dev][step] = *n;
   return cudaSuccess;
 }
 
 template <int BITS, int D> cudaError_t launch_inst(KvPagesAttnArgs a, int64_t most_units, cudaStream_t st) {
   int n = 0;
-  cudaError_t e = resident<BITS, D>(&n);
+  const int step = a.B <= kSeqSteps[0] ? 0 : (a.B <= kSeqSteps[1] ? 1 : 2);
+  cudaError_t e = resident<BITS, D>(step, &n);
   if (e != cudaSuccess) return e;
   const unsigned grid = (unsigned)(most_units < n ? (most_units < 1 ? 1 : most_units) : n);
-  e = launch_kernel(kv_pages_kernel<BITS, D>, dim3(grid), dim3(kWarps * 32), Geo<BITS, D>::SMEM, st, a);
+  e = launch_kernel(kv_pages_kernel<BITS, D>, dim3(grid), dim3(kWarps * 32), smem_of<BITS, D>(step), st, a);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
