@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
   if (parts > 0) {
     const int most = (L.longest + a.min_units - 1) / a.min_units;
     parts = parts > most ? (most < 1 ? 1 : most) : parts;
-    const int pieces = 1 + (int)(((int64_t)per * seqs + U - 1) / (U > 0 ? U : 1));
+    const int pieces = 1 + (int)ceilf(__fdividef((float)per * (float)seqs, (float)(U > 0 ? U : 1)));   // that an even share touches
     if ((L.longest + parts - 1) / parts + kPiece * kWarps > per + pieces * kPiece * kWarps) parts = 0;
   }
   int64_t u_from = (int64_t)blockIdx.x * per;
@@ -228,8 +228,9 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
       sn = few ? seen_from(L, b) : seen_of(a, b);
       const int mine = parts < sn.blocks ? parts : sn.blocks;
       if (part >= mine) return;
-      blk0 = (int)((int64_t)sn.blocks * part / mine);
-      todo = (int)((int64_t)sn.blocks * (part + 1) / mine) - blk0;
+      const int each = sn.blocks / mine, rest = sn.blocks - each * mine;
+      blk0 = each * part + (part < rest ? part : rest);
+      todo = each + (part < rest ? 1 : 0);
       more = mine - 1;
       next = false;
     } else {
@@ -321,9 +322,11 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
     int pid_next = page_at(0), pid_cur = -1, blk_tok = 0;
     uint32_t vm_next = 0;
     bool whole_next = false;
-    auto issue = [&](auto part_c, int j) {                // the copies of stage `part` of block j
-      constexpr int part = decltype(part_c)::value, stage = part % STAGES;
-      if constexpr (part == 0) {
+    // the copies of stage `part` of block j (a constant in the loop over the blocks; the first three stages go through one copy of the
+    // code: a short sequence waits for instructions more than for data)
+    auto issue = [&](const int part, int j) {
+      const int stage = part % STAGES;
+      if (part == 0) {
         pid_cur = pid_next;
         blk_tok = first_token(j);
         vm_next = __ballot_sync(0xffffffffu, pid_cur >= 0) & 15u;
@@ -360,8 +363,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
           }
         }
       }
-      constexpr bool V = part >= ITEMS / 2;
-      constexpr int tk0 = (part % (ITEMS / 2)) * TOK;
+      const bool V = part >= ITEMS / 2;
+      const int tk0 = (part % (ITEMS / 2)) * TOK;
       const uint32_t page_b = a.page_bytes[V], tok_b = a.tok_bytes[V], st = my_ring + stage * GE::STAGE;
       auto copy = [&](auto all_c) {
 #pragma unroll
@@ -382,12 +385,11 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
       if (whole_next) copy(std::true_type{}); else copy(std::false_type{});
     };
 #define QB_PART(n) std::integral_constant<int, (n)>{}
-    if (my_blocks > 0) issue(QB_PART(0), 0);
-    cp_async_commit();
-    if (my_blocks > 0) issue(QB_PART(1), 0);
-    cp_async_commit();
-    if (my_blocks > 0) issue(QB_PART(2), 0);
-    cp_async_commit();
+#pragma unroll 1
+    for (int part = 0; part < STAGES - 1; ++part) {
+      if (my_blocks > 0) issue(part, 0);
+      cp_async_commit();
+    }
 
     // ---- the queries as the B operand ----
     uint32_t qf[D / 16][2];
@@ -456,8 +458,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
     // the next stage of block j: what it takes to stay three stages ahead is issued, and its own copies are complete
     auto acquire = [&](auto it_c, int j) -> const unsigned char* {
       constexpr int it = decltype(it_c)::value, ahead = it + STAGES - 1;
-      if constexpr (ahead < ITEMS) issue(QB_PART(ahead), j);
-      else if (j + 1 < my_blocks) issue(QB_PART(ahead - ITEMS), j + 1);
+      if constexpr (ahead < ITEMS) issue(ahead, j);
+      else if (j + 1 < my_blocks) issue(ahead - ITEMS, j + 1);
       cp_async_commit();
       cp_async_wait<STAGES - 1>();
       __syncwarp();
