@@ -64,6 +64,29 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *(const uint32_t*)&h;
 }
 
+// Two fp32 in a 64-bit register: one instruction does both.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void untwo(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // sigmoid of a bf16 value, rounded to bf16: the two-sided form of MLX's Sigmoid as the reference quotes it
 // (src/transformer.zig:17566-17570).  The approximate exponential and reciprocal give the same bf16 as fp32 libm for every
 // one of the 65536 patterns with |x| <= 80 (the elementwise tests go through all of them); beyond, where the result is

@@ -179,13 +179,12 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const uint16_t* x, uint
   const bool live = i < rg.inner * rg.per_row;
   const int row = live ? row_of(rg, i) : 0, c = live ? i - row * rg.per_row : 0;
   const uint16_t* xp = x + row_base(ax, row) + c * kRowVals;
-  float v[kRowVals];
-#pragma unroll
-  for (int k = 0; k < kRowVals / 8; ++k) unpack8_bf16(((const uint4*)xp)[k], v + 8 * k);
+  const uint4 x0 = ((const uint4*)xp)[0], x1 = ((const uint4*)xp)[1];
+  const uint32_t raw[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
   const int tpg = gs / kRowVals;   // neighbouring lanes share a group: 2, 4 or 8
   float scale, bias;
   uint32_t w[BITS / 2];
-  quantize16<BITS>(v, tpg, w, scale, bias);
+  quantize16<BITS>(raw, tpg, w, scale, bias);
   if (!live) return;
   uint32_t* qp = qo + row_base(aq, row) + c * (BITS / 2);
   if constexpr (BITS == 4) *(uint2*)qp = make_uint2(w[0], w[1]); else *(uint4*)qp = make_uint4(w[0], w[1], w[BITS / 2 - 2], w[BITS / 2 - 1]);

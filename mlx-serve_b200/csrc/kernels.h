@@ -285,6 +285,7 @@ struct KvPagesAppendArgs {
   const int32_t* rows; const int32_t* positions; const int32_t* counts;   // rows, counts may be null
   int64_t M, seqs, P;
   int page_shift, N, H, S, per_row, bits, dense_vec;
+  int tiles, row_shift;                  // by the launcher: blocks of a head's rows, log2 of per_row (-1: no power of two)
 };
 cudaError_t launch_pages_append(const KvPagesAppendArgs& a, cudaStream_t st);
 struct PageState {

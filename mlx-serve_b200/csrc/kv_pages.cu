@@ -16,26 +16,18 @@ namespace {
 // ---------------------------------------------------------------- new rows into pages
 // Row (n, i) of head h goes to slot (pos % page) of page table[r, pos / page], pos = positions[n] + i.  16 values a thread: the four
 // (head dim 64) or eight threads of a row are neighbours, rows of one head follow each other as tokens do, so that both sides are
-// read and written in whole sectors.  Bound by HBM at prompt lengths, by the launch at one token.
+// read and written in whole sectors.  A block has rows of one (sequence, K or V, head); the values are asked for before the table is
+// looked up.  Bound by HBM at prompt lengths, by the launch at one token.
 template <int BITS>
 __global__ void __launch_bounds__(256) pages_append_kernel(const __grid_constant__ KvPagesAppendArgs a) {
-  const uint32_t total = (uint32_t)a.N * 2u * a.H * a.S * a.per_row;
-  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
-  const bool in = i < total;
-  const uint32_t ii = in ? i : total - 1;
-  const uint32_t r = ii / a.per_row, c = ii - r * a.per_row;
-  const uint32_t r2 = r / a.S, s = r - r2 * a.S;
+  const uint32_t r2 = blockIdx.x / a.tiles, tile = blockIdx.x - r2 * a.tiles;
   const uint32_t r3 = r2 / a.H, h = r2 - r3 * a.H;
   const uint32_t kv = r3 & 1u, n = r3 >> 1;
-  const int64_t row = a.rows ? a.rows[n] : (int64_t)n;
-  const int64_t pos = (int64_t)a.positions[n] + s;
-  bool live = in && row >= 0 && row < a.seqs && pos >= 0 && (pos >> a.page_shift) < a.M && (!a.counts || (int64_t)s < a.counts[n]);
-  const int64_t pid = live ? a.table[row * a.table_str + (pos >> a.page_shift)] : -1;
-  live = live && pid >= 0 && pid < a.P;
-  if (!__any_sync(0xffffffffu, live)) return;
-  const KvPoolView& p = a.pool[kv];
-  const int64_t slot = pos & ((1 << a.page_shift) - 1);
-  const uint16_t* x = a.dense[kv] + (int64_t)n * a.dense_str[kv][0] + (int64_t)h * a.dense_str[kv][1] + (int64_t)s * a.dense_str[kv][2] + c * kRowVals;
+  const uint32_t i = tile * blockDim.x + threadIdx.x, s0 = a.row_shift >= 0 ? i >> a.row_shift : i / a.per_row;
+  const bool in = s0 < (uint32_t)a.S;
+  const uint32_t s = in ? s0 : a.S - 1, c = i - s0 * a.per_row;
+  const uint16_t* x = (kv ? a.dense[1] : a.dense[0]) + (int64_t)n * (kv ? a.dense_str[1][0] : a.dense_str[0][0]) + (int64_t)h * (kv ? a.dense_str[1][1] : a.dense_str[0][1]) +
+                      (int64_t)s * (kv ? a.dense_str[1][2] : a.dense_str[0][2]) + c * kRowVals;
   uint4 raw[2];
   if (a.dense_vec) {
     raw[0] = ((const uint4*)x)[0]; raw[1] = ((const uint4*)x)[1];
@@ -45,16 +37,23 @@ __global__ void __launch_bounds__(256) pages_append_kernel(const __grid_constant
     for (int k = 0; k < 8; ++k) e[k] = (uint32_t)x[2 * k] | ((uint32_t)x[2 * k + 1] << 16);
     raw[0] = make_uint4(e[0], e[1], e[2], e[3]); raw[1] = make_uint4(e[4], e[5], e[6], e[7]);
   }
+  const int64_t row = a.rows ? a.rows[n] : (int64_t)n;
+  const int64_t pos = (int64_t)a.positions[n] + s;
+  bool live = in && row >= 0 && row < a.seqs && pos >= 0 && (pos >> a.page_shift) < a.M && (!a.counts || (int64_t)s < a.counts[n]);
+  const int64_t pid = live ? a.table[row * a.table_str + (pos >> a.page_shift)] : -1;
+  live = live && pid >= 0 && pid < a.P;
+  if (!__any_sync(0xffffffffu, live)) return;
+  const KvPoolView& p = kv ? a.pool[1] : a.pool[0];
+  const int64_t slot = pos & ((1 << a.page_shift) - 1);
   if constexpr (BITS == 16) {
     if (!live) return;
     uint4* o = (uint4*)((uint16_t*)p.q + pid * p.q_str[0] + h * p.q_str[1] + slot * p.q_str[2] + c * kRowVals);
     o[0] = raw[0]; o[1] = raw[1];
   } else {
-    float v[kRowVals];
-    unpack8_bf16(raw[0], v); unpack8_bf16(raw[1], v + 8);
+    const uint32_t vals[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
     float scale, bias;
     uint32_t w[BITS / 2];
-    quantize16<BITS>(v, 4, w, scale, bias);
+    quantize16<BITS>(vals, 4, w, scale, bias);
     if (!live) return;
     uint32_t* o = (uint32_t*)p.q + pid * p.q_str[0] + h * p.q_str[1] + slot * p.q_str[2] + c * (BITS / 2);
     if constexpr (BITS == 4) *(uint2*)o = make_uint2(w[0], w[1]); else *(uint4*)o = make_uint4(w[0], w[1], w[BITS / 2 - 2], w[BITS / 2 - 1]);
@@ -431,9 +430,15 @@ int bit_words(int64_t P, int blocks) { return (int)(((P + 31) / 32 + blocks - 1)
 }  // namespace
 
 cudaError_t launch_pages_append(const KvPagesAppendArgs& a, cudaStream_t st) {
-  const int64_t threads = (int64_t)a.N * 2 * a.H * a.S * a.per_row;
+  const int64_t head = (int64_t)a.S * a.per_row;             // threads that the rows of a head take
+  const int block = head >= 256 ? 256 : (int)((head + 31) / 32 * 32);
+  KvPagesAppendArgs k = a;
+  k.tiles = (int)((head + block - 1) / block);
+  k.row_shift = -1;
+  for (int i = 0; i < 16; ++i)
+    if (a.per_row == 1 << i) k.row_shift = i;
   auto kern = a.bits == 4 ? pages_append_kernel<4> : (a.bits == 8 ? pages_append_kernel<8> : pages_append_kernel<16>);
-  return launch_kernel(kern, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);
+  return launch_kernel(kern, dim3((unsigned)((int64_t)k.tiles * a.N * 2 * a.H)), dim3((unsigned)block), 0, st, k);
 }
 cudaError_t launch_pages_free(const PageState& s, const int32_t* rows, const int32_t* begin, const int32_t* end, int n, cudaStream_t st) {
   return launch_kernel(pages_free_kernel, dim3((unsigned)n), dim3(256), 0, st, s, rows, begin, end);

@@ -80,6 +80,32 @@ def test_append_drops_positions_below_zero_and_counts_of_none():
     assert torch.equal(kp[0][0, :, :2], want) and torch.equal(kp[0][1:], before[0][1:])
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+def test_codes_are_those_of_a_division(bits):
+    """Groups whose quotients are ties, or next to one, as often as bf16 values make them so, at every magnitude; the codes by a division
+    in fp32 rounded to nearest even, worked out here."""
+    g = torch.Generator(device="cuda").manual_seed(bits)
+    rows = 4096
+    x = torch.randint(-255, 256, (rows, 64), device="cuda", generator=g).float() * 2.0 ** torch.randint(-30, 30, (rows, 1), device="cuda", generator=g).float()
+    x[::2] = torch.randn(rows // 2, 64, device="cuda", generator=g) * 2.0 ** torch.randint(-40, 100, (rows // 2, 1), device="cuda", generator=g).float()
+    x[:64] = torch.arange(64, device="cuda") * torch.arange(1, 65, device="cuda")[:, None] / 2.0
+    x = x.to(BF16)
+    v = x.float()
+    lo, hi = v.amin(1, keepdim=True), v.amax(1, keepdim=True)
+    bins = torch.full_like(lo, 2.0 ** bits - 1)
+    neg = lo.abs() > hi.abs()
+    s = torch.clamp((hi - lo) / bins, min=1e-7)
+    s = torch.where(neg, s, -s)
+    edge = torch.where(neg, lo, hi)
+    q0 = torch.round(edge / s)
+    s = torch.where(q0 == 0, s, edge / torch.where(q0 == 0, torch.ones_like(q0), q0))
+    bias = torch.where(q0 == 0, torch.zeros_like(edge), edge)
+    want = torch.minimum(torch.clamp(torch.round((v - bias) / s), min=0.0), bins).to(torch.int64)
+    q, sc, b = qb200.quantize(x, 64, bits)
+    got = ((q[..., None].to(torch.int64) >> (torch.arange(32 // bits, device="cuda") * bits)) & (2 ** bits - 1)).reshape(rows, 64)
+    assert torch.equal(got, want) and torch.equal(sc, s.to(BF16)) and torch.equal(b, bias.to(BF16))
+
+
 # ---------------------------------------------------------------- bookkeeping
 
 class Both:
