@@ -430,7 +430,7 @@ QB200_API int qb200_window_attention(qb200_tensor* res, const qb200_tensor* q, c
   if (Hkv <= 0 || Hq % Hkv != 0) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: Hq %lld not a multiple of Hkv %lld", who, (long long)Hq, (long long)Hkv);
   if (D != 64 && D != 128) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: head dim %lld is not served (64, 128)", who, (long long)D);
   if (window < 0 || sinks < 0) return pg_fail(QB200_ERR_BAD_ARG, "%s: window and sinks must not be negative", who);
-  if (!(scale > 0.f) || !(scale <= 3.0e38f)) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: scale must be positive and finite", who);
+  if (!(scale > 0.f) || !(scale <= 1.0e38f)) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: scale must be positive and finite", who);
   if (!empty(kv_lens)) {
     if ((st = expect_list(kv_lens, who, "kv_lens", B))) return st;
   } else if (Tk < Tq) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: %lld queries need as many keys (%lld given)", who, (long long)Tq, (long long)Tk);

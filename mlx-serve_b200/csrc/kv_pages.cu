@@ -13,6 +13,10 @@
 namespace qb {
 namespace {
 
+// These kernels follow each other in a serving loop, each a few microseconds long: they are launched while the one before still runs
+// and wait here for all that it writes.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- new rows into pages
 // Row (n, i) of head h goes to slot (pos % page) of page table[r, pos / page], pos = positions[n] + i.  16 values a thread: the four
 // (head dim 64) or eight threads of a row are neighbours, rows of one head follow each other as tokens do, so that both sides are
@@ -68,6 +72,7 @@ __global__ void __launch_bounds__(256) pages_append_kernel(const __grid_constant
 // ---------------------------------------------------------------- freeing pages
 // A block per listed sequence; the first of several entries that name the same sequence does the work.
 __global__ void __launch_bounds__(256) pages_free_kernel(PageState st, const int32_t* rows, const int32_t* begin, const int32_t* end) {
+  grid_wait();
   const int i = blockIdx.x, tid = threadIdx.x;
   const int r = rows[i];
   if (r < 0 || r >= st.S) return;
@@ -97,6 +102,7 @@ __global__ void __launch_bounds__(256) pages_free_kernel(PageState st, const int
 // Forking, reserving and compacting each read the whole state before they change it.  One cluster of up to eight blocks does
 // that in one launch with the hardware's barrier between the steps; a launch of one block is the same program.
 constexpr int kPageThreads = 512;
+constexpr int kStateBlocks = 8;      // one, two, four or eight blocks take the same for pools of 700 pages; 200,000 pages take 77, 49, 34, 26 us
 
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
   uint32_t v;
@@ -176,6 +182,7 @@ __global__ void __launch_bounds__(kPageThreads) pages_fork_kernel(PageState st, 
   int* s_dst = sm;          // [n]
   int* s_tok = sm + n;      // [n]: tokens shared, -1 = refused
   const int tid = threadIdx.x;
+  grid_wait();
   for (int i = tid; i < n; i += kPageThreads) s_dst[i] = dst[i];
   __syncthreads();
   for (int i = tid; i < n; i += kPageThreads) {
@@ -192,20 +199,25 @@ __global__ void __launch_bounds__(kPageThreads) pages_fork_kernel(PageState st, 
     s_tok[i] = t;
   }
   cluster_sync_all();                    // every block has seen the state before the call
-  const int nr = (int)cluster_size(), me = (int)cluster_rank();
-  for (int i = me; i < n; i += nr) {
-    const int t = s_tok[i];
-    if (t > 0) {
-      const int np = (int)(((int64_t)t + (1 << st.page_shift) - 1) >> st.page_shift);
+  // a warp takes up to 512 pages of an entry at a time
+  constexpr int kChunk = 512;
+  const int nw = (int)cluster_size() * (kPageThreads / 32), w = (int)cluster_rank() * (kPageThreads / 32) + (tid >> 5), lane = tid & 31;
+  const int chunks = (st.M + kChunk - 1) / kChunk > 0 ? (st.M + kChunk - 1) / kChunk : 1;
+  for (int item = w; item < n * chunks; item += nw) {
+    const int i = item / chunks, c = item - i * chunks, t = s_tok[i];
+    const int np = t > 0 ? (int)(((int64_t)t + (1 << st.page_shift) - 1) >> st.page_shift) : 0;
+    const int stop = np < (c + 1) * kChunk ? np : (c + 1) * kChunk;
+    if (c * kChunk < stop) {
       const int32_t* from = st.table + (int64_t)src[i] * st.table_str;
       int32_t* to = st.table + (int64_t)s_dst[i] * st.table_str;
-      for (int p = tid; p < np; p += kPageThreads) {
+#pragma unroll 4
+      for (int p = c * kChunk + lane; p < stop; p += 32) {
         const int32_t pid = from[p];
         to[p] = pid;
         if (pid >= 0 && pid < st.P) atomicAdd(st.refs + pid, 1);
       }
     }
-    if (tid == 0) {
+    if (c == 0 && lane == 0) {
       if (t > 0) st.lens[s_dst[i]] = t;
       shared[i] = t;
     }
@@ -229,6 +241,7 @@ __global__ void __launch_bounds__(kPageThreads) pages_reserve_kernel(PageState s
   __shared__ int block_count;
   const int tid = threadIdx.x;
   const int64_t page = 1ll << st.page_shift;
+  grid_wait();
   for (int i = tid; i < n; i += kPageThreads) s_row[i] = rows[i];
   __syncthreads();
   int run = 0;
@@ -312,6 +325,7 @@ __global__ void __launch_bounds__(kPageThreads) pages_compact_kernel(PageState s
   __shared__ int warp_sums[kPageThreads / 32];
   __shared__ int block_count, in_front;
   const int nr = (int)cluster_size(), me = (int)cluster_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  grid_wait();
   const Share sh = page_bits(st, false, bits, pre, warp_sums, &block_count);
   const int live = sh.total;
   // how many of the first `live` pages are live: the block that holds page `live` knows, and tells the others
@@ -360,6 +374,7 @@ constexpr int kCopyPiece = 8192;
 
 template <typename V>
 __global__ void __launch_bounds__(256) pages_copy_kernel(const __grid_constant__ PagesCopyArgs a) {
+  grid_wait();
   const int64_t n = a.count ? min((int64_t)(*a.count > 0 ? *a.count : 0), a.n) : a.n;
   const int64_t work = n * a.pieces;
   for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
@@ -403,6 +418,23 @@ __global__ void __launch_bounds__(256) pages_copy_kernel(const __grid_constant__
   }
 }
 
+// A launch that may begin while the kernel before it runs; in clusters of `cluster` blocks where that is above 1.
+template <typename... K, typename... A>
+cudaError_t launch_behind(void (*kern)(K...), dim3 grid, int threads, int cluster, size_t smem, cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cluster > 1 ? launch_clusters(cfg, kern, args...) : cudaLaunchKernelEx(&cfg, kern, static_cast<K>(args)...);
+}
 template <typename... K, typename... A>
 cudaError_t launch_page_cluster(void (*kern)(K...), int want, size_t smem, cudaStream_t st, A... args) {
   if (smem > 48 * 1024) {
@@ -410,21 +442,11 @@ cudaError_t launch_page_cluster(void (*kern)(K...), int want, size_t smem, cudaS
     if (e != cudaSuccess) return e;
   }
   if (want > 1) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)want);
-    cfg.blockDim = dim3(kPageThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)want; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = launch_clusters(cfg, kern, args...);
+    const cudaError_t e = launch_behind(kern, dim3((unsigned)want), kPageThreads, want, smem, st, args...);
     if (e == cudaSuccess) return e;
     (void)cudaGetLastError();            // the device places no clusters: one block does it
   }
-  return launch_kernel(kern, dim3(1), dim3(kPageThreads), smem, st, args...);
+  return launch_behind(kern, dim3(1), kPageThreads, 1, smem, st, args...);
 }
 int bit_words(int64_t P, int blocks) { return (int)(((P + 31) / 32 + blocks - 1) / blocks); }
 }  // namespace
@@ -441,28 +463,28 @@ cudaError_t launch_pages_append(const KvPagesAppendArgs& a, cudaStream_t st) {
   return launch_kernel(kern, dim3((unsigned)((int64_t)k.tiles * a.N * 2 * a.H)), dim3((unsigned)block), 0, st, k);
 }
 cudaError_t launch_pages_free(const PageState& s, const int32_t* rows, const int32_t* begin, const int32_t* end, int n, cudaStream_t st) {
-  return launch_kernel(pages_free_kernel, dim3((unsigned)n), dim3(256), 0, st, s, rows, begin, end);
+  return launch_behind(pages_free_kernel, dim3((unsigned)n), 256, 1, 0, st, s, rows, begin, end);
 }
 // One block's bits take 2 words per 32 pages and the list five: both fit where kMaxPages and kMaxPageList hold.
 cudaError_t launch_pages_fork(const PageState& s, const int32_t* src, const int32_t* dst, const int32_t* tokens, int n, int32_t* shared, cudaStream_t st) {
-  return launch_page_cluster(pages_fork_kernel, n < 8 ? n : 8, (size_t)n * 8, st, s, src, dst, tokens, n, shared);
+  return launch_page_cluster(pages_fork_kernel, kStateBlocks, (size_t)n * 8, st, s, src, dst, tokens, n, shared);
 }
 cudaError_t launch_pages_reserve(const PageState& s, const int32_t* rows, const int32_t* counts, int n, int32_t* positions, int32_t* copies, cudaStream_t st) {
   const int bw = bit_words(s.P, 1);
-  return launch_page_cluster(pages_reserve_kernel, 8, (size_t)bw * 8 + (size_t)n * 20, st, s, rows, counts, n, positions, copies, bw);
+  return launch_page_cluster(pages_reserve_kernel, kStateBlocks, (size_t)bw * 8 + (size_t)n * 20, st, s, rows, counts, n, positions, copies, bw);
 }
 cudaError_t launch_pages_compact(const PageState& s, int32_t* remap, int32_t* moves, int64_t cap, int32_t* count, cudaStream_t st) {
   const int bw = bit_words(s.P, 1);
-  return launch_page_cluster(pages_compact_kernel, 8, (size_t)bw * 8, st, s, remap, moves, cap, count, bw);
+  return launch_page_cluster(pages_compact_kernel, kStateBlocks, (size_t)bw * 8, st, s, remap, moves, cap, count, bw);
 }
 cudaError_t launch_pages_copy(const PagesCopyArgs& a, int vec, cudaStream_t st) {
   const int64_t work = a.n * a.pieces, most = (int64_t)sm_count() * 8;
   const dim3 grid((unsigned)(work < most ? work : most));
   switch (vec) {
-    case 16: return launch_kernel(pages_copy_kernel<uint4>, grid, dim3(256), 0, st, a);
-    case 4: return launch_kernel(pages_copy_kernel<uint32_t>, grid, dim3(256), 0, st, a);
-    case 2: return launch_kernel(pages_copy_kernel<uint16_t>, grid, dim3(256), 0, st, a);
-    default: return launch_kernel(pages_copy_kernel<uint8_t>, grid, dim3(256), 0, st, a);
+    case 16: return launch_behind(pages_copy_kernel<uint4>, grid, 256, 1, 0, st, a);
+    case 4: return launch_behind(pages_copy_kernel<uint32_t>, grid, 256, 1, 0, st, a);
+    case 2: return launch_behind(pages_copy_kernel<uint16_t>, grid, 256, 1, 0, st, a);
+    default: return launch_behind(pages_copy_kernel<uint8_t>, grid, 256, 1, 0, st, a);
   }
 }
 int pages_copy_piece() { return kCopyPiece; }

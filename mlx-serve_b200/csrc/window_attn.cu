@@ -7,8 +7,9 @@
 // One CTA of 12 warps takes two tiles of 128 queries that read the same keys: two heads of a group where the group is even, else
 // two neighbouring tiles of one head.
 //   warps 0-3, 4-7 : the softmax of a tile, a thread a row.  Scores come from tensor memory, the probabilities go back in their place as
-//                    bf16, the A operand of the second product.  r follows the row's maximum only when it has fallen 2^8 behind, so the
-//                    result is rescaled in the first steps of a row and hardly ever after.
+//                    bf16, the A operand of the second product.  Blocks that all queries see whole are taken with the reference r as it
+//                    is, without looking for their maximum first; only where a block's sum passes 2^24 (and in masked blocks, where
+//                    the maximum is found anyway and r may lie 2^8 below it) r moves and the result is rescaled.
 //   warp 8         : copies (TMA): both query tiles once, then keys and values of 128 tokens in a ring.
 //   warp 9         : issues the matrix products, S = Q K^T of the next step behind P V of this one, the tiles in turn: while one
 //                    tile's softmax runs, the tensor cores work for the other.
@@ -16,6 +17,13 @@
 //                    some query, rows that no query of the CTA sees are zeroed, and rows with anything not finite are zeroed and
 //                    noted; the queries that see such a row give NaN.
 // Blocks of 128 keys that no query of a tile sees are left out; only those cut by a border of the mask are masked element by element.
+// Where there are few tiles, clusters share a tile's keys and join their sums through distributed shared memory.
+//
+// Floor: 4 D operations per visible pair on the tensor cores.  32 heads of 128, 16384 tokens, window 4096: 0.96 TFLOP, 589 us at 1634
+// TFLOP/s, takes 811 us (1.19 PFLOP/s, 0.73 of the measured peak).  A step of a tile is a chain: softmax of 128 keys 1400 cycles, P V and
+// S 512 each, 450 of hand-over; the other tile fills part of it, and the tensor cores work for 2048 of every 3100 cycles.  Tried and
+// not kept: 16 softmax warps (845 us), scores in halves of 64 keys made ahead (1040: a product of 64 columns takes as long as
+// one of 128), an issuer for each tile (870: they fall into step and wait together), the first half of P handed over early (862).
 #include <mutex>
 #include <type_traits>
 
@@ -45,6 +53,7 @@ struct WindowK {
   const int32_t* kv_lens;
   int B, Hq, gqa, Tq, Tk, window, sinks;
   int qblocks, heads2;                 // 1: the two tiles are two heads; 0: two tiles of one head
+  int split;                           // CTAs of a cluster that share the keys of the tiles (1, 2, 4, 8)
   int mul[3][2];                       // coordinates along (head, sequence) of q, k, v: 0 where the tensor is broadcast
   float c;
   int o_vec;                           // result rows can be stored 16 bytes at a time
@@ -73,6 +82,11 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
       "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
       : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
 }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -127,7 +141,8 @@ struct Plan {
   int lo, hi;               // keys [lo, hi] and the sinks are all that the CTA sees
   int window, sinks;
   int front, skip, blocks;  // blocks [0, front), then i + skip
-  __device__ __forceinline__ int block(int i) const { return i < front ? i : i + skip; }
+  int from;                 // of these, the ones from here on are this CTA's (`blocks` of them)
+  __device__ __forceinline__ int block(int i) const { return i + from < front ? i + from : i + from + skip; }
   __device__ __forceinline__ bool needs(int t, int blk) const {       // some query of tile t sees some key of the block
     const int k0 = blk * kTile, lo_t = t ? p_lo[1] : p_lo[0], hi_t = t ? p_hi[1] : p_hi[0];
     const int first = lo_t > 0 ? lo_t : 0;
@@ -140,7 +155,7 @@ struct Plan {
   __device__ __forceinline__ bool masked(int blk) const { return (needs(0, blk) && !whole(0, blk)) || (needs(1, blk) && !whole(1, blk)); }
 };
 
-__device__ __forceinline__ Plan make_plan(const WindowK& a, int b, int row0) {
+__device__ __forceinline__ Plan make_plan(const WindowK& a, int b, int row0, int rank) {
   Plan p;
   int len = a.kv_lens ? a.kv_lens[b] : a.Tk;
   len = len < 0 ? 0 : (len > a.Tk ? a.Tk : len);
@@ -163,7 +178,9 @@ __device__ __forceinline__ Plan make_plan(const WindowK& a, int b, int row0) {
   p.front = (p.sinks + kTile - 1) / kTile;
   p.skip = p.lo / kTile - p.front;
   if (p.skip < 0) p.skip = 0;
-  p.blocks = nb - p.skip;
+  const int all = nb - p.skip, each = all / a.split, rest = all - each * a.split;
+  p.from = each * rank + (rank < rest ? rank : rest);
+  p.blocks = each + (rank < rest ? 1 : 0);
   return p;
 }
 
@@ -197,12 +214,13 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
 
   // ---- which tiles: the longest rows of the prompt first ----
   const int per_q = (a.heads2 ? a.Hq / 2 : a.Hq) * a.B;
-  const int qb = a.qblocks - 1 - (int)blockIdx.x / per_q;
-  int rem = (int)blockIdx.x % per_q;
+  const int rank = a.split > 1 ? (int)cluster_rank_tc() : 0, unit = a.split > 1 ? (int)blockIdx.x / a.split : (int)blockIdx.x;
+  const int qb = a.qblocks - 1 - unit / per_q;
+  const int rem = unit % per_q;
   const int b = rem / (per_q / a.B), hu = rem % (per_q / a.B);
   const int head0 = a.heads2 ? 2 * hu : hu, head1 = a.heads2 ? head0 + 1 : head0, hk = head0 / a.gqa;
   const int row0 = qb * (a.heads2 ? kTile : 2 * kTile), row1 = a.heads2 ? row0 : row0 + kTile;
-  const Plan plan = make_plan(a, b, row0);
+  const Plan plan = make_plan(a, b, row0, rank);
 
   if (tid >= 32 && tid < 32 + kNotes) note_bits[tid - 32] = 0u;
   if (tid == 0) {
@@ -257,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       Plan pl;
 #pragma unroll
       for (int t = 0; t < 2; ++t) { pl.p_lo[t] = U(plan.p_lo[t]); pl.p_hi[t] = U(plan.p_hi[t]); }
-      pl.window = U(plan.window); pl.sinks = U(plan.sinks); pl.front = U(plan.front); pl.skip = U(plan.skip); pl.blocks = U(plan.blocks);
+      pl.window = U(plan.window); pl.sinks = U(plan.sinks); pl.front = U(plan.front); pl.skip = U(plan.skip); pl.from = U(plan.from); pl.blocks = U(plan.blocks);
       const uint32_t tm = (uint32_t)U((int)tmem), slot = SH::BYTES >> 4;
       const uint64_t hi_k = make_desc(0) & 0xFFFFFFFF00000000ull, hi_v = make_desc_mn(0) & 0xFFFFFFFF00000000ull;
       const uint32_t q_d = (uint32_t)U((int)(uint32_t)make_desc(smem_u32(smem))), k_d = (uint32_t)U((int)(uint32_t)make_desc(ring)),
@@ -378,6 +396,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       }
       if (!ok && lane == 0 && !s_fail) failed(503);
     }
+    __syncwarp();
+    if (a.split > 1) { cluster_sync_tc(); cluster_sync_tc(); }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax: a thread a row ----
@@ -500,49 +520,127 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
     if (ok && done > 0) ok = __all_sync(0xffffffffu, spin_cta(&o_done[t], (uint32_t)(done - 1) & 1));
     fence_after();
     if (!ok && lane == 0 && !s_fail) failed(504);
-    float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+    bool poisoned = false;
     const int notes = *(volatile int*)&noted;
     for (int i = 0; i < notes && i < kNotes; ++i)
       for (uint32_t m = *(volatile uint32_t*)&note_bits[i]; m; m &= m - 1) {
         const int key = *(volatile int*)&note_key[i] + __ffs(m) - 1;
-        if (key <= pos && (plan.window == 0 || key > pos - plan.window || key < plan.sinks)) inv = __uint_as_float(0x7fc00000u);
+        poisoned |= key <= pos && (plan.window == 0 || key > pos - plan.window || key < plan.sinks);
       }
-    // The results go through shared memory, in the place of the warp's own queries, so that a store covers whole rows (a thread a
-    // row, 32 rows a store, took 5000 cycles); 16-byte chunks swizzled by the row.
-    unsigned char* const stage = smem + t * SH::BYTES + (warp & 3) * (32 * D * 2);
-    constexpr int CH = D / 8;
+    if (a.split > 1) {
+      // Every CTA of the cluster takes 256 / split rows of the two tiles.  The sums are laid out in the CTA's own ring, and read by the others a row a warp (written to the others a row a thread, 16 bytes at a time, they took
+      // 40 us).
+      const int r_all = t * kTile + in_tile;
+      if (poisoned) ref = __uint_as_float(0x7fc00000u);
+      __syncwarp();
+      unsigned char* const sums = smem + 2 * SH::BYTES;
+      float2* const stats = (float2*)(sums + 2 * kTile * D * 4);
+      asm volatile("bar.sync 1, 256;" ::: "memory");         // (the other tile is done with the ring, too)
 #pragma unroll 1
-    for (int q = 0; q < D / 32; ++q) {
-      uint32_t o[32];
-      if (done > 0) {
-        tmem_ld32(o_at + 32 * q, o);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      } else {
+      for (int q = 0; q < D / 32; ++q) {
+        uint32_t o[32];
+        if (done > 0) {
+          tmem_ld32(o_at + 32 * q, o);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = 0u;
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          *(uint4*)(sums + r_all * (D * 4) + (((8 * q + c) ^ (r_all & 7)) << 4)) = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
       }
+      stats[r_all] = make_float2(ref, l);
+      __syncwarp();
+      cluster_sync_tc();
+      // out = (sum o_s w_s) / (sum l_s w_s), w_s = 2^(r_s - max r): 4 values of a row a thread
+      const uint32_t sums_a = smem_u32(sums), stats_a = smem_u32(stats);
+      constexpr int CQ = D / 4;
+      auto join = [&](auto split_c) {                        // 16 pieces asked for at a time
+        constexpr int S = decltype(split_c)::value, kItems = 16 / S, kRows = 2 * kTile / S;
+        float2* const got = stats + 2 * kTile;               // [rank][row] of this CTA's rows
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(got[tid].x), "=f"(got[tid].y)
+                     : "r"(cluster_addr(stats_a + (uint32_t)(rank * kRows + tid % kRows) * 8u, (uint32_t)(tid / kRows))));
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll 1
+        for (int i0 = tid; i0 < kRows * CQ; i0 += 2 * kTile * kItems) {
+          float4 x[kItems][S];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t w[4];
+          for (int j = 0; j < kItems; ++j) {
+            const int i = i0 + j * 2 * kTile, mine = rank * kRows + (i < kRows * CQ ? i / CQ : 0), c = i % CQ;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = pack2(__uint_as_float(o[8 * c + 2 * i]) * inv, __uint_as_float(o[8 * c + 2 * i + 1]) * inv);
-        *(uint4*)(stage + lane * (D * 2) + (((4 * q + c) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int k = 0; k < S; ++k) {
+              asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[j][k].x), "=f"(x[j][k].y), "=f"(x[j][k].z), "=f"(x[j][k].w)
+                           : "r"(cluster_addr(sums_a + (uint32_t)(mine * (D * 4) + ((c ^ (mine & 7)) << 4)), (uint32_t)k)));
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < kItems; ++j) {
+            const int i = i0 + j * 2 * kTile, r = i / CQ, c = i % CQ, mine = rank * kRows + r, tt = mine / kTile, rr = (tt ? row1 : row0) + mine - tt * kTile;
+            if (i >= kRows * CQ || rr >= a.Tq) continue;
+            float top = -INFINITY, L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+            float2 rl[S];
+#pragma unroll
+            for (int k = 0; k < S; ++k) { rl[k] = got[k * kRows + r]; top = fmaxf(top, rl[k].x); }
+#pragma unroll
+            for (int k = 0; k < S; ++k)
+              if (!(rl[k].x == -INFINITY)) {                 // (nothing was seen there)
+                const float w = ex2f(rl[k].x - top);
+                L = fmaf(rl[k].y, w, L);
+                o[0] = fmaf(x[j][k].x, w, o[0]); o[1] = fmaf(x[j][k].y, w, o[1]); o[2] = fmaf(x[j][k].z, w, o[2]); o[3] = fmaf(x[j][k].w, w, o[3]);
+              }
+            const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+            uint16_t* p = a.out + (int64_t)b * a.o_str[0] + (int64_t)(tt ? head1 : head0) * a.o_str[1] + (int64_t)rr * a.o_str[2] + 4 * c;
+            const uint32_t w0 = pack2(o[0] * inv, o[1] * inv), w1 = pack2(o[2] * inv, o[3] * inv);
+            if (a.o_vec) *(uint2*)p = make_uint2(w0, w1);
+            else { p[0] = (uint16_t)w0; p[1] = (uint16_t)(w0 >> 16); p[2] = (uint16_t)w1; p[3] = (uint16_t)(w1 >> 16); }
+          }
+        }
+      };
+      if (a.split == 2) join(std::integral_constant<int, 2>{});
+      else if (a.split == 4) join(std::integral_constant<int, 4>{});
+      else join(std::integral_constant<int, 8>{});
+      __syncwarp();
+      cluster_sync_tc();                                     // (shared memory stays until all have read it)
+    } else {
+      const float inv = poisoned ? __uint_as_float(0x7fc00000u) : (l > 0.f ? 1.f / l : (l == l ? 0.f : l));
+      // The results go through shared memory, in the place of the warp's own queries, so that a store covers whole rows (a thread a
+      // row, 32 rows a store, took 5000 cycles); 16-byte chunks swizzled by the row.
+      unsigned char* const stage = smem + t * SH::BYTES + (warp & 3) * (32 * D * 2);
+      constexpr int CH = D / 8;
+#pragma unroll 1
+      for (int q = 0; q < D / 32; ++q) {
+        uint32_t o[32];
+        if (done > 0) {
+          tmem_ld32(o_at + 32 * q, o);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = pack2(__uint_as_float(o[8 * c + 2 * i]) * inv, __uint_as_float(o[8 * c + 2 * i + 1]) * inv);
+          *(uint4*)(stage + lane * (D * 2) + (((4 * q + c) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
       }
-    }
-    __syncwarp();
-    uint16_t* out = a.out + (int64_t)b * a.o_str[0] + (int64_t)(t ? head1 : head0) * a.o_str[1];
-    const int first = row - lane;
+      __syncwarp();
+      uint16_t* out = a.out + (int64_t)b * a.o_str[0] + (int64_t)(t ? head1 : head0) * a.o_str[1];
+      const int first = row - lane;
 #pragma unroll 4
-    for (int i = lane; i < 32 * CH; i += 32) {
-      const int r = i / CH, c = i % CH;
-      if (first + r >= a.Tq) break;
-      const uint4 v = *(const uint4*)(stage + r * (D * 2) + ((c ^ (r & 7)) << 4));
-      uint16_t* p = out + (int64_t)(first + r) * a.o_str[2] + 8 * c;
-      if (a.o_vec) *(uint4*)p = v;
-      else {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      for (int i = lane; i < 32 * CH; i += 32) {
+        const int r = i / CH, c = i % CH;
+        if (first + r >= a.Tq) break;
+        const uint4 v = *(const uint4*)(stage + r * (D * 2) + ((c ^ (r & 7)) << 4));
+        uint16_t* p = out + (int64_t)(first + r) * a.o_str[2] + 8 * c;
+        if (a.o_vec) *(uint4*)p = v;
+        else {
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) { p[2 * k] = (uint16_t)w[k]; p[2 * k + 1] = (uint16_t)(w[k] >> 16); }
+          for (int k = 0; k < 4; ++k) { p[2 * k] = (uint16_t)w[k]; p[2 * k + 1] = (uint16_t)(w[k] >> 16); }
+        }
       }
     }
   }
@@ -594,6 +692,33 @@ template <int D> cudaError_t launch_d(const WindowArgs& w, cudaStream_t st) {
     }
   }
   const int64_t ctas = (int64_t)a.qblocks * (a.heads2 ? a.Hq / 2 : a.Hq) * a.B;
+  // Where the tiles leave SMs without work, clusters share a tile's keys, as many CTAs as there are SMs for.  To join them takes as long
+  // as some five blocks, so it has to save more than that: 16 CTAs of 64 blocks (64 queries, 8192 keys) take 115 us alone and 55
+  // in clusters of 8; 64 CTAs of 11 blocks (512 queries, a window of 1024) take 34 us either way and stay alone.
+  const int64_t rows = a.heads2 ? kTile : 2 * kTile;
+  int64_t most = (w.Tk + kTile - 1) / kTile;
+  if (w.window > 0) {
+    const int64_t seen = (w.window + rows + kTile - 2) / kTile + 1 + (w.sinks + kTile - 1) / kTile;
+    most = most < seen ? most : seen;
+  }
+  a.split = 8;
+  while (a.split > 1 && (ctas * a.split > sm_count() || most - most / a.split < 8)) a.split /= 2;
+  if (a.split > 1) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(ctas * a.split));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Shape<D>::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)a.split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = launch_clusters(cfg, kern, m[0], m[1], m[2], a);
+    if (e == cudaSuccess) return e;
+    (void)cudaGetLastError();            // the device places no clusters: every tile by itself
+    a.split = 1;
+  }
   return launch_kernel(kern, dim3((unsigned)ctas), dim3(kThreads), Shape<D>::SMEM, st, m[0], m[1], m[2], a);
 }
 }  // namespace

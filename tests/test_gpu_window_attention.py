@@ -64,6 +64,19 @@ def test_window_and_sinks(D, gqa, window, sinks, Tq, Tk):
     check(qb200.window_attention(q, k, v, D ** -0.5, window=window, sinks=sinks), q, k, v, D ** -0.5, window, sinks)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,Hq,Hkv,Tq,Tk,window,sinks", [(1, 2, 1, 1, 5000, 0, 0), (1, 4, 4, 130, 3000, 0, 0), (1, 8, 2, 300, 4099, 1024, 4), (3, 2, 1, 100, 2000, 700, 200)])
+@pytest.mark.parametrize("clusters", [True, False])
+def test_tiles_whose_keys_several_blocks_share(D, B, Hq, Hkv, Tq, Tk, window, sinks, clusters, request):
+    if not clusters:
+        request.getfixturevalue("no_clusters")
+    q, k, v = make(B, Hq, Hkv, Tq, Tk, D, Tq)
+    lens = None if B == 1 else [2000, 55, 0]
+    out = qb200.window_attention(q, k, v, D ** -0.5, window=window, sinks=sinks, kv_lens=None if lens is None else torch.tensor(lens, dtype=I32, device="cuda"))
+    check(out, q, k, v, D ** -0.5, window, sinks, lens)
+    assert qb200.lib().qb200_debug_tc_status() == 0
+
+
 def test_a_long_prompt():
     q, k, v = make(1, 4, 2, 3000, 5000, 128)
     for window, sinks in ((0, 0), (1024, 4)):
@@ -97,6 +110,7 @@ def test_what_is_not_finite_shows_where_it_is_seen_and_nowhere_else(D, gqa):
     # (in blocks that a query sees whole the value itself comes through, so only that it is not finite is asked of all channels together)
     fine = torch.where(torch.isfinite(out).all(-1, keepdim=True), out, torch.full_like(out, float("nan")))
     check(fine, q, torch.nan_to_num(k), clean, 0.1, window, sinks, poisoned=poisoned)
+    assert qb200.lib().qb200_debug_tc_status() == 0
     k2 = torch.nan_to_num(k)
     k2[0, 1, 333, 3] = float("nan")
     out = qb200.window_attention(q, k2, clean, 0.1, window=window, sinks=sinks)
