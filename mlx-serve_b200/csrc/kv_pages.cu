@@ -369,16 +369,18 @@ __global__ void __launch_bounds__(kPageThreads) pages_compact_kernel(PageState s
 }
 
 // ---------------------------------------------------------------- copying pages
-// Pair by pair, pool by pool, in pieces of at most 8 KB: a block of 256 threads copies two vectors a thread.
-constexpr int kCopyPiece = 8192;
+// Pair by pair, pool by pool, in pieces that a warp copies with four vectors a lane: pages of codes have many, those of scales one or
+// two, and no warp waits for another's.
+constexpr int kCopyPiece = 2048;
 
 template <typename V>
 __global__ void __launch_bounds__(256) pages_copy_kernel(const __grid_constant__ PagesCopyArgs a) {
   grid_wait();
   const int64_t n = a.count ? min((int64_t)(*a.count > 0 ? *a.count : 0), a.n) : a.n;
   const int64_t work = n * a.pieces;
-  for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
-    const int64_t pair = w / a.pieces;
+  const int lane = threadIdx.x & 31;
+  for (int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); w < work; w += (int64_t)gridDim.x * 8) {
+    const int64_t pair = work <= 0x7fffffff ? (int64_t)((uint32_t)w / (uint32_t)a.pieces) : w / a.pieces;
     const int piece = (int)(w - pair * a.pieces);
     const int64_t src = a.pairs[2 * pair], dst = a.pairs[2 * pair + 1];
     if (src < 0 || src >= a.P || dst < 0 || dst >= a.P || src == dst) continue;
@@ -391,7 +393,7 @@ __global__ void __launch_bounds__(256) pages_copy_kernel(const __grid_constant__
     const char* from = p.base + src * p.page_str;
     char* to = p.base + dst * p.page_str;
     const uint32_t at = (uint32_t)(piece - p.first_piece) * kCopyPiece, left = p.bytes - at;
-    constexpr int kVecs = kCopyPiece / 256 / (int)sizeof(V);
+    constexpr int kVecs = kCopyPiece / 32 / (int)sizeof(V);
     constexpr int kBatch = kVecs < 8 ? kVecs : 8;
 #pragma unroll 1
     for (int k0 = 0; k0 < kVecs; k0 += kBatch) {
@@ -399,7 +401,7 @@ __global__ void __launch_bounds__(256) pages_copy_kernel(const __grid_constant__
       int64_t off[kBatch];
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
-        const uint32_t o = ((k0 + k) * 256 + threadIdx.x) * (uint32_t)sizeof(V);
+        const uint32_t o = ((k0 + k) * 32 + lane) * (uint32_t)sizeof(V);
         off[k] = -1;
         if (o < left) {
           uint32_t e = at + o;
@@ -478,7 +480,7 @@ cudaError_t launch_pages_compact(const PageState& s, int32_t* remap, int32_t* mo
   return launch_page_cluster(pages_compact_kernel, kStateBlocks, (size_t)bw * 8, st, s, remap, moves, cap, count, bw);
 }
 cudaError_t launch_pages_copy(const PagesCopyArgs& a, int vec, cudaStream_t st) {
-  const int64_t work = a.n * a.pieces, most = (int64_t)sm_count() * 8;
+  const int64_t work = (a.n * a.pieces + 7) / 8, most = (int64_t)sm_count() * 8;   // eight warps a block
   const dim3 grid((unsigned)(work < most ? work : most));
   switch (vec) {
     case 16: return launch_behind(pages_copy_kernel<uint4>, grid, 256, 1, 0, st, a);
