@@ -106,3 +106,15 @@ pub extern "c" fn qb200_rope_kv_append_seqs(q: *Tensor, dims: c_int, base: f32, 
 // TurboState's Hadamard rotation of the given seed (0x9E37 ^ layer for K, 0x85EB ^ layer for V) instead of an mlx_matmul by the [D, D] matrix
 pub extern "c" fn qb200_turbo_rotate(res: *Tensor, x: *const Tensor, seed: u64, s: Stream) c_int;
 pub extern "c" fn qb200_turbo_signs(seed: u64, n: c_int, bits: [*]u32) c_int;
+
+// the paged key-value cache (no counterpart in the reference): empty optional tensors are null
+pub extern "c" fn qb200_kv_pages_append(k_q: *Tensor, k_scales: ?*Tensor, k_biases: ?*Tensor, v_q: *Tensor, v_scales: ?*Tensor, v_biases: ?*Tensor, dense_k: *const Tensor, dense_v: *const Tensor, table: *const Tensor, rows: ?*const Tensor, positions: *const Tensor, counts: ?*const Tensor, bits: c_int, group_size: c_int, s: Stream) c_int;
+pub extern "c" fn qb200_kv_pages_free(table: *Tensor, lens: *Tensor, refs: *Tensor, page: c_int, rows: *const Tensor, begin: ?*const Tensor, end: ?*const Tensor, s: Stream) c_int;
+pub extern "c" fn qb200_kv_pages_fork(shared: *Tensor, table: *Tensor, lens: *Tensor, refs: *Tensor, page: c_int, src: *const Tensor, dst: *const Tensor, tokens: ?*const Tensor, s: Stream) c_int;
+pub extern "c" fn qb200_kv_pages_reserve(positions: *Tensor, copies: *Tensor, table: *Tensor, lens: *Tensor, refs: *Tensor, page: c_int, rows: *const Tensor, counts: *const Tensor, s: Stream) c_int;
+pub extern "c" fn qb200_kv_pages_compact(remap: *Tensor, moves: *Tensor, count: *Tensor, table: *Tensor, refs: *Tensor, s: Stream) c_int;
+pub extern "c" fn qb200_kv_pages_copy(pools: [*]const *Tensor, num_pools: c_int, pairs: *const Tensor, count: ?*const Tensor, s: Stream) c_int;
+pub extern "c" fn qb200_kv_pages_decode_attention(res: *Tensor, q: *const Tensor, k_q: *const Tensor, k_scales: ?*const Tensor, k_biases: ?*const Tensor, v_q: *const Tensor, v_scales: ?*const Tensor, v_biases: ?*const Tensor, table: *const Tensor, rows: ?*const Tensor, lens: *const Tensor, bits: c_int, group_size: c_int, scale: f32, window: i64, sinks: i64, workspace: ?*anyopaque, workspace_bytes: usize, s: Stream) c_int;
+pub extern "c" fn qb200_kv_pages_decode_attention_workspace_size(B: i64, Hq: i64, Hkv: i64, D: i64) usize;
+// mlx_fast_scaled_dot_product_attention of a prompt (src/mlx.zig:325) with a sliding window and sinks
+pub extern "c" fn qb200_window_attention(res: *Tensor, q: *const Tensor, k: *const Tensor, v: *const Tensor, scale: f32, window: i64, sinks: i64, kv_lens: ?*const Tensor, s: Stream) c_int;

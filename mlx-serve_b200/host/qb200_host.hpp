@@ -13,6 +13,9 @@
 //   rmsNorm, addRmsNorm, ropeDynamic, computeGeglu, updateAffineBatched   src/transformer.zig:7770-7779, :9678, :8220-8243, :9738-9756
 //   rotateLastDim, quantizeTurbo, dequantizeTurbo   src/kv_quant.zig:362-403
 //   saveChunk / restoreChunk (chunk files of the prefix cache's SSD tier)   src/kv_disk_cache.zig:320-440, :1062-1074
+//   PagedCache: pagesReserve, pagesAppend, pagesFork, pagesFree, pagesCompact, pagesCopy, quantAttentionPaged   no counterpart: slots own
+//                                            one capacity buffer per layer there (src/scheduler.zig:463-480)
+//   windowAttention (dense attention of a prompt with a sliding window)   src/mlx.zig:325
 //   Checkpoint (safetensors triples, f16 narrowing, geometry)   src/model.zig:3030-3061, :3241-3256; src/transformer.zig:16763-16790
 //   moeBlockEp (moeMLP2 over several GPUs; define QB200_HOST_WITH_EP and link libqb200_ep)   src/transformer.zig:14945-15140
 //
@@ -261,6 +264,60 @@ inline void ropeUpdateAffineBatched(Array& q, int dims, float base, float scale,
   check(qb200_rope_kv_append_seqs(&q.t, dims, base, scale, &p[0], &p[slots], &p[2 * slots], &p[3 * slots], &p[4 * slots], &p[5 * slots],
                                   &k_new.t, &v_new.t, offs.data(), slots, entries[0]->keys.bits, entries[0]->keys.group_size, s));
   for (int n = 0; n < slots; ++n) entries[n]->offset += 1;
+}
+
+// ---- a paged cache: one table for all layers, a pool of pages per layer ----
+// `keys` and `values` are the pools [pages, Hkv, page, .] of one layer (scales and biases empty at bits == 16); the state tensors live
+// on the device and are changed there.
+struct PagePool {
+  QuantizedKV keys, values;
+};
+struct PagedCache {
+  Array table, lens, refs;   // [sequences, M], [sequences], [pages]: int32
+  int page = 64;             // tokens of a page
+  std::vector<PagePool> layers;
+};
+// Room for counts[n] more tokens in sequence rows[n]; a half-filled page that others read too is copied in every layer.
+inline void pagesCopy(PagedCache& c, const Array& pairs, const Array* count, qb200_stream s) {
+  std::vector<qb200_tensor*> pools;
+  for (PagePool& l : c.layers)
+    for (QuantizedKV* kv : {&l.keys, &l.values})
+      for (Array* a : {&kv->q, &kv->scales, &kv->biases})
+        if (a->t.data) pools.push_back(&a->t);
+  check(qb200_kv_pages_copy(pools.data(), (int)pools.size(), &pairs.t, count ? &count->t : nullptr, s));
+}
+inline void pagesReserve(PagedCache& c, Array& positions, Array& copies, const Array& rows, const Array& counts, qb200_stream s) {
+  check(qb200_kv_pages_reserve(&positions.t, &copies.t, &c.table.t, &c.lens.t, &c.refs.t, c.page, &rows.t, &counts.t, s));
+  pagesCopy(c, copies, nullptr, s);
+}
+inline void pagesAppend(PagedCache& c, int layer, const Array& k_new, const Array& v_new, const Array* rows, const Array& positions, const Array* counts,
+                        qb200_stream s) {
+  PagePool& l = c.layers[(size_t)layer];
+  check(qb200_kv_pages_append(&l.keys.q.t, &l.keys.scales.t, &l.keys.biases.t, &l.values.q.t, &l.values.scales.t, &l.values.biases.t, &k_new.t, &v_new.t,
+                              &c.table.t, rows ? &rows->t : nullptr, &positions.t, counts ? &counts->t : nullptr, l.keys.bits, l.keys.group_size, s));
+}
+inline void pagesFork(PagedCache& c, Array& shared, const Array& src, const Array& dst, const Array* tokens, qb200_stream s) {
+  check(qb200_kv_pages_fork(&shared.t, &c.table.t, &c.lens.t, &c.refs.t, c.page, &src.t, &dst.t, tokens ? &tokens->t : nullptr, s));
+}
+inline void pagesFree(PagedCache& c, const Array& rows, const Array* begin, const Array* end, qb200_stream s) {
+  check(qb200_kv_pages_free(&c.table.t, &c.lens.t, &c.refs.t, c.page, &rows.t, begin ? &begin->t : nullptr, end ? &end->t : nullptr, s));
+}
+inline void pagesCompact(PagedCache& c, Array& remap, Array& moves, Array& count, qb200_stream s) {
+  check(qb200_kv_pages_compact(&remap.t, &moves.t, &count.t, &c.table.t, &c.refs.t, s));
+  pagesCopy(c, moves, &count, s);
+}
+inline size_t quantAttentionPagedWorkspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) { return qb200_kv_pages_decode_attention_workspace_size(B, Hq, Hkv, D); }
+inline void quantAttentionPaged(Array& out, const Array& q, const PagedCache& c, int layer, const Array* rows, float scale, int64_t window, int64_t sinks,
+                                void* workspace, size_t workspace_bytes, qb200_stream s) {
+  const PagePool& l = c.layers[(size_t)layer];
+  check(qb200_kv_pages_decode_attention(&out.t, &q.t, &l.keys.q.t, &l.keys.scales.t, &l.keys.biases.t, &l.values.q.t, &l.values.scales.t, &l.values.biases.t,
+                                        &c.table.t, rows ? &rows->t : nullptr, &c.lens.t, l.keys.bits, l.keys.group_size, scale, window, sinks, workspace,
+                                        workspace_bytes, s));
+}
+// Causal attention of a prompt (or a chunk behind cached tokens) with a sliding window and a few first tokens that stay visible.
+inline void windowAttention(Array& out, const Array& q, const Array& k, const Array& v, float scale, int64_t window, int64_t sinks, const Array* kv_lens,
+                            qb200_stream s) {
+  check(qb200_window_attention(&out.t, &q.t, &k.t, &v.t, scale, window, sinks, kv_lens ? &kv_lens->t : nullptr, s));
 }
 
 // rmsNorm / rmsNormEps (src/transformer.zig:7770-7779) and the mlx_add that precedes the post-attention and the next

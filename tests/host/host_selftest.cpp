@@ -231,6 +231,66 @@ int main(int argc, char** argv) {
       ok = gate(f32_of(to_host((uint16_t*)out.t.data, (size_t)(B * Hq * D))), ref, 1e-2, "updateAffine + quantAttention") && ok;
     }
 
+    // ---- the paged cache: reserve, append, fork, a token each, attention over pages; and the prompt attention's last position ----
+    {
+      const int64_t H = 2, Hq = 8, D = 128, page = 32, M = 8, P = 20, S = 3, T = 75;
+      PagedCache c;
+      c.page = (int)page;
+      c.table = Array(to_dev(std::vector<int32_t>((size_t)(S * M), -1)), QB200_INT32, {S, M});
+      c.lens = Array(to_dev(std::vector<int32_t>((size_t)S, 0)), QB200_INT32, {S});
+      c.refs = Array(to_dev(std::vector<int32_t>((size_t)P, 0)), QB200_INT32, {P});
+      c.layers.resize(1);
+      for (QuantizedKV* kv : {&c.layers[0].keys, &c.layers[0].values}) {
+        kv->q = Array(dev_alloc<uint32_t>((size_t)(P * H * page * D / 8)), QB200_UINT32, {P, H, page, D / 8});
+        kv->scales = Array(dev_alloc<uint16_t>((size_t)(P * H * page * 2)), QB200_BFLOAT16, {P, H, page, 2});
+        kv->biases = Array(dev_alloc<uint16_t>((size_t)(P * H * page * 2)), QB200_BFLOAT16, {P, H, page, 2});
+        kv->group_size = 64; kv->bits = 4;
+      }
+      std::vector<float> kd = rand_bf16((size_t)(H * (T + 1) * D), 1.0f), vd = rand_bf16((size_t)(H * (T + 1) * D), 1.0f);
+      auto rows = [&](const std::vector<float>& src, int64_t t0, int64_t n) {
+        std::vector<float> out((size_t)(H * n * D));
+        for (int64_t h = 0; h < H; ++h) std::memcpy(&out[(size_t)(h * n * D)], &src[(size_t)((h * (T + 1) + t0) * D)], sizeof(float) * (size_t)(n * D));
+        return out;
+      };
+      auto list = [&](std::vector<int32_t> v) { return Array(to_dev(v), QB200_INT32, {(int64_t)v.size()}); };
+      Array pos = list({0}), copies(dev_alloc<int32_t>(2), QB200_INT32, {1, 2}), shared = list({0});
+      Array r0 = list({0}), r2 = list({2}), many = list({(int32_t)T}), one = list({1});
+      pagesReserve(c, pos, copies, r0, many, stream);
+      Array k0(to_dev(bf16_of(rows(kd, 0, T))), QB200_BFLOAT16, {1, H, T, D}), v0(to_dev(bf16_of(rows(vd, 0, T))), QB200_BFLOAT16, {1, H, T, D});
+      pagesAppend(c, 0, k0, v0, &r0, pos, nullptr, stream);
+      pagesFork(c, shared, r0, r2, nullptr, stream);
+      pagesReserve(c, pos, copies, r2, one, stream);
+      Array k1(to_dev(bf16_of(rows(kd, T, 1))), QB200_BFLOAT16, {1, H, 1, D}), v1(to_dev(bf16_of(rows(vd, T, 1))), QB200_BFLOAT16, {1, H, 1, D});
+      pagesAppend(c, 0, k1, v1, &r2, pos, nullptr, stream);
+      std::vector<float> qv = rand_bf16((size_t)(2 * Hq * D), 1.0f);
+      Array dq(to_dev(bf16_of(qv)), QB200_BFLOAT16, {2, Hq, 1, D}), out(dev_alloc<uint16_t>((size_t)(2 * Hq * D)), QB200_BFLOAT16, {2, Hq, 1, D}), both = list({0, 2});
+      const float scale = 1.0f / std::sqrt((float)D);
+      const size_t need = quantAttentionPagedWorkspace(2, Hq, H, D);
+      void* ws = dev_alloc<char>(need);
+      quantAttentionPaged(out, dq, c, 0, &both, scale, 0, 0, ws, need, stream);
+      std::vector<uint32_t> kq((size_t)(H * (T + 1) * D / 8)), vq(kq.size());
+      std::vector<uint16_t> ks((size_t)(H * (T + 1) * 2)), kb(ks.size()), vs(ks.size()), vb(ks.size());
+      qo_quantize(kd.data(), H * (T + 1), D, 64, 4, kq.data(), ks.data(), kb.data());
+      qo_quantize(vd.data(), H * (T + 1), D, 64, 4, vq.data(), vs.data(), vb.data());
+      const int64_t qstr[3] = {0, (T + 1) * (D / 8), D / 8}, sstr[3] = {0, (T + 1) * 2, 2};   // two sequences over the same rows
+      std::vector<int32_t> lens = {(int32_t)T, (int32_t)T + 1};
+      std::vector<float> ref((size_t)(2 * Hq * D));
+      qo_kv_decode_attention(qv.data(), kq.data(), ks.data(), kb.data(), vq.data(), vs.data(), vb.data(), 2, Hq, H, T + 1, D, D, 64, 4, qstr, sstr, qstr, sstr, scale,
+                             lens.data(), nullptr, ref.data());
+      cudaDeviceSynchronize();
+      ok = gate(f32_of(to_host((uint16_t*)out.t.data, (size_t)(2 * Hq * D))), ref, 1e-2, "paged cache: reserve, append, fork, attention") && ok;
+
+      // a prompt of 32 tokens whose every query sees itself alone: its values come back
+      const int64_t n = 32;
+      Array pq(to_dev(bf16_of(rand_bf16((size_t)(Hq * n * D), 1.0f))), QB200_BFLOAT16, {1, Hq, n, D}), po(dev_alloc<uint16_t>((size_t)(Hq * n * D)), QB200_BFLOAT16, {1, Hq, n, D});
+      Array pk(to_dev(bf16_of(rows(kd, 0, n))), QB200_BFLOAT16, {1, H, n, D}), pv(to_dev(bf16_of(rows(vd, 0, n))), QB200_BFLOAT16, {1, H, n, D});
+      windowAttention(po, pq, pk, pv, scale, 1, 0, nullptr, stream);
+      cudaDeviceSynchronize();
+      std::vector<float> want, vals = rows(vd, 0, n);
+      for (int64_t h = 0; h < Hq; ++h) want.insert(want.end(), vals.begin() + (h / (Hq / H)) * n * D, vals.begin() + (h / (Hq / H) + 1) * n * D);
+      ok = gate(f32_of(to_host((uint16_t*)po.t.data, (size_t)(Hq * n * D))), want, 1e-2, "windowAttention") && ok;
+    }
+
     // ---- a declined request surfaces as Declined, not as a crash (src/transformer.zig:20463-20475) ----
     {
       QWeight odd = QWeight{qw.q, qw.scales, qw.biases, 64, 3};   // 3-bit codes are not served
