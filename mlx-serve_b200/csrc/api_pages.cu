@@ -22,11 +22,22 @@ int pg_fail(int status, const char* fmt, ...) {
 int pg_cuda(cudaError_t e, const char* who) { return pg_fail(QB200_ERR_CUDA, "%s: CUDA error %d (%s)", who, (int)e, cudaGetErrorString(e)); }
 bool empty(const qb200_tensor* t) { return t == nullptr || (t->data == nullptr && t->ndim == 0); }
 
-// A tensor of a given rank and dtype whose last axis is contiguous.
+int elem_size(int dtype) {
+  switch (dtype) {
+    case QB200_UINT8: case QB200_INT8: return 1;
+    case QB200_UINT16: case QB200_INT16: case QB200_FLOAT16: case QB200_BFLOAT16: return 2;
+    case QB200_UINT32: case QB200_INT32: case QB200_FLOAT32: return 4;
+    default: return 0;
+  }
+}
+// A tensor of a given rank and dtype, aligned to its elements, whose last axis is contiguous.
 int expect(const qb200_tensor* t, const char* who, const char* name, int ndim, int dtype) {
   if (t == nullptr) return pg_fail(QB200_ERR_BAD_ARG, "%s: %s: null tensor", who, name);
   if (t->ndim != ndim) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: %s must have %d dimensions, not %d", who, name, ndim, t->ndim);
+  if (ndim > QB200_MAX_DIMS) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: %s has %d dimensions", who, name, ndim);
   if (t->dtype != dtype) return pg_fail(QB200_ERR_BAD_DTYPE, "%s: %s has dtype %d, expected %d", who, name, t->dtype, dtype);
+  const int esz = elem_size(dtype);
+  if (esz > 1 && (uintptr_t)t->data % esz) return pg_fail(QB200_ERR_BAD_STRIDE, "%s: %s does not start on its elements' size", who, name);
   int64_t n = 1;
   for (int d = 0; d < ndim; ++d) {
     if (t->shape[d] < 0) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: %s: negative extent in dim %d", who, name, d);
@@ -43,12 +54,23 @@ int expect_list(const qb200_tensor* t, const char* who, const char* name, int64_
   if (t->shape[0] != n) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: %s has %lld entries, expected %lld", who, name, (long long)t->shape[0], (long long)n);
   return 0;
 }
-// Rows that a kernel writes: no two of them may be the same memory.
-bool rows_distinct(const qb200_tensor* t) {
-  for (int d = 0; d < t->ndim; ++d)
+// What a kernel writes: no two elements may be the same memory.  Axes by growing stride, each has to reach over all that the smaller
+// ones span (so layouts in which the axes are nested in any order pass, and those that are not are refused).
+bool distinct(const qb200_tensor* t) {
+  int order[QB200_MAX_DIMS], n = 0;
+  for (int d = 0; d < t->ndim; ++d) {
     if (t->shape[d] == 0) return true;
-  for (int d = 0; d + 1 < t->ndim; ++d)
-    if (t->shape[d] > 1 && t->stride[d] < t->shape[t->ndim - 1]) return false;
+    if (t->shape[d] == 1) continue;
+    int at = n++;
+    for (; at > 0 && t->stride[order[at - 1]] > t->stride[d]; --at) order[at] = order[at - 1];
+    order[at] = d;
+  }
+  int64_t span = 1;
+  for (int i = 0; i < n; ++i) {
+    const int64_t str = t->stride[order[i]], ext = t->shape[order[i]] - 1;
+    if (str < span || str > (INT64_MAX - span) / ext) return false;
+    span += str * ext;
+  }
   return true;
 }
 int page_shift_of(int64_t page) {
@@ -160,7 +182,7 @@ QB200_API int qb200_kv_pages_append(qb200_tensor* k_q, qb200_tensor* k_scales, q
     return st;
   const qb200_tensor* const written[6] = {k_q, k_scales, k_biases, v_q, v_scales, v_biases};
   for (int i = 0; i < 6; ++i)
-    if (!empty(written[i]) && !rows_distinct(written[i])) return pg_fail(QB200_ERR_BAD_STRIDE, "%s: rows of a pool overlap", who);
+    if (!empty(written[i]) && !distinct(written[i])) return pg_fail(QB200_ERR_BAD_STRIDE, "%s: rows of a pool overlap", who);
   if ((st = expect_list(positions, who, "positions", N))) return st;
   if (!empty(rows)) {
     if ((st = expect_list(rows, who, "rows", N))) return st;
@@ -275,15 +297,9 @@ QB200_API int qb200_kv_pages_copy(qb200_tensor* const* pools, int num_pools, con
       for (int i = p0; i < num_pools && i < p0 + kMaxCopyPools; ++i) {
         const qb200_tensor* t = pools[i];
         if (t == nullptr || t->ndim < 1) return pg_fail(QB200_ERR_BAD_ARG, "%s: pool %d is no tensor of pages", who, i);
-        int esz = 0;
-        switch (t->dtype) {
-          case QB200_UINT8: case QB200_INT8: esz = 1; break;
-          case QB200_UINT16: case QB200_INT16: case QB200_FLOAT16: case QB200_BFLOAT16: esz = 2; break;
-          case QB200_UINT32: case QB200_INT32: case QB200_FLOAT32: esz = 4; break;
-          default: return pg_fail(QB200_ERR_BAD_DTYPE, "%s: pool %d has dtype %d", who, i, t->dtype);
-        }
+        const int esz = elem_size(t->dtype);
+        if (esz == 0) return pg_fail(QB200_ERR_BAD_DTYPE, "%s: pool %d has dtype %d", who, i, t->dtype);
         if ((st = expect(t, who, "pool", t->ndim, t->dtype))) return st;
-        if (t->ndim > QB200_MAX_DIMS) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: pool %d has %d dimensions", who, i, t->ndim);
         if (t->shape[0] != pools[0]->shape[0])
           return pg_fail(QB200_ERR_BAD_SHAPE, "%s: pool %d holds %lld pages, pool 0 %lld", who, i, (long long)t->shape[0], (long long)pools[0]->shape[0]);
         // the page's axes from the innermost stride out, neighbours that follow each other taken as one
@@ -310,11 +326,7 @@ QB200_API int qb200_kv_pages_copy(qb200_tensor* const* pools, int num_pools, con
           while (k < nd && str[k] == outer * outer_str) outer *= ext[k++];
         }
         if (k < nd) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: the pages of pool %d lie in more than two levels of strides", who, i);
-        if ((inner > 1 && inner_str < run) || (outer > 1 && outer_str < inner_str * (inner - 1) + run))
-          return pg_fail(QB200_ERR_BAD_STRIDE, "%s: rows of pool %d overlap", who, i);
-        const int64_t extent = (outer - 1) * outer_str + (inner - 1) * inner_str + run;
-        // (pages may lie between each other's rows; a page stride below a run cannot)
-        if (t->shape[0] > 1 && t->stride[0] < extent && t->stride[0] < run) return pg_fail(QB200_ERR_BAD_STRIDE, "%s: pages of pool %d overlap", who, i);
+        if (!distinct(t)) return pg_fail(QB200_ERR_BAD_STRIDE, "%s: pages or rows of pool %d overlap", who, i);
         const int64_t bytes = none ? 0 : run * inner * outer * esz;
         if (bytes > (1ll << 31)) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: pages of %lld bytes are not served", who, (long long)bytes);
         if (bytes == 0) continue;
@@ -377,7 +389,7 @@ QB200_API int qb200_kv_pages_decode_attention(qb200_tensor* res, const qb200_ten
   } else if (ps.S != B) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: %lld queries for a table of %d sequences (pass rows)", who, (long long)B, ps.S);
   if (!(scale >= -3.0e38f && scale <= 3.0e38f)) return pg_fail(QB200_ERR_BAD_ARG, "%s: scale must be finite", who);
   if (window < 0 || sinks < 0) return pg_fail(QB200_ERR_BAD_ARG, "%s: window and sinks must not be negative", who);
-  if (!rows_distinct(res)) return pg_fail(QB200_ERR_BAD_STRIDE, "%s: rows of res overlap", who);
+  if (!distinct(res)) return pg_fail(QB200_ERR_BAD_STRIDE, "%s: rows of res overlap", who);
   if (B == 0 || Hq == 0) return QB200_OK;
   if (P < 1) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: the pool holds no pages", who);
   if (P > INT32_MAX || B > kMaxPageSeqs) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: %lld sequences are not served (at most %d)", who, (long long)B, kMaxPageSeqs);
@@ -434,7 +446,7 @@ QB200_API int qb200_window_attention(qb200_tensor* res, const qb200_tensor* q, c
   if (!empty(kv_lens)) {
     if ((st = expect_list(kv_lens, who, "kv_lens", B))) return st;
   } else if (Tk < Tq) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: %lld queries need as many keys (%lld given)", who, (long long)Tq, (long long)Tk);
-  if (!rows_distinct(res)) return pg_fail(QB200_ERR_BAD_STRIDE, "%s: rows of res overlap", who);
+  if (!distinct(res)) return pg_fail(QB200_ERR_BAD_STRIDE, "%s: rows of res overlap", who);
   if (B == 0 || Hq == 0 || Tq == 0) return QB200_OK;
   if (Tk == 0) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: no keys", who);
   const int64_t lim = (int64_t)1 << 30;

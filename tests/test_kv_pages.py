@@ -157,3 +157,38 @@ def test_the_binding_refuses_host_tensors():
             call()
     with pytest.raises(ValueError):
         q.kv_pages_append(pages[:2], pages, x, x, table, lens, 16)
+
+
+@pytest.mark.parametrize("k", [
+    t(q.UINT32, [6, 2, 32, 16], stride=[512, 512, 16, 1]),          # pages begin on each other's second head
+    t(q.UINT32, [6, 2, 32, 16], stride=[1024, 16, 16, 1]),          # heads begin on each other's second token
+    t(q.UINT32, [6, 2, 32, 16], stride=[1024, 64, 48, 1]),          # axes that are not nested
+    t(q.UINT32, [6, 2, 32, 16], stride=[1 << 62, 1 << 62, 16, 1]),
+])
+def test_overlapping_pools_are_refused(k):
+    assert append(k=[k, *pool()[1:]]) == 3, q.lib().qb200_last_error()
+    assert copy([k]) in (1, 3)
+
+
+def test_interleaved_pages_are_taken():
+    k = t(q.UINT32, [6, 2, 32, 16], stride=[16, 6 * 16 * 32, 6 * 16, 1])       # the pages' rows lie between each other
+    assert append(k=[k, *pool()[1:]], dk=t(BF16, [3, 2, 0, 128])) == 0 and copy([k]) == 0
+
+
+def test_results_that_overlap_are_refused():
+    assert attend(res=t(BF16, [3, 4, 1, 128], stride=[128, 128, 128, 1])) == 3
+    assert q.lib().qb200_window_attention(*ref(t(BF16, [1, 2, 16, 64], stride=[0, 64, 64, 1]), *[t(BF16, [1, 2, 16, 64])] * 3), 0.1, 0, 0, *ref(NONE), None) == 3
+
+
+def test_tensors_off_their_elements_are_refused():
+    L, li, odd, st = q.lib(), t(I32, [2]), t(I32, [2], ptr=0x1002), state()
+    assert L.qb200_kv_pages_free(*ref(*st), 32, *ref(odd, NONE, NONE), None) == 3
+    assert L.qb200_kv_pages_fork(*ref(li, t(I32, [3, 4], ptr=0x1001), *st[1:]), 32, *ref(li, li, NONE), None) == 3
+    assert append(dk=t(BF16, [3, 2, 5, 128], ptr=0x1001)) == 3 and append(pos=t(I32, [3], ptr=0x1002)) == 3
+    assert attend(lens=t(I32, [3], ptr=0x1001)) == 3 and copy([t(BF16, [6, 4], ptr=0x1001)]) == 3
+
+
+def test_a_rank_beyond_the_descriptor_is_refused():
+    d = t(BF16, [6, 4])
+    d.ndim = 100
+    assert copy([d]) == 2
