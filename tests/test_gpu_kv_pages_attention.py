@@ -255,3 +255,53 @@ def test_replayed_graphs_streams_and_repeated_calls():
                 call(other, ws[1])
         torch.cuda.synchronize()
         assert torch.equal(again.view(torch.int16), out.view(torch.int16)) and torch.equal(other.view(torch.int16), out.view(torch.int16))
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_pages_far_apart(bits):
+    """Pages half a gigabyte apart: written, copied and read at offsets beyond 32 bits, of elements and of bytes."""
+    torch.manual_seed(8)
+    P, H, page, D, lens = 20, 2, 32, 128, [200, 77, 64]
+
+    def far(shape, dtype):
+        stride = 2 ** 29 // dtype.itemsize
+        inner = shape[1] * shape[2] * shape[3]
+        flat = torch.empty((P - 1) * stride + inner, dtype=dtype, device="cuda")
+        return flat.as_strided(shape, [stride, shape[2] * shape[3], shape[3], 1])
+
+    def pool():
+        if bits == 16:
+            p = (far([P, H, page, D], BF16), None, None)
+        else:
+            p = (far([P, H, page, D * bits // 32], I32), far([P, H, page, D // 64], BF16), far([P, H, page, D // 64], BF16))
+        for x in p:
+            if x is not None:
+                x.zero_()
+        return p
+
+    kp, vp = pool(), pool()
+    table = [[19, 0, 17, 3, 18, 9, 15], [12, 14, 16] + [-1] * 4, [13, 11] + [-1] * 5]
+    dense = [torch.randn(3, H, 200, D, device="cuda").to(BF16) for _ in range(2)]
+    qb200.kv_pages_append(kp, vp, *dense, ints(table), ints([0, 0, 0]), bits, counts=ints(lens))
+    qb200.kv_pages_copy([x for x in (*kp, *vp) if x is not None], ints([[19, 1], [0, 10], [16, 8]]))
+    table[0][0], table[0][1], table[1][2] = 1, 10, 8
+    q, out = run(kp, vp, table, lens, bits, 3, 8, D)
+    check(out, q, kp, vp, table, lens, page, bits, D ** -0.5)
+    for x, pl in zip(dense, (kp, vp)):                       # the rows, bit for bit as qb200.quantize makes them
+        for want, got in zip((x,) if bits == 16 else qb200.quantize(x, 64, bits), pl):
+            for b, n in enumerate(lens):
+                rows = torch.stack([got[table[b][t // page], :, t % page] for t in range(n)], 1)
+                assert torch.equal(rows, want[b, :, :n])
+
+
+def test_more_sequences_than_the_smaller_forms_hold():
+    """The cut of the work over 600 and 1024 sequences, empty ones among them, lengths in shared memory."""
+    torch.manual_seed(9)
+    for B in (600, 1024):
+        lens = [(i * 37) % 90 for i in range(B)]
+        page, H, D = 16, 1, 64
+        M, P = 6, sum(-(-n // 16) for n in lens)
+        kp, vp = make_pool(P, H, page, D, 8), make_pool(P, H, page, D, 8)
+        table = make_table(lens, page, M, P)
+        q, out = run(kp, vp, table, lens, 8, B, 2, D)
+        check(out, q, kp, vp, table, lens, page, 8, D ** -0.5)

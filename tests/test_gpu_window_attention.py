@@ -183,3 +183,23 @@ def test_streams_graphs_and_the_status_word():
         check(out, q, k, v, 0.1, 300, 4, [n])
         assert torch.equal(out.view(torch.int16), again.view(torch.int16))
     assert qb200.lib().qb200_debug_tc_status() == 0
+
+
+def test_sequences_far_apart():
+    """Sequences and heads whose elements lie beyond 2^31 of each other, in every operand and in the result."""
+    D, far = 64, 2 ** 31 + 64
+    q, k, v = make(2, 2, 2, 140, 140, D)
+    res = torch.zeros_like(q)
+
+    def spread(x, axis):
+        x = x.contiguous()
+        stride = [far if i == axis else s for i, s in enumerate(x.stride())]
+        flat = torch.empty(far + x.stride(0) * 2, dtype=BF16, device="cuda")
+        y = flat.as_strided(x.shape, stride)
+        y.copy_(x)
+        return y
+
+    for axis in (0, 1):
+        fq, fk, fv, fr = (spread(x, axis) for x in (q, k, v, res))
+        qb200.window_attention(fq, fk, fv, 0.1, window=50, sinks=3, out=fr)
+        check(fr, q, k, v, 0.1, 50, 3)
