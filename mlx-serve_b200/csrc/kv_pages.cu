@@ -355,16 +355,27 @@ __global__ void __launch_bounds__(kPageThreads) pages_compact_kernel(PageState s
     st.refs[mv.y] = st.refs[mv.x];
     st.refs[mv.x] = 0;
   }
-  cluster_sync_all();
-  const int64_t entries = (int64_t)st.S * st.M;
-  for (int64_t i = (int64_t)me * kPageThreads + tid; i < entries; i += (int64_t)nr * kPageThreads) {
-    const int64_t s = i / st.M;
-    int32_t* e = st.table + s * st.table_str + (i - s * st.M);
-    const int32_t pid = *e;
-    if (pid >= 0) {
-      const int32_t to = pid < st.P ? __ldcg(remap + pid) : -1;
-      if (to != pid) *e = to;
-    }
+}
+
+// The table's entries become what remap says: a launch of its own over the whole device, a warp 512 entries of a sequence at a time, all
+// asked for at once.  (By the cluster itself, behind its other steps, 1024 x 2048 entries took 104 us in all, so 55; 24 x 128 take 11 either way.)
+constexpr int kRemapChunk = 512;
+__global__ void __launch_bounds__(256) pages_remap_kernel(PageState st, const int32_t* remap, int chunks) {
+  grid_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t items = (int64_t)st.S * chunks;
+  for (int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); item < items; item += (int64_t)gridDim.x * 8) {
+    const int64_t s = item / chunks;
+    const int p0 = (int)(item - s * chunks) * kRemapChunk + lane;
+    int32_t* row = st.table + s * st.table_str;
+    int32_t pid[kRemapChunk / 32], to[kRemapChunk / 32];
+#pragma unroll
+    for (int k = 0; k < kRemapChunk / 32; ++k) pid[k] = p0 + k * 32 < st.M ? row[p0 + k * 32] : -1;
+#pragma unroll
+    for (int k = 0; k < kRemapChunk / 32; ++k) to[k] = pid[k] < 0 ? pid[k] : (pid[k] < st.P ? remap[pid[k]] : -1);
+#pragma unroll
+    for (int k = 0; k < kRemapChunk / 32; ++k)
+      if (to[k] != pid[k]) row[p0 + k * 32] = to[k];
   }
 }
 
@@ -477,7 +488,11 @@ cudaError_t launch_pages_reserve(const PageState& s, const int32_t* rows, const 
 }
 cudaError_t launch_pages_compact(const PageState& s, int32_t* remap, int32_t* moves, int64_t cap, int32_t* count, cudaStream_t st) {
   const int bw = bit_words(s.P, 1);
-  return launch_page_cluster(pages_compact_kernel, kStateBlocks, (size_t)bw * 8, st, s, remap, moves, cap, count, bw);
+  const cudaError_t e = launch_page_cluster(pages_compact_kernel, kStateBlocks, (size_t)bw * 8, st, s, remap, moves, cap, count, bw);
+  if (e != cudaSuccess || s.S == 0 || s.M == 0) return e;
+  const int chunks = (s.M - 1) / kRemapChunk + 1;
+  const int64_t blocks = ((int64_t)s.S * chunks + 7) / 8, most = (int64_t)sm_count() * 4;
+  return launch_behind(pages_remap_kernel, dim3((unsigned)(blocks < most ? blocks : most)), 256, 1, 0, st, s, remap, chunks);
 }
 cudaError_t launch_pages_copy(const PagesCopyArgs& a, int vec, cudaStream_t st) {
   const int64_t work = (a.n * a.pieces + 7) / 8, most = (int64_t)sm_count() * 8;   // eight warps a block

@@ -308,3 +308,31 @@ def test_bookkeeping_in_a_replayed_graph():
         st.ref.free([2, 3, 4])
         assert shared.tolist() == want and pos.tolist() == wp and [tuple(c) for c in copies.tolist()] == wc
         st.check()
+
+
+@pytest.mark.parametrize("S,M,P", [(3, 1100, 2000), (700, 513, 100000), (1, 1, 1), (5, 0, 64)])
+def test_compact_rewrites_tables_of_any_shape(S, M, P):
+    """Rows of several chunks, more rows than one pass of the device takes, with strides, shared and foreign pages among the entries."""
+    g = torch.Generator(device="cuda").manual_seed(S)
+    wide = torch.full((S, M + 3), -7, dtype=torch.int32, device="cuda")
+    table = wide[:, :M]
+    table.copy_(torch.randint(-P, P, (S, M), device="cuda", generator=g, dtype=torch.int32))
+    if M:
+        table[0, 0] = P + 5                                   # no page of the pool: no page behind the call either
+    refs = torch.zeros(P, dtype=torch.int32, device="cuda")
+    named = table[(table >= 0) & (table < P)].long()
+    refs.scatter_add_(0, named, torch.ones_like(named, dtype=torch.int32))
+    before, counts = table.clone(), refs.clone()
+    remap, moves, count = qb200.kv_pages_compact(table, refs)
+    live = int((counts > 0).sum())
+    back = torch.nonzero((counts > 0) & (torch.arange(P, device="cuda") >= live)).flatten()
+    holes = torch.nonzero((counts == 0) & (torch.arange(P, device="cuda") < live)).flatten()
+    want = torch.where(counts > 0, torch.arange(P, device="cuda"), -1)
+    want[back] = holes
+    assert count.item() == len(back) and torch.equal(remap.long(), want)
+    assert torch.equal(moves[:len(back)].long(), torch.stack([back, holes], 1)) and bool((moves[len(back):] == -1).all())
+    entries = torch.where((before >= 0) & (before < P), want[before.clamp(0, P - 1).long()], torch.where(before < 0, before, -1).long())
+    assert torch.equal(table.long(), entries) and bool((wide[:, M:] == -7).all())
+    moved = torch.zeros_like(counts)
+    moved[want[counts > 0]] = counts[counts > 0]
+    assert torch.equal(refs, moved)
