@@ -606,6 +606,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       const float inv = poisoned ? __uint_as_float(0x7fc00000u) : (l > 0.f ? 1.f / l : (l == l ? 0.f : l));
       // The results go through shared memory, in the place of the warp's own queries, so that a store covers whole rows (a thread a
       // row, 32 rows a store, took 5000 cycles); 16-byte chunks swizzled by the row.
+      // (a tile that saw nothing has not waited for its queries, which must have arrived before anything is put in their place)
+      if (plan.blocks > 0 && done == 0 && !__all_sync(0xffffffffu, wait_cta(&q_full, 0, kPolls)) && lane == 0 && !s_fail) failed(504);
       unsigned char* const stage = smem + t * SH::BYTES + (warp & 3) * (32 * D * 2);
       constexpr int CH = D / 8;
 #pragma unroll 1

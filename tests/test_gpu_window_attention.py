@@ -203,3 +203,62 @@ def test_sequences_far_apart():
         fq, fk, fv, fr = (spread(x, axis) for x in (q, k, v, res))
         qb200.window_attention(fq, fk, fv, 0.1, window=50, sinks=3, out=fr)
         check(fr, q, k, v, 0.1, 50, 3)
+
+
+def crowd(q, k, v, *args, lens=None, **kw):
+    """The call on so many copies of its sequences that every CTA takes two tiles; all copies give the same."""
+    n = 160 // (q.shape[0] * q.shape[1]) + 1
+    rep = lambda x: x.repeat(n, 1, 1, 1)
+    if lens is not None:
+        kw["kv_lens"] = torch.tensor(lens * n, dtype=I32, device="cuda")
+    out = qb200.window_attention(rep(q), rep(k), rep(v), *args, **kw).view(n, *q.shape)
+    bits = out.view(torch.int16)
+    assert torch.equal(bits, bits[:1].expand_as(bits))
+    return out[0]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hq,Hkv", [(2, 1), (3, 1), (2, 2)])
+@pytest.mark.parametrize("Tq,Tk,window,sinks", [(1, 1, 0, 0), (77, 77, 32, 2), (129, 300, 0, 0), (256, 256, 1, 0), (300, 700, 200, 130), (513, 513, 129, 128), (140, 900, 64, 10 ** 12)])
+def test_two_tiles_a_block(D, Hq, Hkv, Tq, Tk, window, sinks):
+    q, k, v = make(1, Hq, Hkv, Tq, Tk, D, Tq)
+    check(crowd(q, k, v, D ** -0.5, window=window, sinks=sinks), q, k, v, D ** -0.5, window, sinks)
+
+
+@pytest.mark.parametrize("D,gqa,window,sinks", [(64, 1, 0, 0), (128, 2, 90, 5), (128, 3, 90, 5)])
+def test_two_tiles_a_block_with_lengths(D, gqa, window, sinks):
+    lens = [400, 250, 130, 1, 0, 1000, -3]
+    q, k, v = make(7, gqa, 1, 200, 400, D)
+    for b, n in enumerate(lens):
+        k[b, :, max(n, 0):], v[b, :, max(n, 0):] = float("nan"), float("nan")
+    check(crowd(q, k, v, 0.1, window=window, sinks=sinks, lens=lens), q, k, v, 0.1, window, sinks, lens)
+
+
+@pytest.mark.parametrize("D,gqa", [(64, 1), (128, 2)])
+def test_two_tiles_a_block_and_what_is_not_finite(D, gqa):
+    Tq, Tk, window, sinks = 400, 600, 100, 3
+    q, k, v = make(1, 2 * gqa, 2, Tq, Tk, D)
+    bad = {0: [(150, float("nan")), (599, float("inf")), (340, float("-inf"))], 1: [(1, float("nan")), (260, float("inf"))]}
+    for h, rows in bad.items():
+        for j, x in rows:
+            v[0, h, j, 7] = x
+    v[0, :, 50], k[0, :, 60] = float("nan"), float("nan")           # no query sees these
+    out = crowd(q, k, v, 0.1, window=window, sinks=sinks)
+    clean = torch.nan_to_num(v, 0.0, 0.0, 0.0)
+    poisoned = lambda b, h, see: see[:, [j for j, _ in bad[h]]].any(1)
+    fine = torch.where(torch.isfinite(out).all(-1, keepdim=True), out, torch.full_like(out, float("nan")))
+    check(fine, q, torch.nan_to_num(k), clean, 0.1, window, sinks, poisoned=poisoned)
+
+
+@pytest.mark.parametrize("std", [1e-3, 8.0])
+def test_two_tiles_a_block_of_any_magnitude(std):
+    q, k, v = make(1, 2, 1, 500, 500, 128, 3, std)
+    k *= torch.linspace(0, 2, 500, device="cuda").to(BF16)[None, None, :, None]
+    check(crowd(q, k, v, 0.1), q, k, v, 0.1)
+
+
+def test_a_long_prompt_of_many_heads():
+    q, k, v = make(1, 16, 2, 3000, 5000, 128)
+    for window, sinks in ((0, 0), (1024, 4)):
+        check(qb200.window_attention(q, k, v, 128 ** -0.5, window=window, sinks=sinks), q, k, v, 128 ** -0.5, window, sinks)
+    assert qb200.lib().qb200_debug_tc_status() == 0
