@@ -5,7 +5,7 @@
 //   o = sum_j P_j v_j / sum_j P_j,  P_j = 2^(c s_j - c r),  s = q . k, c = scale * log2(e), r a running reference of the row.
 //
 // One CTA of 12 warps takes two tiles of 128 queries that read the same keys: two heads of a group where the group is even, else
-// two neighbouring tiles of one head.
+// two neighbouring tiles of one head (one tile where a launch has fewer tiles than the device has SMs).
 //   warps 0-3, 4-7 : the softmax of a tile, a thread a row.  Scores come from tensor memory, the probabilities go back in their place as
 //                    bf16, the A operand of the second product.  Blocks that all queries see whole are taken with the reference r as it
 //                    is, without looking for their maximum first; only where a block's sum passes 2^24 (and in masked blocks, where
@@ -53,6 +53,7 @@ struct WindowK {
   const int32_t* kv_lens;
   int B, Hq, gqa, Tq, Tk, window, sinks;
   int qblocks, heads2;                 // 1: the two tiles are two heads; 0: two tiles of one head
+  int single;                          // one tile (heads2 is 0): the second lies behind the last query
   int split;                           // CTAs of a cluster that share the keys of the tiles (1, 2, 4, 8)
   int mul[3][2];                       // coordinates along (head, sequence) of q, k, v: 0 where the tensor is broadcast
   float c;
@@ -160,7 +161,7 @@ __device__ __forceinline__ Plan make_plan(const WindowK& a, int b, int row0, int
   int len = a.kv_lens ? a.kv_lens[b] : a.Tk;
   len = len < 0 ? 0 : (len > a.Tk ? a.Tk : len);
   const int base = len - a.Tq;
-  const int r1 = a.heads2 ? row0 : row0 + kTile;
+  const int r1 = a.heads2 ? row0 : (a.single ? a.Tq : row0 + kTile);
   const int rows[2] = {row0, r1};
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
   const int rem = unit % per_q;
   const int b = rem / (per_q / a.B), hu = rem % (per_q / a.B);
   const int head0 = a.heads2 ? 2 * hu : hu, head1 = a.heads2 ? head0 + 1 : head0, hk = head0 / a.gqa;
-  const int row0 = qb * (a.heads2 ? kTile : 2 * kTile), row1 = a.heads2 ? row0 : row0 + kTile;
+  const int row0 = qb * (a.heads2 || a.single ? kTile : 2 * kTile), row1 = a.heads2 ? row0 : (a.single ? a.Tq : row0 + kTile);
   const Plan plan = make_plan(a, b, row0, rank);
 
   if (tid >= 32 && tid < 32 + kNotes) note_bits[tid - 32] = 0u;
@@ -246,9 +247,9 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
     if (warp == 8) {
       // ---- copies ----
       if (elect_one() && plan.blocks > 0) {
-        mbar_expect_tx(&q_full, 2 * SH::BYTES);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
+        const int tiles = a.single ? 1 : 2;
+        mbar_expect_tx(&q_full, tiles * SH::BYTES);
+        for (int t = 0; t < tiles; ++t)
 #pragma unroll
           for (int h = 0; h < SH::HALVES; ++h)
             tma_load_4d(smem_u32(smem) + t * SH::BYTES + h * kTile * 128, &mq, &q_full, 64 * h, t ? row1 : row0, (t ? head1 : head0) * a.mul[0][0], b * a.mul[0][1]);
@@ -666,6 +667,40 @@ bool rows_map(CUtensorMap* m, const void* base, int64_t D, const int64_t (&shape
                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// How many CTAs, clusters of 2, 4 and 8 of the kernel the device holds at once.
+template <int D> cudaError_t places(int (&fit)[4]) {
+  auto kern = window_attn_kernel<D>;
+  static int cached[64][4] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> setup_lk(setup_mutex());       // first use on a device, from any thread
+  if (dev < 0 || dev >= 64 || cached[dev][0] == 0) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::SMEM);
+    if (e != cudaSuccess) return e;
+    fit[0] = sm_count();
+    for (int i = 1; i < 4; ++i) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1u << i);
+      cfg.blockDim = dim3(kThreads);
+      cfg.dynamicSmemBytes = Shape<D>::SMEM;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1u << i; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&fit[i], kern, &cfg) != cudaSuccess) {
+        (void)cudaGetLastError();
+        fit[i] = 0;
+      }
+    }
+    if (dev >= 0 && dev < 64)
+      for (int i = 0; i < 4; ++i) cached[dev][i] = fit[i];
+  } else
+    for (int i = 0; i < 4; ++i) fit[i] = cached[dev][i];
+  return cudaSuccess;
+}
+
 template <int D> cudaError_t launch_d(const WindowArgs& w, cudaStream_t st) {
   WindowK a;
   a.out = (uint16_t*)w.out; a.kv_lens = w.kv_lens;
@@ -674,37 +709,38 @@ template <int D> cudaError_t launch_d(const WindowArgs& w, cudaStream_t st) {
   a.B = (int)w.B; a.Hq = (int)w.Hq; a.gqa = (int)(w.Hq / w.Hkv); a.Tq = (int)w.Tq; a.Tk = (int)w.Tk;
   a.window = w.window; a.sinks = w.sinks;
   a.c = w.scale * 1.4426950408889634f;
-  a.heads2 = a.gqa % 2 == 0;
-  a.qblocks = (a.Tq + (a.heads2 ? 1 : 2) * kTile - 1) / ((a.heads2 ? 1 : 2) * kTile);
   CUtensorMap m[3];
   const int64_t qs[3] = {w.B, w.Hq, w.Tq}, ks[3] = {w.B, w.Hkv, w.Tk};
   if (!rows_map(&m[0], w.q, D, qs, w.str[0], a.mul[0]) || !rows_map(&m[1], w.k, D, ks, w.str[1], a.mul[1]) || !rows_map(&m[2], w.v, D, ks, w.str[2], a.mul[2]))
     return cudaErrorInvalidValue;
   auto kern = window_attn_kernel<D>;
-  static bool done[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  int fit[4];
+  cudaError_t e = places<D>(fit);
   if (e != cudaSuccess) return e;
-  {
-    std::lock_guard<std::mutex> setup_lk(setup_mutex());   // first use on a device, from any thread
-    if (dev < 0 || dev >= 64 || !done[dev]) {
-      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::SMEM);
-      if (e != cudaSuccess) return e;
-      if (dev >= 0 && dev < 64) done[dev] = true;
-    }
-  }
-  const int64_t ctas = (int64_t)a.qblocks * (a.heads2 ? a.Hq / 2 : a.Hq) * a.B;
-  // Where the tiles leave SMs without work, clusters share a tile's keys, as many CTAs as there are SMs for.  To join them takes as long
-  // as some five blocks, so it has to save more than that: 16 CTAs of 64 blocks (64 queries, 8192 keys) take 115 us alone and 55
-  // in clusters of 8; 64 CTAs of 11 blocks (512 queries, a window of 1024) take 34 us either way and stay alone.
-  const int64_t rows = a.heads2 ? kTile : 2 * kTile;
+  // Two tiles a CTA, as they fill the tensor cores between them.  Where that leaves SMs without work, clusters share a tile's keys, as
+  // many CTAs as the device places at once (16 clusters of 8 are more than it does: 64 queries on 8192 keys took 57 us by them and 45 by
+  // clusters of 4, 115 alone).  To join them takes as long as some five blocks, so it has to save more than that: 64 CTAs of 11
+  // blocks (512 queries, a window of 1024) take 33 us by clusters of 2 and 35 alone.  Where there are SMs still, a CTA takes one
+  // tile: its steps are no longer than those of two, which wait for each other now and then (these 64: 31 us).  Clusters come first:
+  // 256 queries of 32 heads on 4096 keys take 33 us in 128 CTAs of two tiles by clusters of 4 and 43 of one tile by clusters of 2.
+  auto shape = [&](bool single) {
+    a.single = single;
+    a.heads2 = !single && a.gqa % 2 == 0;
+    const int rows = a.heads2 || single ? kTile : 2 * kTile;
+    a.qblocks = (a.Tq + rows - 1) / rows;
+    return (int64_t)a.qblocks * (a.heads2 ? a.Hq / 2 : a.Hq) * a.B;
+  };
+  const int64_t singles = shape(true);
+  int64_t ctas = shape(false);
   int64_t most = (w.Tk + kTile - 1) / kTile;
   if (w.window > 0) {
-    const int64_t seen = (w.window + rows + kTile - 2) / kTile + 1 + (w.sinks + kTile - 1) / kTile;
+    const int64_t rows = a.heads2 ? kTile : 2 * kTile, seen = (w.window + rows + kTile - 2) / kTile + 1 + (w.sinks + kTile - 1) / kTile;
     most = most < seen ? most : seen;
   }
-  a.split = 8;
-  while (a.split > 1 && (ctas * a.split > sm_count() || most - most / a.split < 8)) a.split /= 2;
+  int step = 3;
+  while (step > 0 && (ctas > fit[step] || most - (most >> step) < 8)) --step;
+  a.split = 1 << step;
+  if (singles <= fit[step]) ctas = shape(true);
   if (a.split > 1) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(ctas * a.split));
@@ -718,7 +754,7 @@ template <int D> cudaError_t launch_d(const WindowArgs& w, cudaStream_t st) {
     cfg.numAttrs = 1;
     e = launch_clusters(cfg, kern, m[0], m[1], m[2], a);
     if (e == cudaSuccess) return e;
-    (void)cudaGetLastError();            // the device places no clusters: every tile by itself
+    (void)cudaGetLastError();            // the device places no clusters after all: every tile by itself
     a.split = 1;
   }
   return launch_kernel(kern, dim3((unsigned)ctas), dim3(kThreads), Shape<D>::SMEM, st, m[0], m[1], m[2], a);
