@@ -21,7 +21,9 @@ __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;
 // Row (n, i) of head h goes to slot (pos % page) of page table[r, pos / page], pos = positions[n] + i.  16 values a thread: the four
 // (head dim 64) or eight threads of a row are neighbours, rows of one head follow each other as tokens do, so that both sides are
 // read and written in whole sectors.  A block has rows of one (sequence, K or V, head); the values are asked for before the table is
-// looked up.  Bound by HBM at prompt lengths, by the launch at one token.
+// looked up.  Bound by the launch at one token a sequence (16 sequences of 8 heads of 128: 5 us), by instructions at prompt lengths:
+// a warp's 512 values take 388, most of them to divide as the quantiser defines it, and 68 % of the issue slots are used (8192 tokens
+// of 8 heads at 8 bits, 45 MB in and out: 20.4 us, floor 6.9).
 template <int BITS>
 __global__ void __launch_bounds__(256) pages_append_kernel(const __grid_constant__ KvPagesAppendArgs a) {
   const uint32_t r2 = blockIdx.x / a.tiles, tile = blockIdx.x - r2 * a.tiles;
@@ -381,7 +383,8 @@ __global__ void __launch_bounds__(256) pages_remap_kernel(PageState st, const in
 
 // ---------------------------------------------------------------- copying pages
 // Pair by pair, pool by pool, in pieces that a warp copies with four vectors a lane: pages of codes have many, those of scales one or
-// two, and no warp waits for another's.
+// two, and no warp waits for another's.  Bound by HBM: 336 MB of moved pages, read and written, take 105 us, 6.4 TB/s (pieces of 1024, 8192
+// and 16384 bytes: 158, 150, 160 us).
 constexpr int kCopyPiece = 2048;
 
 template <typename V>
