@@ -21,6 +21,23 @@ inline cudaError_t launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, 
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
+// The same, begun while the kernel before it in the stream still runs: for kernels that wait (griddepcontrol.wait) before they read or
+// write anything, which saves the launch's own latency.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_behind(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
 int report_error(int status, const char* msg);  // api.cu: last-error string + handler
 int sm_count();                                 // device.cu: SMs of the current device
 std::mutex& setup_mutex();                      // device.cu: guards every first-use-per-device set-up

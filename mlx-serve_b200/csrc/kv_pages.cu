@@ -26,6 +26,7 @@ __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;
 // of 8 heads at 8 bits, 45 MB in and out: 20.4 us, floor 6.9).
 template <int BITS>
 __global__ void __launch_bounds__(256) pages_append_kernel(const __grid_constant__ KvPagesAppendArgs a) {
+  grid_wait();
   const uint32_t r2 = blockIdx.x / a.tiles, tile = blockIdx.x - r2 * a.tiles;
   const uint32_t r3 = r2 / a.H, h = r2 - r3 * a.H;
   const uint32_t kv = r3 & 1u, n = r3 >> 1;
@@ -434,23 +435,6 @@ __global__ void __launch_bounds__(256) pages_copy_kernel(const __grid_constant__
   }
 }
 
-// A launch that may begin while the kernel before it runs; in clusters of `cluster` blocks where that is above 1.
-template <typename... K, typename... A>
-cudaError_t launch_behind(void (*kern)(K...), dim3 grid, int threads, int cluster, size_t smem, cudaStream_t st, A&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cluster > 1 ? launch_clusters(cfg, kern, args...) : cudaLaunchKernelEx(&cfg, kern, static_cast<K>(args)...);
-}
 template <typename... K, typename... A>
 cudaError_t launch_page_cluster(void (*kern)(K...), int want, size_t smem, cudaStream_t st, A... args) {
   if (smem > 48 * 1024) {
@@ -458,11 +442,23 @@ cudaError_t launch_page_cluster(void (*kern)(K...), int want, size_t smem, cudaS
     if (e != cudaSuccess) return e;
   }
   if (want > 1) {
-    const cudaError_t e = launch_behind(kern, dim3((unsigned)want), kPageThreads, want, smem, st, args...);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)want);
+    cfg.blockDim = dim3(kPageThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)want; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = launch_clusters(cfg, kern, args...);
     if (e == cudaSuccess) return e;
     (void)cudaGetLastError();            // the device places no clusters: one block does it
   }
-  return launch_behind(kern, dim3(1), kPageThreads, 1, smem, st, args...);
+  return launch_behind(kern, dim3(1), dim3(kPageThreads), smem, st, args...);
 }
 int bit_words(int64_t P, int blocks) { return (int)(((P + 31) / 32 + blocks - 1) / blocks); }
 }  // namespace
@@ -476,10 +472,10 @@ cudaError_t launch_pages_append(const KvPagesAppendArgs& a, cudaStream_t st) {
   for (int i = 0; i < 16; ++i)
     if (a.per_row == 1 << i) k.row_shift = i;
   auto kern = a.bits == 4 ? pages_append_kernel<4> : (a.bits == 8 ? pages_append_kernel<8> : pages_append_kernel<16>);
-  return launch_kernel(kern, dim3((unsigned)((int64_t)k.tiles * a.N * 2 * a.H)), dim3((unsigned)block), 0, st, k);
+  return launch_behind(kern, dim3((unsigned)((int64_t)k.tiles * a.N * 2 * a.H)), dim3((unsigned)block), 0, st, k);
 }
 cudaError_t launch_pages_free(const PageState& s, const int32_t* rows, const int32_t* begin, const int32_t* end, int n, cudaStream_t st) {
-  return launch_behind(pages_free_kernel, dim3((unsigned)n), 256, 1, 0, st, s, rows, begin, end);
+  return launch_behind(pages_free_kernel, dim3((unsigned)n), dim3(256), 0, st, s, rows, begin, end);
 }
 // One block's bits take 2 words per 32 pages and the list five: both fit where kMaxPages and kMaxPageList hold.
 cudaError_t launch_pages_fork(const PageState& s, const int32_t* src, const int32_t* dst, const int32_t* tokens, int n, int32_t* shared, cudaStream_t st) {
@@ -495,16 +491,16 @@ cudaError_t launch_pages_compact(const PageState& s, int32_t* remap, int32_t* mo
   if (e != cudaSuccess || s.S == 0 || s.M == 0) return e;
   const int chunks = (s.M - 1) / kRemapChunk + 1;
   const int64_t blocks = ((int64_t)s.S * chunks + 7) / 8, most = (int64_t)sm_count() * 4;
-  return launch_behind(pages_remap_kernel, dim3((unsigned)(blocks < most ? blocks : most)), 256, 1, 0, st, s, remap, chunks);
+  return launch_behind(pages_remap_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, s, remap, chunks);
 }
 cudaError_t launch_pages_copy(const PagesCopyArgs& a, int vec, cudaStream_t st) {
   const int64_t work = (a.n * a.pieces + 7) / 8, most = (int64_t)sm_count() * 8;   // eight warps a block
   const dim3 grid((unsigned)(work < most ? work : most));
   switch (vec) {
-    case 16: return launch_behind(pages_copy_kernel<uint4>, grid, 256, 1, 0, st, a);
-    case 4: return launch_behind(pages_copy_kernel<uint32_t>, grid, 256, 1, 0, st, a);
-    case 2: return launch_behind(pages_copy_kernel<uint16_t>, grid, 256, 1, 0, st, a);
-    default: return launch_behind(pages_copy_kernel<uint8_t>, grid, 256, 1, 0, st, a);
+    case 16: return launch_behind(pages_copy_kernel<uint4>, grid, dim3(256), 0, st, a);
+    case 4: return launch_behind(pages_copy_kernel<uint32_t>, grid, dim3(256), 0, st, a);
+    case 2: return launch_behind(pages_copy_kernel<uint16_t>, grid, dim3(256), 0, st, a);
+    default: return launch_behind(pages_copy_kernel<uint8_t>, grid, dim3(256), 0, st, a);
   }
 }
 int pages_copy_piece() { return kCopyPiece; }

@@ -193,6 +193,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
   int* const units = (int*)(smem + GE::SMEM);      // [B + 1], above 32 sequences
   __shared__ int warp_sums[2 * kWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   const bool few = a.B <= 32;
   const Lengths L = read_lengths(a, units, warp_sums);
@@ -854,18 +855,9 @@ template <int BITS, int D> cudaError_t launch_inst(KvPagesAttnArgs a, int64_t mo
   cudaError_t e = resident<BITS, D>(step, &n);
   if (e != cudaSuccess) return e;
   const unsigned grid = (unsigned)(most_units < n ? (most_units < 1 ? 1 : most_units) : n);
-  e = launch_kernel(kv_pages_kernel<BITS, D>, dim3(grid), dim3(kWarps * 32), smem_of<BITS, D>(step), st, a);
+  e = launch_behind(kv_pages_kernel<BITS, D>, dim3(grid), dim3(kWarps * 32), smem_of<BITS, D>(step), st, a);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kMergeWarps * 32);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv_pages_join_kernel<D>, a);
+  return launch_behind(kv_pages_join_kernel<D>, dim3(grid), dim3(kMergeWarps * 32), 0, st, a);
 }
 }  // namespace
 

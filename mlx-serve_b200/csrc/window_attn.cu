@@ -213,6 +213,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
   __shared__ uint32_t note_bits[kNotes];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+  asm volatile("griddepcontrol.wait;" ::: "memory");         // (before tensor memory is taken, too: the kernel before may hold it)
+
   // ---- which tiles: the longest rows of the prompt first ----
   const int per_q = (a.heads2 ? a.Hq / 2 : a.Hq) * a.B;
   const int rank = a.split > 1 ? (int)cluster_rank_tc() : 0, unit = a.split > 1 ? (int)blockIdx.x / a.split : (int)blockIdx.x;
@@ -747,17 +749,19 @@ template <int D> cudaError_t launch_d(const WindowArgs& w, cudaStream_t st) {
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = Shape<D>::SMEM;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)a.split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     e = launch_clusters(cfg, kern, m[0], m[1], m[2], a);
     if (e == cudaSuccess) return e;
     (void)cudaGetLastError();            // the device places no clusters after all: every tile by itself
     a.split = 1;
   }
-  return launch_kernel(kern, dim3((unsigned)ctas), dim3(kThreads), Shape<D>::SMEM, st, m[0], m[1], m[2], a);
+  return launch_behind(kern, dim3((unsigned)ctas), dim3(kThreads), Shape<D>::SMEM, st, m[0], m[1], m[2], a);
 }
 }  // namespace
 
