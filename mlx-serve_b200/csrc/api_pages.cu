@@ -288,10 +288,11 @@ QB200_API int qb200_kv_pages_copy(qb200_tensor* const* pools, int num_pools, con
   if (pairs->shape[1] != 2 || (pairs->shape[0] > 1 && pairs->stride[0] != 2)) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: pairs must be a contiguous [n, 2]", who);
   if (!empty(count) && (st = expect_list(count, who, "count", 1))) return st;
   const int piece = pages_copy_piece();
-  for (int pass = 0; pass < 2; ++pass) {       // every pool is checked before the first launch
+  const int launches = (num_pools + kMaxCopyPools - 1) / kMaxCopyPools;
+  for (int pass = launches > 1 ? 0 : 1; pass < 2; ++pass) {    // every pool is checked before the first launch
     for (int p0 = 0; p0 < num_pools; p0 += kMaxCopyPools) {
       PagesCopyArgs a;
-      std::memset(&a, 0, sizeof(a));
+      a.pools = 0;
       uint64_t bits = 0;                       // every address, stride and run, or-ed: what they are all multiples of
       int64_t pieces = 0;
       for (int i = p0; i < num_pools && i < p0 + kMaxCopyPools; ++i) {

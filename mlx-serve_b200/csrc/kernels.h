@@ -324,12 +324,13 @@ struct PagesCopyPool {
   int first_piece;
 };
 constexpr int kMaxCopyPools = 96;        // pools per launch
-struct PagesCopyArgs {
+template <int N> struct PagesCopyList {
   const int32_t* pairs; const int32_t* count;   // count may be null
   int64_t n, P;
   int pools, pieces;
-  PagesCopyPool pool[kMaxCopyPools];
+  PagesCopyPool pool[N];
 };
+using PagesCopyArgs = PagesCopyList<kMaxCopyPools>;
 cudaError_t launch_pages_copy(const PagesCopyArgs& a, int vec, cudaStream_t st);   // vec: bytes every offset and length is a multiple of (16, 4, 2, 1)
 int pages_copy_piece();
 
