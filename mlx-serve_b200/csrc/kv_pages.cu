@@ -23,7 +23,7 @@ __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;
 // read and written in whole sectors.  A block has rows of one (sequence, K or V, head); the values are asked for before the table is
 // looked up.  Bound by the launch at one token a sequence (16 sequences of 8 heads of 128: 5 us), by instructions at prompt lengths:
 // a warp's 512 values take 388, most of them to divide as the quantiser defines it, and 68 % of the issue slots are used (8192 tokens
-// of 8 heads at 8 bits, 45 MB in and out: 20.4 us, floor 6.9).
+// of 8 heads at 8 bits, 45 MB in and out: 17.9 us, floor 6.9).
 template <int BITS>
 __global__ void __launch_bounds__(256) pages_append_kernel(const __grid_constant__ KvPagesAppendArgs a) {
   grid_wait();

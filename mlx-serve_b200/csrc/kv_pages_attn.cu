@@ -21,11 +21,11 @@
 //    layout becomes the B operand of the next product by movmatrix.
 //
 // Floor: the visible rows' bytes at the copy bandwidth (6.54 TB/s measured).  Sequences of 16k to 32k tokens, 16 of them, 32 query heads on 8 of
-// 128, pages of 64: 4 bits 463 MB, floor 71 us, takes 111 (4.2 TB/s); 8 bits 874 MB, 134 and 162 us; bf16 1.64 GB, 251 and 268 us.  At
+// 128, pages of 64: 4 bits 463 MB, floor 71 us, takes 107 to 111 (4.2 to 4.3 TB/s); 8 bits 874 MB, 134 and 162 us; bf16 1.64 GB, 251 and 268 us.  At
 // 4 bits the issue slots bound it: 271 warp instructions per 16 tokens (406 before a token's four neighbours were placed for wide
 // scale loads and the rescaling became lazy), 56 % of the slots used with the 12 warps an SM that 168 registers leave; 128 registers
 // and 16 warps spill and take 126 to 137 us, 5 warps a CTA 127.  Short calls wait for dependent reads (lengths, table, rows) and the
-// join: one sequence of 700 tokens takes 12.3 us, of it 4.7 in the second launch.
+// join: one sequence of 700 tokens takes 9.6 us, 12.3 before the kernels were launched behind one another.
 #include <mutex>
 #include <type_traits>
 
