@@ -17,7 +17,8 @@
 //                    some query, rows that no query of the CTA sees are zeroed, and rows with anything not finite are zeroed and
 //                    noted; the queries that see such a row give NaN.
 // Blocks of 128 keys that no query of a tile sees are left out; only those cut by a border of the mask are masked element by element.
-// Where there are few tiles, clusters share a tile's keys and join their sums through distributed shared memory.
+// Where there are few tiles, a CTA takes one, whose scores are made two steps ahead in the place of the other tile's (the tensor cores then
+// wait for the softmax alone: 1.03 us a step), or clusters share a tile's keys and join their sums through distributed shared memory.
 //
 // Floor: 4 D operations per visible pair on the tensor cores.  32 heads of 128, 16384 tokens, window 4096: 0.96 TFLOP, 589 us at 1634
 // TFLOP/s, takes 811 us (1.19 PFLOP/s, 0.73 of the measured peak).  A step of a tile is a chain: softmax of 128 keys 1400 cycles, P V and
@@ -53,7 +54,6 @@ struct WindowK {
   const int32_t* kv_lens;
   int B, Hq, gqa, Tq, Tk, window, sinks;
   int qblocks, heads2;                 // 1: the two tiles are two heads; 0: two tiles of one head
-  int single;                          // one tile (heads2 is 0): the second lies behind the last query
   int split;                           // CTAs of a cluster that share the keys of the tiles (1, 2, 4, 8)
   int mul[3][2];                       // coordinates along (head, sequence) of q, k, v: 0 where the tensor is broadcast
   float c;
@@ -156,12 +156,12 @@ struct Plan {
   __device__ __forceinline__ bool masked(int blk) const { return (needs(0, blk) && !whole(0, blk)) || (needs(1, blk) && !whole(1, blk)); }
 };
 
-__device__ __forceinline__ Plan make_plan(const WindowK& a, int b, int row0, int rank) {
+template <bool SINGLE> __device__ __forceinline__ Plan make_plan(const WindowK& a, int b, int row0, int rank) {
   Plan p;
   int len = a.kv_lens ? a.kv_lens[b] : a.Tk;
   len = len < 0 ? 0 : (len > a.Tk ? a.Tk : len);
   const int base = len - a.Tq;
-  const int r1 = a.heads2 ? row0 : (a.single ? a.Tq : row0 + kTile);
+  const int r1 = a.heads2 ? row0 : (SINGLE ? a.Tq : row0 + kTile);
   const int rows[2] = {row0, r1};
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -199,7 +199,8 @@ __device__ __forceinline__ uint64_t make_desc_mn(uint32_t saddr) {
 
 constexpr int kNotes = 48;    // groups of 32 keys of masked blocks: at most 3 blocks at the diagonal, 3 at the window's start, 2 where the sinks end
 
-template <int D>
+// SINGLE: one tile (heads2 is 0; the second lies behind the last query), whose steps take the places and barriers of the two tiles in turn.
+template <int D, bool SINGLE>
 __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                                                                   const __grid_constant__ CUtensorMap mv, const __grid_constant__ WindowK a) {
   using SH = Shape<D>;
@@ -222,8 +223,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
   const int rem = unit % per_q;
   const int b = rem / (per_q / a.B), hu = rem % (per_q / a.B);
   const int head0 = a.heads2 ? 2 * hu : hu, head1 = a.heads2 ? head0 + 1 : head0, hk = head0 / a.gqa;
-  const int row0 = qb * (a.heads2 || a.single ? kTile : 2 * kTile), row1 = a.heads2 ? row0 : (a.single ? a.Tq : row0 + kTile);
-  const Plan plan = make_plan(a, b, row0, rank);
+  const int row0 = qb * (a.heads2 || SINGLE ? kTile : 2 * kTile), row1 = a.heads2 ? row0 : (SINGLE ? a.Tq : row0 + kTile);
+  const Plan plan = make_plan<SINGLE>(a, b, row0, rank);
 
   if (tid >= 32 && tid < 32 + kNotes) note_bits[tid - 32] = 0u;
   if (tid == 0) {
@@ -249,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
     if (warp == 8) {
       // ---- copies ----
       if (elect_one() && plan.blocks > 0) {
-        const int tiles = a.single ? 1 : 2;
+        constexpr int tiles = SINGLE ? 1 : 2;
         mbar_expect_tx(&q_full, tiles * SH::BYTES);
         for (int t = 0; t < tiles; ++t)
 #pragma unroll
@@ -284,11 +285,11 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       const uint32_t q_d = (uint32_t)U((int)(uint32_t)make_desc(smem_u32(smem))), k_d = (uint32_t)U((int)(uint32_t)make_desc(ring)),
                      v_d = (uint32_t)U((int)(uint32_t)make_desc_mn(ring));
       auto wait = [&](uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, spin_cta(bar, phase & 1)); };
-      auto scores = [&](int t, uint32_t st) {                // S of tile t with the keys in ring slot st (by the elected lane)
+      auto scores = [&](int t, uint32_t st) {                // S of tile t (or step t of one tile) with the keys in ring slot st (by the elected lane)
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t o = (k >> 2) * ((kTile * 128) >> 4) + (k & 3) * 2;
-          umma_ss(tm + t * 128, hi_k | (q_d + t * slot + o), hi_k | (k_d + st * slot + o), idesc_s, k > 0);
+          umma_ss(tm + t * 128, hi_k | (q_d + (SINGLE ? 0 : t) * slot + o), hi_k | (k_d + st * slot + o), idesc_s, k > 0);
         }
         commit(&s_full[t]);
       };
@@ -343,7 +344,40 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
           if (done[t] > 0 && !wait(&o_done[t], done[t] - 1)) return false;
         return true;
       };
-      if (pl.blocks > 0 && !products()) {
+      // One tile: S of the step after the next follows P V of this one, in the place of its probabilities, so that the softmax finds the next
+      // scores done.  Steps take turns with all barriers: two of them may be complete before a waiter looks.
+      auto products_single = [&]() -> bool {
+        if (!wait(&q_full, 0)) return false;
+        uint32_t sv = 1, sk = 0, rk = 0;
+        for (int n = -2; n < pl.blocks; ++n) {
+          const int step = n & 1;
+          if (n >= 0) {
+            if (!wait(&p_ready[step], (uint32_t)(n >> 1))) return false;
+            fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 0; k < kTile / 16; ++k)
+                umma_ts(tm + 256, tm + step * 128 + k * 8, hi_v | (v_d + sv * slot + k * (2048 >> 4)), idesc_o, k > 0 ? 1u : (n > 0 ? 1u : 0u));
+              commit(&o_done[step]);
+              commit(&kv_empty[sv]);
+            }
+            __syncwarp();
+            sv = sv + 2 < ST ? sv + 2 : sv + 2 - ST;
+          }
+          if (n + 2 < pl.blocks) {
+            if (!wait(&kv_full[sk], rk)) return false;
+            if (elect_one()) {
+              scores(step, sk);
+              commit(&kv_empty[sk]);
+            }
+            __syncwarp();
+            sk += 2;
+            if (sk >= ST) { sk -= ST; ++rk; }
+          }
+        }
+        return wait(&o_done[(pl.blocks - 1) & 1], (uint32_t)((pl.blocks - 1) >> 1));
+      };
+      if (pl.blocks > 0 && !(SINGLE ? products_single() : products())) {
         if (lane == 0 && !s_fail) failed(502);
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);    // (products may still be on their way)
       }
@@ -386,10 +420,10 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        if (ok && n + 1 < plan.blocks) ok = __all_sync(0xffffffffu, wait_cta(&kv_full[(iv + 1) % ST], (uint32_t)((iv + 1) / ST) & 1, kPolls));
+        if (!SINGLE && ok && n + 1 < plan.blocks) ok = __all_sync(0xffffffffu, wait_cta(&kv_full[(iv + 1) % ST], (uint32_t)((iv + 1) / ST) & 1, kPolls));
 #pragma unroll
         for (int t = 0; t < 2; ++t)
-          if (plan.needs(t, blk)) {
+          if (SINGLE ? t == (n & 1) : plan.needs(t, blk)) {
             // (the phase before is complete, so that this arrival is not taken for one of its own)
             if (ok && cnt[t] > 0) ok = __all_sync(0xffffffffu, wait_cta(&p_ready[t], (uint32_t)(cnt[t] - 1) & 1, kPolls));
             __syncwarp();
@@ -405,17 +439,20 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax: a thread a row ----
     const int t = warp >> 2, in_tile = tid & 127, row = (t ? row1 : row0) + in_tile, pos = (t ? plan.p_lo[1] : plan.p_lo[0]) + in_tile;
-    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21), s_at = lanes + (uint32_t)t * 128, o_at = lanes + 256 + (uint32_t)t * D;
+    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21), o_at = lanes + 256 + (uint32_t)t * D;
     float ref = -INFINITY, l = 0.f;
     int done = 0;
     bool ok = true;
     const uint64_t c2 = two(a.c, a.c);
+    auto turn = [&](int n) { return SINGLE ? n & 1 : t; };                        // whose place and barriers step n of the tile takes
+    auto phase = [&](int n) { return (uint32_t)(SINGLE ? n >> 1 : n) & 1u; };
     for (int n = 0; n < plan.blocks; ++n) {
       const int blk = plan.block(n);
       if (!plan.needs(t, blk)) continue;
-      ok = __all_sync(0xffffffffu, wait_cta(&s_full[t], (uint32_t)done & 1, kPolls));
+      ok = __all_sync(0xffffffffu, wait_cta(&s_full[turn(done)], phase(done), kPolls));
       if (!ok) break;
       fence_after();
+      const uint32_t s_at = lanes + (uint32_t)turn(done) * 128;
       // A block that all queries see whole is taken with the reference as it is, scores and all in one pass: the sum tells afterwards
       // whether that was right (a maximum of more than 2^24 would be among it, and what is not finite shows).
       uint32_t p[64];
@@ -486,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
           if (grow) ref = mx;
           l *= f;
           if (done > 0) {
-            ok = __all_sync(0xffffffffu, wait_cta(&o_done[t], (uint32_t)(done - 1) & 1, kPolls));
+            ok = __all_sync(0xffffffffu, wait_cta(&o_done[turn(done - 1)], phase(done - 1), kPolls));
             if (!ok) break;
             fence_after();
 #pragma unroll 1
@@ -516,11 +553,11 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[t]);
+      if (lane == 0) mbar_arrive(&p_ready[turn(done)]);
       l += sum;
       ++done;
     }
-    if (ok && done > 0) ok = __all_sync(0xffffffffu, spin_cta(&o_done[t], (uint32_t)(done - 1) & 1));
+    if (ok && done > 0) ok = __all_sync(0xffffffffu, spin_cta(&o_done[turn(done - 1)], phase(done - 1)));
     fence_after();
     if (!ok && lane == 0 && !s_fail) failed(504);
     bool poisoned = false;
@@ -671,7 +708,7 @@ bool rows_map(CUtensorMap* m, const void* base, int64_t D, const int64_t (&shape
 
 // How many CTAs, clusters of 2, 4 and 8 of the kernel the device holds at once.
 template <int D> cudaError_t places(int (&fit)[4]) {
-  auto kern = window_attn_kernel<D>;
+  auto kern = window_attn_kernel<D, false>;
   static int cached[64][4] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -679,6 +716,7 @@ template <int D> cudaError_t places(int (&fit)[4]) {
   std::lock_guard<std::mutex> setup_lk(setup_mutex());       // first use on a device, from any thread
   if (dev < 0 || dev >= 64 || cached[dev][0] == 0) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(window_attn_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::SMEM);
     if (e != cudaSuccess) return e;
     fit[0] = sm_count();
     for (int i = 1; i < 4; ++i) {
@@ -715,34 +753,39 @@ template <int D> cudaError_t launch_d(const WindowArgs& w, cudaStream_t st) {
   const int64_t qs[3] = {w.B, w.Hq, w.Tq}, ks[3] = {w.B, w.Hkv, w.Tk};
   if (!rows_map(&m[0], w.q, D, qs, w.str[0], a.mul[0]) || !rows_map(&m[1], w.k, D, ks, w.str[1], a.mul[1]) || !rows_map(&m[2], w.v, D, ks, w.str[2], a.mul[2]))
     return cudaErrorInvalidValue;
-  auto kern = window_attn_kernel<D>;
+  auto kern = window_attn_kernel<D, false>;
   int fit[4];
   cudaError_t e = places<D>(fit);
   if (e != cudaSuccess) return e;
-  // Two tiles a CTA, as they fill the tensor cores between them.  Where that leaves SMs without work, clusters share a tile's keys, as
-  // many CTAs as the device places at once (16 clusters of 8 are more than it does: 64 queries on 8192 keys took 57 us by them and 45 by
-  // clusters of 4, 115 alone).  To join them takes as long as some five blocks, so it has to save more than that: 64 CTAs of 11
-  // blocks (512 queries, a window of 1024) take 33 us by clusters of 2 and 35 alone.  Where there are SMs still, a CTA takes one
-  // tile: its steps are no longer than those of two, which wait for each other now and then (these 64: 31 us).  Clusters come first:
-  // 256 queries of 32 heads on 4096 keys take 33 us in 128 CTAs of two tiles by clusters of 4 and 43 of one tile by clusters of 2.
+  // Two tiles a CTA, which fill the tensor cores between them, where there are enough for all SMs.  Where there are not: one tile a CTA,
+  // whose step takes 1.03 us (two tiles' 1.75), or clusters that share a tile's keys, as many as the device places at once (of 8
+  // CTAs it places fewer than 16), which takes 8 to 10 us for the join.  Of the forms that run in one wave the one that
+  // should end first is taken.  (32 query heads of 128 on 8, two tiles by clusters / one tile: 512 queries, 4099 keys, a window of 1024 35 us
+  // alone / 27 alone; without a window 51 by 2 / 48 alone; 512 on 16384 130 by 2 / 142 alone; 256 on 4096 34 by 4 / 36 by 2;
+  // 64 on 8192 46 by 4 / 35 by 4; 128 on 32768 125 by 4 / 85 by 4.)
   auto shape = [&](bool single) {
-    a.single = single;
     a.heads2 = !single && a.gqa % 2 == 0;
     const int rows = a.heads2 || single ? kTile : 2 * kTile;
     a.qblocks = (a.Tq + rows - 1) / rows;
     return (int64_t)a.qblocks * (a.heads2 ? a.Hq / 2 : a.Hq) * a.B;
   };
-  const int64_t singles = shape(true);
-  int64_t ctas = shape(false);
-  int64_t most = (w.Tk + kTile - 1) / kTile;
+  const int64_t tiles[2] = {shape(false), shape(true)};
+  int64_t most = (w.Tk + kTile - 1) / kTile;                 // steps of a tile
   if (w.window > 0) {
-    const int64_t rows = a.heads2 ? kTile : 2 * kTile, seen = (w.window + rows + kTile - 2) / kTile + 1 + (w.sinks + kTile - 1) / kTile;
+    const int64_t seen = (w.window + (int64_t)kTile + kTile - 2) / kTile + 1 + (w.sinks + kTile - 1) / kTile;
     most = most < seen ? most : seen;
   }
-  int step = 3;
-  while (step > 0 && (ctas > fit[step] || most - (most >> step) < 8)) --step;
-  a.split = 1 << step;
-  if (singles <= fit[step]) ctas = shape(true);
+  bool single = false;
+  float best = 1.7f * (float)most;
+  a.split = 1;
+  for (int one = 0; one < 2; ++one)
+    for (int i = 0; i < 4; ++i) {
+      if (tiles[one] > fit[i]) continue;
+      const float steps = (one ? 1.f : 1.7f) * (float)((most + (1 << i) - 1) >> i) + (i ? 8.f : 0.f);
+      if (steps < best) { best = steps; single = one; a.split = 1 << i; }
+    }
+  if (single) kern = window_attn_kernel<D, true>;
+  const int64_t ctas = shape(single);
   if (a.split > 1) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(ctas * a.split));
