@@ -262,3 +262,27 @@ def test_a_long_prompt_of_many_heads():
     for window, sinks in ((0, 0), (1024, 4)):
         check(qb200.window_attention(q, k, v, 128 ** -0.5, window=window, sinks=sinks), q, k, v, 128 ** -0.5, window, sinks)
     assert qb200.lib().qb200_debug_tc_status() == 0
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,Tq,Tk,D,window,sinks,lens", [
+    (1, 32, 8, 256, 4096, 128, 0, 0, None), (1, 28, 4, 250, 4099, 64, 0, 0, None), (1, 32, 8, 500, 16384, 128, 0, 0, None),
+    (4, 8, 4, 200, 4096, 128, 0, 0, [4096, 3001, 150, 0]), (1, 32, 8, 200, 6000, 128, 4000, 300, None)])
+@pytest.mark.parametrize("clusters", [True, False])
+def test_two_tiles_a_block_whose_keys_several_blocks_share(B, Hq, Hkv, Tq, Tk, D, window, sinks, lens, clusters, request):
+    """More tiles than fit one a block with as many clusters; a value that is not finite shows in the heads that see it."""
+    if not clusters:
+        request.getfixturevalue("no_clusters")
+    q, k, v = make(B, Hq, Hkv, Tq, Tk, D, Tq)
+    kl = None if lens is None else torch.tensor(lens, dtype=I32, device="cuda")
+    call = lambda v: qb200.window_attention(q, k, v, D ** -0.5, window=window, sinks=sinks, kv_lens=kl)
+    out = call(v)
+    check(out, q, k, v, D ** -0.5, window, sinks, lens)
+    bad = v.clone()
+    n = Tk if lens is None else lens[0]
+    bad[0, 1, n - 1, 5] = float("inf")                        # seen by the last query alone
+    bits = call(bad).view(torch.int16) != out.view(torch.int16)
+    g = Hq // Hkv
+    assert bool(bits[0, g:2 * g, -1].any(-1).all())
+    bits[0, g:2 * g, -1] = False
+    assert not bool(bits.any())
+    assert qb200.lib().qb200_debug_tc_status() == 0
