@@ -387,7 +387,8 @@ QB200_API int qb200_rope_kv_append_seqs(qb200_tensor* q, int dims, float base, f
 
 /* New rows of K and V into the pages of their sequences, quantised as qb200_quantize does (16 bits: as they are).
  * dense_k / dense_v [N, heads, S, D] bf16; token i of entry n goes to position positions[n] + i of sequence rows[n] (rows empty: n),
- * for i < counts[n] (counts empty: S).  Tokens whose position has no page are dropped; all other rows of the pool stay as they are.
+ * for i < counts[n] (counts empty: S).  positions[n] below 0, as qb200_kv_pages_reserve marks an entry that it refused: nothing of entry n
+ * is written.  Tokens whose position has no page are dropped; all other rows of the pool stay as they are.
  * Two tokens for one position: either one is kept. */
 QB200_API int qb200_kv_pages_append(qb200_tensor* k_q, qb200_tensor* k_scales, qb200_tensor* k_biases, qb200_tensor* v_q, qb200_tensor* v_scales,
                                     qb200_tensor* v_biases, const qb200_tensor* dense_k, const qb200_tensor* dense_v, const qb200_tensor* table,

@@ -45,8 +45,9 @@ __global__ void __launch_bounds__(256) pages_append_kernel(const __grid_constant
     raw[0] = make_uint4(e[0], e[1], e[2], e[3]); raw[1] = make_uint4(e[4], e[5], e[6], e[7]);
   }
   const int64_t row = a.rows ? a.rows[n] : (int64_t)n;
-  const int64_t pos = (int64_t)a.positions[n] + s;
-  bool live = in && row >= 0 && row < a.seqs && pos >= 0 && (pos >> a.page_shift) < a.M && (!a.counts || (int64_t)s < a.counts[n]);
+  const int64_t first = a.positions[n], pos = first + s;
+  // (below 0: an entry that reserve refused, none of whose rows has a place -- not even those whose own position would be 0 or above)
+  bool live = in && row >= 0 && row < a.seqs && first >= 0 && (pos >> a.page_shift) < a.M && (!a.counts || (int64_t)s < a.counts[n]);
   const int64_t pid = live ? a.table[row * a.table_str + (pos >> a.page_shift)] : -1;
   live = live && pid >= 0 && pid < a.P;
   if (!__any_sync(0xffffffffu, live)) return;

