@@ -5,6 +5,7 @@
 // forks, grows and frees sequences without reading anything back.  Integer work throughout: results do not depend on the order
 // in which blocks or atomics run.
 #include <cstring>
+#include <mutex>
 
 #include "kernels.h"
 #include "quant_rows.cuh"
@@ -436,12 +437,26 @@ __global__ void __launch_bounds__(256) pages_copy_kernel(const __grid_constant__
   }
 }
 
-template <typename... K, typename... A>
-cudaError_t launch_page_cluster(void (*kern)(K...), int want, size_t smem, cudaStream_t st, A... args) {
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPageSmem);
-    if (e != cudaSuccess) return e;
-  }
+// The kernel may take kPageSmem bytes on the current device: set once for each, whatever the first call needs (without it a launch has
+// 48 KB less what the kernel holds statically).
+template <auto KERN>
+cudaError_t allow_page_smem() {
+  static bool done[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> setup_lk(setup_mutex());       // first use on a device, from any thread
+  if (dev >= 0 && dev < 64 && done[dev]) return cudaSuccess;
+  e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, kPageSmem);
+  if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+  return e;
+}
+
+template <auto KERN, typename... A>
+cudaError_t launch_page_cluster(int want, size_t smem, cudaStream_t st, A... args) {
+  constexpr auto kern = KERN;
+  const cudaError_t ready = allow_page_smem<KERN>();
+  if (ready != cudaSuccess) return ready;
   if (want > 1) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)want);
@@ -480,15 +495,15 @@ cudaError_t launch_pages_free(const PageState& s, const int32_t* rows, const int
 }
 // One block's bits take 2 words per 32 pages and the list five: both fit where kMaxPages and kMaxPageList hold.
 cudaError_t launch_pages_fork(const PageState& s, const int32_t* src, const int32_t* dst, const int32_t* tokens, int n, int32_t* shared, cudaStream_t st) {
-  return launch_page_cluster(pages_fork_kernel, kStateBlocks, (size_t)n * 8, st, s, src, dst, tokens, n, shared);
+  return launch_page_cluster<pages_fork_kernel>(kStateBlocks, (size_t)n * 8, st, s, src, dst, tokens, n, shared);
 }
 cudaError_t launch_pages_reserve(const PageState& s, const int32_t* rows, const int32_t* counts, int n, int32_t* positions, int32_t* copies, cudaStream_t st) {
   const int bw = bit_words(s.P, 1);
-  return launch_page_cluster(pages_reserve_kernel, kStateBlocks, (size_t)bw * 8 + (size_t)n * 20, st, s, rows, counts, n, positions, copies, bw);
+  return launch_page_cluster<pages_reserve_kernel>(kStateBlocks, (size_t)bw * 8 + (size_t)n * 20, st, s, rows, counts, n, positions, copies, bw);
 }
 cudaError_t launch_pages_compact(const PageState& s, int32_t* remap, int32_t* moves, int64_t cap, int32_t* count, cudaStream_t st) {
   const int bw = bit_words(s.P, 1);
-  const cudaError_t e = launch_page_cluster(pages_compact_kernel, kStateBlocks, (size_t)bw * 8, st, s, remap, moves, cap, count, bw);
+  const cudaError_t e = launch_page_cluster<pages_compact_kernel>(kStateBlocks, (size_t)bw * 8, st, s, remap, moves, cap, count, bw);
   if (e != cudaSuccess || s.S == 0 || s.M == 0) return e;
   const int chunks = (s.M - 1) / kRemapChunk + 1;
   const int64_t blocks = ((int64_t)s.S * chunks + 7) / 8, most = (int64_t)sm_count() * 4;

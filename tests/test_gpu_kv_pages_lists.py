@@ -73,3 +73,28 @@ def test_an_entry_of_a_negative_position_writes_nothing(bits):
         qb200.kv_pages_append(kp, vp, x, x, table, ints(positions), bits)
         qb200.kv_pages_append(kp, vp, x, x, table, ints(positions), bits, rows=ints([3, 2, 1, 0]), counts=ints([S, S, S + 9, 0]))
         assert same(tensors(kp) + tensors(vp), before)
+
+
+def test_reserve_where_the_lists_take_the_last_of_the_usual_shared_memory():
+    """817 entries on 131072 pages: 49108 bytes, next to the 48 KB that a launch has without asking for more."""
+    st = Both(820, 3, 131072, 16)
+    st.reserve([(7 * i) % 820 for i in range(817)], [i % 49 for i in range(817)])
+    st.free(list(range(0, 820, 2)))
+    st.reserve([(11 * i) % 820 for i in range(817)], [i % 5 for i in range(817)])
+
+
+@pytest.mark.parametrize("P", [196289, 196400, 196608])
+def test_compact_where_the_pages_take_the_last_of_the_usual_shared_memory(P):
+    st = Both(40, 30, P, 16)
+    st.reserve(list(range(40)), [(97 * i) % 480 + 1 for i in range(40)])
+    st.free(list(range(0, 40, 3)))
+    st.compact()
+    st.refs.zero_()                                  # live pages all over the pool, a table entry for each
+    st.ref.refs = [0] * P
+    ids = [(i * 163 + 5) % P for i in range(1200)]
+    st.table.copy_(ints(ids).view(40, 30))
+    st.refs[torch.tensor(ids, device="cuda")] = 1
+    st.ref.table = [ids[30 * i:30 * i + 30] for i in range(40)]
+    for p in ids:
+        st.ref.refs[p] = 1
+    st.compact()
