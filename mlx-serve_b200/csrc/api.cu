@@ -41,6 +41,7 @@ int fail(int status, const char* fmt, ...) {
 }
 
 int cuda_fail(cudaError_t e, const char* what) {
+  (void)cudaGetLastError();              // (reported here, so that no later entry takes it for its own)
   return fail(QB200_ERR_CUDA, "%s: CUDA error %d (%s)", what, (int)e, cudaGetErrorString(e));
 }
 

@@ -19,7 +19,10 @@ int pg_fail(int status, const char* fmt, ...) {
   va_end(ap);
   return report_error(status, buf);
 }
-int pg_cuda(cudaError_t e, const char* who) { return pg_fail(QB200_ERR_CUDA, "%s: CUDA error %d (%s)", who, (int)e, cudaGetErrorString(e)); }
+int pg_cuda(cudaError_t e, const char* who) {
+  (void)cudaGetLastError();              // (reported here, so that no later entry takes it for its own)
+  return pg_fail(QB200_ERR_CUDA, "%s: CUDA error %d (%s)", who, (int)e, cudaGetErrorString(e));
+}
 bool empty(const qb200_tensor* t) { return t == nullptr || (t->data == nullptr && t->ndim == 0); }
 
 int elem_size(int dtype) {
