@@ -274,6 +274,8 @@ __global__ void __launch_bounds__(kPageThreads) pages_reserve_kernel(PageState s
             col = none ? have - 1 : ~(have - 1);
           }
         }
+        // (an entry that asks for more pages than there are is refused by one too many as well, and so 2048 of them stay below 2^31)
+        need = need < st.P + 1 ? need : st.P + 1;
       }
       s_len[i] = len; s_cnt[i] = c; s_col[i] = col;
     }

@@ -98,3 +98,20 @@ def test_compact_where_the_pages_take_the_last_of_the_usual_shared_memory(P):
     for p in ids:
         st.ref.refs[p] = 1
     st.compact()
+
+
+def test_reserve_of_a_list_that_asks_for_more_pages_than_an_int_counts():
+    """17 entries of 2^27 - 1 pages each, far more than the pool has: they and the later ones that need pages are refused, those before them
+    and those that need none are served."""
+    S, M, P, page = 20, 2 ** 27 - 1, 64, 16
+    table = torch.full((S, M), -1, dtype=I32, device="cuda")
+    lens, refs = ints([0] * S), ints([0] * P)
+    most = M * page - 1
+    counts = [40] + [most] * 17 + [5, 0]
+    pos, copies = qb200.kv_pages_reserve(table, lens, refs, page, ints(list(range(S))), ints(counts))
+    assert pos.tolist() == [0] + [-1] * 18 + [0] and bool((copies == -1).all())
+    assert lens.tolist() == [40] + [0] * 19 and refs.tolist() == [1] * 3 + [0] * (P - 3)
+    assert table[0, :4].tolist() == [0, 1, 2, -1]
+    table[0, :3] = -1
+    assert all(bool((row == -1).all()) for row in table)
+    assert qb200.kv_pages_reserve(table, lens, refs, page, ints([18, 19]), ints([5, 0]))[0].tolist() == [0, 0]
