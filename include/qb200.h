@@ -389,7 +389,8 @@ QB200_API int qb200_rope_kv_append_seqs(qb200_tensor* q, int dims, float base, f
  * dense_k / dense_v [N, heads, S, D] bf16; token i of entry n goes to position positions[n] + i of sequence rows[n] (rows empty: n),
  * for i < counts[n] (counts empty: S).  positions[n] below 0, as qb200_kv_pages_reserve marks an entry that it refused: nothing of entry n
  * is written.  Tokens whose position has no page are dropped; all other rows of the pool stay as they are.
- * Two tokens for one position: either one is kept. */
+ * No two tokens of a call may have one row of a page for their place (one position of a sequence named twice, or of two sequences that
+ * share the page): the row then holds parts of both, codes of one beside scales of the other; no other row is touched by it. */
 QB200_API int qb200_kv_pages_append(qb200_tensor* k_q, qb200_tensor* k_scales, qb200_tensor* k_biases, qb200_tensor* v_q, qb200_tensor* v_scales,
                                     qb200_tensor* v_biases, const qb200_tensor* dense_k, const qb200_tensor* dense_v, const qb200_tensor* table,
                                     const qb200_tensor* rows, const qb200_tensor* positions, const qb200_tensor* counts, int bits, int group_size,

@@ -353,7 +353,8 @@ def kv_append_seqs(k_triples, v_triples, dense_k, dense_v, offsets, bits, group_
 
 def kv_pages_append(k_pool, v_pool, dense_k, dense_v, table, positions, bits, group_size=64, rows=None, counts=None):
     """New rows dense_k / dense_v [N, heads, S, D] into pages: token i of entry n at position positions[n] + i of sequence rows[n]
-    (default n), for i < counts[n] (default S).  Entries with a position below 0, which ``kv_pages_reserve`` refused, write nothing."""
+    (default n), for i < counts[n] (default S).  Entries with a position below 0, which ``kv_pages_reserve`` refused, write nothing.
+    No two tokens may have the same row of a page for their place: it would hold parts of both."""
     _native.kv_pages_append(k_pool, v_pool, dense_k, dense_v, table, positions, bits, group_size, rows, counts)
 
 

@@ -115,3 +115,21 @@ def test_reserve_of_a_list_that_asks_for_more_pages_than_an_int_counts():
     table[0, :3] = -1
     assert all(bool((row == -1).all()) for row in table)
     assert qb200.kv_pages_reserve(table, lens, refs, page, ints([18, 19]), ints([5, 0]))[0].tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("bits", [4, 8, 16])
+def test_two_tokens_for_one_row_touch_no_other(bits):
+    """The row holds parts of both; every other one is written or left as ever."""
+    torch.manual_seed(bits)
+    page, H, D = 16, 3, 128
+    kp, vp = make_pool(6, H, page, D, bits), make_pool(6, H, page, D, bits)
+    want = [t.clone() for t in tensors(kp) + tensors(vp)]
+    x = torch.randn(3, H, 2, D, device="cuda").to(BF16)
+    qb200.kv_pages_append(kp, vp, x, x, ints([[2, 4], [5, 4]]), ints([15, 7, 16]), bits, rows=ints([0, 1, 1]))      # (0, 16) and (1, 16) are one row
+    new = (x,) if bits == 16 else qb200.quantize(x, 64, bits)
+    for w, t, v in zip(want, tensors(kp) + tensors(vp), new * 2):
+        w[2, :, 15], w[5, :, 7], w[5, :, 8], w[4, :, 1] = v[0, :, 0], v[1, :, 0], v[1, :, 1], v[2, :, 1]
+        row, one, two = as_ints(t[4, :, 0]), as_ints(v[0, :, 1]), as_ints(v[2, :, 0])
+        assert bool(((row == one) | (row == two)).all())
+        w[4, :, 0] = t[4, :, 0]
+    assert same(tensors(kp) + tensors(vp), want)
