@@ -15,10 +15,13 @@
 //    8 queries the B operand, so that a matrix instruction takes 256 codes (as the B operand it would take 128).  A code in the low
 //    bits of a 16-bit word IS the fp16 subnormal c * 2^-24: one AND makes an operand register; the next nibble is 16 times that.
 //    The value operand comes out of ldmatrix.m16n16.trans.b8, four tokens of a byte column a lane.
-//  * Queries are scaled by a power of two into fp16's range (exact for bf16 down to 2^-38 of the row's largest), the probabilities
-//    times the value scale are rounded once to fp16 (2^-11 relative, against 2^-8 of the bf16 result) with the softmax's reference
-//    kept low enough by the block's largest value scale; at 16 bits they stay a sum of two bf16 (16 bits).  The score tile's
-//    layout becomes the B operand of the next product by movmatrix.
+//  * Queries are scaled by a power of two into fp16's range: the row's largest lies in [2^14, 2^15), so that a bf16 is exact down to 2^-31
+//    of it (2^-27 for the odd dims at 4 bits, whose operand is a sixteenth), with an error of half of fp16's smallest step, 2^-24, below.
+//    The probabilities times the value scale are rounded once to fp16 (2^-11 relative, against 2^-8 of the bf16 result); the value
+//    scales of a group are multiplied by a power of two of the group's own that keeps p * v_scale below 2^15, so that neither the other
+//    group's size nor what is not finite there counts for it.  Tokens whose p * v_scale is so far below the largest that some query of
+//    the tile meets (2^29) that it drops under fp16's normal range keep an error of 2^-25 in its place.  At 16 bits the probabilities stay a sum of two bf16 (16 bits).  The score
+//    tile's layout becomes the B operand of the next product by movmatrix.
 //
 // Floor: the visible rows' bytes at the copy bandwidth (6.54 TB/s measured).  Sequences of 16k to 32k tokens, 16 of them, 32 query heads on 8 of
 // 128, pages of 64: 4 bits 463 MB, floor 71 us, takes 107 to 111 (4.2 to 4.3 TB/s); 8 bits 874 MB, 134 and 162 us; bf16 1.64 GB, 251 and 268 us.  At
@@ -41,6 +44,7 @@ constexpr int kRows = 8;              // queries per tile
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegBig = -1e30f;
 constexpr int kMergeWarps = 16;
+constexpr int kLowExp = 60;           // the exponent (biased by 127) that a group's value scales are taken to have at least: 2^-67
 constexpr int kPiece = 3;             // what a piece of a sequence takes beside its blocks, in blocks of a warp
 
 template <int BITS, int D> struct Geo {
@@ -85,6 +89,12 @@ __device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32
 __device__ __forceinline__ void mma_bf16_1688_z(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(b), "f"(0.f));
+}
+// bf16 pairs times bf16 pairs: exact for powers of two
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 // bf16 parameters of four consecutive tokens, G a token, each token's in one register (at G = 1 in its low half)
 template <int G> __device__ __forceinline__ void load4(uint32_t (&r)[4], const unsigned char* p) {
@@ -476,6 +486,10 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
     };
 
     float r_run[2] = {kNegBig, kNegBig}, l_part[2] = {0.f, 0.f};
+    // A group's value scales are multiplied by 2^(141 - e), e the largest exponent (biased by 127) of p * v_scale so far: as a pair of bf16,
+    // whose own biased exponents are 268 - e.
+    uint32_t v_unit = (uint32_t)(268 - kLowExp) << 7 | (G == 2 ? (uint32_t)(268 - kLowExp) << 23 : 0u);
+    auto v_exp = [&](int grp) { return 268 - (int)((v_unit >> (16 * grp + 7)) & 0xFFu); };
     float O[GE::NT][4];
     float ob[G][2];
 #pragma unroll
@@ -582,19 +596,25 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
           }
       }
       // ---------------- the block's softmax ----------------
-      int ex = 141;
-      if constexpr (BITS != 16) {      // exponent of the block's largest |v_scale|
-        uint32_t m;
+      int ex[G];                         // exponents of the block's largest |v_scale| of a group
+      bool larger = false;
+      if constexpr (BITS != 16) {
         if constexpr (G == 2) {
           const uint2 v = *(const uint2*)(sbb + 2 * GE::SB + lane * 8);
-          m = __vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu);
+          const uint32_t m = __vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu);
+          ex[0] = (int)(__reduce_max_sync(0xffffffffu, m & 0xFFFFu) >> 7);
+          ex[G - 1] = (int)(__reduce_max_sync(0xffffffffu, m >> 16) >> 7);
         } else {
-          m = *(const uint32_t*)(sbb + 2 * GE::SB + lane * 4) & 0x7FFF7FFFu;
+          const uint32_t m = *(const uint32_t*)(sbb + 2 * GE::SB + lane * 4) & 0x7FFF7FFFu;
+          ex[0] = (int)(__reduce_max_sync(0xffffffffu, max(m >> 16, m & 0xFFFFu)) >> 7);
         }
-        ex = (int)(__reduce_max_sync(0xffffffffu, max(m >> 16, m & 0xFFFFu)) >> 7);
-        ex = ex < 60 ? 60 : ex;          // (p <= 2^81: its sum stays finite over any length)
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          ex[i] = ex[i] > 254 ? 254 : ex[i];
+          larger |= ex[i] > v_exp(i);
+        }
       }
-      float mb[2];     // the least reference that this block allows: p = 2^(s - r), r >= max s + ex - 141 keeps p * v_scale below 2^15
+      float mb[2];     // the least reference that this block allows: p = 2^(s - r) <= 1
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float m = fmaxf(sc[0][c], sc[0][2 + c]);
@@ -603,14 +623,35 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        mb[c] = fmaf(m, c ? C1 : C0, (float)(ex - 141));
+        mb[c] = m * (c ? C1 : C0);
       }
-      // a reference that has to move moves 6 further, so that few blocks have to rescale (from 12 of 21 blocks of a warp to 2)
-      if (__any_sync(0xffffffffu, mb[0] > r_run[0] || mb[1] > r_run[1])) {
+      // a reference that has to move moves 6 further, an exponent 1, so that few blocks have to rescale (from 12 of 21 blocks of a warp to 2)
+      if (larger || __any_sync(0xffffffffu, mb[0] > r_run[0] || mb[1] > r_run[1])) {
         const float n0 = mb[0] > r_run[0] ? mb[0] + 6.f : r_run[0], n1 = mb[1] > r_run[1] ? mb[1] + 6.f : r_run[1];
         const float al0 = ex2(r_run[0] - n0), al1 = ex2(r_run[1] - n1);
+        float f[G];
+        if constexpr (BITS != 16) {
+          // A group's unit has to fit the largest p * v_scale.  No probability of this block is above 2^-gap, and those before shrink by
+          // 2^-rise for every query, so that large values that no query looks at, or that are forgotten, do not cost the others' bits (up
+          // to 100, so that v_scale times the unit is a bf16).  What the references' slack explains does not count, else most blocks
+          // would move the unit: 110 us for 104.
+          const int q0 = qt * kRows + 2 * t;
+          int gap = __reduce_min_sync(0xffffffffu, (int)fminf(fminf(q0 < a.gqa ? n0 - mb[0] : 100.f, q0 + 1 < a.gqa ? n1 - mb[1] : 100.f), 100.f));
+          int rise = __reduce_min_sync(0xffffffffu, (int)fminf(fminf(q0 < a.gqa ? n0 - r_run[0] : 100.f, q0 + 1 < a.gqa ? n1 - r_run[1] : 100.f), 100.f));
+          gap = gap < 16 ? 0 : gap;
+          rise = rise < 16 ? 0 : rise;
 #pragma unroll
-        for (int i = 0; i < GE::NT; ++i) { O[i][0] *= al0; O[i][1] *= al1; O[i][2] *= al0; O[i][3] *= al1; }
+          for (int grp = 0; grp < G; ++grp) {
+            const int was = v_exp(grp), before = max(was - rise, kLowExp), now = ex[grp] - gap > before ? min(ex[grp] - gap + 1, 254) : before;
+            f[grp] = pow2i(max(was - now, -126));
+            v_unit += (uint32_t)(was - now) << (16 * grp + 7);
+          }
+        } else f[0] = 1.f;
+#pragma unroll
+        for (int i = 0; i < GE::NT; ++i) {
+          const float g0 = al0 * f[i / (GE::NT / G)], g1 = al1 * f[i / (GE::NT / G)];
+          O[i][0] *= g0; O[i][1] *= g1; O[i][2] *= g0; O[i][3] *= g1;
+        }
 #pragma unroll
         for (int i = 0; i < G; ++i) { ob[i][0] *= al0; ob[i][1] *= al1; }
         l_part[0] *= al0; l_part[1] *= al1;
@@ -631,6 +672,8 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
         uint32_t vs4[4], vb4[4];
         if constexpr (BITS != 16) {
           load4<G>(vs4, sbb + 2 * GE::SB + (it * TOK + 4 * g) * G * 2);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vs4[i] = mul_bf16x2(vs4[i], v_unit);
           load4<G>(vb4, sbb + 3 * GE::SB + (it * TOK + 4 * g) * G * 2);
         }
 #pragma unroll
@@ -709,6 +752,9 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
         for (int grp = 0; grp < G; ++grp) ob[grp][c] += __shfl_xor_sync(0xffffffffu, ob[grp][c], o);
       }
     }
+    float v_back[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) v_back[i] = pow2i(v_exp(i) - 141);
     __syncthreads();      // every warp is done with its ring
     float* wm = (float*)smem;                     // [warp][8]
     float* wl = wm + kWarps * kRows;
@@ -725,10 +771,10 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
         int dim; float v = O[n][i];
         if constexpr (BITS == 4) {      // codes came in as c * 2^-24 (even dims) or 16 c * 2^-24 (odd)
           dim = 32 * (n >> 1) + 2 * m + (n & 1);
-          v = fmaf(v, (n & 1) ? 1048576.f : 16777216.f, ob[(n >> 2) % G][c]);
+          v = fmaf(v * ((n & 1) ? 1048576.f : 16777216.f), v_back[(n >> 2) % G], ob[(n >> 2) % G][c]);
         } else if constexpr (BITS == 8) {
           dim = 16 * n + m;
-          v = fmaf(v, 16777216.f, ob[(n >> 2) % G][c]);
+          v = fmaf(v * 16777216.f, v_back[(n >> 2) % G], ob[(n >> 2) % G][c]);
         } else dim = 16 * n + m;
         wo[(warp * kRows + 2 * t + c) * GE::WROW + dim] = v;
       }
