@@ -408,7 +408,9 @@ QB200_API int qb200_kv_pages_fork(qb200_tensor* shared, qb200_tensor* table, qb2
                                   const qb200_tensor* dst, const qb200_tensor* tokens, qb200_stream s);
 /* Room for counts[n] more tokens in sequence rows[n]: positions[n] = its length before, which grows by counts[n]; missing pages are
  * the free pages of the pool in ascending order, handed out in the order of the list.  A half-filled last page that others read too
- * is replaced by a fresh one: copies[n] = (old, new), else (-1, -1), for qb200_kv_pages_copy before the next change of the table.
+ * is replaced by a fresh one: copies[n] = (old, new), else (-1, -1), for qb200_kv_pages_copy before the next change of the table.  Where
+ * the half-filled last page is missing (the sequence was forked or shortened to a token whose page a window had given back), a fresh one
+ * takes its place as well: its rows in front of the sequence's end hold what the page held before, and are seen.
  * positions[n] = -1 and nothing changed where an entry is refused: no such sequence, a count below 0, listed before, beyond the table's
  * M pages, or the pool ran out (then also for all later entries that need pages).  At most 2048 entries and 2^19 pages. */
 QB200_API int qb200_kv_pages_reserve(qb200_tensor* positions, qb200_tensor* copies, qb200_tensor* table, qb200_tensor* lens, qb200_tensor* refs, int page,

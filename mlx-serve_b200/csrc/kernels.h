@@ -22,7 +22,9 @@ inline cudaError_t launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, 
 }
 
 // The same, begun while the kernel before it in the stream still runs: for kernels that wait (griddepcontrol.wait) before they read or
-// write anything, which saves the launch's own latency.
+// write anything, which saves the launch's own latency: the paged cache's calls and the prompt attention, timed each behind itself (one
+// sequence of 700 tokens 12.3 -> 9.6 us, a prompt of 77 8.2 -> 6.6).  How it does in a tick between weight-streaming kernels, where it was not
+// kept for the kernels above, is not measured.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_behind(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
   cudaLaunchConfig_t cfg = {};

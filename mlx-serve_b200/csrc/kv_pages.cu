@@ -22,7 +22,7 @@ __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;
 // Row (n, i) of head h goes to slot (pos % page) of page table[r, pos / page], pos = positions[n] + i.  16 values a thread: the four
 // (head dim 64) or eight threads of a row are neighbours, rows of one head follow each other as tokens do, so that both sides are
 // read and written in whole sectors.  A block has rows of one (sequence, K or V, head); the values are asked for before the table is
-// looked up.  Bound by the launch at one token a sequence (16 sequences of 8 heads of 128: 5 us), by instructions at prompt lengths:
+// looked up.  Bound by the launch at one token a sequence (13 sequences of 8 heads of 128: 5.5 to 6.1 us), by instructions at prompt lengths:
 // a warp's 512 values take 388, most of them to divide as the quantiser defines it, and 68 % of the issue slots are used (8192 tokens
 // of 8 heads at 8 bits, 45 MB in and out: 17.9 us, floor 6.9).
 template <int BITS>

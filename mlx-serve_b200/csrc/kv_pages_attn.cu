@@ -20,15 +20,15 @@
 //    The probabilities times the value scale are rounded once to fp16 (2^-11 relative, against 2^-8 of the bf16 result); the value
 //    scales of a group are multiplied by a power of two of the group's own that keeps p * v_scale below 2^15, so that neither the other
 //    group's size nor what is not finite there counts for it.  Tokens whose p * v_scale is so far below the largest that some query of
-//    the tile meets (2^29) that it drops under fp16's normal range keep an error of 2^-25 in its place.  At 16 bits the probabilities stay a sum of two bf16 (16 bits).  The score
-//    tile's layout becomes the B operand of the next product by movmatrix.
+//    the tile meets (2^29) that it drops under fp16's normal range keep an error of 2^-25 in its place.  At 16 bits the probabilities
+//    stay a sum of two bf16 (16 bits).  The score tile's layout becomes the B operand of the next product by movmatrix.
 //
 // Floor: the visible rows' bytes at the copy bandwidth (6.54 TB/s measured).  Sequences of 16k to 32k tokens, 16 of them, 32 query heads on 8 of
-// 128, pages of 64: 4 bits 463 MB, floor 71 us, takes 107 to 111 (4.2 to 4.3 TB/s); 8 bits 874 MB, 134 and 162 us; bf16 1.64 GB, 251 and 268 us.  At
-// 4 bits the issue slots bound it: 271 warp instructions per 16 tokens (406 before a token's four neighbours were placed for wide
+// 128, pages of 64: 4 bits 463 MB, floor 71 us, takes 104 to 112 on different GPUs (4.1 to 4.4 TB/s); 8 bits 874 MB, 134 and 156; bf16 1.64 GB, 251
+// and 258 us.  At 4 bits the issue slots bound it: 278 warp instructions per 16 tokens, 7 of them for the groups' units (406 before a token's four neighbours were placed for wide
 // scale loads and the rescaling became lazy), 56 % of the slots used with the 12 warps an SM that 168 registers leave; 128 registers
 // and 16 warps spill and take 126 to 137 us, 5 warps a CTA 127.  Short calls wait for dependent reads (lengths, table, rows) and the
-// join: one sequence of 700 tokens takes 9.6 us, 12.3 before the kernels were launched behind one another.
+// join: one sequence of 700 tokens takes 9.7 to 10.1 us, 12.3 before the kernels were launched behind one another.
 #include <mutex>
 #include <type_traits>
 
@@ -214,8 +214,9 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_pages_kernel(const __grid_c
 
   // The cut: an even share of all units for every CTA, or every sequence in the same number of parts, whichever ends first by blocks a
   // warp walks and what a piece takes beside them (about kPiece blocks' time): even shares cut long ragged batches best, parts keep a
-  // CTA from working on the ends of two short sequences.  (16 sequences of 16k to 32k tokens: 112 us by even shares, 132 in parts; 48 of
-  // 1k to 2k: 44 and 38; 32 windows of 1024 tokens at 16 bits: 34 and 28; 13 of 4k to 8k: 40 and 38.)
+  // CTA from working on the ends of two short sequences.  (By even shares and in parts, us: 16 sequences of 16k to 32k tokens 110 and 122; 48
+  // of 1k to 2k 41 and 31; 32 windows of 1024 tokens at 16 bits 24.4 and 18.3; 13 of 4k to 8k at 8 bits 32.1 and 28.6; one of 700 tokens 13.8
+  // and 10.1; these go by the better one.  4 of 4k to 8k, 16.4 and 18.3, go in parts: the estimate is off there.)
   const int U = L.all, ctas = (int)gridDim.x, seqs = a.B * a.tiles;
   int per = (U + ctas - 1) / ctas;
   per = per < a.min_units ? a.min_units : per;

@@ -21,7 +21,8 @@
 // wait for the softmax alone: 1.03 us a step), or clusters share a tile's keys and join their sums through distributed shared memory.
 //
 // Floor: 4 D operations per visible pair on the tensor cores.  32 heads of 128, 16384 tokens, window 4096: 0.96 TFLOP, 589 us at 1634
-// TFLOP/s, takes 811 us (1.19 PFLOP/s, 0.73 of the measured peak).  A step of a tile is a chain: softmax of 128 keys 1400 cycles, P V and
+// TFLOP/s, takes 955 us pass after pass, where the power cap holds the clock down (1.01 PFLOP/s, 0.62 of the measured burst peak), 820 with a
+// pause before each (1.17 PFLOP/s, 0.72).  The variants below were timed with pauses, against 811.  A step of a tile is a chain: softmax of 128 keys 1400 cycles, P V and
 // S 512 each, 450 of hand-over; the other tile fills part of it, and the tensor cores work for 2048 of every 3100 cycles.  Tried and
 // not kept: 16 softmax warps (845 us), scores in halves of 64 keys made ahead (1040: a product of 64 columns takes as long as
 // one of 128), an issuer for each tile (870: they fall into step and wait together), the first half of P handed over early (862).
@@ -38,7 +39,7 @@ __device__ int g_window_error = 0;   // 0 = ok; otherwise the code of the wait t
 constexpr int kThreads = 384;
 constexpr int kTile = 128;           // queries of a tile, keys of a block
 constexpr uint32_t kPolls = 1u << 18, kSpins = 1u << 23;
-constexpr int kPolyOf8 = 2;          // pairs of 8 whose exponentials the fp32 units work out
+constexpr int kPolyOf8 = 2;          // pairs of 8 whose exponentials the fp32 units work out (chosen at head dim 128)
 constexpr float kMostSum = 16777216.f;   // of a block's probabilities, with the reference as it was
 constexpr float kSlack = 8.f;        // exponents that the reference may lie below the maximum
 
@@ -762,7 +763,8 @@ template <int D> cudaError_t launch_d(const WindowArgs& w, cudaStream_t st) {
   // CTAs it places fewer than 16), which takes 8 to 10 us for the join.  Of the forms that run in one wave the one that
   // should end first is taken.  (32 query heads of 128 on 8, two tiles by clusters / one tile: 512 queries, 4099 keys, a window of 1024 35 us
   // alone / 27 alone; without a window 51 by 2 / 48 alone; 512 on 16384 130 by 2 / 142 alone; 256 on 4096 34 by 4 / 36 by 2;
-  // 64 on 8192 46 by 4 / 35 by 4; 128 on 32768 125 by 4 / 85 by 4.)
+  // 64 on 8192 46 by 4 / 35 by 4; 128 on 32768 125 by 4 / 85 by 4.  All at head dim 128; at 64, where a step and a join move half as much,
+  // the same constants choose, unmeasured.)
   auto shape = [&](bool single) {
     a.heads2 = !single && a.gqa % 2 == 0;
     const int rows = a.heads2 || single ? kTile : 2 * kTile;

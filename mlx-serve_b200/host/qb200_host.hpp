@@ -277,7 +277,7 @@ struct PagedCache {
   int page = 64;             // tokens of a page
   std::vector<PagePool> layers;
 };
-// Room for counts[n] more tokens in sequence rows[n]; a half-filled page that others read too is copied in every layer.
+// Pages pairs[n][0] to pairs[n][1] in every pool of every layer.
 inline void pagesCopy(PagedCache& c, const Array& pairs, const Array* count, qb200_stream s) {
   std::vector<qb200_tensor*> pools;
   for (PagePool& l : c.layers)
@@ -286,6 +286,7 @@ inline void pagesCopy(PagedCache& c, const Array& pairs, const Array* count, qb2
         if (a->t.data) pools.push_back(&a->t);
   check(qb200_kv_pages_copy(pools.data(), (int)pools.size(), &pairs.t, count ? &count->t : nullptr, s));
 }
+// Room for counts[n] more tokens in sequence rows[n]; a half-filled page that others read too is copied in every layer.
 inline void pagesReserve(PagedCache& c, Array& positions, Array& copies, const Array& rows, const Array& counts, qb200_stream s) {
   check(qb200_kv_pages_reserve(&positions.t, &copies.t, &c.table.t, &c.lens.t, &c.refs.t, c.page, &rows.t, &counts.t, s));
   pagesCopy(c, copies, nullptr, s);
