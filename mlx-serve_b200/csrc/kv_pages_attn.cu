@@ -24,11 +24,12 @@
 //    stay a sum of two bf16 (16 bits).  The score tile's layout becomes the B operand of the next product by movmatrix.
 //
 // Floor: the visible rows' bytes at the copy bandwidth (6.54 TB/s measured).  Sequences of 16k to 32k tokens, 16 of them, 32 query heads on 8 of
-// 128, pages of 64: 4 bits 463 MB, floor 71 us, takes 104 to 112 on different GPUs (4.1 to 4.4 TB/s); 8 bits 874 MB, 134 and 156; bf16 1.64 GB, 251
-// and 258 us.  At 4 bits the issue slots bound it: 278 warp instructions per 16 tokens, 7 of them for the groups' units (406 before a token's four neighbours were placed for wide
-// scale loads and the rescaling became lazy), 56 % of the slots used with the 12 warps an SM that 168 registers leave; 128 registers
-// and 16 warps spill and take 126 to 137 us, 5 warps a CTA 127.  Short calls wait for dependent reads (lengths, table, rows) and the
-// join: one sequence of 700 tokens takes 9.7 to 10.1 us, 12.3 before the kernels were launched behind one another.
+// 128, pages of 64: 4 bits 463 MB, floor 71 us, takes 104 to 112 on different GPUs (4.1 to 4.4 TB/s); 8 bits 874 MB, 134 and 156; bf16
+// 1.64 GB, 251 and 258.  At 4 bits the issue slots bound it: 278 warp instructions per 16 tokens, 7 of them for the groups' units (406 before
+// a token's four neighbours were placed for wide scale loads and the rescaling became lazy), 56 % of the slots used with the 12 warps
+// an SM that 168 registers leave; 128 registers and 16 warps spill and take 126 to 137 us, 5 warps a CTA 127.  Short calls wait for
+// dependent reads (lengths, table, rows) and the join: one sequence of 700 tokens takes 9.7 to 10.1 us, 12.3 before the kernels were launched
+// behind one another.
 #include <mutex>
 #include <type_traits>
 
