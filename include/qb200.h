@@ -434,6 +434,43 @@ QB200_API int qb200_kv_pages_decode_attention(qb200_tensor* res, const qb200_ten
                                               int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes, qb200_stream s);
 QB200_API size_t qb200_kv_pages_decode_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
 
+/* ---- drafted tokens over a paged cache: a round of speculative decoding ----
+ * The drafted tokens of a sequence are the nodes of a tree and the sequence's last n = counts[b] tokens (empty: T; at most T and the
+ * sequence's length): reserved and appended like any others, node t at place len - n + t, up to 64 of them.  parents [B, T] int32:
+ * the node before, which has a lower number (any other: the node stands behind the cached tokens).  A chain is parents[t] = t - 1. */
+/* Attention of all nodes at once over the pages: node t stands at position p = len - n + (nodes before it on its line) and sees the cached
+ * tokens, itself and the nodes before it on its line; with a window > 0 those at positions > p - window or < sinks.  q, res [B, Hq, T, D]
+ * bf16, D 64 or 128; tree b belongs to sequence rows[b] (empty: b).  Nodes at or behind n and nodes that see nothing give zeros.  What no
+ * node sees may hold anything; a node that sees a key or value which is not finite gives results that are not.  Otherwise as
+ * qb200_kv_pages_decode_attention, the workspace too. */
+QB200_API int qb200_kv_pages_tree_attention(qb200_tensor* res, const qb200_tensor* q, const qb200_tensor* k_q, const qb200_tensor* k_scales,
+                                            const qb200_tensor* k_biases, const qb200_tensor* v_q, const qb200_tensor* v_scales, const qb200_tensor* v_biases,
+                                            const qb200_tensor* table, const qb200_tensor* rows, const qb200_tensor* lens, const qb200_tensor* parents,
+                                            const qb200_tensor* counts, int bits, int group_size, float scale, int64_t window, int64_t sinks, void* workspace,
+                                            size_t workspace_bytes, qb200_stream s);
+QB200_API size_t qb200_kv_pages_tree_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D);
+/* A token from every row of logits [N, V] (bf16, f16 or f32; sampleTokenLazy, src/generate.zig:6929), by a random number in [0, 1) of the
+ * row's own.  With m the row's largest logit, w_i = exp((l_i - m) / temperature) and the order "larger first, equal ones by index": the first
+ * top_k of the order stay (0 or less: all), of these the fewest whose weights reach top_p of their sum (at least one; 1 or more: all),
+ * of these the ones with w_i >= min_p (and the first); the token is the first, by index, at which the running sum of what stays passes
+ * random times the whole.  A temperature that is not above 0 takes the first of the order.  Sums and borders are those of 64-bit
+ * arithmetic to 2^-45 of the largest weight.  temperature, random, top_p, min_p f32 and top_k int32, [N] on the device, of any stride
+ * (0: one for all); all but random may be empty (1, 0, 1, 0).  tokens [N] int32, -1 for a row of -inf alone (a NaN counts as -inf); logprobs
+ * [N] f32 (or empty): log softmax of the row at the token, before temperature and filters (0 beside -1).  V up to 2^19. */
+QB200_API int qb200_sample(qb200_tensor* tokens, qb200_tensor* logprobs, const qb200_tensor* logits, const qb200_tensor* random,
+                           const qb200_tensor* temperature, const qb200_tensor* top_k, const qb200_tensor* top_p, const qb200_tensor* min_p, qb200_stream s);
+/* Which drafted tokens the samples confirm: from node 0 (the last token that was certain) to the lowest child whose token is the one
+ * sampled behind it, and on from there.  tokens, sampled [B, T] int32: of every node, and sampled from its logits.  path [B, T] = the nodes
+ * passed, next [B, T] = the tokens sampled behind them (the new tokens; the last one is the next round's node 0), -1 behind both;
+ * accepted [B] = how many; ends [B] = the length that the sequence has with them alone.  In every pool [pages, heads, page, cols] (codes,
+ * scales and biases of all layers) the rows of the path's nodes move to the places behind the cached tokens, in the path's order; lens
+ * stays, and qb200_kv_pages_free(begin = ends) gives back the rest.  A sequence that does not exist, or is listed again, has accepted 0
+ * (and ends at 0, or its length).  At most 1024 trees.  No page of the drafted tokens may be another sequence's too, which
+ * qb200_kv_pages_reserve sees to. */
+QB200_API int qb200_kv_pages_accept(qb200_tensor* path, qb200_tensor* next, qb200_tensor* accepted, qb200_tensor* ends, qb200_tensor* const* pools, int num_pools,
+                                    const qb200_tensor* table, const qb200_tensor* lens, int page, const qb200_tensor* rows, const qb200_tensor* parents,
+                                    const qb200_tensor* tokens, const qb200_tensor* sampled, const qb200_tensor* counts, qb200_stream s);
+
 /* ---- causal attention of a prompt, or of a chunk behind cached tokens, with a sliding window and sinks ----
  * The dense attention of the reference's prefill (mlx_fast_scaled_dot_product_attention, src/mlx.zig:325; its window as the mask of the
  * sliding layers).  q, res [B, Hq, Tq, D], k, v [B, Hkv, Tk, D], all bf16, D 64 or 128, rows of q, k and v on 16 bytes.  Sequence b has

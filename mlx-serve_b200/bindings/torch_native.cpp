@@ -715,6 +715,81 @@ PyObject* kv_pages_decode_attention(Args a) {
   return a[12] == Py_None ? wrap(std::move(out)) : ret(a[12]);
 }
 
+// q, k_pool, v_pool, table, lens, parents, bits, group_size, scale, window, sinks, rows, counts, workspace, out
+PyObject* kv_pages_tree_attention(Args a) {
+  OnDevice dev;
+  const int nb = (int)as_long(a[6]), gs = (int)as_long(a[7]);
+  PagePool k(a[1], nb, dev), v(a[2], nb, dev);
+  for (int i : {0, 3, 4, 5, 11, 12, 13, 14}) dev.add(a[i]);
+  const at::Tensor& q = tensor(a[0]);
+  const float scale = (float)as_double(a[8]);
+  const int64_t window = as_index(a[9]), sinks = as_index(a[10]);
+  void* st = dev.stream();
+  at::Tensor out = a[14] == Py_None ? at::empty(q.sizes(), q.options().requires_grad(false)) : tensor(a[14]), ws;
+  if (a[13] == Py_None) {
+    const bool known = q.dim() == 4 && k.codes->dim() == 4;
+    const size_t need = known ? qb200_kv_pages_tree_attention_workspace_size(q.size(0), q.size(1), k.codes->size(1), q.size(2), q.size(3)) : 0;
+    ws = empty({(int64_t)(need > 16 ? need : 16)}, q, at::kByte);
+  } else {
+    ws = tensor(a[13]);
+    if (!ws.is_contiguous()) throw std::invalid_argument("qb200: the workspace must be contiguous");
+  }
+  T y = plain(out), dq = plain(q), t = plain(a[3]), l = plain(a[4]), p = plain(a[5]), r = plain(a[11]), c = plain(a[12]);
+  void* wp = ws.data_ptr();
+  const size_t wn = (size_t)ws.nbytes();
+  call([&] {
+    return qb200_kv_pages_tree_attention(&y.d, &dq.d, &k.d[0].d, &k.d[1].d, &k.d[2].d, &v.d[0].d, &v.d[1].d, &v.d[2].d, &t.d, &r.d, &l.d, &p.d, &c.d, nb, gs,
+                                         scale, window, sinks, wp, wn, st);
+  });
+  return a[14] == Py_None ? wrap(std::move(out)) : ret(a[14]);
+}
+
+// pools, table, lens, page, parents, tokens, sampled, rows, counts
+PyObject* kv_pages_accept(Args a) {
+  OnDevice dev;
+  Seq list(a[0]);
+  const Py_ssize_t n = list.size();
+  std::vector<T> d((size_t)n);
+  std::vector<qb200_tensor*> p((size_t)n);
+  for (int i : {1, 2, 4, 5, 6, 7, 8}) dev.add(a[i]);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    dev.add(tensor(list[i]));
+    d[i] = plain(list[i]);
+    p[i] = &d[i].d;
+  }
+  T t = plain(a[1]), l = plain(a[2]), pa = plain(a[4]), to = plain(a[5]), sa = plain(a[6]), r = plain(a[7]), c = plain(a[8]);
+  const int page = (int)as_long(a[3]);
+  void* st = dev.stream();
+  const at::Tensor& parents = tensor(a[4]);
+  const int64_t B = parents.dim() > 0 ? parents.size(0) : 0;
+  at::Tensor path = empty(parents.sizes(), parents, at::kInt), next = empty(parents.sizes(), parents, at::kInt), accepted = empty({B}, parents, at::kInt),
+             ends = empty({B}, parents, at::kInt);
+  T dp = plain(path), dn = plain(next), da = plain(accepted), de = plain(ends);
+  call([&] {
+    return qb200_kv_pages_accept(&dp.d, &dn.d, &da.d, &de.d, p.data(), (int)n, &t.d, &l.d, page, &r.d, &pa.d, &to.d, &sa.d, &c.d, st);
+  });
+  return pack({wrap(std::move(path)), wrap(std::move(next)), wrap(std::move(accepted)), wrap(std::move(ends))});
+}
+
+// logits, random, temperature, top_k, top_p, min_p, want_logprobs
+PyObject* sample(Args a) {
+  OnDevice dev;
+  for (int i : {0, 1, 2, 3, 4, 5}) dev.add(a[i]);
+  const at::Tensor& x = tensor(a[0]);
+  const bool want = as_bool(a[6]);
+  void* st = dev.stream();
+  const int64_t N = x.dim() > 0 ? x.size(0) : 0;
+  at::Tensor tokens = empty({N}, x, at::kInt), logprobs;
+  T dx = plain(x), r = plain(a[1]), te = plain(a[2]), k = plain(a[3]), p = plain(a[4]), m = plain(a[5]), dt = plain(tokens), dl;
+  dl.none();
+  if (want) {
+    logprobs = empty({N}, x, at::kFloat);
+    dl = plain(logprobs);
+  }
+  call([&] { return qb200_sample(&dt.d, &dl.d, &dx.d, &r.d, &te.d, &k.d, &p.d, &m.d, st); });
+  return want ? pack({wrap(std::move(tokens)), wrap(std::move(logprobs))}) : wrap(std::move(tokens));
+}
+
 // q, k, v, scale, window, sinks, kv_lens, out
 PyObject* window_attention(Args a) {
   OnDevice dev;
@@ -745,6 +820,7 @@ PyMethodDef methods[] = {
     QB_ENTRY(rope, 6), QB_ENTRY(turbo_rotate, 3), QB_ENTRY(swiglu, 3), QB_ENTRY(kv_append_seqs, 11), QB_ENTRY(set_error_class, 1),
     QB_ENTRY(kv_pages_append, 10), QB_ENTRY(kv_pages_free, 7), QB_ENTRY(kv_pages_fork, 7), QB_ENTRY(kv_pages_reserve, 6), QB_ENTRY(kv_pages_compact, 2),
     QB_ENTRY(kv_pages_copy, 3), QB_ENTRY(kv_pages_decode_attention, 13), QB_ENTRY(window_attention, 8),
+    QB_ENTRY(kv_pages_tree_attention, 15), QB_ENTRY(kv_pages_accept, 9), QB_ENTRY(sample, 7),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native half of the qb200 Python binding", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

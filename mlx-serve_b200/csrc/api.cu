@@ -688,6 +688,46 @@ QB200_API int qb200_moe_route(qb200_tensor* inds, qb200_tensor* norm_scores, con
   return QB200_OK;
 }
 
+QB200_API int qb200_sample(qb200_tensor* tokens, qb200_tensor* logprobs, const qb200_tensor* logits, const qb200_tensor* random,
+                           const qb200_tensor* temperature, const qb200_tensor* top_k, const qb200_tensor* top_p, const qb200_tensor* min_p,
+                           qb200_stream s) {
+  int st;
+  if ((st = check_tensor(logits, "sample: logits", 2))) return st;
+  if (logits->ndim != 2) return fail(QB200_ERR_BAD_SHAPE, "sample: logits must be [N, V]");
+  if (!is_float_dtype(logits->dtype)) return fail(QB200_ERR_UNSUPPORTED, "sample: logits must be bf16, f16 or f32");
+  const int64_t N = logits->shape[0], V = logits->shape[1];
+  if ((uintptr_t)logits->data % dtype_size(logits->dtype)) return fail(QB200_ERR_BAD_STRIDE, "sample: logits do not start on their elements' size");
+  // per row: values that may repeat (stride 0), results that may not
+  struct { const qb200_tensor* t; const char* name; int dtype; bool needed, result; } const lists[7] = {
+      {random, "random", QB200_FLOAT32, true, false}, {temperature, "temperature", QB200_FLOAT32, false, false}, {top_k, "top_k", QB200_INT32, false, false},
+      {top_p, "top_p", QB200_FLOAT32, false, false}, {min_p, "min_p", QB200_FLOAT32, false, false}, {tokens, "tokens", QB200_INT32, true, true},
+      {logprobs, "logprobs", QB200_FLOAT32, false, true}};
+  SampleArgs a;
+  std::memset(&a, 0, sizeof(a));
+  for (int i = 0; i < 7; ++i) {
+    const auto& l = lists[i];
+    if (!l.needed && is_empty(l.t)) continue;
+    if (l.t == nullptr) return fail(QB200_ERR_BAD_ARG, "sample: %s: null tensor", l.name);
+    if (l.t->ndim != 1 || l.t->shape[0] != N) return fail(QB200_ERR_BAD_SHAPE, "sample: %s must be [N]", l.name);
+    if (l.t->dtype != l.dtype) return fail(QB200_ERR_BAD_DTYPE, "sample: %s has dtype %d, expected %d", l.name, l.t->dtype, l.dtype);
+    if (N > 0 && l.t->data == nullptr) return fail(QB200_ERR_BAD_ARG, "sample: %s: null data pointer", l.name);
+    if ((uintptr_t)l.t->data % 4) return fail(QB200_ERR_BAD_STRIDE, "sample: %s does not start on its elements' size", l.name);
+    if (l.t->stride[0] < 0 || (l.result && N > 1 && l.t->stride[0] != 1)) return fail(QB200_ERR_BAD_STRIDE, "sample: %s has stride %lld", l.name, (long long)l.t->stride[0]);
+    if (i < 5) a.str[i] = l.t->stride[0];
+  }
+  if (V < 1 || V > kMaxVocab) return fail(QB200_ERR_UNSUPPORTED, "sample: rows of %lld logits are not served (1 to %d)", (long long)V, kMaxVocab);
+  if (N > (1 << 24)) return fail(QB200_ERR_UNSUPPORTED, "sample: %lld rows are too many for one call", (long long)N);
+  if (N == 0) return QB200_OK;
+  auto at = [](const qb200_tensor* t) { return is_empty(t) ? nullptr : t->data; };
+  a.logits = logits->data; a.row_bytes = logits->stride[0] * dtype_size(logits->dtype);
+  a.random = (const float*)random->data; a.temperature = (const float*)at(temperature); a.top_k = (const int32_t*)at(top_k);
+  a.top_p = (const float*)at(top_p); a.min_p = (const float*)at(min_p);
+  a.tokens = (int32_t*)tokens->data; a.logprobs = (float*)at(logprobs);
+  a.N = (int)N; a.V = (int)V; a.dtype = logits->dtype;
+  const cudaError_t e = launch_sample(a, (cudaStream_t)s);
+  return e == cudaSuccess ? QB200_OK : cuda_fail(e, "sample");
+}
+
 QB200_API int qb200_moe_sort_by_expert(qb200_tensor* order, qb200_tensor* inv_order, qb200_tensor* sorted_inds,
                                        qb200_tensor* token_rows, qb200_tensor* expert_offsets, const qb200_tensor* inds,
                                        int num_experts, qb200_stream s) {

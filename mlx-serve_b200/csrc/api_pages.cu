@@ -1,4 +1,4 @@
-// C ABI of the paged key-value cache and of windowed prompt attention: argument validation and dispatch (include/qb200.h).
+// C ABI of the paged key-value cache, of drafted trees over it and of windowed prompt attention: argument validation and dispatch (include/qb200.h).
 // As in the other entries everything is checked on the host before any CUDA call; what only the device knows (page numbers,
 // lengths, listed sequences) is checked by the kernels, which skip what lies outside the tensors.
 #include <cstdarg>
@@ -55,6 +55,13 @@ int expect(const qb200_tensor* t, const char* who, const char* name, int ndim, i
 int expect_list(const qb200_tensor* t, const char* who, const char* name, int64_t n) {
   if (int st = expect(t, who, name, 1, QB200_INT32)) return st;
   if (t->shape[0] != n) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: %s has %lld entries, expected %lld", who, name, (long long)t->shape[0], (long long)n);
+  return 0;
+}
+// A list for the nodes of every tree: [B, T], rows any distance apart.
+int expect_tree(const qb200_tensor* t, const char* who, const char* name, int64_t B, int64_t T) {
+  if (int st = expect(t, who, name, 2, QB200_INT32)) return st;
+  if (t->shape[0] != B || t->shape[1] != T)
+    return pg_fail(QB200_ERR_BAD_SHAPE, "%s: %s is [%lld, %lld], expected [%lld, %lld]", who, name, (long long)t->shape[0], (long long)t->shape[1], (long long)B, (long long)T);
   return 0;
 }
 // What a kernel writes: no two elements may be the same memory.  Axes by growing stride, each has to reach over all that the smaller
@@ -359,17 +366,20 @@ QB200_API size_t qb200_kv_pages_decode_attention_workspace_size(int64_t B, int64
   return kv_pages_workspace_bytes(D);
 }
 
-QB200_API int qb200_kv_pages_decode_attention(qb200_tensor* res, const qb200_tensor* q, const qb200_tensor* k_q, const qb200_tensor* k_scales,
-                                              const qb200_tensor* k_biases, const qb200_tensor* v_q, const qb200_tensor* v_scales, const qb200_tensor* v_biases,
-                                              const qb200_tensor* table, const qb200_tensor* rows, const qb200_tensor* lens, int bits, int group_size, float scale,
-                                              int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes, qb200_stream s) {
-  const char* who = "kv_pages_decode_attention";
+// What the attentions over pages have in common: q and res [B, Hq, 1 .. most_nodes, D], the pools, the table and the lengths.
+static int parse_attention(KvPagesAttnArgs& a, bool* nothing, const char* who, int most_nodes, const qb200_tensor* res, const qb200_tensor* q,
+                           const qb200_tensor* k_q, const qb200_tensor* k_scales, const qb200_tensor* k_biases, const qb200_tensor* v_q,
+                           const qb200_tensor* v_scales, const qb200_tensor* v_biases, const qb200_tensor* table, const qb200_tensor* rows,
+                           const qb200_tensor* lens, int bits, int group_size, float scale, int64_t window, int64_t sinks) {
   int st;
-  if (q == nullptr || q->ndim != 4) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: q must be [B, Hq, 1, D]", who);
+  std::memset(&a, 0, sizeof(a));
+  if (q == nullptr || q->ndim != 4) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: q must be [B, Hq, %s, D]", who, most_nodes == 1 ? "1" : "T");
   if (q->dtype != QB200_BFLOAT16) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: q must be bf16", who);
   if ((st = expect(q, who, "q", 4, QB200_BFLOAT16)) || (st = expect(res, who, "res", 4, QB200_BFLOAT16))) return st;
   const int64_t B = q->shape[0], Hq = q->shape[1], D = q->shape[3];
-  if (q->shape[2] != 1) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: T_q=%lld (only one new token is served)", who, (long long)q->shape[2]);
+  if (most_nodes == 1 ? q->shape[2] != 1 : q->shape[2] < 1 || q->shape[2] > most_nodes)
+    return most_nodes == 1 ? pg_fail(QB200_ERR_UNSUPPORTED, "%s: T_q=%lld (only one new token is served)", who, (long long)q->shape[2])
+                           : pg_fail(QB200_ERR_UNSUPPORTED, "%s: %lld nodes a tree are not served (1 to %d)", who, (long long)q->shape[2], most_nodes);
   for (int d = 0; d < 4; ++d)
     if (res->shape[d] != q->shape[d]) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: res must have q's shape", who);
   if ((st = check_format(who, bits, group_size, D))) return st;
@@ -380,8 +390,6 @@ QB200_API int qb200_kv_pages_decode_attention(qb200_tensor* res, const qb200_ten
   if (page > 65536) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: pages of %lld tokens are not served (a power of two from 16 to 65536)", who, (long long)page);
   PageState ps;
   if ((st = parse_state(&ps, who, table, nullptr, nullptr, (int)page))) return st;
-  KvPagesAttnArgs a;
-  std::memset(&a, 0, sizeof(a));
   bool vec[2];
   if ((st = parse_pool(&a.pool[0], &vec[0], who, "K", k_q, k_scales, k_biases, bits, P, Hkv, page, D)) ||
       (st = parse_pool(&a.pool[1], &vec[1], who, "V", v_q, v_scales, v_biases, bits, P, Hkv, page, D)))
@@ -394,17 +402,14 @@ QB200_API int qb200_kv_pages_decode_attention(qb200_tensor* res, const qb200_ten
   if (!(scale >= -3.0e38f && scale <= 3.0e38f)) return pg_fail(QB200_ERR_BAD_ARG, "%s: scale must be finite", who);
   if (window < 0 || sinks < 0) return pg_fail(QB200_ERR_BAD_ARG, "%s: window and sinks must not be negative", who);
   if (!distinct(res)) return pg_fail(QB200_ERR_BAD_STRIDE, "%s: rows of res overlap", who);
-  if (B == 0 || Hq == 0) return QB200_OK;
+  *nothing = B == 0 || Hq == 0;
+  if (*nothing) return QB200_OK;
   if (P < 1) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: the pool holds no pages", who);
   if (P > INT32_MAX || B > kMaxPageSeqs) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: %lld sequences are not served (at most %d)", who, (long long)B, kMaxPageSeqs);
-  const int64_t gqa = Hq / Hkv, tiles = Hkv * ((gqa + 7) / 8), most = (((int64_t)ps.M << ps.page_shift) + 63) / 64;
+  const int64_t gqa = Hq / Hkv, tiles = Hkv * ((gqa * q->shape[2] + 7) / 8), most = (((int64_t)ps.M << ps.page_shift) + 63) / 64;
   if (Hq > 65536 || B * tiles * most > INT32_MAX)
     return pg_fail(QB200_ERR_UNSUPPORTED, "%s: %lld sequences of %lld heads and up to %lld tokens are too many for one call", who, (long long)B, (long long)Hq,
                    (long long)ps.M << ps.page_shift);
-  const size_t need = kv_pages_workspace_bytes(D);
-  if (workspace == nullptr || workspace_bytes < need)
-    return pg_fail(QB200_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace_bytes);
-  if ((uintptr_t)workspace & 15) return pg_fail(QB200_ERR_WORKSPACE, "%s: the workspace must start on 16 bytes", who);
   a.q = q->data; a.out = res->data;
   a.q_vec = ((uintptr_t)q->data & 15) == 0;
   for (int d = 0; d < 2; ++d) {
@@ -423,8 +428,146 @@ QB200_API int qb200_kv_pages_decode_attention(qb200_tensor* res, const qb200_ten
   a.window = (int)(window < INT32_MAX ? window : 0);      // (no sequence is longer: everything is inside)
   a.sinks = (int)(sinks < INT32_MAX ? sinks : INT32_MAX);
   a.bits = bits; a.scale = scale; a.sb_vec = vec[0] && vec[1];
+  return QB200_OK;
+}
+static int check_workspace(const char* who, const void* workspace, size_t given, size_t need) {
+  if (workspace == nullptr || given < need) return pg_fail(QB200_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, given);
+  if ((uintptr_t)workspace & 15) return pg_fail(QB200_ERR_WORKSPACE, "%s: the workspace must start on 16 bytes", who);
+  return QB200_OK;
+}
+
+QB200_API int qb200_kv_pages_decode_attention(qb200_tensor* res, const qb200_tensor* q, const qb200_tensor* k_q, const qb200_tensor* k_scales,
+                                              const qb200_tensor* k_biases, const qb200_tensor* v_q, const qb200_tensor* v_scales, const qb200_tensor* v_biases,
+                                              const qb200_tensor* table, const qb200_tensor* rows, const qb200_tensor* lens, int bits, int group_size, float scale,
+                                              int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes, qb200_stream s) {
+  const char* who = "kv_pages_decode_attention";
+  int st;
+  KvPagesAttnArgs a;
+  bool nothing = false;
+  if ((st = parse_attention(a, &nothing, who, 1, res, q, k_q, k_scales, k_biases, v_q, v_scales, v_biases, table, rows, lens, bits, group_size, scale, window, sinks)))
+    return st;
+  if (nothing) return QB200_OK;
+  const int64_t D = q->shape[3];
+  if ((st = check_workspace(who, workspace, workspace_bytes, kv_pages_workspace_bytes(D)))) return st;
   const cudaError_t e = launch_kv_pages_attn(a, (int)D, workspace, (cudaStream_t)s);
   return e == cudaSuccess ? QB200_OK : pg_cuda(e, who);
+}
+
+QB200_API size_t qb200_kv_pages_tree_attention_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || T < 1 || T > kMaxNodes || (D != 64 && D != 128)) return 0;
+  return kv_pages_tree_workspace_bytes(B, Hq, Hkv, T, D);
+}
+
+QB200_API int qb200_kv_pages_tree_attention(qb200_tensor* res, const qb200_tensor* q, const qb200_tensor* k_q, const qb200_tensor* k_scales,
+                                            const qb200_tensor* k_biases, const qb200_tensor* v_q, const qb200_tensor* v_scales, const qb200_tensor* v_biases,
+                                            const qb200_tensor* table, const qb200_tensor* rows, const qb200_tensor* lens, const qb200_tensor* parents,
+                                            const qb200_tensor* counts, int bits, int group_size, float scale, int64_t window, int64_t sinks, void* workspace,
+                                            size_t workspace_bytes, qb200_stream s) {
+  const char* who = "kv_pages_tree_attention";
+  int st;
+  KvPagesTreeArgs t;
+  std::memset(&t, 0, sizeof(t));
+  bool nothing = false;
+  if ((st = parse_attention(t.a, &nothing, who, kMaxNodes, res, q, k_q, k_scales, k_biases, v_q, v_scales, v_biases, table, rows, lens, bits, group_size, scale,
+                            window, sinks)))
+    return st;
+  const int64_t B = q->shape[0], Hq = q->shape[1], T = q->shape[2], D = q->shape[3];
+  if ((st = expect_tree(parents, who, "parents", B, T))) return st;
+  if (!empty(counts)) {
+    if ((st = expect_list(counts, who, "counts", B))) return st;
+    t.counts = (const int32_t*)counts->data;
+  }
+  if (nothing) return QB200_OK;
+  if ((st = check_workspace(who, workspace, workspace_bytes, kv_pages_tree_workspace_bytes(B, Hq, k_q->shape[1], T, D)))) return st;
+  t.parents = (const int32_t*)parents->data; t.par_str = parents->stride[0];
+  t.T = (int)T; t.q_tok = q->stride[2]; t.o_tok = res->stride[2];
+  if (T > 1 && q->stride[2] % 8 != 0) t.a.q_vec = 0;
+  const cudaError_t e = launch_kv_pages_tree(t, (int)D, workspace, (cudaStream_t)s);
+  return e == cudaSuccess ? QB200_OK : pg_cuda(e, who);
+}
+
+QB200_API int qb200_kv_pages_accept(qb200_tensor* path, qb200_tensor* next, qb200_tensor* accepted, qb200_tensor* ends, qb200_tensor* const* pools, int num_pools,
+                                    const qb200_tensor* table, const qb200_tensor* lens, int page, const qb200_tensor* rows, const qb200_tensor* parents,
+                                    const qb200_tensor* tokens, const qb200_tensor* sampled, const qb200_tensor* counts, qb200_stream s) {
+  const char* who = "kv_pages_accept";
+  int st;
+  PageState ps;
+  if (num_pools < 0 || (num_pools > 0 && pools == nullptr)) return pg_fail(QB200_ERR_BAD_ARG, "%s: null pool list", who);
+  if (lens == nullptr) return pg_fail(QB200_ERR_BAD_ARG, "%s: lens are needed", who);
+  if ((st = parse_state(&ps, who, table, lens, nullptr, page)) || (st = expect(parents, who, "parents", 2, QB200_INT32))) return st;
+  const int64_t B = parents->shape[0], T = parents->shape[1];
+  if (T < 1 || T > kMaxNodes) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: %lld nodes a tree are not served (1 to %d)", who, (long long)T, kMaxNodes);
+  if (B > kMaxPageSeqs) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: %lld sequences are not served (at most %d)", who, (long long)B, kMaxPageSeqs);
+  const qb200_tensor* const lists[3] = {parents, tokens, sampled};
+  const char* const names[5] = {"parents", "tokens", "sampled", "path", "next"};
+  qb200_tensor* const wide[2] = {path, next};
+  PagesAcceptArgs a;
+  std::memset((void*)&a, 0, sizeof(a));
+  for (int i = 0; i < 3; ++i) {
+    if ((st = expect_tree(lists[i], who, names[i], B, T))) return st;
+    a.lists[i] = (const int32_t*)lists[i]->data; a.list_str[i] = lists[i]->stride[0];
+  }
+  for (int i = 0; i < 2; ++i) {
+    if ((st = expect_tree(wide[i], who, names[3 + i], B, T))) return st;
+    if (B > 1 && wide[i]->stride[0] != T) return pg_fail(QB200_ERR_BAD_STRIDE, "%s: %s must be contiguous", who, names[3 + i]);
+  }
+  if ((st = expect_list(accepted, who, "accepted", B)) || (st = expect_list(ends, who, "ends", B))) return st;
+  if (!empty(rows)) {
+    if ((st = expect_list(rows, who, "rows", B))) return st;
+    a.rows = (const int32_t*)rows->data;
+  } else if (ps.S != B) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: %lld trees for a table of %d sequences (pass rows)", who, (long long)B, ps.S);
+  if (!empty(counts)) {
+    if ((st = expect_list(counts, who, "counts", B))) return st;
+    a.counts = (const int32_t*)counts->data;
+  }
+  a.table = ps.table; a.table_str = ps.table_str; a.lens = ps.lens;
+  a.seqs = ps.S; a.M = ps.M; a.page_shift = ps.page_shift; a.B = (int)B; a.T = (int)T;
+  const int launches = num_pools > kMaxCopyPools ? (num_pools + kMaxCopyPools - 1) / kMaxCopyPools : 1;
+  for (int pass = 0; pass < 2; ++pass) {                       // every pool is checked before the first launch
+    for (int l = 0; l < launches; ++l) {
+      const int p0 = l * kMaxCopyPools, p1 = p0 + kMaxCopyPools < num_pools ? p0 + kMaxCopyPools : num_pools;
+      uint64_t bits = 0;                                       // every address, stride and row, or-ed: what they are all multiples of
+      for (int i = p0; i < p1; ++i) {
+        const qb200_tensor* t = pools[i];
+        if (t == nullptr || t->ndim != 4) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: pool %d must be [pages, heads, page, cols]", who, i);
+        const int esz = elem_size(t->dtype);
+        if (esz == 0) return pg_fail(QB200_ERR_BAD_DTYPE, "%s: pool %d has dtype %d", who, i, t->dtype);
+        if (pass == 0) {
+          if ((st = expect(t, who, "pool", 4, t->dtype))) return st;
+          if (t->shape[0] != pools[0]->shape[0])
+            return pg_fail(QB200_ERR_BAD_SHAPE, "%s: pool %d holds %lld pages, pool 0 %lld", who, i, (long long)t->shape[0], (long long)pools[0]->shape[0]);
+          if (t->shape[2] != page) return pg_fail(QB200_ERR_BAD_SHAPE, "%s: pool %d has pages of %lld tokens, expected %d", who, i, (long long)t->shape[2], page);
+          if (!distinct(t)) return pg_fail(QB200_ERR_BAD_STRIDE, "%s: rows of pool %d overlap", who, i);
+          if (t->shape[1] > 65536 || t->shape[3] > 65536) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: pool %d has %lld heads of %lld columns", who, i,
+                                                                         (long long)t->shape[1], (long long)t->shape[3]);
+        }
+        bits |= (uint64_t)(uintptr_t)t->data | (uint64_t)(t->shape[3] * esz);
+        for (int d = 0; d < 3; ++d) bits |= t->shape[d] > 1 ? (uint64_t)(t->stride[d] * esz) : 0;
+      }
+      const int vec = bits % 16 == 0 ? 16 : (bits % 4 == 0 ? 4 : (bits % 2 == 0 ? 2 : 1));
+      int64_t cols = 0;
+      a.pools = 0;
+      for (int i = p0; i < p1; ++i) {
+        const qb200_tensor* t = pools[i];
+        const int esz = elem_size(t->dtype);
+        const int64_t vecs = t->shape[3] * esz / vec;
+        if (vecs * t->shape[1] == 0 || t->shape[0] == 0) continue;
+        AcceptPool& p = a.pool[a.pools++];
+        p.base = (char*)t->data;
+        p.page_str = t->stride[0] * esz; p.head_str = t->stride[1] * esz; p.tok_str = t->stride[2] * esz;
+        p.vecs = (int)vecs; p.first = (int)cols;
+        cols += vecs * t->shape[1];
+        if (cols > INT32_MAX) return pg_fail(QB200_ERR_UNSUPPORTED, "%s: rows of so many heads are not served in one call", who);
+      }
+      a.cols = (int)cols; a.P = num_pools ? pools[0]->shape[0] : 0;
+      if (pass == 0 || B == 0) continue;
+      a.path = l ? nullptr : (int32_t*)path->data; a.next = (int32_t*)next->data;
+      a.accepted = (int32_t*)accepted->data; a.ends = (int32_t*)ends->data;
+      const cudaError_t e = launch_pages_accept(a, vec, (cudaStream_t)s);
+      if (e != cudaSuccess) return pg_cuda(e, who);
+    }
+  }
+  return QB200_OK;
 }
 
 QB200_API int qb200_window_attention(qb200_tensor* res, const qb200_tensor* q, const qb200_tensor* k, const qb200_tensor* v, float scale, int64_t window,

@@ -359,6 +359,47 @@ struct KvPagesAttnArgs {
 size_t kv_pages_workspace_bytes(int64_t D);
 cudaError_t launch_kv_pages_attn(KvPagesAttnArgs a, int D, void* workspace, cudaStream_t st);
 
+// ---- kv_pages_tree.cu: attention of a tree of drafted tokens over pages ----
+constexpr int kMaxNodes = 64;            // nodes of a tree
+struct KvPagesTreeArgs {
+  KvPagesAttnArgs a;                     // (its workspace pointers and what its launcher sets are not used)
+  int64_t q_tok, o_tok;                  // strides from node to node
+  const int32_t* parents; int64_t par_str;
+  const int32_t* counts;                 // may be null
+  int T;
+};
+size_t kv_pages_tree_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D);
+cudaError_t launch_kv_pages_tree(KvPagesTreeArgs a, int D, void* workspace, cudaStream_t st);
+
+// ---- kv_pages.cu: the walk through drafted trees, and the rows of the nodes that stay ----
+// A pool's rows: `vecs` vectors a (head, token), strides in bytes.
+struct AcceptPool {
+  char* base; int64_t page_str, head_str, tok_str;
+  int vecs, first;                       // first: of the launch's (head, vector) columns
+};
+template <int N> struct PagesAcceptList {
+  const int32_t* table; int64_t table_str;
+  const int32_t* lens; const int32_t* rows; const int32_t* counts;   // rows, counts may be null
+  const int32_t* lists[3]; int64_t list_str[3];                      // parents, tokens, sampled: [B, T]
+  int32_t* path; int32_t* next; int32_t* accepted; int32_t* ends;    // path, next: contiguous [B, T]; null where another launch wrote them
+  int64_t P;
+  int seqs, M, page_shift, B, T, pools, cols, blocks;
+  AcceptPool pool[N];
+};
+using PagesAcceptArgs = PagesAcceptList<kMaxCopyPools>;
+cudaError_t launch_pages_accept(const PagesAcceptArgs& a, int vec, cudaStream_t st);   // vec: bytes of a vector (16, 4, 2, 1)
+
+// ---- sample.cu: a token from every row of logits ----
+struct SampleArgs {
+  const void* logits; int64_t row_bytes;
+  const float* random; const float* temperature; const int32_t* top_k; const float* top_p; const float* min_p;   // all but random may be null
+  int64_t str[5];                        // from row to row of the five
+  int32_t* tokens; float* logprobs;      // logprobs may be null
+  int N, V, dtype;
+};
+constexpr int kMaxVocab = 1 << 19;
+cudaError_t launch_sample(const SampleArgs& a, cudaStream_t st);
+
 // ---- window_attn.cu: causal attention of a prompt, sliding window and sinks ----
 struct WindowArgs {
   const void* q; const void* k; const void* v; void* out;

@@ -4,6 +4,7 @@
 // lens the tokens, refs how many table entries name a page (0: free).  All three live on the device, so that a serving loop
 // forks, grows and frees sequences without reading anything back.  Integer work throughout: results do not depend on the order
 // in which blocks or atomics run.
+#include <cstddef>
 #include <cstring>
 #include <mutex>
 
@@ -439,6 +440,97 @@ __global__ void __launch_bounds__(256) pages_copy_kernel(const __grid_constant__
   }
 }
 
+// ---------------------------------------------------------------- the nodes of drafted trees that stay
+// The walk: from node 0 to the first child that carries the token sampled behind it, and on from there.  A warp holds the tree, two nodes
+// a lane, and finds a child with two ballots; every block walks again, so that one launch does it all.  A path's nodes ascend and stand
+// at or behind the places they go to, path[i] >= i: taken in ascending order, no row is overwritten that is still to be read, and a
+// thread's column of a row (16 bytes of one head in one pool) needs no other thread.  Eight rows are asked for at a time.
+template <typename V, int N>
+__global__ void __launch_bounds__(256) pages_accept_kernel(const __grid_constant__ PagesAcceptList<N> a) {
+  __shared__ int s_path[kMaxNodes], s_pid[kMaxNodes + 1][2], s_n;   // of a place: its page and the page of the node that goes there
+  grid_wait();
+  const int b = (int)(blockIdx.x / (unsigned)a.blocks), part = (int)(blockIdx.x - (unsigned)b * (unsigned)a.blocks), tid = threadIdx.x;
+  const int64_t row = a.rows ? a.rows[b] : (int64_t)b;
+  const bool known = row >= 0 && row < a.seqs;
+  int64_t len = known ? a.lens[row] : 0;
+  const int64_t cap = (int64_t)a.M << a.page_shift;
+  len = len < 0 ? 0 : (len > cap ? cap : len);
+  bool again = false;                                  // (a sequence listed before: its rows move once)
+  if (a.rows)
+    for (int j = tid; j < b; j += 256) again |= a.rows[j] == row;
+  again = __syncthreads_or(again);
+  int64_t n64 = a.counts ? a.counts[b] : a.T;
+  n64 = n64 < 0 ? 0 : (n64 > a.T ? a.T : n64);
+  const int n = again ? 0 : (int)(n64 > len ? len : n64);
+  const int64_t base = len - n;
+  if (tid < 32) {
+    int parent[2], token[2], behind[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = tid + 32 * h;
+      parent[h] = -1; token[h] = 0; behind[h] = 0;
+      if (i < n) {
+        parent[h] = a.lists[0][b * a.list_str[0] + i];
+        token[h] = a.lists[1][b * a.list_str[1] + i];
+        behind[h] = a.lists[2][b * a.list_str[2] + i];
+      }
+      if (parent[h] >= i) parent[h] = -1;              // (no parent stands at its node or behind it)
+    }
+    int at = 0, len_path = 0;
+    while (len_path < n) {                             // (nodes ascend: at most n steps)
+      const int want = __shfl_sync(0xffffffffu, at & 32 ? behind[1] : behind[0], at & 31);
+      if (tid == 0) s_path[len_path] = at;
+      if (part == 0 && a.path != nullptr && tid == 0) { a.path[(int64_t)b * a.T + len_path] = at; a.next[(int64_t)b * a.T + len_path] = want; }
+      ++len_path;
+      const uint32_t lo = __ballot_sync(0xffffffffu, parent[0] == at && token[0] == want), hi = __ballot_sync(0xffffffffu, parent[1] == at && token[1] == want);
+      if ((lo | hi) == 0) break;
+      at = lo ? __ffs(lo) - 1 : 31 + __ffs(hi);
+    }
+    if (part == 0 && a.path != nullptr) {
+      for (int i = len_path + tid; i < a.T; i += 32) { a.path[(int64_t)b * a.T + i] = -1; a.next[(int64_t)b * a.T + i] = -1; }
+      if (tid == 0) { a.accepted[b] = len_path; a.ends[b] = (int32_t)(base + len_path); }
+    }
+    __syncwarp();
+    const int32_t* const tab = a.table + row * a.table_str;
+    for (int i = tid; i < len_path; i += 32) {
+      const int64_t to = base + i, from = base + s_path[i];
+      int p0 = tab[to >> a.page_shift], p1 = tab[from >> a.page_shift];
+      if (p0 >= a.P) p0 = -1;
+      if (p1 >= a.P) p1 = -1;
+      s_pid[i][0] = p0; s_pid[i][1] = from == to ? -1 : p1;
+    }
+    if (tid == 0) s_n = len_path;
+  }
+  __syncthreads();
+  const int rows = s_n;
+  const int mask = (1 << a.page_shift) - 1;
+  for (int c = part * 256 + tid; c < a.cols; c += a.blocks * 256) {
+    int lo = 0, hi = a.pools - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (a.pool[mid].first <= c) lo = mid; else hi = mid - 1;
+    }
+    const AcceptPool& p = a.pool[lo];
+    const int in = c - p.first, head = in / p.vecs;
+    char* const column = p.base + (int64_t)head * p.head_str + (int64_t)(in - head * p.vecs) * (int64_t)sizeof(V);
+#pragma unroll 1
+    for (int i0 = 0; i0 < rows; i0 += 8) {
+      V v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = i0 + k;
+        if (i < rows && s_pid[i][0] >= 0 && s_pid[i][1] >= 0)
+          v[k] = *(const V*)(column + (int64_t)s_pid[i][1] * p.page_str + ((base + s_path[i]) & mask) * p.tok_str);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = i0 + k;
+        if (i < rows && s_pid[i][0] >= 0 && s_pid[i][1] >= 0) *(V*)(column + (int64_t)s_pid[i][0] * p.page_str + ((base + i) & mask) * p.tok_str) = v[k];
+      }
+    }
+  }
+}
+
 // The kernel may take kPageSmem bytes on the current device: set once for each, whatever the first call needs (without it a launch has
 // 48 KB less what the kernel holds statically).
 template <auto KERN>
@@ -529,5 +621,24 @@ cudaError_t launch_pages_copy(const PagesCopyArgs& a, int vec, cudaStream_t st) 
   return a.pools <= 12 ? launch_copy<12>(a, vec, st) : launch_copy<kMaxCopyPools>(a, vec, st);
 }
 int pages_copy_piece() { return kCopyPiece; }
+
+template <int N> cudaError_t launch_accept(const PagesAcceptArgs& a, int vec, cudaStream_t st) {
+  PagesAcceptList<N> k;
+  std::memcpy((void*)&k, (const void*)&a, offsetof(PagesAcceptArgs, pool));
+  std::memcpy(k.pool, a.pool, sizeof(AcceptPool) * (size_t)a.pools);
+  // blocks a sequence: a column a thread, as far as the device has room for at once
+  const int64_t need = ((int64_t)a.cols + 255) / 256, most = (int64_t)sm_count() * 8 / a.B;
+  k.blocks = (int)(need < 1 ? 1 : (need < most ? need : (most < 1 ? 1 : most)));
+  const dim3 grid((unsigned)((int64_t)k.blocks * a.B));
+  switch (vec) {
+    case 16: return launch_behind(pages_accept_kernel<uint4, N>, grid, dim3(256), 0, st, k);
+    case 4: return launch_behind(pages_accept_kernel<uint32_t, N>, grid, dim3(256), 0, st, k);
+    case 2: return launch_behind(pages_accept_kernel<uint16_t, N>, grid, dim3(256), 0, st, k);
+    default: return launch_behind(pages_accept_kernel<uint8_t, N>, grid, dim3(256), 0, st, k);
+  }
+}
+cudaError_t launch_pages_accept(const PagesAcceptArgs& a, int vec, cudaStream_t st) {
+  return a.pools <= 12 ? launch_accept<12>(a, vec, st) : launch_accept<kMaxCopyPools>(a, vec, st);
+}
 
 }  // namespace qb

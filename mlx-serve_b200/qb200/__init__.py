@@ -157,9 +157,15 @@ def lib():
         L.qb200_kv_pages_decode_attention.argtypes = [TP] * 11 + [C.c_int, C.c_int, C.c_float, C.c_int64, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]
         L.qb200_kv_pages_decode_attention_workspace_size.argtypes = [C.c_int64] * 4
         L.qb200_kv_pages_decode_attention_workspace_size.restype = C.c_size_t
+        L.qb200_kv_pages_tree_attention.argtypes = [TP] * 13 + [C.c_int, C.c_int, C.c_float, C.c_int64, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]
+        L.qb200_kv_pages_tree_attention_workspace_size.argtypes = [C.c_int64] * 5
+        L.qb200_kv_pages_tree_attention_workspace_size.restype = C.c_size_t
+        L.qb200_kv_pages_accept.argtypes = [TP] * 4 + [C.POINTER(TP), C.c_int, TP, TP, C.c_int] + [TP] * 5 + [C.c_void_p]
+        L.qb200_sample.argtypes = [TP] * 8 + [C.c_void_p]
+        L.qb200_sample.restype = C.c_int
         L.qb200_window_attention.argtypes = [TP] * 4 + [C.c_float, C.c_int64, C.c_int64, TP, C.c_void_p]
         L.qb200_window_attention.restype = C.c_int
-        for name in ("append", "free", "fork", "reserve", "compact", "copy", "decode_attention"):
+        for name in ("append", "free", "fork", "reserve", "compact", "copy", "decode_attention", "tree_attention", "accept"):
             getattr(L, "qb200_kv_pages_" + name).restype = C.c_int
         for name in ("qb200_rms_norm", "qb200_add_rms_norm", "qb200_rope", "qb200_swiglu", "qb200_kv_append_seqs"):
             getattr(L, name).restype = C.c_int
@@ -395,6 +401,32 @@ def kv_pages_decode_attention(q, k_pool, v_pool, table, lens, bits, group_size, 
     """Attention of one new token per sequence over its pages; q [B, Hq, 1, D] bf16, query b of sequence rows[b] (default b).  With a
     window the query sees the last ``window`` tokens and the first ``sinks``."""
     return _native.kv_pages_decode_attention(q, k_pool, v_pool, table, lens, bits, group_size, scale, window, sinks, rows, workspace, out)
+
+
+def kv_pages_tree_attention_workspace_size(B, Hq, Hkv, T, D) -> int:
+    return int(lib().qb200_kv_pages_tree_attention_workspace_size(B, Hq, Hkv, T, D))
+
+
+def kv_pages_tree_attention(q, k_pool, v_pool, table, lens, parents, bits, group_size, scale, window=0, sinks=0, rows=None, counts=None, workspace=None,
+                            out=None):
+    """Attention of a tree of drafted tokens per sequence over its pages; q [B, Hq, T, D] bf16, T up to 64 nodes, the sequence's last
+    counts[b] tokens (default T).  parents [B, T] int32: the node before each, -1 behind the cached tokens.  A node sees the cached tokens,
+    itself and the nodes before it on its line, with a window those at the last ``window`` positions and the first ``sinks``."""
+    return _native.kv_pages_tree_attention(q, k_pool, v_pool, table, lens, parents, bits, group_size, scale, window, sinks, rows, counts, workspace, out)
+
+
+def kv_pages_accept(pools, table, lens, page, parents, tokens, sampled, rows=None, counts=None):
+    """The nodes of drafted trees that the samples confirm (from node 0 on, each the lowest child that carries the token sampled behind its
+    parent), and their rows moved together in every tensor of the list ``pools`` [pages, heads, page, cols].  Returns (path, next, accepted,
+    ends): the nodes, the tokens sampled behind them, how many, and the length for ``kv_pages_free(..., begin=ends)``."""
+    return _native.kv_pages_accept(pools, table, lens, page, parents, tokens, sampled, rows, counts)
+
+
+def sample(logits, random, temperature=None, top_k=None, top_p=None, min_p=None, want_logprobs=False):
+    """A token from every row of logits [N, V] by its number random[n] in [0, 1) (sampleTokenLazy, src/generate.zig:6929): temperature, then
+    top-k, top-p and min-p, each a tensor [N] (top_k int32, the others fp32) or None.  With want_logprobs (tokens, logprobs): of the token by
+    the logits as they are."""
+    return _native.sample(logits, random, temperature, top_k, top_p, min_p, want_logprobs)
 
 
 def window_attention(q, k, v, scale, window=0, sinks=0, kv_lens=None, out=None):
