@@ -224,7 +224,7 @@ QB200_API void qb200_set_error_handler(qb200_error_handler_func handler, void* d
 QB200_API const char* qb200_last_error(void) { return g_last_error.c_str(); }
 QB200_API const char* qb200_version(void) { return "qb200 0.1 (sm_100a)"; }
 QB200_API int qb200_debug_tc_status(void) {
-  for (int code : {qmm_tc_error_code(), qmm_pair_error_code(), qmv_f16_error_code(), qmv_tmem_error_code(), window_attn_error_code()})
+  for (int code : {qmm_tc_error_code(), qmm_pair_error_code(), qmv_f16_error_code(), qmv_tmem_error_code(), window_attn_error_code(), tree_attn_error_code()})
     if (code) return code;
   return qmv_wide_error_code();
 }
@@ -235,6 +235,7 @@ QB200_API void qb200_debug_tc_reset(void) {
   qmm_pair_error_reset();
   qmv_tmem_error_reset();
   window_attn_error_reset();
+  tree_attn_error_reset();
 }
 
 QB200_API void qb200_debug_wait_polls(int polls) { wait_polls() = polls; }

@@ -370,6 +370,8 @@ struct KvPagesTreeArgs {
 };
 size_t kv_pages_tree_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D);
 cudaError_t launch_kv_pages_tree(KvPagesTreeArgs a, int D, void* workspace, cudaStream_t st);
+void tree_attn_error_reset();
+int tree_attn_error_code();    // 0, or the code of a bounded wait that expired in it
 
 // ---- kv_pages.cu: the walk through drafted trees, and the rows of the nodes that stay ----
 // A pool's rows: `vecs` vectors a (head, token), strides in bytes.

@@ -1,92 +1,1011 @@
-// Attention of a tree of drafted tokens over a paged key-value cache: a warp a query row, one pass over the tokens that some node may see.
-#include "kernels.h"
+// Attention of a tree of drafted tokens over a paged key-value cache, 4- or 8-bit codes or bf16 rows, head dim 64 or 128, with an
+// optional window and a few first tokens that stay visible, on the tensor cores (tcgen05) with keys, scores and results in tensor memory.
+//
+// Node t of a sequence stands at position p(t) = base + depth(t) behind `base` cached tokens; it sees the cached tokens, itself and the
+// nodes before it on its line (with a window those at positions > p(t) - window or < sinks).
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c s_j - r),  s = q . k, c = scale * log2(e), r a running reference of the row.
+//
+// A tile is N (16, 32 or 64) query rows of one cache head: nodes times the heads of its group, node after node, so that a tree with few nodes
+// fills few tiles.  The products are transposed, S^T = K Q^T and O^T = V^T P^T: the 128 tokens of a block are the rows (lanes), the queries the
+// columns, so that a product takes time in proportion to N, a thread of the softmax has one token, and what belongs to a token is a
+// register of its thread:
+//  * Codes are dequantised to fp16, rounded once, in a unit of the token's own (a power of two, its largest |q s + b| in [2^14, 2^15)), so that the
+//    range of fp16 holds for each token by itself; a key's unit is a factor of its thread's scores, a value's goes to its probabilities: P' = p * unit, and the
+//    row's sum takes P' / unit.  Tokens and groups 2^28 apart in size keep fp16's 11 bits.  At 16 bits the operands are the cache's bf16.
+//  * r moves only where some P' would pass 2^15: then it is placed 2^8 below the block's maximum, and O is rescaled.
+//  * Roles of a CTA's warps: four a 32 columns of the softmax; four read keys and dequantise them into tensor memory (the A operand of S^T); four
+//    read values and dequantise them into shared memory; one issues the products, S^T two blocks ahead of O^T.  A warp's codes come through a cp.async
+//    ring of its own, page numbers a block ahead; at 16 bits the ring's slots are the operands themselves.
+//  * The grid is one CTA an SM; every CTA works out all sequences' blocks from `lens` and takes an even share of them, or every tile is cut in the
+//    same number of parts.  Parts of a tile go to the workspace and are joined by a second kernel.
+#include <mutex>
+#include <type_traits>
+
 #include "stream_ptx.cuh"
+#include "tc_ptx.cuh"
 
 namespace qb {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+__device__ int g_tree_error = 0;     // 0 = ok; otherwise the code of the wait that expired
 
-template <int BITS, int D>
-__global__ void __launch_bounds__(256) tree_simple_kernel(const __grid_constant__ KvPagesTreeArgs t) {
+constexpr int kBlk = 128;            // tokens of a block
+constexpr uint32_t kPolls = 1u << 18, kSpins = 1u << 23;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegBig = -1e30f;
+constexpr float kTop = 15.f, kAim = 8.f;   // exponents of P': the reference moves above the first, and then aims at the second
+constexpr int kLowExp = -80, kHighExp = 113;   // of a token's largest value, beyond which its unit does not follow
+constexpr int kNotes = 2 * kMaxNodes;       // the drafted tokens, and where a window begins the tokens that its deepest node sees no more
+constexpr int kPiece = 5;            // what a piece of a tile takes beside its blocks, in blocks
+constexpr int kJoinRows = 8, kJoinWarps = 16;
+
+template <int BITS, int D, int N> struct Shape {
+  static constexpr int G = BITS == 16 ? 1 : D / 64;          // scale groups of a token
+  static constexpr int HALVES = D / 64;                      // blocks of 64 columns (128 bytes) side by side
+  static constexpr int ROWB = D * BITS / 8, CH = ROWB / 16;  // bytes of a token, 16-byte chunks of it
+  static constexpr int NC = N < 32 ? N : 32;                 // columns of a softmax warp
+  static constexpr int WGS = N / NC, SW = 4 * WGS;           // groups of four softmax warps
+  static constexpr int THREADS = (SW + 9) * 32;
+  static constexpr int TILE = kBlk * 128 * HALVES;           // a block's keys or values as an operand
+  static constexpr int STAGES = BITS == 4 ? 4 : (BITS == 8 ? 3 : (D == 64 ? 4 : 2));
+  static constexpr int VT = BITS == 16 ? STAGES : 2, KT = BITS == 16 ? STAGES : 0;
+  static constexpr int PS = BITS == 8 && D == 128 ? 1 : 2;   // places for P
+  static constexpr int PTILE = kBlk * 128;
+  static constexpr int SB = 32 * G * 2;                      // bytes of a warp's scales (or biases) of a block
+  static constexpr int RS = BITS == 16 ? 0 : 32 * ROWB + 4 * SB;
+  static constexpr int V0 = 0, K0 = VT * TILE, Q0 = K0 + KT * TILE, P0 = Q0 + N * 128 * HALVES, R0 = P0 + PS * PTILE;
+  static constexpr int SMEM = R0 + 8 * STAGES * RS + 1024;
+  static_assert(SMEM + 2 * (kMaxPageSeqs + 1) * 4 + 12 * 1024 <= 227 * 1024, "shared memory");
+  static constexpr uint32_t S_AT = 0, O_AT = 128, K_AT = 192;   // columns of tensor memory: two of S, O, two of K
+};
+
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accum) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(accum) : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bd, uint32_t idesc, uint32_t accum) {   // A in tensor memory
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(bd), "r"(idesc), "r"(accum) : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                 "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+               ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+                 "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+               : "memory");
+}
+template <int NC> __device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t (&r)[NC]) {
+  if constexpr (NC == 32) tmem_ld32(taddr, r); else tmem_ld16(taddr, r);
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+template <int NC> __device__ __forceinline__ void tmem_put(uint32_t taddr, const uint32_t (&r)[NC]) {
+  if constexpr (NC == 32) tmem_st32(taddr, r); else tmem_st16(taddr, r);
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ bool bar_any(int id, int n, bool v) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbar.red.or.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(r) : "r"(id), "r"(n), "r"((uint32_t)v) : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {   // (a NaN does not count)
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// A bounded wait that polls without sleeping.
+__device__ __forceinline__ bool spin_cta(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  for (uint32_t it = 0; it < kSpins; ++it) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(addr), "r"(parity) : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+// Rows of 128 bytes with their 64 columns contiguous, swizzled, as an operand whose columns are its M or N: 8 rows 1024 bytes apart, the next
+// 64 columns a block of 128 rows further.
+__device__ __forceinline__ uint64_t make_desc_mn(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+  d |= (uint64_t)((kBlk * 128) >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+// The largest |code * s + b| of a group, and its unit: values times 2^(14 - e) lie below 2^15.  What is not finite does not count.
+template <int BITS> __device__ __forceinline__ float group_top(float s, float b) { return fmaxf(fabsf(b), fabsf(fmaf(s, (float)((1 << (BITS & 15)) - 1), b))); }
+__device__ __forceinline__ int unit_exp(float top) {
+  const int e = (int)(__float_as_uint(top) >> 23) - 127;
+  return e < kLowExp ? kLowExp : (e > kHighExp ? kHighExp : e);
+}
+// Codes of a packed word as fp16 values c * s + b, rounded once: a code in the low bits of 1024, or at 4 bits a nibble further up of 64, is exact,
+// and so is taking that away.  Pairs come out of a word in the order its bits allow: dims 0 4, 1 5, 2 6, 3 7 at 4 bits, 0 2, 1 3 at 8.
+template <int BITS> __device__ __forceinline__ void dequant_word(uint32_t w, __half2 s, __half2 b, uint32_t* o) {
+  const __half2 c1024 = __float2half2_rn(1024.f), c64 = __float2half2_rn(64.f);
+  auto out = [&](uint32_t bits, __half2 off) {
+    const __half2 v = __hfma2(__hsub2(*(const __half2*)&bits, off), s, b);
+    return *(const uint32_t*)&v;
+  };
+  if constexpr (BITS == 4) {
+    const uint32_t w8 = w >> 8;
+    o[0] = out(lop3_and_or(w, 0x000F000Fu, 0x64006400u), c1024);
+    o[1] = out(lop3_and_or(w, 0x00F000F0u, 0x54005400u), c64);
+    o[2] = out(lop3_and_or(w8, 0x000F000Fu, 0x64006400u), c1024);
+    o[3] = out(lop3_and_or(w8, 0x00F000F0u, 0x54005400u), c64);
+  } else {
+    o[0] = out(lop3_and_or(w, 0x00FF00FFu, 0x64006400u), c1024);
+    o[1] = out(lop3_and_or(w >> 8, 0x00FF00FFu, 0x64006400u), c1024);
+  }
+}
+// the dim that stands at a place of the operands
+template <int BITS> __device__ __forceinline__ int dim_at(int place) {
+  if constexpr (BITS == 4) return (place & ~7) | ((place & 1) << 2) | ((place >> 1) & 3);
+  else if constexpr (BITS == 8) return (place & ~3) | ((place & 1) << 1) | ((place >> 1) & 1);
+  else return place;
+}
+
+// A sequence's tree, and the blocks that its nodes see: [0, front) and, from there on, block i + skip.
+struct Seq {
+  int row, base, n, len, w0, sinks, front, skip, blocks, tiles;
+};
+__device__ __forceinline__ Seq seq_of(const KvPagesTreeArgs& t, int b, int N) {
   const KvPagesAttnArgs& a = t.a;
-  constexpr int E = D / 32;
-  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (w >= (int64_t)a.B * a.Hq * t.T) return;
-  const int node = (int)(w % t.T), h = (int)(w / t.T % a.Hq), b = (int)(w / t.T / a.Hq), hk = h / a.gqa;
+  Seq s;
   const int64_t row = a.rows ? a.rows[b] : b;
-  int64_t len = row >= 0 && row < a.seqs ? a.lens[row] : 0;
+  const bool known = row >= 0 && row < a.seqs;
+  int64_t len = known ? a.lens[row] : 0, n = t.counts ? t.counts[b] : t.T;
   const int64_t cap = (int64_t)a.M << a.page_shift;
   len = len < 0 ? 0 : (len > cap ? cap : len);
-  int64_t n = t.counts ? t.counts[b] : t.T;
   n = n < 0 ? 0 : (n > t.T ? t.T : n);
   n = n > len ? len : n;
-  const int64_t base = len - n;
-  uint16_t* out = (uint16_t*)a.out + (int64_t)b * a.o_str[0] + (int64_t)h * a.o_str[1] + (int64_t)node * t.o_tok;
-  const uint16_t* q = (const uint16_t*)a.q + (int64_t)b * a.q_str[0] + (int64_t)h * a.q_str[1] + (int64_t)node * t.q_tok;
-  const int32_t* par = t.parents + (int64_t)b * t.par_str;
-  if (node >= n) {
-    for (int e = 0; e < E; ++e) out[lane * E + e] = 0;
-    return;
+  s.row = known ? (int)row : 0; s.len = (int)len; s.n = (int)n; s.base = (int)(len - n);
+  s.w0 = a.window > 0 && s.base - a.window + 1 > 0 ? s.base - a.window + 1 : 0;
+  s.sinks = a.sinks < s.len ? a.sinks : s.len;
+  s.front = (int)(((int64_t)s.sinks + kBlk - 1) / kBlk);
+  s.skip = s.w0 / kBlk - s.front;
+  if (s.skip < 0) s.skip = 0;
+  s.blocks = n > 0 ? (int)((len + kBlk - 1) / kBlk) - s.skip : 0;
+  s.tiles = n > 0 ? a.Hkv * (int)(((int64_t)n * a.gqa + N - 1) / N) : 0;
+  return s;
+}
+
+// What a CTA works on: blocks [blk0, blk0 + todo) of a tile, and how many CTAs behind this one share it.
+struct Piece {
+  Seq s;
+  int b, hk, rt, blk0, todo, more;
+  __device__ __forceinline__ int first_token(int j) const { const int i = blk0 + j; return (i < s.front ? i : i + s.skip) * kBlk; }
+  __device__ __forceinline__ bool some_see(int tok) const { return tok < s.len && (tok >= s.w0 || tok < s.sinks); }
+  __device__ __forceinline__ bool all_see(const KvPagesTreeArgs& t, int tok) const {    // (no node is deeper than n - 1)
+    return tok < s.base && (t.a.window == 0 || tok < s.sinks || tok > s.base + s.n - 1 - t.a.window);
   }
-  uint64_t line = 0;
-  int depth[64];
-  for (int i = 0; i < n; ++i) { const int p = par[i]; depth[i] = p >= 0 && p < i ? depth[p] + 1 : 0; }
-  for (int i = node; ; ) { line |= 1ull << i; const int p = par[i]; if (p < 0 || p >= i) break; i = p; }
-  const int64_t me = base + depth[node];
-  float qv[E], o[E], m = -INFINITY, l = 0.f;
-  for (int e = 0; e < E; ++e) { qv[e] = bf16_bits_to_f32(q[lane * E + e]) * a.scale * kLog2e; o[e] = 0.f; }
-  for (int64_t j = 0; j < len; ++j) {
-    int64_t at = j;
-    if (j >= base) {
-      if (!((line >> (j - base)) & 1)) continue;
-      at = base + depth[j - base];
+  __device__ __forceinline__ bool whole(const KvPagesTreeArgs& t, int k0) const {
+    return k0 + kBlk <= s.base && (t.a.window == 0 || k0 + kBlk <= s.sinks || k0 > s.base + s.n - 1 - t.a.window);
+  }
+};
+// The pieces of a CTA, one after the other; every role goes through them by itself.
+struct Pieces {
+  const KvPagesTreeArgs& t;
+  const int *units, *tiles;      // [B + 1]: blocks, tiles before each sequence
+  int N, per, parts, u, u_to;
+  bool more;
+  __device__ __forceinline__ Pieces(const KvPagesTreeArgs& t_, const int* units_, const int* tiles_, int longest, int N_) : t(t_), units(units_), tiles(tiles_), N(N_) {
+    const int U = units[t.a.B], all = tiles[t.a.B], ctas = (int)gridDim.x;
+    per = (U + ctas - 1) / ctas;
+    if (per < 1) per = 1;
+    parts = all > 0 ? ctas / all : 0;
+    if (parts > 0) {
+      parts = parts > longest ? (longest < 1 ? 1 : longest) : parts;
+      const int pieces = 1 + (int)ceilf(__fdividef((float)per * (float)all, (float)(U > 0 ? U : 1)));   // that an even share touches
+      if ((longest + parts - 1) / parts + kPiece > per + pieces * kPiece) parts = 0;
     }
-    if (a.window > 0 && at >= a.sinks && at <= me - a.window) continue;
-    const int64_t pid = a.table[row * a.table_str + (j >> a.page_shift)], slot = j & ((1 << a.page_shift) - 1);
-    if (pid < 0 || pid >= a.P) continue;
-    float kv[2][E];
-    for (int s = 0; s < 2; ++s) {
-      const KvPoolView& p = a.pool[s];
-      const int64_t at_q = pid * p.q_str[0] + hk * p.q_str[1] + slot * p.q_str[2];
-      for (int e = 0; e < E; ++e) {
-        const int d = lane * E + e;
-        if (BITS == 16) kv[s][e] = bf16_bits_to_f32(((const uint16_t*)p.q)[at_q + d]);
+    const int64_t from = (int64_t)blockIdx.x * per;
+    u = from < U ? (int)from : U;
+    u_to = u + per < U ? u + per : U;
+    more = parts > 0 ? (int)blockIdx.x < all * parts : u < U;
+  }
+  __device__ __forceinline__ int find(const int* before, int x) const {       // the last sequence that begins at x or before
+    int lo = 0, hi = t.a.B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (before[mid] <= x) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+  }
+  __device__ __forceinline__ bool next(Piece& p) {
+    if (!more) return false;
+    int tile;
+    if (parts > 0) {
+      more = false;
+      const int at = (int)blockIdx.x / parts, part = (int)blockIdx.x - at * parts;
+      p.b = find(tiles, at);
+      p.s = seq_of(t, p.b, N);
+      tile = at - tiles[p.b];
+      const int mine = parts < p.s.blocks ? parts : p.s.blocks;
+      if (part >= mine) return false;
+      const int each = p.s.blocks / mine, rest = p.s.blocks - each * mine;
+      p.blk0 = each * part + (part < rest ? part : rest);
+      p.todo = each + (part < rest ? 1 : 0);
+      p.more = mine - 1;
+    } else {
+      p.b = find(units, u);
+      p.s = seq_of(t, p.b, N);
+      const int before = units[p.b];
+      tile = (u - before) / p.s.blocks;
+      p.blk0 = u - before - tile * p.s.blocks;
+      const int left = p.s.blocks - p.blk0;
+      p.todo = left < u_to - u ? left : u_to - u;
+      p.more = (before + (tile + 1) * p.s.blocks - 1) / per - (int)blockIdx.x;
+      u += p.todo;
+      more = u < u_to;
+    }
+    const int rts = p.s.tiles / t.a.Hkv;
+    p.hk = tile / rts;
+    p.rt = tile - p.hk * rts;
+    return true;
+  }
+};
+
+template <int BITS, int D, int N>
+__global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(const __grid_constant__ KvPagesTreeArgs t) {
+  using SH = Shape<BITS, D, N>;
+  constexpr int G = SH::G, CH = SH::CH, NC = SH::NC, SW = SH::SW, STAGES = SH::STAGES, THREADS = SH::THREADS;
+  constexpr bool QUANT = BITS != 16;
+  const KvPagesAttnArgs& a = t.a;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* const smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  int* const units = (int*)(smem + SH::SMEM - 1024);          // [B + 1], [B + 1]
+  int* const tiles = units + a.B + 1;
+  __shared__ uint64_t q_ready, k_ready[2], v_ready[2], s_ready[2], p_ready[2], o_done[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int s_fail, s_longest[32], warp_sums[2][32];
+  __shared__ __align__(16) float s_nr[N], s_kunit[4][kBlk];     // -r of the columns; of a block's tokens
+  __shared__ int s_vexp[4][kBlk];
+  __shared__ uint32_t s_kmask[4][4], s_vm[8][STAGES];
+  __shared__ float s_wmax[SH::WGS][4][NC];
+  __shared__ int s_par[kMaxNodes], s_depth[kMaxNodes], s_clo[N], s_qe[N];
+  __shared__ uint64_t s_line[kMaxNodes], s_cline[N];
+  __shared__ int note_count[4], note_key[4][kNotes];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  asm volatile("griddepcontrol.wait;" ::: "memory");         // (before tensor memory is taken, too: the kernel before may hold it)
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  // ---- all sequences' blocks and tiles ----
+  {
+    const int each = (a.B + THREADS - 1) / THREADS, b0 = tid * each;
+    int mine = 0, mine_t = 0, longest = 0;
+    for (int i = 0; i < each && b0 + i < a.B; ++i) {
+      const Seq s = seq_of(t, b0 + i, N);
+      units[b0 + i] = mine; tiles[b0 + i] = mine_t;
+      mine += s.blocks * s.tiles;
+      mine_t += s.tiles;
+      longest = s.blocks > longest ? s.blocks : longest;
+    }
+    int upto = mine, upto_t = mine_t;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o), y = __shfl_up_sync(0xffffffffu, upto_t, o);
+      if (lane >= o) { upto += x; upto_t += y; }
+    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (lane == 31) { warp_sums[0][warp] = upto; warp_sums[1][warp] = upto_t; s_longest[warp] = longest; }
+    if (tid == 0) {
+      s_fail = 0;
+      mbar_init(&q_ready, SW);
+      for (int i = 0; i < 2; ++i) { mbar_init(&k_ready[i], 4); mbar_init(&v_ready[i], 4); mbar_init(&s_ready[i], 1); mbar_init(&p_ready[i], SW); mbar_init(&o_done[i], 1); }
+      for (int i = 0; i < 4; ++i) note_count[i] = 0;
+      a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+      asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == SW + 8) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    __syncthreads();
+    int before = upto - mine, before_t = upto_t - mine_t;
+    for (int w = 0; w < warp; ++w) { before += warp_sums[0][w]; before_t += warp_sums[1][w]; }
+    for (int i = 0; i < each && b0 + i < a.B; ++i) { units[b0 + i] += before; tiles[b0 + i] += before_t; }
+    if (tid == THREADS - 1) { units[a.B] = before + mine; tiles[a.B] = before_t + mine_t; }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  int longest = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) longest = s_longest[w] > longest ? s_longest[w] : longest;
+  const uint32_t tmem = tmem_slot;
+  Pieces pieces(t, units, tiles, longest, N);
+  Piece pc;
+  // A wait that runs out is noted once; the warp then goes on without waiting (on data that is not there yet, within its bounds), so that
+  // all warps meet at every barrier and the CTA ends.
+  bool dead = false;
+  auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
+    if (dead) return;
+    dead = !__all_sync(0xffffffffu, wait_cta(bar, phase & 1, kPolls));
+    if (dead && lane == 0 && !s_fail) { s_fail = code; atomicCAS(&g_tree_error, 0, code); }
+  };
+  const int pmask = (1 << a.page_shift) - 1;
+  int J0 = 0;                        // blocks before this piece
+
+  if (warp >= SW && warp < SW + 8) {
+    // ---------------- keys, values ----------------
+    const bool V = warp >= SW + 4;
+    const int wq = warp & 3, w8 = warp - SW;                   // quarter of the block: 32 tokens
+    const KvPoolView& pool = a.pool[V];
+    const uint32_t page_b = a.page_bytes[V], tok_b = a.tok_bytes[V];
+    unsigned char* const ring = smem + SH::R0 + w8 * STAGES * SH::RS;
+    constexpr int RPI = 32 / CH;                               // token rows of one copy instruction
+    const int cc = lane % CH, r0 = lane / CH;
+    auto swz = [](int r) { return CH >= 8 ? (r & 7) & (CH - 1) : (r / (8 / CH)) % CH; };   // so that 8 neighbours' rows lie in different banks
+    int piece_no = 0;
+    while (pieces.next(pc)) {
+      const int32_t* const tab = a.table + (int64_t)pc.s.row * a.table_str;
+      const unsigned char* const base = (const unsigned char*)pool.q + (int64_t)pc.hk * a.q_head[V] + (int64_t)r0 * tok_b + cc * 16;
+      // lane l holds the page of the 16 tokens from 16 * (l & 1) of the warp's 32 on, -1 where there is none
+      auto page_at = [&](int j) {
+        int pid = -1;
+        if (j < pc.todo) {
+          const int tok = pc.first_token(j) + 32 * wq + 16 * (lane & 1);
+          if (tok < pc.s.len) pid = tab[tok >> a.page_shift];
+          if (pid >= a.P) pid = -1;
+        }
+        return pid;
+      };
+      int pid_next = page_at(0);
+      auto issue = [&](int j, int given) {                     // (given: blocks that the products have been given, or soon will be)
+        const int J = J0 + j, st = J % STAGES;
+        const int pid_cur = pid_next, tok0 = pc.first_token(j) + 32 * wq;
+        pid_next = page_at(j + 1);
+        const int p0 = __shfl_sync(0xffffffffu, pid_cur, 0), p1 = __shfl_sync(0xffffffffu, pid_cur, 1);
+        const bool mine = pc.some_see(tok0 + lane) && (lane < 16 ? p0 : p1) >= 0;
+        const uint32_t vm = __ballot_sync(0xffffffffu, mine);
+        if (lane == 0) s_vm[w8][st] = vm;
+        uint32_t dst0;
+        if constexpr (QUANT) dst0 = smem_u32(ring + st * SH::RS);
         else {
-          const uint32_t word = ((const uint32_t*)p.q)[at_q + d * BITS / 32];
-          const int64_t g = pid * p.sb_str[0] + hk * p.sb_str[1] + slot * p.sb_str[2] + d / 64;
-          kv[s][e] = fmaf((float)((word >> (d % (32 / BITS) * BITS)) & ((1u << (BITS & 15)) - 1)), bf16_bits_to_f32(((const uint16_t*)p.s)[g]), bf16_bits_to_f32(((const uint16_t*)p.b)[g]));
+          dst0 = smem_u32(smem + (V ? SH::V0 : SH::K0) + st * SH::TILE);
+          // the products that read the slot, or later ones: two blocks back the barrier may already be a phase further
+          const int read = J - STAGES > given - 2 ? J - STAGES : given - 2;
+          if (read >= 0) wait((V ? o_done : s_ready) + (read & 1), (uint32_t)(read >> 1), 605);
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          const int r = i * RPI + r0, pid = i * RPI < 16 ? p0 : p1;
+          const unsigned char* const src = base + (uint64_t)(uint32_t)(pid < 0 ? 0 : pid) * page_b + (uint64_t)(uint32_t)((tok0 + i * RPI) & pmask) * tok_b;
+          uint32_t dst;
+          if constexpr (QUANT) dst = dst0 + r * SH::ROWB + ((cc ^ swz(r)) << 4);
+          else dst = dst0 + (cc >> 3) * (kBlk * 128) + (32 * wq + r) * 128 + (((cc & 7) ^ (r & 7)) << 4);
+          cp_async16_z(dst, src, (vm >> r) & 1u ? 16u : 0u);
+        }
+        if constexpr (QUANT) {
+          // [scales, biases of this pool][of the values: the keys' warps give their units on], 32 tokens each
+          const int arrays = V ? 2 : 4;
+          unsigned char* const sb = ring + st * SH::RS + 32 * SH::ROWB;
+          if (a.sb_vec) {
+            constexpr int TP = 8 / G;                          // tokens of a 16-byte piece
+            if (lane < arrays * 4 * G) {
+              const int arr = lane / (4 * G), tok = lane % (4 * G) * TP, pid = tok < 16 ? p0 : p1;
+              const KvPoolView& pl = arr >= 2 ? a.pool[1] : pool;
+              const uint16_t* const src = (const uint16_t*)((arr & 1) ? pl.b : pl.s) + (int64_t)(pid < 0 ? 0 : pid) * pl.sb_str[0] + (int64_t)pc.hk * pl.sb_str[1] +
+                                          (int64_t)((tok0 + tok) & pmask) * G;
+              cp_async16_z(smem_u32(sb + arr * SH::SB + tok * G * 2), src, pid >= 0 && tok0 + tok < pc.s.len ? 16u : 0u);
+            }
+          } else {
+            const int pid = lane < 16 ? p0 : p1;
+            for (int arr = 0; arr < arrays; ++arr) {
+              const KvPoolView& pl = arr >= 2 ? a.pool[1] : pool;
+              const uint16_t* const src = (const uint16_t*)((arr & 1) ? pl.b : pl.s) + (int64_t)(pid < 0 ? 0 : pid) * pl.sb_str[0] + (int64_t)pc.hk * pl.sb_str[1] +
+                                          (int64_t)((tok0 + lane) & pmask) * pl.sb_str[2];
+#pragma unroll
+              for (int g = 0; g < G; ++g) ((uint16_t*)(sb + arr * SH::SB))[lane * G + g] = mine ? src[g] : (uint16_t)0;
+            }
+          }
+        }
+      };
+#pragma unroll 1
+      for (int j = 0; j < STAGES - 1; ++j) {
+        if (j < pc.todo) issue(j, J0);
+        cp_async_commit();
+      }
+#pragma unroll 1
+      for (int j = 0; j < pc.todo; ++j) {
+        const int J = J0 + j, st = J % STAGES, key = 32 * wq + lane;
+        if (j + STAGES - 1 < pc.todo) issue(j + STAGES - 1, J);
+        cp_async_commit();
+        cp_async_wait<STAGES - 1>();
+        __syncwarp();
+        const uint32_t vm = s_vm[w8][st];
+        const bool mine = (vm >> lane) & 1u;
+        if (!V && lane == 0) s_kmask[J & 3][wq] = vm;
+        // a value that some nodes see and others do not must not meet their 0 if it is not finite: it is zeroed and noted
+        const int tok = pc.first_token(j) + key;
+        const bool partly = V && mine && !pc.all_see(t, tok);
+        bool bad = false;
+        if constexpr (QUANT) {
+          const unsigned char* const codes = ring + st * SH::RS;
+          const unsigned char* const sb = codes + 32 * SH::ROWB;
+          float s[G], b[G], top = 0.f;
+          auto params = [&](int arr, float (&x)[G]) {
+            if constexpr (G == 2) {
+              const uint32_t v = mine ? *(const uint32_t*)(sb + arr * SH::SB + lane * 4) : 0u;
+              x[0] = bf16lo(v); x[G - 1] = bf16hi(v);
+            } else x[0] = mine ? bf16_bits_to_f32(*(const uint16_t*)(sb + arr * SH::SB + lane * 2)) : 0.f;
+          };
+          auto largest = [&]() {
+            float m = 0.f;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              const float x = group_top<BITS>(s[g], b[g]);
+              const bool off = !(x < INFINITY) || !(fabsf(s[g]) < INFINITY);
+              bad |= off;
+              m = fmaxf(m, off ? 0.f : x);
+            }
+            return m;
+          };
+          if (!V) {
+            params(2, s); params(3, b);
+            s_vexp[J & 3][key] = unit_exp(largest()) - 14;
+          }
+          bad = false;
+          params(0, s); params(1, b);
+          top = largest();
+          const int e = unit_exp(top);
+          const float up = pow2i(14 - e);
+          if (!V) s_kunit[J & 3][key] = pow2i(e - 14);
+          const bool drop = partly && bad;
+          __half2 s2[G], b2[G];
+#pragma unroll
+          for (int g = 0; g < G; ++g) { s2[g] = __float2half2_rn(drop ? 0.f : s[g] * up); b2[g] = __float2half2_rn(drop ? 0.f : b[g] * up); }
+          if (J >= 2) wait((V ? o_done : s_ready) + (J & 1), (uint32_t)((J >> 1) - 1), V ? 602 : 601);
+          unsigned char* const vrow = smem + SH::V0 + (J & 1) * SH::TILE + key * 128;
+          constexpr int CG = CH / G;                           // chunks of a group
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            uint32_t o[32];
+#pragma unroll
+            for (int c = 0; c < CG; ++c) {
+              const uint4 x = *(const uint4*)(codes + lane * SH::ROWB + (((g * CG + c) ^ swz(lane)) << 4));
+              constexpr int W = 32 / BITS / 2;                 // registers of a word
+              dequant_word<BITS>(x.x, s2[g], b2[g], &o[(4 * c + 0) * W]); dequant_word<BITS>(x.y, s2[g], b2[g], &o[(4 * c + 1) * W]);
+              dequant_word<BITS>(x.z, s2[g], b2[g], &o[(4 * c + 2) * W]); dequant_word<BITS>(x.w, s2[g], b2[g], &o[(4 * c + 3) * W]);
+            }
+            if (!V) tmem_st32(tmem + SH::K_AT + (J & 1) * 64 + g * 32 + ((uint32_t)wq << 21), o);
+            else {
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                *(uint4*)(vrow + g * (kBlk * 128) + ((c ^ (key & 7)) << 4)) = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+            }
+          }
+          if (!V) {
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            fence_before();
+          } else fence_async();
+        } else {
+          // (the products two blocks back are done, so that this arrival is not taken for one of theirs)
+          if (STAGES > 2 && J >= 2) wait((V ? o_done : s_ready) + (J & 1), (uint32_t)((J >> 1) - 1), V ? 602 : 601);
+          if (__any_sync(0xffffffffu, partly)) {
+            unsigned char* const vrow = smem + SH::V0 + st * SH::TILE + key * 128;
+            if (partly) {
+              uint32_t acc = 0;
+#pragma unroll
+              for (int c = 0; c < D / 8; ++c) {
+                const uint4 x = *(const uint4*)(vrow + (c >> 3) * (kBlk * 128) + (((c & 7) ^ (key & 7)) << 4));
+                acc |= ((x.x & 0x7F807F80u) + 0x00800080u) | ((x.y & 0x7F807F80u) + 0x00800080u) | ((x.z & 0x7F807F80u) + 0x00800080u) | ((x.w & 0x7F807F80u) + 0x00800080u);
+              }
+              bad = (acc & 0x80008000u) != 0;                  // an exponent of all ones
+              if (bad)
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) *(uint4*)(vrow + (c >> 3) * (kBlk * 128) + (((c & 7) ^ (key & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          fence_async();
+        }
+        if (partly && bad) {
+          const int at = atomicAdd(&note_count[piece_no & 3], 1);
+          if (at < kNotes) note_key[piece_no & 3][at] = tok;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive((V ? v_ready : k_ready) + (J & 1));
+      }
+      cp_async_wait<0>();
+      J0 += pc.todo;
+      ++piece_no;
+    }
+  } else if (warp == SW + 8) {
+    // ---------------- products ----------------
+    constexpr uint32_t type = QUANT ? 0u : 1u;                 // fp16, bf16
+    constexpr uint32_t idesc0 = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
+    constexpr uint32_t idesc_s = idesc0, idesc_o = idesc0 | (1u << 15) | (1u << 16);   // the values and P: columns contiguous
+    auto U = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    const uint32_t tm = (uint32_t)U((int)tmem), sm = (uint32_t)U((int)smem_u32(smem));
+    const uint64_t hi_k = make_desc(0) & 0xFFFFFFFF00000000ull, hi_v = make_desc_mn(0) & 0xFFFFFFFF00000000ull;
+    const uint32_t q_d = (uint32_t)make_desc(sm + SH::Q0), k_d = (uint32_t)make_desc(sm + SH::K0), v_d = (uint32_t)make_desc_mn(sm + SH::V0), p_d = (uint32_t)make_desc_mn(sm + SH::P0);
+    auto spin = [&](uint64_t* bar, uint32_t phase, int code) {
+      if (dead) return;
+      dead = !__all_sync(0xffffffffu, spin_cta(bar, phase & 1));
+      if (dead && lane == 0 && !s_fail) { s_fail = code; atomicCAS(&g_tree_error, 0, code); }
+    };
+    int piece_no = 0;
+    auto scores = [&](int J) {
+      spin(&k_ready[J & 1], (uint32_t)(J >> 1), 603);
+      fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t q = hi_k | (q_d + (k >> 2) * ((N * 128) >> 4) + (k & 3) * 2);
+          if constexpr (QUANT) umma_ts(tm + SH::S_AT + (J & 1) * 64, tm + SH::K_AT + (J & 1) * 64 + k * 8, q, idesc_s, k > 0);
+          else umma_ss(tm + SH::S_AT + (J & 1) * 64, hi_k | (k_d + (J % STAGES) * (SH::TILE >> 4) + (k >> 2) * ((kBlk * 128) >> 4) + (k & 3) * 2), q, idesc_s, k > 0);
+        }
+        commit(&s_ready[J & 1]);
+      }
+      __syncwarp();
+    };
+    while (pieces.next(pc)) {
+      const int todo = U(pc.todo);
+      spin(&q_ready, (uint32_t)piece_no, 604);
+      for (int j = -2; j < todo; ++j) {
+        if (j >= 0) {
+          const int J = J0 + j;
+          spin(&v_ready[J & 1], (uint32_t)(J >> 1), 606);
+          spin(&p_ready[J & 1], (uint32_t)(J >> 1), 607);
+          fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < kBlk / 16; ++k)
+              umma_ss(tm + SH::O_AT, hi_v | (v_d + (J % SH::VT) * (SH::TILE >> 4) + k * (2048 >> 4)), hi_v | (p_d + (J % SH::PS) * (SH::PTILE >> 4) + k * (2048 >> 4)), idesc_o,
+                      k > 0 ? 1u : (j > 0 ? 1u : 0u));
+            commit(&o_done[J & 1]);
+          }
+          __syncwarp();
+        }
+        if (j + 2 < todo) scores(J0 + j + 2);
+      }
+      J0 += todo;
+      ++piece_no;
+    }
+    // every product is complete before tensor memory and shared memory go
+    if (J0 > 0) spin(&o_done[(J0 - 1) & 1], (uint32_t)((J0 - 1) >> 1), 608);
+    if (s_fail)
+      for (int i = 0; i < 1000; ++i) __nanosleep(1000);        // (products may still be on their way)
+  } else {
+    // ---------------- softmax: a thread a token ----------------
+    const int wg = warp >> 2, wq = warp & 3, key = tid & 127, col0 = wg * NC;
+    const uint32_t lanes = tmem + ((uint32_t)wq << 21);
+    constexpr int ALL = SW * 32;
+    const float factor = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);   // (a factor of 0 would meet scores of -inf)
+    int piece_no = 0;
+    while (pieces.next(pc)) {
+      const Seq& s = pc.s;
+      // ---- the tree, the queries ----
+      constexpr int LPR = D / 4, RPW = 32 / LPR, IT = N / (SW * RPW);    // lanes of a row, rows of a warp at a time
+      uint32_t raw[IT][2];
+      const int live = s.n * a.gqa;
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const int n = (i * SW + warp) * RPW + lane / LPR, R = pc.rt * N + n;
+        raw[i][0] = raw[i][1] = 0u;
+        if (R < live) {
+          const int node = R / a.gqa, h = R - node * a.gqa;
+          const uint16_t* const p = (const uint16_t*)a.q + (int64_t)pc.b * a.q_str[0] + (int64_t)(pc.hk * a.gqa + h) * a.q_str[1] + (int64_t)node * t.q_tok + (lane % LPR) * 4;
+          if (a.q_vec) { const uint2 x = *(const uint2*)p; raw[i][0] = x.x; raw[i][1] = x.y; }
+          else { raw[i][0] = (uint32_t)p[0] | ((uint32_t)p[1] << 16); raw[i][1] = (uint32_t)p[2] | ((uint32_t)p[3] << 16); }
+        }
+        if (a.scale < 0.f) { raw[i][0] ^= 0x80008000u; raw[i][1] ^= 0x80008000u; }   // so that the largest score is the largest sum
+      }
+      if (piece_no > 0) bar_sync(5, ALL);                      // (all are done with the last tile's lists)
+      if (tid < kMaxNodes && tid < s.n) {
+        const int p = t.parents[(int64_t)pc.b * t.par_str + tid];
+        s_par[tid] = p >= 0 && p < tid ? p : -1;
+      }
+      if (tid < N) s_nr[tid] = -kNegBig;
+      if constexpr (QUANT) {
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+          float mx = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float x = fabsf((k & 1) ? bf16hi(raw[i][k >> 1]) : bf16lo(raw[i][k >> 1]));
+            mx = x < INFINITY ? fmaxf(mx, x) : mx;
+          }
+#pragma unroll
+          for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          const int e = (int)(__float_as_uint(mx) >> 23) - 127;
+          if (lane % LPR == 0) s_qe[(i * SW + warp) * RPW + lane / LPR] = mx > 0.f ? (e < -100 ? -100 : (e > 110 ? 110 : e)) : -1000;
+        }
+      }
+      bar_sync(5, ALL);
+      if (tid < s.n && tid < kMaxNodes) {
+        uint64_t line = 0;
+        int depth = -1;
+        for (int i = tid; i >= 0; i = s_par[i]) { line |= 1ull << i; ++depth; }
+        s_line[tid] = line; s_depth[tid] = depth;
+      }
+      // queries in fp16: all in the unit of the largest, where their sizes are near one another, else each in its own
+      int emax = 0;
+      bool alike = true;
+      if constexpr (QUANT) {
+        int hi = -1000, lo = 1000;
+        for (int i = lane; i < N; i += 32) { const int e = s_qe[i]; if (e > -1000) { hi = e > hi ? e : hi; lo = e < lo ? e : lo; } }
+        hi = __reduce_max_sync(0xffffffffu, hi); lo = __reduce_min_sync(0xffffffffu, lo);
+        emax = hi > -1000 ? hi : 0;
+        alike = hi - lo <= 12;
+      }
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const int n = (i * SW + warp) * RPW + lane / LPR, l = lane % LPR;
+        uint32_t w0 = raw[i][0], w1 = raw[i][1];
+        if constexpr (QUANT) {
+          const int e = alike || s_qe[n] == -1000 ? emax : s_qe[n];
+          const float up = pow2i(14 - e);
+          const uint32_t h0 = pack_f16x2(bf16lo(raw[i][0]) * up, bf16hi(raw[i][0]) * up), h1 = pack_f16x2(bf16lo(raw[i][1]) * up, bf16hi(raw[i][1]) * up);
+          if constexpr (BITS == 4) {       // eight dims of two lanes: 0 4 1 5 in the first, 2 6 3 7 in the second
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, l & 1 ? h0 : h1, 1);
+            const uint32_t x = l & 1 ? got : h0, y = l & 1 ? h1 : got;
+            w0 = __byte_perm(x, y, 0x5410); w1 = __byte_perm(x, y, 0x7632);
+          } else { w0 = __byte_perm(h0, h1, 0x5410); w1 = __byte_perm(h0, h1, 0x7632); }
+        }
+        const int d = 4 * l, c = (d & 63) >> 3;
+        *(uint2*)(smem + SH::Q0 + (d >> 6) * (N * 128) + n * 128 + ((c ^ (n & 7)) << 4) + (l & 1) * 8) = make_uint2(w0, w1);
+      }
+      fence_async();
+      bar_sync(5, ALL);
+      if (lane == 0) mbar_arrive(&q_ready);
+      if (tid < N) {
+        const int R = pc.rt * N + tid, node = R < live ? R / a.gqa : -1;
+        s_cline[tid] = node >= 0 ? s_line[node] : 0ull;
+        s_clo[tid] = node >= 0 ? s.base + s_depth[node] - a.window : 0;
+      }
+      if (tid == 0) note_count[(piece_no + 3) & 3] = 0;        // (read before, and not yet used again: the other roles are two blocks ahead at most)
+      bar_sync(5, ALL);
+      const float Cq = QUANT ? factor * pow2i(emax - 14) : factor;
+
+      uint64_t l2[NC / 2];
+#pragma unroll
+      for (int i = 0; i < NC / 2; ++i) l2[i] = 0ull;
+#pragma unroll 1
+      for (int j = 0; j < pc.todo; ++j) {
+        const int J = J0 + j, k0 = pc.first_token(j), tok = k0 + key;
+        wait(&s_ready[J & 1], (uint32_t)(J >> 1), 609);
+        fence_after();
+        const uint32_t vm = s_kmask[J & 3][wq];
+        float ck = Cq, w = 1.f, ev = 0.f;
+        if constexpr (QUANT) {
+          const int e = s_vexp[J & 3][key];
+          ck *= s_kunit[J & 3][key];
+          ev = (float)e;
+          w = pow2i(-e);
+        }
+        const bool masked = vm != 0xffffffffu || !pc.whole(t, k0);
+        const uint32_t s_at = lanes + SH::S_AT + (J & 1) * 64 + col0;
+        uint32_t z[NC];
+        auto exponents = [&](bool with_reference) {            // of P' (or, without the reference, of P' 2^r)
+          tmem_get<NC>(s_at, z);
+          if (QUANT && !alike)
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+              const int e = s_qe[col0 + i];
+              z[i] = __float_as_uint(__uint_as_float(z[i]) * (e == -1000 ? 1.f : pow2i(e - emax < -126 ? -126 : e - emax)));
+            }
+          const uint64_t ck2 = two(ck, ck), ev2 = two(ev, ev);
+#pragma unroll
+          for (int i = 0; i < NC / 4; ++i) {
+            uint64_t r0 = ev2, r1 = ev2;
+            if (with_reference) {
+              const ulonglong2 nr = *(const ulonglong2*)&s_nr[col0 + 4 * i];
+              if constexpr (QUANT) { r0 = add2(nr.x, ev2); r1 = add2(nr.y, ev2); } else { r0 = nr.x; r1 = nr.y; }
+            }
+            const uint64_t x = fma2(two(__uint_as_float(z[4 * i]), __uint_as_float(z[4 * i + 1])), ck2, r0), y = fma2(two(__uint_as_float(z[4 * i + 2]), __uint_as_float(z[4 * i + 3])), ck2, r1);
+            float f0, f1, f2, f3;
+            untwo(x, f0, f1); untwo(y, f2, f3);
+            z[4 * i] = __float_as_uint(f0); z[4 * i + 1] = __float_as_uint(f1); z[4 * i + 2] = __float_as_uint(f2); z[4 * i + 3] = __float_as_uint(f3);
+          }
+          if (masked) {
+            const bool mine = (vm >> lane) & 1u, drafted = tok >= s.base;
+            const int m = drafted ? tok - s.base : 0, at = drafted ? s.base + (mine ? s_depth[m] : 0) : tok;
+            const bool inside = a.window == 0 || at < a.sinks;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+              const bool sees = mine && (!drafted || ((s_cline[col0 + i] >> m) & 1ull)) && (inside || at > s_clo[col0 + i]);
+              if (!sees) z[i] = 0xff800000u;
+            }
+          }
+        };
+        exponents(true);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NC; i += 2) mx = max3(mx, __uint_as_float(z[i]), __uint_as_float(z[i + 1]));
+        if (bar_any(1 + wg, 128, mx > kTop)) {
+          exponents(false);
+          // the columns' maxima over the warp's tokens: lane n ends with that of column n
+          float v[NC];
+#pragma unroll
+          for (int i = 0; i < NC; ++i) v[i] = __uint_as_float(z[i]);
+#pragma unroll
+          for (int o = NC / 2; o > 0; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < o; ++i) {
+              const bool up = (lane & o) != 0;
+              const float keep = up ? v[i + o] : v[i], give = up ? v[i] : v[i + o];
+              v[i] = fmaxf(fmaxf(keep, -INFINITY), __shfl_xor_sync(0xffffffffu, give, o));
+            }
+          if constexpr (NC == 16) v[0] = fmaxf(v[0], __shfl_xor_sync(0xffffffffu, v[0], 16));
+          if (lane < NC) s_wmax[wg][wq][lane] = v[0];
+          bar_sync(3 + wg, 128);
+          float f = 1.f, nr = 0.f;
+          if (lane < NC) {
+            nr = s_nr[col0 + lane];
+            const float top = fmaxf(fmaxf(s_wmax[wg][0][lane], s_wmax[wg][1][lane]), fmaxf(s_wmax[wg][2][lane], s_wmax[wg][3][lane]));
+            if (top + nr > kTop) {
+              f = ex2(kAim - top - nr);
+              nr = kAim - top;
+            }
+          }
+          bar_sync(3 + wg, 128);                               // (all have read the old ones)
+          if (wq == 0 && lane < NC) s_nr[col0 + lane] = nr;
+          if (j > 0) {
+            wait(&o_done[(J - 1) & 1], (uint32_t)((J - 1) >> 1), 610);
+            fence_after();
+            uint32_t o[NC];
+            tmem_get<NC>(lanes + SH::O_AT + col0, o);
+#pragma unroll
+            for (int i = 0; i < NC; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * __shfl_sync(0xffffffffu, f, i));
+            tmem_put<NC>(lanes + SH::O_AT + col0, o);
+#pragma unroll
+            for (int i = 0; i < NC / 2; ++i) l2[i] = mul2(l2[i], two(__shfl_sync(0xffffffffu, f, 2 * i), __shfl_sync(0xffffffffu, f, 2 * i + 1)));
+          }
+          bar_sync(3 + wg, 128);
+          exponents(true);
+        }
+        uint32_t p[NC / 2];
+        const uint64_t w2 = two(w, w);
+#pragma unroll
+        for (int i = 0; i < NC / 2; ++i) {
+          const float x0 = ex2(__uint_as_float(z[2 * i])), x1 = ex2(__uint_as_float(z[2 * i + 1]));
+          if constexpr (QUANT) { l2[i] = fma2(two(x0, x1), w2, l2[i]); p[i] = pack_f16x2(x0, x1); }
+          else { l2[i] = add2(l2[i], two(x0, x1)); p[i] = pack2(x0, x1); }
+        }
+        if (J >= SH::PS) wait(&o_done[(J - SH::PS) & 1], (uint32_t)((J - SH::PS) >> 1), 611);
+        unsigned char* const prow = smem + SH::P0 + (J % SH::PS) * SH::PTILE + key * 128;
+#pragma unroll
+        for (int c = 0; c < NC / 8; ++c)
+          *(uint4*)(prow + (((col0 / 8 + c) ^ (key & 7)) << 4)) = make_uint4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
+        fence_async();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[J & 1]);
+      }
+      // ---- the tile's results, a thread a dim ----
+      const int last = J0 + pc.todo - 1;
+      float l[NC];
+#pragma unroll
+      for (int i = 0; i < NC / 2; ++i) untwo(l2[i], l[2 * i], l[2 * i + 1]);
+#pragma unroll
+      for (int o = NC / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+          const bool up = (lane & o) != 0;
+          const float keep = up ? l[i + o] : l[i], give = up ? l[i] : l[i + o];
+          l[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+      if constexpr (NC == 16) l[0] += __shfl_xor_sync(0xffffffffu, l[0], 16);
+      if (lane < NC) s_wmax[wg][wq][lane] = l[0];
+      wait(&o_done[last & 1], (uint32_t)(last >> 1), 612);
+      fence_after();
+      uint32_t o[NC];
+      tmem_get<NC>(lanes + SH::O_AT + col0, o);
+      fence_before();
+      bar_sync(3 + wg, 128);
+      float L = 0.f, r = 0.f;
+      if (lane < NC) {
+        L = (s_wmax[wg][0][lane] + s_wmax[wg][1][lane]) + (s_wmax[wg][2][lane] + s_wmax[wg][3][lane]);
+        r = -s_nr[col0 + lane];
+        const int notes = note_count[piece_no & 3];
+        for (int i = 0; i < notes && i < kNotes; ++i) {
+          const int k = note_key[piece_no & 3][i];
+          const bool drafted = k >= s.base;
+          const int at = drafted ? s.base + s_depth[k - s.base] : k;
+          if ((!drafted || ((s_cline[col0 + lane] >> (k - s.base)) & 1ull)) && (a.window == 0 || at < a.sinks || at > s_clo[col0 + lane])) L = __uint_as_float(0x7fc00000u);
+        }
+      }
+      const bool all = pc.blk0 == 0 && pc.todo == s.blocks;
+      const int rows = live - pc.rt * N < N ? live - pc.rt * N : N;
+      if (all) {
+        const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+        const int dim = dim_at<BITS>(key);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const float v = __uint_as_float(o[i]) * __shfl_sync(0xffffffffu, inv, i);
+          if (col0 + i < rows && key < D) {
+            const int R = pc.rt * N + col0 + i, node = R / a.gqa, h = R - node * a.gqa;
+            ((uint16_t*)a.out)[(int64_t)pc.b * a.o_str[0] + (int64_t)(pc.hk * a.gqa + h) * a.o_str[1] + (int64_t)node * t.o_tok + dim] = f32_to_bf16_bits(v);
+          }
+        }
+      } else {
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (pc.blk0 == 0 ? 1 : 0);
+        if (pc.blk0 == 0 && tid == 0) a.joins[blockIdx.x] = make_int4(pc.b, pc.hk, pc.rt, pc.more);
+        if (wq == 0 && lane < NC) a.part_ml[slot * N + col0 + lane] = make_float2(r, L);
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+          if (col0 + i < rows && key < D) a.part_o[(slot * N + col0 + i) * D + key] = __uint_as_float(o[i]);
+      }
+      J0 += pc.todo;
+      ++piece_no;
+    }
+    // nodes that are not there: zeros
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+      const int n = seq_of(t, b, N).n;
+      for (int64_t i = tid; i < (int64_t)(t.T - n) * a.Hq * D; i += ALL) {
+        const int e = (int)(i % D), h = (int)(i / D % a.Hq), node = n + (int)(i / D / a.Hq);
+        ((uint16_t*)a.out)[(int64_t)b * a.o_str[0] + (int64_t)h * a.o_str[1] + (int64_t)node * t.o_tok + e] = 0;
+      }
+    }
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  if (warp == SW + 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+}
+
+// ---- the parts of a tile that several CTAs share: out = (sum_i o_i w_i) / (sum_i l_i w_i), w_i = 2^(r_i - max r) ----
+// CTA (c, y) joins 8 rows of the tile that begins in CTA c's share and ends behind it: its own part (slot 2c + 1) and those of the next
+// CTAs (slots 2(c + k)).  A warp takes one row's every second part.
+template <int BITS, int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const __grid_constant__ KvPagesTreeArgs t, int N) {
+  __shared__ float red[kJoinWarps][D + 2];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const KvPagesAttnArgs& a = t.a;
+  const int4 jn = a.joins[blockIdx.x];
+  if (jn.x < 0) return;
+  const Seq s = seq_of(t, jn.x, N);
+  const int row0 = (int)blockIdx.y * kJoinRows, left = s.n * a.gqa - jn.z * N - row0;
+  if (left <= 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = jn.w + 1;
+  constexpr int parts = kJoinWarps / kJoinRows;
+  const int rows = left < kJoinRows ? left : kJoinRows, h = warp % kJoinRows, part = warp / kJoinRows;
+  constexpr int E = D / 32;
+  auto slot = [&](int k) { return (int64_t)(k == 0 ? 2 * (int)blockIdx.x + 1 : 2 * ((int)blockIdx.x + k)); };
+  float M = kNegBig, L = 0.f, o[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) o[i] = 0.f;
+  if (h < rows) {
+    for (int k0 = part; k0 < n; k0 += parts * 32) {
+      const int k = k0 + lane * parts;
+      float2 ml = make_float2(kNegBig, 0.f);
+      if (k < n) ml = __ldcg(a.part_ml + slot(k) * N + row0 + h);
+      float m = ml.x;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+      const float Mn = fmaxf(M, m), f = ex2(M - Mn), w = ex2(ml.x - Mn);
+      L = L * f + w * ml.y;          // a lane's own parts
+#pragma unroll
+      for (int i = 0; i < E; ++i) o[i] *= f;
+      M = Mn;
+      const int cnt = (n - k0 + parts - 1) / parts < 32 ? (n - k0 + parts - 1) / parts : 32;
+#pragma unroll 8
+      for (int q = 0; q < cnt; ++q) {
+        const float wq = __shfl_sync(0xffffffffu, w, q);
+        const float* src = a.part_o + (slot(k0 + q * parts) * N + row0 + h) * D + lane * E;
+        if constexpr (E == 4) {
+          const float4 x = __ldcg((const float4*)src);
+          o[0] = fmaf(wq, x.x, o[0]); o[1] = fmaf(wq, x.y, o[1]); o[2] = fmaf(wq, x.z, o[2]); o[3] = fmaf(wq, x.w, o[3]);
+        } else {
+          const float2 x = __ldcg((const float2*)src);
+          o[0] = fmaf(wq, x.x, o[0]); o[1] = fmaf(wq, x.y, o[1]);
         }
       }
     }
-    float s = 0.f;
-    for (int e = 0; e < E; ++e) s = fmaf(qv[e], kv[0][e], s);
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    if (s == -INFINITY) continue;
-    const float mn = fmaxf(m, s), f = m == mn ? 1.f : exp2f(m - mn), pr = exp2f(s - mn);
-    l = l * f + pr;
-    for (int e = 0; e < E; ++e) o[e] = fmaf(pr, kv[1][e], o[e] * f);
-    m = mn;
+    for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+#pragma unroll
+    for (int i = 0; i < E; ++i) red[warp][lane * E + i] = o[i];
+    if (lane == 0) { red[warp][D] = M; red[warp][D + 1] = L; }
   }
-  const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-  for (int e = 0; e < E; ++e) out[lane * E + e] = f32_to_bf16_bits(o[e] * inv);
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * D; i += kJoinWarps * 32) {
+    const int r = i / D, e = i - r * D;
+    float Mx = kNegBig;
+#pragma unroll
+    for (int p = 0; p < parts; ++p) Mx = fmaxf(Mx, red[p * kJoinRows + r][D]);
+    float Ls = 0.f, Os = 0.f;
+#pragma unroll
+    for (int p = 0; p < parts; ++p) {
+      const float f = ex2(red[p * kJoinRows + r][D] - Mx);
+      Ls += red[p * kJoinRows + r][D + 1] * f;
+      Os += red[p * kJoinRows + r][e] * f;
+    }
+    const float v = Os * (Ls > 0.f ? 1.f / Ls : (Ls == Ls ? 0.f : Ls));
+    const int R = jn.z * N + row0 + r, node = R / a.gqa, hh = R - node * a.gqa;
+    ((uint16_t*)a.out)[(int64_t)jn.x * a.o_str[0] + (int64_t)(jn.y * a.gqa + hh) * a.o_str[1] + (int64_t)node * t.o_tok + dim_at<BITS>(e)] = f32_to_bf16_bits(v);
+  }
+}
+
+// Columns of a tile: as many as the widest tree has rows of a cache head, up to 64.
+int columns(int64_t T, int64_t gqa) { return T * gqa <= 16 ? 16 : (T * gqa <= 32 ? 32 : 64); }
+
+template <int BITS, int D, int N> cudaError_t launch_n(const KvPagesTreeArgs& t, cudaStream_t st) {
+  auto kern = tree_kernel<BITS, D, N>;
+  static bool done[64] = {};
+  const size_t most = Shape<BITS, D, N>::SMEM + 2 * (kMaxPageSeqs + 1) * 4, smem = Shape<BITS, D, N>::SMEM + 2 * (size_t)(t.a.B + 1) * 4;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  {
+    std::lock_guard<std::mutex> setup_lk(setup_mutex());     // first use on a device, from any thread
+    if (dev < 0 || dev >= 64 || !done[dev]) {
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+      if (e != cudaSuccess) return e;
+      if (dev >= 0 && dev < 64) done[dev] = true;
+    }
+  }
+  const unsigned grid = (unsigned)sm_count();
+  e = launch_behind(kern, dim3(grid), dim3(Shape<BITS, D, N>::THREADS), smem, st, t);
+  if (e != cudaSuccess) return e;
+  return launch_behind(tree_join_kernel<BITS, D>, dim3(grid, (N + kJoinRows - 1) / kJoinRows), dim3(kJoinWarps * 32), 0, st, t, N);
+}
+template <int BITS, int D> cudaError_t launch_d(const KvPagesTreeArgs& t, cudaStream_t st) {
+  switch (columns(t.T, t.a.gqa)) {
+    case 16: return launch_n<BITS, D, 16>(t, st);
+    case 32: return launch_n<BITS, D, 32>(t, st);
+    default: return launch_n<BITS, D, 64>(t, st);
+  }
 }
 }  // namespace
 
-size_t kv_pages_tree_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t) { return 16; }
+// [joins: int4 per CTA][r, l: float2 per slot and row][o: D floats per slot and row], two slots a CTA
+size_t kv_pages_tree_workspace_bytes(int64_t, int64_t Hq, int64_t Hkv, int64_t T, int64_t D) {
+  const size_t ctas = (size_t)sm_count(), rows = (size_t)columns(T, Hq / Hkv);
+  return ctas * 16 + ctas * 2 * rows * (8 + (size_t)D * 4);
+}
 
-cudaError_t launch_kv_pages_tree(KvPagesTreeArgs t, int D, void*, cudaStream_t st) {
-  const unsigned grid = (unsigned)(((int64_t)t.a.B * t.a.Hq * t.T + 7) / 8);
+cudaError_t launch_kv_pages_tree(KvPagesTreeArgs t, int D, void* workspace, cudaStream_t st) {
+  const size_t ctas = (size_t)sm_count(), rows = (size_t)columns(t.T, t.a.gqa);
+  t.a.joins = (int4*)workspace;
+  t.a.part_ml = (float2*)((char*)workspace + ctas * 16);
+  t.a.part_o = (float*)((char*)workspace + ctas * 16 + ctas * 2 * rows * 8);
   switch (t.a.bits * 1000 + D) {
-    case 4064: return launch_kernel(tree_simple_kernel<4, 64>, dim3(grid), dim3(256), 0, st, t);
-    case 4128: return launch_kernel(tree_simple_kernel<4, 128>, dim3(grid), dim3(256), 0, st, t);
-    case 8064: return launch_kernel(tree_simple_kernel<8, 64>, dim3(grid), dim3(256), 0, st, t);
-    case 8128: return launch_kernel(tree_simple_kernel<8, 128>, dim3(grid), dim3(256), 0, st, t);
-    case 16064: return launch_kernel(tree_simple_kernel<16, 64>, dim3(grid), dim3(256), 0, st, t);
-    case 16128: return launch_kernel(tree_simple_kernel<16, 128>, dim3(grid), dim3(256), 0, st, t);
+    case 4064: return launch_d<4, 64>(t, st);
+    case 4128: return launch_d<4, 128>(t, st);
+    case 8064: return launch_d<8, 64>(t, st);
+    case 8128: return launch_d<8, 128>(t, st);
+    case 16064: return launch_d<16, 64>(t, st);
+    case 16128: return launch_d<16, 128>(t, st);
     default: return cudaErrorInvalidValue;
   }
 }
+
+void tree_attn_error_reset() {
+  const int zero = 0;
+  cudaMemcpyToSymbol(g_tree_error, &zero, sizeof(int));
+}
+int tree_attn_error_code() {
+  int v = 0;
+  cudaMemcpyFromSymbol(&v, g_tree_error, sizeof(int));
+  return v;
+}
+
 }  // namespace qb

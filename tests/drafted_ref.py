@@ -40,15 +40,21 @@ def attention(q, k, v, scale):
     return p @ v, p @ v.abs(), (abs(scale) * q.abs() @ k.abs().T).amax(-1, keepdim=True)
 
 
-def tolerance(o, A, S, bits):
-    """Of one output o = sum p v of the tree attention: half a bf16 step of the result, 2^-8 |o|, and against A = sum p |v|: half a step of every
-    probability (bf16 beside bf16 values, 2^-8; else fp16, 2^-11, with 2^-18 for the sum of those that drop under its normal range), half an
-    fp16 step of the values at 4 and 8 bits (2^-11), the approximate exponential (a cubic of 7.5e-5 may stand for it: 2^-12 for sum and normaliser), and
-    twice the scores' error: at 4 and 8 bits half an fp16 step of every key, 2^-11 of S = scale * sum |q| |k|, and fp32 sums whose
-    roundings, truncating ones too, are off by 2^-23 of S each step of 16 products and for the reference, 20 in all."""
+def tolerance(o, A, S, bits, v):
+    """Of one output o = sum p v of the tree attention over the values v: half a bf16 step of the result, 2^-8 |o|, and against A = sum p |v|:
+    half a step of every probability (bf16 beside bf16 values, 2^-8; else fp16, 2^-11), half an fp16 step of the values at 4 and 8 bits
+    (2^-11), the approximate exponential (a cubic of 7.5e-5 may stand for it: 2^-12 for sum and normaliser), and twice the scores' error: at 4
+    and 8 bits half an fp16 step of every key, 2^-11 of S = scale * sum |q| |k|, and fp32 sums whose roundings, truncating ones too, are off
+    by 2^-23 of S each step of 16 products and for the reference, 20 in all.
+
+    Probabilities under fp16's normal range are off by 2^-25 each, whatever the sum A at that dim: a token's P' = p 2^(e - r) meets
+    v 2^-e < 2^15, so n of them move the sum by at most n 2^-25 2^15.  The reference was placed where the largest P' was 2^8, of a token with a
+    value of M >= 2^14 2^e: its p alone makes the normaliser at least 2^8 2^-e >= 2^22 / M.  So the result moves by at most
+    n 2^-10 M 2^-22 = n 2^-32 M, M at most the largest |v|."""
     quantised = bits != 16
-    part = 2.0 ** -8 if not quantised else 2.0 ** -11 + 2.0 ** -18 + 2.0 ** -11
-    return 2.0 ** -8 * o.abs() + A * (part + 2.0 ** -12 + S * (40 * 2.0 ** -23 + (2.0 ** -10 if quantised else 0.0))) * 1.01 + 1e-30
+    part = 2.0 ** -8 if not quantised else 2.0 ** -11 + 2.0 ** -11
+    small = v.shape[0] * 2.0 ** -32 * float(v.abs().max()) if quantised and v.numel() else 0.0
+    return 2.0 ** -8 * o.abs() + A * (part + 2.0 ** -12 + S * (40 * 2.0 ** -23 + (2.0 ** -10 if quantised else 0.0))) * 1.01 + small + 1e-30
 
 
 def sample(x, u, t, k, p, least):

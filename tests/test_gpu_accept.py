@@ -254,4 +254,4 @@ def test_rounds_of_drafted_decoding(bits):
         pid = table[s][(at // page)].long()
         for h in range(Hkv):
             o, A, sc = attention(q[s, h * 4:(h + 1) * 4, 0].to(F64), kd[pid, h, at % page], vd[pid, h, at % page], scale)
-            assert ((out[s, h * 4:(h + 1) * 4, 0].to(F64) - o).abs() <= tolerance(o, A, sc, bits)).all()
+            assert ((out[s, h * 4:(h + 1) * 4, 0].to(F64) - o).abs() <= tolerance(o, A, sc, bits, vd[pid, h, at % page])).all()

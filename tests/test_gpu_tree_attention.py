@@ -54,7 +54,7 @@ def check(out, q, kp, vp, table, lens, trees, counts, page, bits, scale, window=
                     assert not torch.isfinite(got).all(-1).any(), f"b {b} node {t}: sees what is not finite"
                     continue
                 o, A, S = attention(q[b, h * rep:(h + 1) * rep, t].to(F64), k[pid, h, at % page], v[pid, h, at % page], scale)
-                tol = tolerance(o, A, S, bits)
+                tol = tolerance(o, A, S, bits, v[pid, h, at % page])
                 err = (got - o).abs()
                 assert not torch.isnan(got).any(), f"b {b} node {t} head {h}: NaN"
                 worst = max(worst, float((err / tol).max()))
