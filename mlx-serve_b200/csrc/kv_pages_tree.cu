@@ -40,23 +40,36 @@ constexpr int kPiece = 5;            // what a piece of a tile takes beside its 
 constexpr int kJoinRows = 8, kJoinWarps = 16;
 
 template <int BITS, int D, int N> struct Shape {
+  static constexpr bool QUANT = BITS != 16;
   static constexpr int G = BITS == 16 ? 1 : D / 64;          // scale groups of a token
   static constexpr int HALVES = D / 64;                      // blocks of 64 columns (128 bytes) side by side
   static constexpr int ROWB = D * BITS / 8, CH = ROWB / 16;  // bytes of a token, 16-byte chunks of it
   static constexpr int NC = N < 32 ? N : 32;                 // columns of a softmax warp
   static constexpr int WGS = N / NC, SW = 4 * WGS;           // groups of four softmax warps
-  static constexpr int THREADS = (SW + 9) * 32;
+  static constexpr int KW = QUANT ? 4 : 0;                   // warps that read keys
+  static constexpr int V_AT = SW + KW, MMA_AT = V_AT + 4, COPY_AT = MMA_AT + 1;   // first warp of the values, of the products, of the copies
+  static constexpr bool SPLIT = QUANT && WGS == 2;           // registers dealt out by role
+  static constexpr int THREADS = SPLIT ? 640 : (COPY_AT + 1) * 32;
   static constexpr int TILE = kBlk * 128 * HALVES;           // a block's keys or values as an operand
-  static constexpr int STAGES = BITS == 4 ? 4 : (BITS == 8 ? 3 : (D == 64 ? 4 : 2));
-  static constexpr int VT = BITS == 16 ? STAGES : 2, KT = BITS == 16 ? STAGES : 0;
-  static constexpr int PS = BITS == 8 && D == 128 ? 1 : 2;   // places for P
+  static constexpr int SB = kBlk * G * 2;                    // bytes of a block's scales (or biases)
+  static constexpr int VT = 2;                               // places for values as operands
+  static constexpr int PS = D == 128 && (BITS == 8 || (BITS == 16 && N == 64)) ? 1 : 2;   // places for P
   static constexpr int PTILE = kBlk * 128;
-  static constexpr int SB = 32 * G * 2;                      // bytes of a warp's scales (or biases) of a block
-  static constexpr int RS = BITS == 16 ? 0 : 32 * ROWB + 4 * SB;
-  static constexpr int V0 = 0, K0 = VT * TILE, Q0 = K0 + KT * TILE, P0 = Q0 + N * 128 * HALVES, R0 = P0 + PS * PTILE;
-  static constexpr int SMEM = R0 + 8 * STAGES * RS + 1024;
-  static_assert(SMEM + 2 * (kMaxPageSeqs + 1) * 4 + 12 * 1024 <= 227 * 1024, "shared memory");
+  // the rings: codes with scales and biases (the keys' with the values' too, for their units), or at 16 bits the operands themselves
+  static constexpr int KS = BITS == 4 ? 4 : (BITS == 8 ? 3 : (D == 64 ? 4 : 2)), VS = BITS == 4 ? 4 : (BITS == 8 ? 3 : (D == 64 ? 4 : 3));
+  static constexpr int K_STAGE = QUANT ? kBlk * ROWB + 4 * SB : TILE, V_STAGE = QUANT ? kBlk * ROWB + 2 * SB : TILE;
+  static constexpr int V0 = 0, Q0 = QUANT ? VT * TILE : 0, P0 = Q0 + N * 128 * HALVES, KR = P0 + PS * PTILE, VR = KR + KS * K_STAGE;
+  static constexpr int SMEM = VR + VS * V_STAGE + (QUANT || D == 128 ? 0 : TILE) + 1024;   // (a product of 128 rows reads a tile past the last one of 64)
+  static constexpr int ATOM = QUANT && ROWB < 128 ? 512 : 1024;
+  static_assert(KR % 1024 == 0 && K_STAGE % ATOM == 0 && V_STAGE % ATOM == 0, "places of boxes");
+  static_assert(SMEM + 2 * (kMaxPageSeqs + 1) * 4 + 11 * 1024 <= 227 * 1024, "shared memory");
   static constexpr uint32_t S_AT = 0, O_AT = 128, K_AT = 192;   // columns of tensor memory: two of S, O, two of K
+};
+
+// A pool's codes (or rows) as boxes of up to 128 tokens of one head in one page, and what a box takes along head and page (0: broadcast).
+struct TreeMaps {
+  int mul[2][2];
+  int piece;                 // tokens of a box
 };
 
 __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accum) {
@@ -113,6 +126,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {   // (a NaN d
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+               ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 // A bounded wait that polls without sleeping.
 __device__ __forceinline__ bool spin_cta(uint64_t* bar, uint32_t parity) {
@@ -271,21 +292,22 @@ struct Pieces {
 };
 
 template <int BITS, int D, int N>
-__global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(const __grid_constant__ KvPagesTreeArgs t) {
+__global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                                                                             const __grid_constant__ KvPagesTreeArgs t, const __grid_constant__ TreeMaps maps) {
   using SH = Shape<BITS, D, N>;
-  constexpr int G = SH::G, CH = SH::CH, NC = SH::NC, SW = SH::SW, STAGES = SH::STAGES, THREADS = SH::THREADS;
-  constexpr bool QUANT = BITS != 16;
+  constexpr int G = SH::G, CH = SH::CH, NC = SH::NC, SW = SH::SW, KS = SH::KS, VS = SH::VS, THREADS = SH::THREADS;
+  constexpr bool QUANT = SH::QUANT;
   const KvPagesAttnArgs& a = t.a;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* const smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   int* const units = (int*)(smem + SH::SMEM - 1024);          // [B + 1], [B + 1]
   int* const tiles = units + a.B + 1;
-  __shared__ uint64_t q_ready, k_ready[2], v_ready[2], s_ready[2], p_ready[2], o_done[2];
+  __shared__ uint64_t q_ready, k_ready[2], v_ready[2], s_ready[2], p_ready[2], o_done[2], k_full[KS], k_empty[KS], v_full[VS], v_empty[VS];
   __shared__ uint32_t tmem_slot;
   __shared__ int s_fail, s_longest[32], warp_sums[2][32];
   __shared__ __align__(16) float s_nr[N], s_kunit[4][kBlk];     // -r of the columns; of a block's tokens
   __shared__ int s_vexp[4][kBlk];
-  __shared__ uint32_t s_kmask[4][4], s_vm[8][STAGES];
+  __shared__ uint32_t s_pages[16];       // of a block: which of its 16 tokens have a page
   __shared__ float s_wmax[SH::WGS][4][NC];
   __shared__ int s_par[kMaxNodes], s_depth[kMaxNodes], s_clo[N], s_qe[N];
   __shared__ uint64_t s_line[kMaxNodes], s_cline[N];
@@ -318,11 +340,13 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
       s_fail = 0;
       mbar_init(&q_ready, SW);
       for (int i = 0; i < 2; ++i) { mbar_init(&k_ready[i], 4); mbar_init(&v_ready[i], 4); mbar_init(&s_ready[i], 1); mbar_init(&p_ready[i], SW); mbar_init(&o_done[i], 1); }
+      for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], QUANT ? 4 : 1); }
+      for (int i = 0; i < VS; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], QUANT ? 4 : 1); }
       for (int i = 0; i < 4; ++i) note_count[i] = 0;
       a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
       asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == SW + 8) {
+    if (warp == SH::MMA_AT) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u));
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
@@ -352,115 +376,53 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
   const int pmask = (1 << a.page_shift) - 1;
   int J0 = 0;                        // blocks before this piece
 
-  if (warp >= SW && warp < SW + 8) {
+  if (warp >= SW && warp < SH::MMA_AT) {
     // ---------------- keys, values ----------------
-    const bool V = warp >= SW + 4;
-    const int wq = warp & 3, w8 = warp - SW;                   // quarter of the block: 32 tokens
-    const KvPoolView& pool = a.pool[V];
-    const uint32_t page_b = a.page_bytes[V], tok_b = a.tok_bytes[V];
-    unsigned char* const ring = smem + SH::R0 + w8 * STAGES * SH::RS;
-    constexpr int RPI = 32 / CH;                               // token rows of one copy instruction
-    const int cc = lane % CH, r0 = lane / CH;
-    auto swz = [](int r) { return CH >= 8 ? (r & 7) & (CH - 1) : (r / (8 / CH)) % CH; };   // so that 8 neighbours' rows lie in different banks
-    int piece_no = 0;
+    if constexpr (SH::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    const bool V = warp >= SH::V_AT;
+    const int wq = warp & 3, key = 32 * wq + lane;             // quarter of the block: 32 tokens, one a lane
+    uint64_t* const full = V ? v_full : k_full;
+    uint64_t* const empty = V ? v_empty : k_empty;
+    const int stages = V ? VS : KS, stage_b = V ? SH::V_STAGE : SH::K_STAGE;
+    unsigned char* const ring = smem + (V ? SH::VR : SH::KR);
+    const int swz = CH >= 8 ? lane & 7 & (CH - 1) : (lane / (8 / CH)) % CH;       // (16-byte chunks of a row, as the copies place them)
+    int piece_no = 0, st = 0;
+    uint32_t round = 0;
     while (pieces.next(pc)) {
-      const int32_t* const tab = a.table + (int64_t)pc.s.row * a.table_str;
-      const unsigned char* const base = (const unsigned char*)pool.q + (int64_t)pc.hk * a.q_head[V] + (int64_t)r0 * tok_b + cc * 16;
-      // lane l holds the page of the 16 tokens from 16 * (l & 1) of the warp's 32 on, -1 where there is none
-      auto page_at = [&](int j) {
-        int pid = -1;
-        if (j < pc.todo) {
-          const int tok = pc.first_token(j) + 32 * wq + 16 * (lane & 1);
-          if (tok < pc.s.len) pid = tab[tok >> a.page_shift];
-          if (pid >= a.P) pid = -1;
-        }
-        return pid;
-      };
-      int pid_next = page_at(0);
-      auto issue = [&](int j, int given) {                     // (given: blocks that the products have been given, or soon will be)
-        const int J = J0 + j, st = J % STAGES;
-        const int pid_cur = pid_next, tok0 = pc.first_token(j) + 32 * wq;
-        pid_next = page_at(j + 1);
-        const int p0 = __shfl_sync(0xffffffffu, pid_cur, 0), p1 = __shfl_sync(0xffffffffu, pid_cur, 1);
-        const bool mine = pc.some_see(tok0 + lane) && (lane < 16 ? p0 : p1) >= 0;
-        const uint32_t vm = __ballot_sync(0xffffffffu, mine);
-        if (lane == 0) s_vm[w8][st] = vm;
-        uint32_t dst0;
-        if constexpr (QUANT) dst0 = smem_u32(ring + st * SH::RS);
-        else {
-          dst0 = smem_u32(smem + (V ? SH::V0 : SH::K0) + st * SH::TILE);
-          // the products that read the slot, or later ones: two blocks back the barrier may already be a phase further
-          const int read = J - STAGES > given - 2 ? J - STAGES : given - 2;
-          if (read >= 0) wait((V ? o_done : s_ready) + (read & 1), (uint32_t)(read >> 1), 605);
-        }
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          const int r = i * RPI + r0, pid = i * RPI < 16 ? p0 : p1;
-          const unsigned char* const src = base + (uint64_t)(uint32_t)(pid < 0 ? 0 : pid) * page_b + (uint64_t)(uint32_t)((tok0 + i * RPI) & pmask) * tok_b;
-          uint32_t dst;
-          if constexpr (QUANT) dst = dst0 + r * SH::ROWB + ((cc ^ swz(r)) << 4);
-          else dst = dst0 + (cc >> 3) * (kBlk * 128) + (32 * wq + r) * 128 + (((cc & 7) ^ (r & 7)) << 4);
-          cp_async16_z(dst, src, (vm >> r) & 1u ? 16u : 0u);
-        }
-        if constexpr (QUANT) {
-          // [scales, biases of this pool][of the values: the keys' warps give their units on], 32 tokens each
-          const int arrays = V ? 2 : 4;
-          unsigned char* const sb = ring + st * SH::RS + 32 * SH::ROWB;
-          if (a.sb_vec) {
-            constexpr int TP = 8 / G;                          // tokens of a 16-byte piece
-            if (lane < arrays * 4 * G) {
-              const int arr = lane / (4 * G), tok = lane % (4 * G) * TP, pid = tok < 16 ? p0 : p1;
-              const KvPoolView& pl = arr >= 2 ? a.pool[1] : pool;
-              const uint16_t* const src = (const uint16_t*)((arr & 1) ? pl.b : pl.s) + (int64_t)(pid < 0 ? 0 : pid) * pl.sb_str[0] + (int64_t)pc.hk * pl.sb_str[1] +
-                                          (int64_t)((tok0 + tok) & pmask) * G;
-              cp_async16_z(smem_u32(sb + arr * SH::SB + tok * G * 2), src, pid >= 0 && tok0 + tok < pc.s.len ? 16u : 0u);
-            }
-          } else {
-            const int pid = lane < 16 ? p0 : p1;
-            for (int arr = 0; arr < arrays; ++arr) {
-              const KvPoolView& pl = arr >= 2 ? a.pool[1] : pool;
-              const uint16_t* const src = (const uint16_t*)((arr & 1) ? pl.b : pl.s) + (int64_t)(pid < 0 ? 0 : pid) * pl.sb_str[0] + (int64_t)pc.hk * pl.sb_str[1] +
-                                          (int64_t)((tok0 + lane) & pmask) * pl.sb_str[2];
-#pragma unroll
-              for (int g = 0; g < G; ++g) ((uint16_t*)(sb + arr * SH::SB))[lane * G + g] = mine ? src[g] : (uint16_t)0;
-            }
-          }
-        }
-      };
-#pragma unroll 1
-      for (int j = 0; j < STAGES - 1; ++j) {
-        if (j < pc.todo) issue(j, J0);
-        cp_async_commit();
-      }
 #pragma unroll 1
       for (int j = 0; j < pc.todo; ++j) {
-        const int J = J0 + j, st = J % STAGES, key = 32 * wq + lane;
-        if (j + STAGES - 1 < pc.todo) issue(j + STAGES - 1, J);
-        cp_async_commit();
-        cp_async_wait<STAGES - 1>();
-        __syncwarp();
-        const uint32_t vm = s_vm[w8][st];
-        const bool mine = (vm >> lane) & 1u;
-        if (!V && lane == 0) s_kmask[J & 3][wq] = vm;
+        const int J = J0 + j, tok = pc.first_token(j) + key;
+        wait(&full[st], round, 605);
+        const bool mine = pc.some_see(tok) && ((s_pages[J & 15] >> (key >> 4)) & 1u);
         // a value that some nodes see and others do not must not meet their 0 if it is not finite: it is zeroed and noted
-        const int tok = pc.first_token(j) + key;
         const bool partly = V && mine && !pc.all_see(t, tok);
         bool bad = false;
         if constexpr (QUANT) {
-          const unsigned char* const codes = ring + st * SH::RS;
-          const unsigned char* const sb = codes + 32 * SH::ROWB;
-          float s[G], b[G], top = 0.f;
+          const unsigned char* const codes = ring + st * stage_b;
+          const unsigned char* const sb = codes + kBlk * SH::ROWB;
+          float s[G], b[G];
           auto params = [&](int arr, float (&x)[G]) {
-            if constexpr (G == 2) {
-              const uint32_t v = mine ? *(const uint32_t*)(sb + arr * SH::SB + lane * 4) : 0u;
-              x[0] = bf16lo(v); x[G - 1] = bf16hi(v);
-            } else x[0] = mine ? bf16_bits_to_f32(*(const uint16_t*)(sb + arr * SH::SB + lane * 2)) : 0.f;
+            uint32_t v = 0u;
+            if (a.sb_vec) {
+              if constexpr (G == 2) v = *(const uint32_t*)(sb + arr * SH::SB + key * 4);
+              else v = *(const uint16_t*)(sb + arr * SH::SB + key * 2);
+            } else if (mine) {
+              const KvPoolView& pl = a.pool[V || arr >= 2];
+              const int pid = a.table[(int64_t)pc.s.row * a.table_str + (tok >> a.page_shift)];
+              const uint16_t* const src = (const uint16_t*)((arr & 1) ? pl.b : pl.s) + (int64_t)pid * pl.sb_str[0] + (int64_t)pc.hk * pl.sb_str[1] + (int64_t)(tok & pmask) * pl.sb_str[2];
+              v = src[0];
+              if constexpr (G == 2) v |= (uint32_t)src[1] << 16;
+            }
+            v = mine ? v : 0u;
+            x[0] = bf16lo(v);
+            if constexpr (G == 2) x[G - 1] = bf16hi(v);
           };
           auto largest = [&]() {
             float m = 0.f;
+            bad = false;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-              const float x = group_top<BITS>(s[g], b[g]);
+              const float x = group_top<BITS>(s[g], b[g]);     // (a NaN where s or b is one or both are infinite)
               const bool off = !(x < INFINITY) || !(fabsf(s[g]) < INFINITY);
               bad |= off;
               m = fmaxf(m, off ? 0.f : x);
@@ -471,10 +433,8 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
             params(2, s); params(3, b);
             s_vexp[J & 3][key] = unit_exp(largest()) - 14;
           }
-          bad = false;
           params(0, s); params(1, b);
-          top = largest();
-          const int e = unit_exp(top);
+          const int e = unit_exp(largest());
           const float up = pow2i(14 - e);
           if (!V) s_kunit[J & 3][key] = pow2i(e - 14);
           const bool drop = partly && bad;
@@ -489,7 +449,8 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
             uint32_t o[32];
 #pragma unroll
             for (int c = 0; c < CG; ++c) {
-              const uint4 x = *(const uint4*)(codes + lane * SH::ROWB + (((g * CG + c) ^ swz(lane)) << 4));
+              // (a token that is not seen: 0 * 0 + 0 whatever the codes are)
+              const uint4 x = *(const uint4*)(codes + key * SH::ROWB + (((g * CG + c) ^ swz) << 4));
               constexpr int W = 32 / BITS / 2;                 // registers of a word
               dequant_word<BITS>(x.x, s2[g], b2[g], &o[(4 * c + 0) * W]); dequant_word<BITS>(x.y, s2[g], b2[g], &o[(4 * c + 1) * W]);
               dequant_word<BITS>(x.z, s2[g], b2[g], &o[(4 * c + 2) * W]); dequant_word<BITS>(x.w, s2[g], b2[g], &o[(4 * c + 3) * W]);
@@ -507,9 +468,9 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
           } else fence_async();
         } else {
           // (the products two blocks back are done, so that this arrival is not taken for one of theirs)
-          if (STAGES > 2 && J >= 2) wait((V ? o_done : s_ready) + (J & 1), (uint32_t)((J >> 1) - 1), V ? 602 : 601);
-          if (__any_sync(0xffffffffu, partly)) {
-            unsigned char* const vrow = smem + SH::V0 + st * SH::TILE + key * 128;
+          if (J >= 2) wait(&o_done[J & 1], (uint32_t)((J >> 1) - 1), 602);
+          if (__any_sync(0xffffffffu, partly || !mine)) {
+            unsigned char* const vrow = ring + st * stage_b + key * 128;
             if (partly) {
               uint32_t acc = 0;
 #pragma unroll
@@ -518,52 +479,126 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
                 acc |= ((x.x & 0x7F807F80u) + 0x00800080u) | ((x.y & 0x7F807F80u) + 0x00800080u) | ((x.z & 0x7F807F80u) + 0x00800080u) | ((x.w & 0x7F807F80u) + 0x00800080u);
               }
               bad = (acc & 0x80008000u) != 0;                  // an exponent of all ones
-              if (bad)
-#pragma unroll
-                for (int c = 0; c < D / 8; ++c) *(uint4*)(vrow + (c >> 3) * (kBlk * 128) + (((c & 7) ^ (key & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
             }
+            if (bad || !mine)
+#pragma unroll
+              for (int c = 0; c < D / 8; ++c) *(uint4*)(vrow + (c >> 3) * (kBlk * 128) + (((c & 7) ^ (key & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+            fence_async();
           }
-          fence_async();
         }
         if (partly && bad) {
           const int at = atomicAdd(&note_count[piece_no & 3], 1);
           if (at < kNotes) note_key[piece_no & 3][at] = tok;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive((V ? v_ready : k_ready) + (J & 1));
+        if (lane == 0) {
+          mbar_arrive((V ? v_ready : k_ready) + (J & 1));
+          if (QUANT) mbar_arrive(&empty[st]);
+        }
+        if (++st == stages) { st = 0; ++round; }
       }
-      cp_async_wait<0>();
       J0 += pc.todo;
       ++piece_no;
     }
-  } else if (warp == SW + 8) {
+  } else if (warp == SH::COPY_AT) {
+    // ---------------- copies: a lane a piece of a block ----------------
+    if constexpr (SH::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    const int pieces_of = kBlk / maps.piece, groups = maps.piece / 16;
+    int ks = 0, vs = 0;
+    uint32_t kr = 0, vr = 0;
+    while (pieces.next(pc)) {
+      const int32_t* const tab = a.table + (int64_t)pc.s.row * a.table_str;
+      auto page_at = [&](int j) {
+        int pid = -1;
+        if (j < pc.todo && lane < pieces_of) {
+          const int tok = pc.first_token(j) + lane * maps.piece;
+          if (tok < pc.s.len) pid = tab[tok >> a.page_shift];
+          if (pid >= a.P) pid = -1;
+        }
+        return pid;
+      };
+      int pid_next = page_at(0);
+#pragma unroll 1
+      for (int j = 0; j < pc.todo; ++j) {
+        const int J = J0 + j, pid = pid_next, tok = pc.first_token(j) + lane * maps.piece, row = tok & pmask;
+        pid_next = page_at(j + 1);
+        const uint32_t have = __ballot_sync(0xffffffffu, pid >= 0);
+        const int n = __popc(have);
+        uint32_t bits = 0;                                     // of 16 tokens each
+        for (int i = 0; i < pieces_of; ++i)
+          if ((have >> i) & 1u) bits |= ((1u << groups) - 1u) << (i * groups);
+        const uint32_t codes_b = (uint32_t)maps.piece * SH::ROWB, sb_b = (uint32_t)maps.piece * G * 2;
+        auto scales = [&](const KvPoolView& pl, unsigned char* to, uint64_t* bar) {
+          const int64_t at = (int64_t)pid * pl.sb_str[0] + (int64_t)pc.hk * pl.sb_str[1] + (int64_t)row * G;
+          bulk_load(smem_u32(to) + lane * sb_b, (const uint16_t*)pl.s + at, sb_b, bar);
+          bulk_load(smem_u32(to) + SH::SB + lane * sb_b, (const uint16_t*)pl.b + at, sb_b, bar);
+        };
+        const bool vec = QUANT && a.sb_vec;
+        if (kr > 0) wait(&k_empty[ks], kr - 1, 613);
+        unsigned char* const kst = smem + SH::KR + ks * SH::K_STAGE;
+        if (lane == 0) {
+          s_pages[J & 15] = bits;
+          mbar_expect_tx(&k_full[ks], (uint32_t)n * (codes_b + (vec ? 4 * sb_b : 0u)));
+        }
+        __syncwarp();
+        if (pid >= 0) {
+#pragma unroll
+          for (int h = 0; h < (QUANT ? 1 : SH::HALVES); ++h)
+            tma_load_4d(smem_u32(kst) + h * kBlk * 128 + lane * (QUANT ? codes_b : (uint32_t)maps.piece * 128u), &mk, &k_full[ks], 64 * h, row, pc.hk * maps.mul[0][0], pid * maps.mul[0][1]);
+          if (vec) { scales(a.pool[0], kst + kBlk * SH::ROWB, &k_full[ks]); scales(a.pool[1], kst + kBlk * SH::ROWB + 2 * SH::SB, &k_full[ks]); }
+        }
+        __syncwarp();
+        if (vr > 0) wait(&v_empty[vs], vr - 1, 614);
+        unsigned char* const vst = smem + SH::VR + vs * SH::V_STAGE;
+        if (lane == 0) mbar_expect_tx(&v_full[vs], (uint32_t)n * (codes_b + (vec ? 2 * sb_b : 0u)));
+        __syncwarp();
+        if (pid >= 0) {
+#pragma unroll
+          for (int h = 0; h < (QUANT ? 1 : SH::HALVES); ++h)
+            tma_load_4d(smem_u32(vst) + h * kBlk * 128 + lane * (QUANT ? codes_b : (uint32_t)maps.piece * 128u), &mv, &v_full[vs], 64 * h, row, pc.hk * maps.mul[1][0], pid * maps.mul[1][1]);
+          if (vec) scales(a.pool[1], vst + kBlk * SH::ROWB, &v_full[vs]);
+        }
+        __syncwarp();
+        if (++ks == KS) { ks = 0; ++kr; }
+        if (++vs == VS) { vs = 0; ++vr; }
+      }
+      J0 += pc.todo;
+    }
+    if (dead)
+      for (int i = 0; i < 1000; ++i) __nanosleep(1000);        // (copies may still be on their way)
+  } else if (warp == SH::MMA_AT) {
     // ---------------- products ----------------
+    if constexpr (SH::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     constexpr uint32_t type = QUANT ? 0u : 1u;                 // fp16, bf16
     constexpr uint32_t idesc0 = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
     constexpr uint32_t idesc_s = idesc0, idesc_o = idesc0 | (1u << 15) | (1u << 16);   // the values and P: columns contiguous
     auto U = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
     const uint32_t tm = (uint32_t)U((int)tmem), sm = (uint32_t)U((int)smem_u32(smem));
     const uint64_t hi_k = make_desc(0) & 0xFFFFFFFF00000000ull, hi_v = make_desc_mn(0) & 0xFFFFFFFF00000000ull;
-    const uint32_t q_d = (uint32_t)make_desc(sm + SH::Q0), k_d = (uint32_t)make_desc(sm + SH::K0), v_d = (uint32_t)make_desc_mn(sm + SH::V0), p_d = (uint32_t)make_desc_mn(sm + SH::P0);
+    const uint32_t q_d = (uint32_t)make_desc(sm + SH::Q0), k_d = (uint32_t)make_desc(sm + SH::KR), v_d = (uint32_t)make_desc_mn(sm + (QUANT ? SH::V0 : SH::VR)), p_d = (uint32_t)make_desc_mn(sm + SH::P0);
     auto spin = [&](uint64_t* bar, uint32_t phase, int code) {
       if (dead) return;
       dead = !__all_sync(0xffffffffu, spin_cta(bar, phase & 1));
       if (dead && lane == 0 && !s_fail) { s_fail = code; atomicCAS(&g_tree_error, 0, code); }
     };
-    int piece_no = 0;
+    int piece_no = 0, ks = 0, vs = 0;                          // (at 16 bits the operands are the rings' places)
+    uint32_t kr = 0;
     auto scores = [&](int J) {
-      spin(&k_ready[J & 1], (uint32_t)(J >> 1), 603);
+      if constexpr (QUANT) spin(&k_ready[J & 1], (uint32_t)(J >> 1), 603);
+      else spin(&k_full[ks], kr, 603);
       fence_after();
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint64_t q = hi_k | (q_d + (k >> 2) * ((N * 128) >> 4) + (k & 3) * 2);
           if constexpr (QUANT) umma_ts(tm + SH::S_AT + (J & 1) * 64, tm + SH::K_AT + (J & 1) * 64 + k * 8, q, idesc_s, k > 0);
-          else umma_ss(tm + SH::S_AT + (J & 1) * 64, hi_k | (k_d + (J % STAGES) * (SH::TILE >> 4) + (k >> 2) * ((kBlk * 128) >> 4) + (k & 3) * 2), q, idesc_s, k > 0);
+          else umma_ss(tm + SH::S_AT + (J & 1) * 64, hi_k | (k_d + ks * (SH::TILE >> 4) + (k >> 2) * ((kBlk * 128) >> 4) + (k & 3) * 2), q, idesc_s, k > 0);
         }
         commit(&s_ready[J & 1]);
+        if (!QUANT) commit(&k_empty[ks]);
       }
       __syncwarp();
+      if (!QUANT && ++ks == KS) { ks = 0; ++kr; }
     };
     while (pieces.next(pc)) {
       const int todo = U(pc.todo);
@@ -577,11 +612,13 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < kBlk / 16; ++k)
-              umma_ss(tm + SH::O_AT, hi_v | (v_d + (J % SH::VT) * (SH::TILE >> 4) + k * (2048 >> 4)), hi_v | (p_d + (J % SH::PS) * (SH::PTILE >> 4) + k * (2048 >> 4)), idesc_o,
+              umma_ss(tm + SH::O_AT, hi_v | (v_d + (QUANT ? J & 1 : vs) * (SH::TILE >> 4) + k * (2048 >> 4)), hi_v | (p_d + (J % SH::PS) * (SH::PTILE >> 4) + k * (2048 >> 4)), idesc_o,
                       k > 0 ? 1u : (j > 0 ? 1u : 0u));
             commit(&o_done[J & 1]);
+            if (!QUANT) commit(&v_empty[vs]);
           }
           __syncwarp();
+          if (!QUANT && ++vs == VS) vs = 0;
         }
         if (j + 2 < todo) scores(J0 + j + 2);
       }
@@ -592,8 +629,9 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
     if (J0 > 0) spin(&o_done[(J0 - 1) & 1], (uint32_t)((J0 - 1) >> 1), 608);
     if (s_fail)
       for (int i = 0; i < 1000; ++i) __nanosleep(1000);        // (products may still be on their way)
-  } else {
+  } else if (warp < SW) {
     // ---------------- softmax: a thread a token ----------------
+    if constexpr (SH::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     const int wg = warp >> 2, wq = warp & 3, key = tid & 127, col0 = wg * NC;
     const uint32_t lanes = tmem + ((uint32_t)wq << 21);
     constexpr int ALL = SW * 32;
@@ -692,7 +730,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
         const int J = J0 + j, k0 = pc.first_token(j), tok = k0 + key;
         wait(&s_ready[J & 1], (uint32_t)(J >> 1), 609);
         fence_after();
-        const uint32_t vm = s_kmask[J & 3][wq];
+        const bool mine = pc.some_see(tok) && ((s_pages[J & 15] >> (key >> 4)) & 1u);
         float ck = Cq, w = 1.f, ev = 0.f;
         if constexpr (QUANT) {
           const int e = s_vexp[J & 3][key];
@@ -700,7 +738,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
           ev = (float)e;
           w = pow2i(-e);
         }
-        const bool masked = vm != 0xffffffffu || !pc.whole(t, k0);
+        const bool masked = s_pages[J & 15] != 0xffu || !pc.whole(t, k0);
         const uint32_t s_at = lanes + SH::S_AT + (J & 1) * 64 + col0;
         uint32_t z[NC];
         auto exponents = [&](bool with_reference) {            // of P' (or, without the reference, of P' 2^r)
@@ -725,7 +763,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
             z[4 * i] = __float_as_uint(f0); z[4 * i + 1] = __float_as_uint(f1); z[4 * i + 2] = __float_as_uint(f2); z[4 * i + 3] = __float_as_uint(f3);
           }
           if (masked) {
-            const bool mine = (vm >> lane) & 1u, drafted = tok >= s.base;
+            const bool drafted = tok >= s.base;
             const int m = drafted ? tok - s.base : 0, at = drafted ? s.base + (mine ? s_depth[m] : 0) : tok;
             const bool inside = a.window == 0 || at < a.sinks;
 #pragma unroll
@@ -865,10 +903,11 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
       }
     }
   }
+  else if constexpr (SH::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");   // (two warps without a role complete the group of four)
   __syncwarp();
   fence_before();
   __syncthreads();
-  if (warp == SW + 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  if (warp == SH::MMA_AT) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
 }
 
 // ---- the parts of a tile that several CTAs share: out = (sum_i o_i w_i) / (sum_i l_i w_i), w_i = 2^(r_i - max r) ----
@@ -947,6 +986,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const __grid
 // Columns of a tile: as many as the widest tree has rows of a cache head, up to 64.
 int columns(int64_t T, int64_t gqa) { return T * gqa <= 16 ? 16 : (T * gqa <= 32 ? 32 : 64); }
 
+// [pages, heads, page, cols] as boxes of `piece` tokens; axes that repeat one entry as one entry at coordinate 0.
+template <int BITS, int D> bool pool_map(CUtensorMap* m, const KvPagesAttnArgs& a, int side, int piece, int* mul) {
+  const EncodeFn enc = get_encode();
+  constexpr int ROWB = D * BITS / 8, COLS = BITS == 16 ? D : ROWB / 4, BOX = BITS == 16 ? 64 : COLS;
+  const cuuint64_t page = (cuuint64_t)1 << a.page_shift;
+  cuuint64_t dims[4] = {(cuuint64_t)COLS, page, 1, 1}, strides[3] = {(cuuint64_t)a.tok_bytes[side], (cuuint64_t)ROWB, (cuuint64_t)ROWB};
+  const int64_t shape[2] = {a.Hkv, a.P}, str[2] = {a.q_head[side], (int64_t)a.page_bytes[side]};
+  for (int d = 0; d < 2; ++d) {
+    mul[d] = shape[d] > 1 && str[d] > 0 ? 1 : 0;
+    if (mul[d]) { dims[2 + d] = (cuuint64_t)shape[d]; strides[1 + d] = (cuuint64_t)str[d]; }
+  }
+  const cuuint32_t box[4] = {(cuuint32_t)BOX, (cuuint32_t)piece, 1, 1}, es[4] = {1, 1, 1, 1};
+  constexpr CUtensorMapSwizzle swizzle = BITS == 16 || ROWB == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : (ROWB == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
+  return enc && enc(m, BITS == 16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, (void*)a.pool[side].q, dims, strides, box, es,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int BITS, int D, int N> cudaError_t launch_n(const KvPagesTreeArgs& t, cudaStream_t st) {
   auto kern = tree_kernel<BITS, D, N>;
   static bool done[64] = {};
@@ -962,8 +1018,12 @@ template <int BITS, int D, int N> cudaError_t launch_n(const KvPagesTreeArgs& t,
       if (dev >= 0 && dev < 64) done[dev] = true;
     }
   }
+  CUtensorMap mk, mv;
+  TreeMaps maps;
+  maps.piece = t.a.page_shift >= 7 ? kBlk : 1 << t.a.page_shift;
+  if (!pool_map<BITS, D>(&mk, t.a, 0, maps.piece, maps.mul[0]) || !pool_map<BITS, D>(&mv, t.a, 1, maps.piece, maps.mul[1])) return cudaErrorInvalidValue;
   const unsigned grid = (unsigned)sm_count();
-  e = launch_behind(kern, dim3(grid), dim3(Shape<BITS, D, N>::THREADS), smem, st, t);
+  e = launch_behind(kern, dim3(grid), dim3(Shape<BITS, D, N>::THREADS), smem, st, mk, mv, t, maps);
   if (e != cudaSuccess) return e;
   return launch_behind(tree_join_kernel<BITS, D>, dim3(grid, (N + kJoinRows - 1) / kJoinRows), dim3(kJoinWarps * 32), 0, st, t, N);
 }
