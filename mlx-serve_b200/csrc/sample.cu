@@ -68,6 +68,34 @@ __device__ __forceinline__ uint32_t add32(void* p, uint32_t rank, uint32_t v) {
   return r;
 }
 
+// 2^(i / 32)
+__constant__ double kRoots[32] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
+// round(2^44 * 2^(d * c / 32)) for d <= 0, c > 0: d c = 32 n + i + f with |f| <= 1/2 (the nearest whole number by adding 1.5 * 2^52), 2^(f / 32)
+// as its series to f^5 (the next term is below 2.3e-15), 2^(i / 32) from a table, 2^n into the exponent, the whole number out of the low bits of a
+// sum with 2^52.  0 where the exponent is below -46.
+__device__ __forceinline__ uint64_t weight64(double d, double c, const double* roots) {
+  const double t = d * c;
+  if (!(t > -46.0 * 32.0)) return 0;
+  const double shifted = t + 6755399441055744.0, f = t - (shifted - 6755399441055744.0);
+  const int n = __double2loint(shifted);
+  double y = fma(f, 3.973709984549416e-11, 9.172562701824643e-09);
+  y = fma(y, f, 1.693850972437182e-06);
+  y = fma(y, f, 0.0002345961982022468);
+  y = fma(y, f, 0.02166084939249829);
+  const double root = roots[n & 31];
+  y = fma(y * f, root, root);
+  const double w = __hiloint2double(__double2hiint(y) + (((n >> 5) + 44) << 20), __double2loint(y));
+  return (uint64_t)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
+}
+
 // What stays: everything in front of (key, index) in the order, and that itself.
 struct Border { uint32_t key; int index; };
 
@@ -76,6 +104,7 @@ struct alignas(16) Shared {
   uint64_t red[kWarps];
   double red_d[kWarps];
   double part[kMaxCtas];                       // of the sum for the log-probability
+  double roots[32];
   uint64_t above, whole;
   union {                                      // (never of use at the same time)
     uint64_t list[kList];                      // pattern, then V - 1 - index: larger ones come first in the order
@@ -163,6 +192,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     }
   }
   if (tid == 0) sh.listed = 0;
+  if (tid < 32) sh.roots[tid] = kRoots[tid];
   for (int i = tid; i < kBins; i += kThreads) sh.hist[i] = 0;
 
   int turn = 0;
@@ -199,11 +229,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     top = value_of(key);
   }
   const bool greedy = !(temp > 0.f), nothing = top == -INFINITY;
-  const double per_t = 1.0 / (double)temp;
-  auto weigh = [&](float x) -> uint64_t {
+  const double per_t = 1.0 / (double)temp, c64 = 32.0 * 1.4426950408889634 * per_t, top64 = top;
+  auto weigh = [&](float x) -> uint64_t {        // (of an infinite temperature: all alike)
     if (x == top) return (uint64_t)kOne;
     if (x == -INFINITY || top == INFINITY) return 0;
-    return (uint64_t)__double2ll_rn(exp(((double)x - (double)top) * per_t) * kOne);
+    return weight64((double)x - top64, c64, sh.roots);
   };
   auto enough = [&](float x) { return !(least > 0.f) || x == top || exp(((double)x - (double)top) * per_t) >= (double)least; };
 
@@ -276,6 +306,115 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       }
       const uint32_t hit = __ballot_sync(0xffffffffu, at >= 0);
       at = hit ? __shfl_sync(0xffffffffu, at, __ffs(hit) - 1) : V - 1;
+      if (lane < (int)C) put32(&sh.answer[0], (uint32_t)lane, (uint32_t)at);
+    }
+    cluster_sync_all();
+    return sh.answer[0];
+  };
+  // The token among those of which `stay(x, i)` says so, by weights in fp32 from the approximate exponential (relative error 2^-22), whose argument is
+  // carried in two parts: eight of them are added in fp32 (three roundings of 2^-24), the rest in 64 bits, so that every sum is within
+  // 2^-20 of itself.  -1 where the place to find lies within that of an element's border (or a weight that near min_p): then the whole numbers decide.
+  auto find_fast = [&](auto stay) -> int {
+    const double c = 1.4426950408889634 * per_t;
+    const float ch = (float)c, cl = (float)(c - (double)ch), floor_d = fmaxf(-200.f / ch, -1e30f);
+    const uint64_t ch2 = two(ch, ch), cl2 = two(cl, cl), top2 = two(-top, -top), ln2 = two(0.6931471805599453f, 0.6931471805599453f), minus = two(-1.f, -1.f);
+    auto weights = [&](const float (&f)[8], int v, float (&w)[8]) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float d0, d1, y0, y1;
+        untwo(add2(two(f[2 * q], f[2 * q + 1]), top2), d0, d1);
+        const uint64_t d = two(fmaxf(d0, floor_d), fmaxf(d1, floor_d)), y = mul2(d, ch2);
+        const uint64_t rest = fma2(d, cl2, fma2(d, ch2, mul2(y, minus)));
+        untwo(y, y0, y1);
+        const uint64_t e = two(ex2(y0), ex2(y1));
+        untwo(fma2(e, mul2(rest, ln2), e), w[2 * q], w[2 * q + 1]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (least > 0.f) {
+          const float off = w[e] - least;
+          if (fabsf(off) <= least * 1.9073486328125e-6f && f[e] != top) w[e] = __uint_as_float(0x7fc00000u);    // 2^-19
+          else if (off < 0.f && f[e] != top) w[e] = 0.f;
+        }
+        if (!stay(f[e], r.index(v, e))) w[e] = 0.f;
+      }
+    };
+    const int strips = (r.vecs + kThreads - 1) / kThreads;
+    double* const sums = (double*)sh.sums;
+    double mine = 0.0;
+    for (int s = 0; s < strips; ++s) {
+      const int v = s * kThreads + tid;
+      double t = 0.0;
+      if (v < r.vecs) {
+        float f[8], w[8];
+        r.load8(v, f);
+        weights(f, v, w);
+        t = (double)(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+      }
+      t = warp_sum(t);
+      if (lane == 0) sums[s * kWarps + warp] = t;
+      mine += t;
+    }
+    __syncthreads();
+    if (lane == 0) sh.red_d[warp] = mine;
+    __syncthreads();
+    mine = warp_sum(lane < kWarps ? sh.red_d[lane] : 0.0);
+    const uint64_t* const g = gather((uint64_t)__double_as_longlong(mine));
+    double all = 0.0;
+    for (uint32_t c1 = 0; c1 < C; ++c1) all += __longlong_as_double((long long)g[c1]);
+    const double slack = all * 9.5367431640625e-7;           // 2^-20
+    double t = u > 0.f ? (u < 1.f ? (double)u * all : all) : 0.0;
+    uint32_t who = 0;
+    double before = 0.0;
+    for (; who + 1 < C; ++who) {
+      const double n = __longlong_as_double((long long)g[who]);
+      if (t < before + n) break;
+      before += n;
+    }
+    if (who == me && warp == 0) {
+      int q = 0;
+      bool found = false;
+      for (int q0 = 0; q0 < strips * kWarps && !found; q0 += 32) {
+        const double x = q0 + lane < strips * kWarps ? sums[q0 + lane] : 0.0;
+        double upto = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double n = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += n;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, before + upto > t);
+        if (hit) {
+          const int l = __ffs(hit) - 1;
+          q = q0 + l;
+          before += __shfl_sync(0xffffffffu, upto - x, l);
+          found = true;
+        } else before += __shfl_sync(0xffffffffu, upto, 31);
+      }
+      const int v = q / kWarps * kThreads + q % kWarps * 32 + lane;
+      float f[8], w[8];
+      if (found && v < r.vecs) { r.load8(v, f); weights(f, v, w); }
+      else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = 0.f;
+      }
+      double s = 0.0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += (double)w[e];
+      double upto = s;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double n = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += n;
+      }
+      double run = before + upto - s;
+      int at = -1;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {              // (the first element of the row begins at 0 exactly, the last one ends at the whole)
+        if (at < 0 && run + slack < t && t < run + (double)w[e] - slack) at = r.index(v, e);
+        run += (double)w[e];
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, at >= 0);
+      at = hit ? __shfl_sync(0xffffffffu, at, __ffs(hit) - 1) : -1;
       if (lane < (int)C) put32(&sh.answer[0], (uint32_t)lane, (uint32_t)at);
     }
     cluster_sync_all();
@@ -395,12 +534,15 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       auto in_list = [&](auto amount, uint64_t target) {
         if (me == 0) {
           const int n = (int)min(sh.listed, (uint32_t)kList);
+          uint64_t* const weight = (uint64_t*)sh.hist;       // (the histogram has been added up)
+          static_assert(kList * 8 <= sizeof(sh.hist), "weights");
+          for (int i = tid; i < n; i += kThreads) weight[i] = amount(value_of((uint32_t)(sh.list[i] >> 32)));
+          __syncthreads();
           for (int i = tid; i < n; i += kThreads) {
-            const uint64_t x = sh.list[i];
+            const uint64_t x = sh.list[i], w = weight[i];
             uint64_t sum = 0;
-            for (int j = 0; j < n; ++j)
-              if (sh.list[j] > x) sum += amount(value_of((uint32_t)(sh.list[j] >> 32)));
-            const uint64_t w = amount(value_of((uint32_t)(x >> 32)));
+#pragma unroll 4
+            for (int j = 0; j < n; ++j) sum += sh.list[j] > x ? weight[j] : 0ull;
             if (sum < target && target <= sum + w)
               for (uint32_t c = 0; c < C; ++c) { put32(&sh.answer[2], c, (uint32_t)(x >> 32)); put32(&sh.answer[3], c, (uint32_t)(V - 1 - (int)(uint32_t)x)); }
           }
@@ -416,7 +558,6 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
           const int n = list_n;
           // ranks and sums in the order; the weights in place of the histogram
           uint64_t* const weight = (uint64_t*)sh.hist;
-          static_assert(kList * 8 <= sizeof(sh.hist), "weights");
           for (int i = tid; i < n; i += kThreads) weight[i] = weigh(value_of((uint32_t)(sh.list[i] >> 32)));
           __syncthreads();
           uint64_t sum_k = 0;                                // of the first k
@@ -546,6 +687,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
         }
       }
     }
+    // (at temperatures like these -200 / c, which stands in for all that lies further down, weighs 0 and is itself exact enough)
+    if (token < 0 && top < INFINITY && temp >= 1e-6f && temp <= 1e6f) token = find_fast([&](float x, int i) { return !(by_k || by_p) || stays(b, x, i); });
     if (token < 0) {
       uint64_t Z;
       token = find([&](float x, int i) { return stays(b, x, i) && enough(x) ? weigh(x) : 0ull; },
