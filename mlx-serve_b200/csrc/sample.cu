@@ -103,48 +103,72 @@ struct alignas(16) Shared {
   uint64_t gather[2][kMaxCtas];                // a value of every block; two, taken in turn
   uint64_t red[kWarps];
   double red_d[kWarps];
-  double part[kMaxCtas];                       // of the sum for the log-probability
+  double part[kMaxCtas], part_top[kMaxCtas];   // of the sum for the log-probability: a block's sum and its largest
+  double once_sum[kMaxCtas];
   double roots[32];
   uint64_t above, whole;
   union {                                      // (never of use at the same time)
     uint64_t list[kList];                      // pattern, then V - 1 - index: larger ones come first in the order
     uint64_t sums[kMaxStrips * kWarps];        // of every warp's part of every strip
   };
-  uint32_t hist[kBins], merged[kBins];
+  uint32_t hist[kBins];
+  union {
+    uint32_t merged[kBins];
+    float refs[kMaxStrips * kWarps];           // of the parts: what their sums are relative to
+  };
   uint32_t scan[kWarps];
   uint32_t listed;
   int answer[4];
 };
 
-static_assert(sizeof(Shared) % 16 == 0 && offsetof(Shared, hist) % 8 == 0, "vectors behind it, weights in it");
+static_assert(sizeof(Shared) % 16 == 0, "vectors behind it");
 
 template <typename T> struct Row {
+  static constexpr int W = (int)sizeof(T) / 2;   // 16-byte vectors of eight elements
   const T* x;                  // this block's share
-  const unsigned char* held;   // the same in shared memory, element e of it at place e + off; null: read from memory
+  const unsigned char* held;   // the same in shared memory, cleaned, element e of it at place e + off; null: read from memory
   int begin, n, off, vecs;
+  struct Raw { uint4 w[W]; };
   // eight elements from place 8 v on; -inf where the row has none
-  __device__ __forceinline__ void load8(int v, float (&f)[8]) const {
-    if (held) {
-      if constexpr (sizeof(T) == 4) {
-        const float4 a = *(const float4*)(held + v * 32), b = *(const float4*)(held + v * 32 + 16);
-        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-      } else {
-        const uint4 a = *(const uint4*)(held + v * 16);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+  __device__ __forceinline__ Raw load_raw(int v) const {
+    const int i0 = 8 * v - off;
+    Raw r;
+    if (i0 >= 0 && i0 + 8 <= n) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if constexpr (std::is_same<T, __half>::value) {
-            const float2 h = __half22float2(*(const __half2*)&w[k]);
-            f[2 * k] = h.x; f[2 * k + 1] = h.y;
-          } else { f[2 * k] = bf16lo(w[k]); f[2 * k + 1] = bf16hi(w[k]); }
-        }
-      }
+      for (int q = 0; q < W; ++q) r.w[q] = ((const uint4*)(x + i0))[q];
     } else {
+      alignas(16) T e8[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int i = 8 * v + e - off;
-        f[e] = i >= 0 && i < n ? clean(IO<T>::load(x, i)) : -INFINITY;
+      for (int e = 0; e < 8; ++e) e8[e] = i0 + e >= 0 && i0 + e < n ? x[i0 + e] : (T)(-INFINITY);
+#pragma unroll
+      for (int q = 0; q < W; ++q) r.w[q] = ((const uint4*)e8)[q];
+    }
+    return r;
+  }
+  __device__ __forceinline__ static void unpack(const Raw& r, float (&f)[8]) {
+#pragma unroll
+    for (int q = 0; q < W; ++q) {
+      const uint32_t w[4] = {r.w[q].x, r.w[q].y, r.w[q].z, r.w[q].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 4) f[4 * q + k] = __uint_as_float(w[k]);
+        else if constexpr (std::is_same<T, __half>::value) {
+          const float2 h = __half22float2(*(const __half2*)&w[k]);
+          f[2 * k] = h.x; f[2 * k + 1] = h.y;
+        } else { f[2 * k] = bf16lo(w[k]); f[2 * k + 1] = bf16hi(w[k]); }
       }
+    }
+  }
+  __device__ __forceinline__ void load8(int v, float (&f)[8]) const {
+    Raw r;
+    if (held) {
+#pragma unroll
+      for (int q = 0; q < W; ++q) r.w[q] = *(const uint4*)(held + v * (16 * W) + 16 * q);
+      unpack(r, f);
+    } else {
+      unpack(load_raw(v), f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = clean(f[e]);
     }
   }
   __device__ __forceinline__ int index(int v, int e) const { return begin + 8 * v + e - off; }
@@ -155,6 +179,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *(Shared*)raw;
   const uint32_t C = cluster_size(), me = cluster_rank();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int row_no = (int)(blockIdx.x / C), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
   const float temp = a.temperature ? a.temperature[row_no * a.str[1]] : 1.f, u = a.random[row_no * a.str[0]];
   const int k = a.top_k ? a.top_k[row_no * a.str[2]] : 0;
@@ -168,33 +193,13 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   r.off = (int)((uintptr_t)r.x & (8 * sizeof(T) - 1)) / (int)sizeof(T);
   r.vecs = (r.n + r.off + 7) / 8;
   unsigned char* const held = raw + sizeof(Shared);
-  r.held = r.vecs * 8 * (int)sizeof(T) <= held_bytes ? held : nullptr;
-  float mx = -INFINITY;
-  for (int v = tid; v < r.vecs; v += kThreads) {
-    const int i0 = 8 * v - r.off;
-    alignas(16) T raw8[8];
-    if (i0 >= 0 && i0 + 8 <= r.n) {
-#pragma unroll
-      for (int q = 0; q < (int)sizeof(T) / 2; ++q) ((uint4*)raw8)[q] = ((const uint4*)(r.x + i0))[q];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) raw8[e] = i0 + e >= 0 && i0 + e < r.n ? r.x[i0 + e] : (T)(-INFINITY);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float f = clean((float)raw8[e]);
-      mx = fmaxf(mx, f);
-      raw8[e] = (T)f;
-    }
-    if (r.held) {
-#pragma unroll
-      for (int q = 0; q < (int)sizeof(T) / 2; ++q) *(uint4*)(held + v * 8 * sizeof(T) + 16 * q) = ((const uint4*)raw8)[q];
-    }
-  }
+  const bool greedy = !(temp > 0.f), by_k = k > 0 && k < V, by_p = p < 1.f;
+  // by temperature alone the row is read once, each warp's 256 elements at a time with a largest of their own
+  const bool once = !greedy && !by_k && !by_p && !(least > 0.f) && temp >= 1e-6f && temp <= 1e6f;
   if (tid == 0) sh.listed = 0;
   if (tid < 32) sh.roots[tid] = kRoots[tid];
-  for (int i = tid; i < kBins; i += kThreads) sh.hist[i] = 0;
-
+  if (by_k || by_p)
+    for (int i = tid; i < kBins; i += kThreads) sh.hist[i] = 0;
   int turn = 0;
   // a value of every block, in all blocks
   auto gather = [&](uint64_t mine) {
@@ -217,19 +222,227 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     for (uint32_t c = 0; c < C; ++c) s += g[c];
     return s;
   };
-  float top;
-  {
-    const uint32_t w = __reduce_max_sync(0xffffffffu, pattern(mx));
-    if (lane == 0) sh.red[warp] = w;
+  constexpr int kAhead = 4;                      // loads of a thread in flight
+  constexpr float kLog2e = 1.4426950408889634f;
+  const double per_t = 1.0 / (double)temp, c64 = 32.0 * 1.4426950408889634 * per_t, c_all = 1.4426950408889634 * per_t;
+  const float ch = (float)c_all, cl = (float)(c_all - (double)ch);
+  const int strips = (r.vecs + kThreads - 1) / kThreads;
+  // Weights in fp32, relative to `largest`, from the approximate exponential (relative error 2^-22), whose argument is carried in two parts and
+  // whose product with the rest rounds twice (2^-23).
+  auto weights32 = [&](const float (&f)[8], float largest, float (&w)[8]) {
+    const float floor_d = -200.f / ch;           // (what lies further down weighs 0, as this does)
+    const uint64_t ch2 = two(ch, ch), cl2 = two(cl, cl), top2 = two(-largest, -largest), ln2 = two(0.6931471805599453f, 0.6931471805599453f), minus = two(-1.f, -1.f);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float d0, d1, y0, y1;
+      untwo(add2(two(f[2 * q], f[2 * q + 1]), top2), d0, d1);
+      const uint64_t d = two(fmaxf(d0, floor_d), fmaxf(d1, floor_d)), y = mul2(d, ch2);
+      const uint64_t rest = fma2(d, cl2, fma2(d, ch2, mul2(y, minus)));
+      untwo(y, y0, y1);
+      const uint64_t e = two(ex2(y0), ex2(y1));
+      untwo(fma2(e, mul2(rest, ln2), e), w[2 * q], w[2 * q + 1]);
+    }
+  };
+  auto add8 = [](const float (&w)[8]) { return ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])); };
+  // How far a sum of such weights and u times their whole may lie from one another's true place: every weight is within e = 2^-20.7 (2^-22, 2^-23,
+  // three roundings of 2^-24 where eight are added) of itself, those before the place count 1 - u times and those behind it u times.
+  auto slack_of = [&](double all) { const double v = u > 0.f ? (u < 1.f ? (double)u : 1.0) : 0.0; return all * (2.0 * v * (1.0 - v) * 5.9e-7 + 1e-11); };
+  double lp_sum = 0.0;                           // of exp(x - this block's largest), for the log-probability
+  float top, mine_top;
+  int token = -1;
+  double* const sums_d = (double*)sh.sums;
+  // The element of a warp's part q of a strip at which the sum passes t (all given relative to `largest` of that part), by a warp; -1: too near a border.
+  auto within = [&](int q, double before, double t, double slack, auto weights) -> int {
+    const int v = q / kWarps * kThreads + q % kWarps * 32 + lane;
+    float w[8];
+    if (v < r.vecs) weights(v, w);
+    else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = 0.f;
+    }
+    double s = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += (double)w[e];
+    double upto = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double n = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += n;
+    }
+    double run = before + upto - s;
+    int at = -1;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (at < 0 && run + slack < t && t < run + (double)w[e] - slack) at = r.index(v, e);
+      run += (double)w[e];
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, at >= 0);
+    return hit ? __shfl_sync(0xffffffffu, at, __ffs(hit) - 1) : -1;
+  };
+  // The part at which the running sum of sums_d passes t, by a warp; *before = the sum before it; -1: none.
+  auto part_of = [&](double t, double* before) -> int {
+    double b = *before;
+    for (int q0 = 0; q0 < strips * kWarps; q0 += 32) {
+      const double x = q0 + lane < strips * kWarps ? sums_d[q0 + lane] : 0.0;
+      double upto = x;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double n = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += n;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, b + upto > t);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        *before = b + __shfl_sync(0xffffffffu, upto - x, l);
+        return q0 + l;
+      }
+      b += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return -1;
+  };
+  auto block_sum_d = [&](double v) {
+    v = warp_sum(v);
     __syncthreads();
-    const uint32_t b = __reduce_max_sync(0xffffffffu, lane < kWarps ? (uint32_t)sh.red[lane] : 0u);
-    const uint64_t* const g = gather(b);
-    uint32_t key = 0;
-    for (uint32_t c = 0; c < C; ++c) key = max(key, (uint32_t)g[c]);
-    top = value_of(key);
+    if (lane == 0) sh.red_d[warp] = v;
+    __syncthreads();
+    return warp_sum(lane < kWarps ? sh.red_d[lane] : 0.0);
+  };
+  {
+    // ---- the row's largest; where the row is read once, sums of the weights too ----
+    r.held = nullptr;
+    const bool hold = !greedy && !once && r.vecs * 8 * (int)sizeof(T) <= held_bytes;
+    uint64_t best = 0;                           // pattern, V - 1 - index
+    for (int v0 = tid; v0 < strips * kThreads; v0 += kAhead * kThreads) {   // (by whole warps)
+      typename Row<T>::Raw got[kAhead];
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q)
+        if (v0 + q * kThreads < r.vecs) got[q] = r.load_raw(v0 + q * kThreads);
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) {
+        const int v = v0 + q * kThreads;
+        if (v - lane >= r.vecs) continue;
+        float f[8];
+        if (v < r.vecs) {
+          Row<T>::unpack(got[q], f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = clean(f[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = -INFINITY;
+        }
+        float mx = f[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) mx = fmaxf(mx, f[e]);
+        if (hold && v < r.vecs) {
+          alignas(16) T e8[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) e8[e] = (T)f[e];
+#pragma unroll
+          for (int x = 0; x < Row<T>::W; ++x) *(uint4*)(held + v * (16 * Row<T>::W) + 16 * x) = ((const uint4*)e8)[x];
+        }
+        if (once) {
+          const uint32_t key = __reduce_max_sync(0xffffffffu, pattern(mx));
+          const float largest = value_of(key);
+          double t = 0.0;
+          if (largest > -INFINITY && largest < INFINITY) {
+            float w[8];
+            weights32(f, largest, w);
+            t = warp_sum((double)add8(w));
+          }
+          const int part = v / kThreads * kWarps + warp;
+          if (lane == 0) { sums_d[part] = t; sh.refs[part] = largest; }
+          best = max(best, (uint64_t)key << 32);
+        } else {
+          int at = 0;
+#pragma unroll
+          for (int e = 7; e >= 0; --e) at = f[e] == mx ? e : at;
+          const int index = r.index(v, at);
+          best = max(best, (uint64_t)pattern(mx) << 32 | (uint32_t)(index >= 0 && index < V ? V - 1 - index : 0));
+        }
+      }
+    }
+    if (hold) r.held = held;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(0xffffffffu, best, o));
+    __syncthreads();
+    if (lane == 0) sh.red[warp] = best;
+    __syncthreads();
+    best = lane < kWarps ? sh.red[lane] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(0xffffffffu, best, o));
+    mine_top = r.vecs > 0 ? value_of((uint32_t)(best >> 32)) : -INFINITY;
+    double mine = 0.0;
+    if (once) {
+      // parts relative to the block's largest (both below infinity, else the row is not decided here)
+      for (int q = tid; q < strips * kWarps; q += kThreads) {
+        const int v = q / kWarps * kThreads + q % kWarps * 32;
+        const float ref = v < r.vecs ? sh.refs[q] : -INFINITY;
+        const double w = ref > -INFINITY && mine_top < INFINITY ? sums_d[q] * exp2(((double)ref - (double)mine_top) * c_all) : 0.0;
+        sums_d[q] = w;
+        mine += w;
+      }
+      mine = block_sum_d(mine);
+    }
+    if (a.logprobs) {
+      // (the row is in shared memory, or has just been read)
+      for (int v = tid; v < r.vecs; v += kThreads) {
+        float f[8], t = 0.f;
+        r.load8(v, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t += f[e] == mine_top ? 1.f : ex2((f[e] - mine_top) * kLog2e);
+        lp_sum += (double)t;
+      }
+      lp_sum = block_sum_d(lp_sum);
+      if (tid == 0) put64((uint64_t*)&sh.part[me], 0, (uint64_t)__double_as_longlong(lp_sum));
+      if (tid == 32) put64((uint64_t*)&sh.part_top[me], 0, (uint64_t)__double_as_longlong((double)mine_top));
+    }
+    if (once && tid < (int)C) put64((uint64_t*)&sh.once_sum[me], (uint32_t)tid, (uint64_t)__double_as_longlong(mine));
+    const uint64_t* const g = gather(best);
+    for (uint32_t c = 0; c < C; ++c) best = max(best, g[c]);
+    top = value_of((uint32_t)(best >> 32));
+    if (greedy && top > -INFINITY) token = V - 1 - (int)(uint32_t)best;
+    if (once && top > -INFINITY && top < INFINITY) {
+      double all = 0.0, part[kMaxCtas];
+#pragma unroll
+      for (uint32_t c = 0; c < kMaxCtas; ++c) {
+        part[c] = 0.0;
+        if (c < C) {
+          const float ref = value_of((uint32_t)(g[c] >> 32));
+          part[c] = g[c] && ref > -INFINITY ? sh.once_sum[c] * exp2(((double)ref - (double)top) * c_all) : 0.0;
+          all += part[c];
+        }
+      }
+      const double slack = slack_of(all), t = u > 0.f ? (u < 1.f ? (double)u * all : all) : 0.0;
+      uint32_t who = C;
+      double before = 0.0, run = 0.0;
+#pragma unroll
+      for (uint32_t c = 0; c < kMaxCtas; ++c) {
+        if (c < C && who == C && t < run + part[c]) { who = c; before = run; }
+        run += part[c];
+      }
+      if (who == C) who = C - 1;
+      if (who == me && warp == 0) {
+        // everything relative to this block's largest
+        const double up = exp2(((double)top - (double)mine_top) * c_all);
+        double b = before * up;
+        const int q = mine_top > -INFINITY ? part_of(t * up, &b) : -1;
+        int at = -1;
+        if (q >= 0) {
+          const double there = exp2(((double)mine_top - (double)sh.refs[q]) * c_all);
+          at = within(q, b * there, t * up * there, slack * up * there, [&](int v, float (&w)[8]) {
+            float f[8];
+            r.load8(v, f);
+            weights32(f, sh.refs[q], w);
+          });
+        }
+        if (lane < (int)C) put32(&sh.answer[0], (uint32_t)lane, (uint32_t)at);
+      }
+      cluster_sync_all();
+      token = sh.answer[0];
+    }
   }
-  const bool greedy = !(temp > 0.f), nothing = top == -INFINITY;
-  const double per_t = 1.0 / (double)temp, c64 = 32.0 * 1.4426950408889634 * per_t, top64 = top;
+  const bool nothing = top == -INFINITY;
+  const double top64 = top;
   auto weigh = [&](float x) -> uint64_t {        // (of an infinite temperature: all alike)
     if (x == top) return (uint64_t)kOne;
     if (x == -INFINITY || top == INFINITY) return 0;
@@ -239,7 +452,6 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
 
   // The first index at which the sum of `amount` passes `target(whole sum)`, all blocks' answer; *whole = the sum.
   auto find = [&](auto amount, auto target, uint64_t* whole) -> int {
-    const int strips = (r.vecs + kThreads - 1) / kThreads;
     uint64_t mine = 0;
     for (int s = 0; s < strips; ++s) {
       const int v = s * kThreads + tid;
@@ -311,24 +523,13 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     cluster_sync_all();
     return sh.answer[0];
   };
-  // The token among those of which `stay(x, i)` says so, by weights in fp32 from the approximate exponential (relative error 2^-22), whose argument is
-  // carried in two parts: eight of them are added in fp32 (three roundings of 2^-24), the rest in 64 bits, so that every sum is within
-  // 2^-20 of itself.  -1 where the place to find lies within that of an element's border (or a weight that near min_p): then the whole numbers decide.
+  // The token among those of which `stay(x, i)` says so, by weights in fp32.  -1 where the place to find lies too near an element's border (or a weight
+  // too near min_p): then the whole numbers decide.
   auto find_fast = [&](auto stay) -> int {
-    const double c = 1.4426950408889634 * per_t;
-    const float ch = (float)c, cl = (float)(c - (double)ch), floor_d = fmaxf(-200.f / ch, -1e30f);
-    const uint64_t ch2 = two(ch, ch), cl2 = two(cl, cl), top2 = two(-top, -top), ln2 = two(0.6931471805599453f, 0.6931471805599453f), minus = two(-1.f, -1.f);
-    auto weights = [&](const float (&f)[8], int v, float (&w)[8]) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float d0, d1, y0, y1;
-        untwo(add2(two(f[2 * q], f[2 * q + 1]), top2), d0, d1);
-        const uint64_t d = two(fmaxf(d0, floor_d), fmaxf(d1, floor_d)), y = mul2(d, ch2);
-        const uint64_t rest = fma2(d, cl2, fma2(d, ch2, mul2(y, minus)));
-        untwo(y, y0, y1);
-        const uint64_t e = two(ex2(y0), ex2(y1));
-        untwo(fma2(e, mul2(rest, ln2), e), w[2 * q], w[2 * q + 1]);
-      }
+    auto weights = [&](int v, float (&w)[8]) {
+      float f[8];
+      r.load8(v, f);
+      weights32(f, top, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if (least > 0.f) {
@@ -339,20 +540,17 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
         if (!stay(f[e], r.index(v, e))) w[e] = 0.f;
       }
     };
-    const int strips = (r.vecs + kThreads - 1) / kThreads;
-    double* const sums = (double*)sh.sums;
     double mine = 0.0;
     for (int s = 0; s < strips; ++s) {
       const int v = s * kThreads + tid;
       double t = 0.0;
       if (v < r.vecs) {
-        float f[8], w[8];
-        r.load8(v, f);
-        weights(f, v, w);
-        t = (double)(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+        float w[8];
+        weights(v, w);
+        t = (double)add8(w);
       }
       t = warp_sum(t);
-      if (lane == 0) sums[s * kWarps + warp] = t;
+      if (lane == 0) sums_d[s * kWarps + warp] = t;
       mine += t;
     }
     __syncthreads();
@@ -361,9 +559,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     mine = warp_sum(lane < kWarps ? sh.red_d[lane] : 0.0);
     const uint64_t* const g = gather((uint64_t)__double_as_longlong(mine));
     double all = 0.0;
-    for (uint32_t c1 = 0; c1 < C; ++c1) all += __longlong_as_double((long long)g[c1]);
-    const double slack = all * 9.5367431640625e-7;           // 2^-20
-    double t = u > 0.f ? (u < 1.f ? (double)u * all : all) : 0.0;
+    for (uint32_t c = 0; c < C; ++c) all += __longlong_as_double((long long)g[c]);
+    const double t = u > 0.f ? (u < 1.f ? (double)u * all : all) : 0.0;
     uint32_t who = 0;
     double before = 0.0;
     for (; who + 1 < C; ++who) {
@@ -372,49 +569,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       before += n;
     }
     if (who == me && warp == 0) {
-      int q = 0;
-      bool found = false;
-      for (int q0 = 0; q0 < strips * kWarps && !found; q0 += 32) {
-        const double x = q0 + lane < strips * kWarps ? sums[q0 + lane] : 0.0;
-        double upto = x;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double n = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += n;
-        }
-        const uint32_t hit = __ballot_sync(0xffffffffu, before + upto > t);
-        if (hit) {
-          const int l = __ffs(hit) - 1;
-          q = q0 + l;
-          before += __shfl_sync(0xffffffffu, upto - x, l);
-          found = true;
-        } else before += __shfl_sync(0xffffffffu, upto, 31);
-      }
-      const int v = q / kWarps * kThreads + q % kWarps * 32 + lane;
-      float f[8], w[8];
-      if (found && v < r.vecs) { r.load8(v, f); weights(f, v, w); }
-      else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = 0.f;
-      }
-      double s = 0.0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s += (double)w[e];
-      double upto = s;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double n = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += n;
-      }
-      double run = before + upto - s;
-      int at = -1;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {              // (the first element of the row begins at 0 exactly, the last one ends at the whole)
-        if (at < 0 && run + slack < t && t < run + (double)w[e] - slack) at = r.index(v, e);
-        run += (double)w[e];
-      }
-      const uint32_t hit = __ballot_sync(0xffffffffu, at >= 0);
-      at = hit ? __shfl_sync(0xffffffffu, at, __ffs(hit) - 1) : -1;
+      const int q = part_of(t, &before);
+      const int at = q >= 0 ? within(q, before, t, slack_of(all), weights) : -1;
       if (lane < (int)C) put32(&sh.answer[0], (uint32_t)lane, (uint32_t)at);
     }
     cluster_sync_all();
@@ -456,13 +612,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     return d < (float)kBins ? (int)d : kBins;
   };
 
-  int token = -1;
-  if (greedy && !nothing) {
-    uint64_t all;
-    token = find([&](float x, int) { return (uint64_t)(x == top); }, [](uint64_t) { return 0ull; }, &all);
-  } else if (!nothing) {
+  if (!greedy && !nothing && token < 0) {
     Border b = {0u, V - 1};
-    const bool by_k = k > 0 && k < V, by_p = p < 1.f;
     if (by_k || by_p) {
       // ---- how many logits in which step ----
       for (int v = tid; v < r.vecs; v += kThreads) {
@@ -530,21 +681,59 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
         }
         cluster_sync_all();
       };
+      // the first n entries of the list in descending order (bitonic; the rest of the power of two that is sorted is 0), by the first block
+      auto sort_list = [&](int n) {
+        int m = 32;
+        while (m < n) m *= 2;
+        for (int i = n + tid; i < m; i += kThreads) sh.list[i] = 0;
+        for (int span = 2; span <= m; span *= 2)
+          for (int d = span / 2; d > 0; d /= 2) {
+            __syncthreads();
+            for (int i = tid; i < m / 2; i += kThreads) {
+              const int lo = 2 * i - (i & (d - 1)), hi = lo + d;
+              const uint64_t x = sh.list[lo], y = sh.list[hi];
+              if ((x < y) == ((lo & span) == 0)) { sh.list[lo] = y; sh.list[hi] = x; }
+            }
+          }
+        __syncthreads();
+      };
+      constexpr int LPT = kList / kThreads;      // neighbours of a thread
+      // sums before each of a thread's entries, of amounts in order; *all = their sum
+      auto list_sums = [&](const uint64_t (&w)[LPT], uint64_t (&before)[LPT], uint64_t* all) {
+        uint64_t mine = 0;
+#pragma unroll
+        for (int q = 0; q < LPT; ++q) { before[q] = mine; mine += w[q]; }
+        uint64_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += x;
+        }
+        __syncthreads();
+        if (lane == 31) sh.red[warp] = upto;
+        __syncthreads();
+        uint64_t base = upto - mine, sum = 0;
+        for (int x = 0; x < kWarps; ++x) { if (x < warp) base += sh.red[x]; sum += sh.red[x]; }
+#pragma unroll
+        for (int q = 0; q < LPT; ++q) before[q] += base;
+        *all = sum;
+      };
+      auto list_value = [&](int i) { return value_of((uint32_t)(sh.list[i] >> 32)); };
+      auto list_index = [&](int i) { return V - 1 - (int)(uint32_t)sh.list[i]; };
       // the element at which the sum of the list's amounts, in order, reaches `target`; by the first block, told to all
       auto in_list = [&](auto amount, uint64_t target) {
         if (me == 0) {
           const int n = (int)min(sh.listed, (uint32_t)kList);
-          uint64_t* const weight = (uint64_t*)sh.hist;       // (the histogram has been added up)
-          static_assert(kList * 8 <= sizeof(sh.hist), "weights");
-          for (int i = tid; i < n; i += kThreads) weight[i] = amount(value_of((uint32_t)(sh.list[i] >> 32)));
-          __syncthreads();
-          for (int i = tid; i < n; i += kThreads) {
-            const uint64_t x = sh.list[i], w = weight[i];
-            uint64_t sum = 0;
-#pragma unroll 4
-            for (int j = 0; j < n; ++j) sum += sh.list[j] > x ? weight[j] : 0ull;
-            if (sum < target && target <= sum + w)
-              for (uint32_t c = 0; c < C; ++c) { put32(&sh.answer[2], c, (uint32_t)(x >> 32)); put32(&sh.answer[3], c, (uint32_t)(V - 1 - (int)(uint32_t)x)); }
+          sort_list(n);
+          uint64_t w[LPT], before[LPT], all;
+#pragma unroll
+          for (int q = 0; q < LPT; ++q) w[q] = LPT * tid + q < n ? amount(list_value(LPT * tid + q)) : 0;
+          list_sums(w, before, &all);
+#pragma unroll
+          for (int q = 0; q < LPT; ++q) {
+            const int i = LPT * tid + q;
+            if (i < n && before[q] < target && target <= before[q] + w[q])
+              for (uint32_t c = 0; c < C; ++c) { put32(&sh.answer[2], c, (uint32_t)(sh.list[i] >> 32)); put32(&sh.answer[3], c, (uint32_t)list_index(i)); }
           }
           __syncthreads();
           if (tid == 0) sh.listed = 0;
@@ -556,58 +745,45 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
         into_list(0, last_bin, nullptr);
         if (me == 0) {
           const int n = list_n;
-          // ranks and sums in the order; the weights in place of the histogram
-          uint64_t* const weight = (uint64_t*)sh.hist;
-          for (int i = tid; i < n; i += kThreads) weight[i] = weigh(value_of((uint32_t)(sh.list[i] >> 32)));
-          __syncthreads();
-          uint64_t sum_k = 0;                                // of the first k
-          uint64_t before_w[kList / kThreads];
-          bool in_k[kList / kThreads];
+          sort_list(n);
+          uint64_t w[LPT], before[LPT], Z;
 #pragma unroll
-          for (int q = 0; q < kList / kThreads; ++q) {
-            const int i = tid + q * kThreads;
-            before_w[q] = 0; in_k[q] = false;
-            if (i < n) {
-              const uint64_t x = sh.list[i];
-              uint32_t rank = 0;
-              uint64_t sum = 0;
-              for (int j = 0; j < n; ++j)
-                if (sh.list[j] > x) { ++rank; sum += weight[j]; }
-              before_w[q] = sum;
-              in_k[q] = rank < want;
-              if (in_k[q]) sum_k += weight[i];
-            }
-          }
-          const uint64_t Zk = block_sum(sum_k);
+          for (int q = 0; q < LPT; ++q) w[q] = LPT * tid + q < n && (uint32_t)(LPT * tid + q) < want ? weigh(list_value(LPT * tid + q)) : 0;
+          list_sums(w, before, &Z);
           uint64_t target = ~0ull;
           if (by_p) {
-            const double t = ceil((double)p * (double)Zk);
-            target = p > 0.f ? (uint64_t)t : 1ull;
+            target = p > 0.f ? (uint64_t)ceil((double)p * (double)Z) : 1ull;
             target = target < 1 ? 1 : target;
           }
-          uint64_t sum_s = 0;
+          // what stays is a first part of the order: how long, and back by index
+          int stay = 0;
+#pragma unroll
+          for (int q = 0; q < LPT; ++q) {
+            const int i = LPT * tid + q;
+            if (w[q] > 0 && before[q] < target && enough(list_value(i))) stay = i + 1;
+          }
+          stay = __reduce_max_sync(0xffffffffu, stay);
+          __syncthreads();
+          if (lane == 0) sh.red[warp] = (uint64_t)stay;
+          __syncthreads();
+          for (int x = 0; x < kWarps; ++x) stay = max(stay, (int)sh.red[x]);
+          uint64_t turned[LPT];
+#pragma unroll
+          for (int q = 0; q < LPT; ++q) turned[q] = LPT * tid + q < stay ? sh.list[LPT * tid + q] : 0;
           __syncthreads();
 #pragma unroll
-          for (int q = 0; q < kList / kThreads; ++q) {
-            const int i = tid + q * kThreads;
-            if (i >= n) continue;
-            const bool stay = in_k[q] && before_w[q] < target && enough(value_of((uint32_t)(sh.list[i] >> 32)));
-            if (!stay) weight[i] = 0;
-            else sum_s += weight[i];
-          }
-          const uint64_t Z = block_sum(sum_s);
-          __syncthreads();
+          for (int q = 0; q < LPT; ++q)
+            if (LPT * tid + q < stay) sh.list[LPT * tid + q] = turned[q] << 32 | turned[q] >> 32;      // V - 1 - index, pattern
+          sort_list(stay);
+#pragma unroll
+          for (int q = 0; q < LPT; ++q) w[q] = LPT * tid + q < stay ? weigh(value_of((uint32_t)sh.list[LPT * tid + q])) : 0;
+          list_sums(w, before, &Z);
           uint64_t t = u > 0.f ? (u < 1.f ? (uint64_t)((double)u * (double)Z) : Z) : 0;
           t = t < Z ? t : Z - 1;
-          for (int i = tid; i < n; i += kThreads) {
-            if (weight[i] == 0) continue;
-            const uint32_t x = (uint32_t)sh.list[i];         // V - 1 - index
-            uint64_t sum = 0;
-            for (int j = 0; j < n; ++j)
-              if ((uint32_t)sh.list[j] > x) sum += weight[j];
-            if (sum <= t && t < sum + weight[i])
-              for (uint32_t c = 0; c < C; ++c) put32(&sh.answer[0], c, (uint32_t)(V - 1 - (int)x));
-          }
+#pragma unroll
+          for (int q = 0; q < LPT; ++q)
+            if (before[q] <= t && t < before[q] + w[q])
+              for (uint32_t c = 0; c < C; ++c) put32(&sh.answer[0], c, (uint32_t)(V - 1 - (int)(uint32_t)(sh.list[LPT * tid + q] >> 32)));
         }
         cluster_sync_all();
         token = sh.answer[0];
@@ -688,7 +864,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       }
     }
     // (at temperatures like these -200 / c, which stands in for all that lies further down, weighs 0 and is itself exact enough)
-    if (token < 0 && top < INFINITY && temp >= 1e-6f && temp <= 1e6f) token = find_fast([&](float x, int i) { return !(by_k || by_p) || stays(b, x, i); });
+    if (token < 0 && !once && top < INFINITY && temp >= 1e-6f && temp <= 1e6f) token = find_fast([&](float x, int i) { return !(by_k || by_p) || stays(b, x, i); });
     if (token < 0) {
       uint64_t Z;
       token = find([&](float x, int i) { return stays(b, x, i) && enough(x) ? weigh(x) : 0ull; },
@@ -698,32 +874,19 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
                    }, &Z);
     }
   }
-  if (a.logprobs && !nothing) {
-    double s = 0.0;
-    for (int v = tid; v < r.vecs; v += kThreads) {
-      float f[8], t = 0.f;
-      r.load8(v, f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) t += f[e] == top ? 1.f : ex2((f[e] - top) * 1.4426950408889634f);
-      s += (double)t;
-    }
-    s = warp_sum(s);
-    __syncthreads();
-    if (lane == 0) sh.red_d[warp] = s;
-    __syncthreads();
-    if (tid == 0) {
+  if (a.logprobs && me == 0 && tid == 0) {
+    float y = 0.f;
+    if (!nothing) {
       double all = 0.0;
-      for (int w = 0; w < kWarps; ++w) all += sh.red_d[w];
-      put64((uint64_t*)&sh.part[me], 0, (uint64_t)__double_as_longlong(all));
-    }
-    cluster_sync_all();
-    if (me == 0 && tid == 0) {
-      double all = 0.0;
-      for (uint32_t c = 0; c < C; ++c) all += sh.part[c];
+      for (uint32_t c = 0; c < C; ++c) {
+        const double ref = sh.part_top[c];
+        if (ref > -INFINITY) all += ref == top64 ? sh.part[c] : sh.part[c] * exp(ref - top64);
+      }
       const float x = clean(IO<T>::load((const char*)a.logits + (int64_t)row_no * a.row_bytes, token));
-      a.logprobs[row_no] = (float)((x == top ? 0.0 : (double)x - (double)top) - log(all));
+      y = (float)((x == top ? 0.0 : (double)x - top64) - log(all));
     }
-  } else if (a.logprobs && me == 0 && tid == 0) a.logprobs[row_no] = 0.f;
+    a.logprobs[row_no] = y;
+  }
   if (me == 0 && tid == 0) a.tokens[row_no] = token;
   cluster_sync_all();                            // (shared memory stays until all have read it)
 }
@@ -754,12 +917,14 @@ template <typename T> cudaError_t launch_t(const SampleArgs& a, cudaStream_t st)
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = sizeof(Shared) + (size_t)bytes;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    if (ctas == 1) return cudaLaunchKernelEx(&cfg, kern, a, share, bytes);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)ctas; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = ctas == 1 ? 1 : 2;
+    if (ctas == 1) return cudaLaunchKernelEx(&cfg, kern, a, share, bytes);
     e = launch_clusters(cfg, kern, a, share, bytes);
     if (e == cudaSuccess) return e;
     (void)cudaGetLastError();                    // the device places no clusters: a block a row
