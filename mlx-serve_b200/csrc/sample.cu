@@ -108,16 +108,16 @@ struct alignas(16) Shared {
   double roots[32];
   uint64_t above, whole;
   union {                                      // (never of use at the same time)
+    uint32_t hist[kBins];
     uint64_t list[kList];                      // pattern, then V - 1 - index: larger ones come first in the order
     uint64_t sums[kMaxStrips * kWarps];        // of every warp's part of every strip
   };
-  uint32_t hist[kBins];
   union {
     uint32_t merged[kBins];
     float refs[kMaxStrips * kWarps];           // of the parts: what their sums are relative to
   };
   uint32_t scan[kWarps];
-  uint32_t listed;
+  uint32_t listed, staged, place;
   int answer[4];
 };
 
@@ -175,7 +175,7 @@ template <typename T> struct Row {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ SampleArgs a, int share, int held_bytes) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a, int share, int held_bytes) {
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *(Shared*)raw;
   const uint32_t C = cluster_size(), me = cluster_rank();
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   const bool greedy = !(temp > 0.f), by_k = k > 0 && k < V, by_p = p < 1.f;
   // by temperature alone the row is read once, each warp's 256 elements at a time with a largest of their own
   const bool once = !greedy && !by_k && !by_p && !(least > 0.f) && temp >= 1e-6f && temp <= 1e6f;
-  if (tid == 0) sh.listed = 0;
+  if (tid == 0) sh.listed = sh.staged = 0;
   if (tid < 32) sh.roots[tid] = kRoots[tid];
   if (by_k || by_p)
     for (int i = tid; i < kBins; i += kThreads) sh.hist[i] = 0;
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     for (uint32_t c = 0; c < C; ++c) s += g[c];
     return s;
   };
-  constexpr int kAhead = 4;                      // loads of a thread in flight
+  constexpr int kAhead = sizeof(T) == 4 ? 4 : 8;   // loads of a thread in flight
   constexpr float kLog2e = 1.4426950408889634f;
   const double per_t = 1.0 / (double)temp, c64 = 32.0 * 1.4426950408889634 * per_t, c_all = 1.4426950408889634 * per_t;
   const float ch = (float)c_all, cl = (float)(c_all - (double)ch);
@@ -666,38 +666,87 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       bool few = list_n <= kList;                            // all that may stay fits the list
       bool by_list = few;
       uint64_t above = 0, whole = 0;
-      auto into_list = [&](int lo, int hi, const Border* from) {
+      // Entries are gathered in a block's own list, then put into the first block's, behind its own and one another.
+      auto enlist = [&](float x, int index) {
+        const uint32_t at = atomicAdd(&sh.staged, 1u);
+        if (at < kList) sh.list[at] = (uint64_t)pattern(x) << 32 | (uint32_t)(V - 1 - index);
+      };
+      auto deliver = [&]() {
+        __syncthreads();
+        const uint32_t n = min(sh.staged, (uint32_t)kList);
+        if (me == 0 && tid == 0) sh.listed = n;
+        cluster_sync_all();                      // (the first block's own entries are in place)
+        if (me != 0) {
+          if (tid == 0 && n > 0) sh.place = add32(&sh.listed, 0, n);
+          __syncthreads();
+          for (uint32_t i = tid; i < n; i += kThreads)
+            if (sh.place + i < kList) put64(&sh.list[sh.place + i], 0, sh.list[i]);
+        }
+        cluster_sync_all();
+        if (tid == 0) sh.staged = 0;
+        __syncthreads();
+      };
+      auto into_list = [&](int lo, int hi) {
         for (int v = tid; v < r.vecs; v += kThreads) {
           float f[8];
           r.load8(v, f);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int bin = bin_of(f[e]);
-            if (bin >= lo && bin <= hi && bin < kBins && (from == nullptr || stays(*from, f[e], r.index(v, e)))) {
-              const uint32_t at = add32(&sh.listed, 0, 1u);
-              if (at < kList) put64(&sh.list[at], 0, (uint64_t)pattern(f[e]) << 32 | (uint32_t)(V - 1 - r.index(v, e)));   // (larger first: larger logit, then lower index)
-            }
+            if (bin >= lo && bin <= hi && bin < kBins) enlist(f[e], r.index(v, e));
           }
         }
-        cluster_sync_all();
+        deliver();
       };
-      // the first n entries of the list in descending order (bitonic; the rest of the power of two that is sorted is 0), by the first block
+      constexpr int LPT = kList / kThreads;      // neighbours of a thread
+      // The first n entries of the list in descending order, by the first block: bitonic, an entry's partner in the same thread, in the same
+      // warp, or through shared memory (ten of 55 steps for 1024).  What fills up the power of two is 0.
       auto sort_list = [&](int n) {
-        int m = 32;
+        int m = LPT * 32;
         while (m < n) m *= 2;
-        for (int i = n + tid; i < m; i += kThreads) sh.list[i] = 0;
+        uint64_t x[LPT];
+#pragma unroll
+        for (int q = 0; q < LPT; ++q) x[q] = LPT * tid + q < n ? sh.list[LPT * tid + q] : 0;
         for (int span = 2; span <= m; span *= 2)
           for (int d = span / 2; d > 0; d /= 2) {
-            __syncthreads();
-            for (int i = tid; i < m / 2; i += kThreads) {
-              const int lo = 2 * i - (i & (d - 1)), hi = lo + d;
-              const uint64_t x = sh.list[lo], y = sh.list[hi];
-              if ((x < y) == ((lo & span) == 0)) { sh.list[lo] = y; sh.list[hi] = x; }
+            if (d < LPT) {
+#pragma unroll
+              for (int dd = 1; dd < LPT; dd *= 2)
+                if (dd == d)
+#pragma unroll
+                  for (int q = 0; q < LPT; ++q)
+                    if ((q & dd) == 0) {
+                      const bool down = ((LPT * tid + q) & span) == 0;
+                      const uint64_t a0 = x[q], a1 = x[q + dd];
+                      if ((a0 < a1) == down) { x[q] = a1; x[q + dd] = a0; }
+                    }
+            } else if (d < LPT * 32) {
+              const bool first = (lane & (d / LPT)) == 0;
+#pragma unroll
+              for (int q = 0; q < LPT; ++q) {
+                const uint64_t y = __shfl_xor_sync(0xffffffffu, x[q], d / LPT);
+                const bool larger = (((LPT * tid + q) & span) == 0) == first;
+                x[q] = (x[q] < y) == larger ? y : x[q];
+              }
+            } else {
+              __syncthreads();
+#pragma unroll
+              for (int q = 0; q < LPT; ++q) sh.list[LPT * tid + q] = x[q];
+              __syncthreads();
+              const bool first = (LPT * tid & d) == 0;
+#pragma unroll
+              for (int q = 0; q < LPT; ++q) {
+                const uint64_t y = sh.list[(LPT * tid + q) ^ d];
+                const bool larger = (((LPT * tid + q) & span) == 0) == first;
+                x[q] = (x[q] < y) == larger ? y : x[q];
+              }
             }
           }
         __syncthreads();
+#pragma unroll
+        for (int q = 0; q < LPT; ++q) sh.list[LPT * tid + q] = x[q];
+        __syncthreads();
       };
-      constexpr int LPT = kList / kThreads;      // neighbours of a thread
       // sums before each of a thread's entries, of amounts in order; *all = their sum
       auto list_sums = [&](const uint64_t (&w)[LPT], uint64_t (&before)[LPT], uint64_t* all) {
         uint64_t mine = 0;
@@ -735,14 +784,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
             if (i < n && before[q] < target && target <= before[q] + w[q])
               for (uint32_t c = 0; c < C; ++c) { put32(&sh.answer[2], c, (uint32_t)(sh.list[i] >> 32)); put32(&sh.answer[3], c, (uint32_t)list_index(i)); }
           }
-          __syncthreads();
-          if (tid == 0) sh.listed = 0;
         }
         cluster_sync_all();
       };
       if (few) {
         // ---- all that may stay is in the list: the first block draws the token ----
-        into_list(0, last_bin, nullptr);
+        into_list(0, last_bin);
         if (me == 0) {
           const int n = list_n;
           sort_list(n);
@@ -790,7 +837,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       } else {
         if (cut) {
           if (list_n - k_before <= kList) {
-            into_list(k_bin, k_bin, nullptr);
+            into_list(k_bin, k_bin);
             in_list([](float) { return 1ull; }, (uint64_t)(want - (uint32_t)k_before));
             b = {(uint32_t)sh.answer[2], sh.answer[3]};
           } else b = border([](float) { return 1ull; }, (uint64_t)want, b);
@@ -843,13 +890,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
               else if (bin > last_bin) s_rest += w;
               else {
                 s_list += w;
-                if (by_list) {
-                  const uint32_t at = add32(&sh.listed, 0, 1u);
-                  if (at < kList) put64(&sh.list[at], 0, (uint64_t)pattern(f[e]) << 32 | (uint32_t)(V - 1 - r.index(v, e)));
-                }
+                if (by_list) enlist(f[e], r.index(v, e));
               }
             }
           }
+          if (by_list) deliver();
           above = total(s_above);
           const uint64_t inside = total(s_list);
           whole = above + inside + total(s_rest);
@@ -906,8 +951,10 @@ template <typename T> cudaError_t launch_t(const SampleArgs& a, cudaStream_t st)
       if (dev >= 0 && dev < 64) done[dev] = true;
     }
   }
+  // Blocks a row: enough that there are two for every SM, of at least 8192 elements each.  (What the blocks of a row say to one another takes 0.7 us
+  // each time, so that many rows are better off with a block or two each; one row of 128256 takes 23 us by one, 13 by eight.)
   int ctas = 1;
-  while (ctas < kMaxCtas && a.V > ctas * 2 * kStrip) ctas *= 2;
+  while (ctas < kMaxCtas && (int64_t)a.N * ctas < 2 * sm_count() && a.V > ctas * 2 * kStrip) ctas *= 2;
   for (;; ctas = 1) {
     const int share = ((a.V + ctas - 1) / ctas + 7) / 8 * 8;
     const int need = (share + 16) * (int)sizeof(T);
