@@ -25,13 +25,14 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kStrip = kThreads * 8;           // elements that the block takes at a time, eight a thread
-constexpr int kMaxStrips = kMaxVocab / kStrip + 2;
 constexpr int kBins = 4096;
 constexpr float kRange = 32.f;                 // temperatures below the largest that the bins cover: e^-32 < 2^-45
 constexpr int kList = 2048;
+constexpr int kPairs = 128;                    // entries of a list that are compared pair by pair rather than sorted
 constexpr double kOne = 17592186044416.0;      // 2^44
 constexpr int kMaxCtas = 8;
+constexpr int kDeep = 2;                       // vectors of eight elements a lane has of a warp's part of a row
+constexpr int kMaxParts = kMaxVocab / (32 * 8 * kDeep) + 2;
 
 // larger patterns for larger floats (no NaN, no -0 comes here)
 __device__ __forceinline__ uint32_t pattern(float x) {
@@ -106,21 +107,20 @@ struct alignas(16) Shared {
   double part[kMaxCtas], part_top[kMaxCtas];   // of the sum for the log-probability: a block's sum and its largest
   double once_sum[kMaxCtas];
   double roots[32];
-  uint64_t above, whole;
   union {                                      // (never of use at the same time)
     uint32_t hist[kBins];
     uint64_t list[kList];                      // pattern, then V - 1 - index: larger ones come first in the order
-    uint64_t sums[kMaxStrips * kWarps];        // of every warp's part of every strip
+    uint64_t sums[kMaxParts];                  // of every warp's part
   };
   union {
     uint32_t merged[kBins];
-    float refs[kMaxStrips * kWarps];           // of the parts: what their sums are relative to
+    uint64_t weight[kPairs];                   // of the list's entries
+    float refs[kMaxParts];                     // of the parts: what their sums are relative to
   };
   uint32_t scan[kWarps];
   uint32_t listed, staged, place;
   int answer[4];
 };
-
 static_assert(sizeof(Shared) % 16 == 0, "vectors behind it");
 
 template <typename T> struct Row {
@@ -176,6 +176,8 @@ template <typename T> struct Row {
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a, int share, int held_bytes) {
+  constexpr int DEEP = kDeep;
+  constexpr float kLog2e = 1.4426950408889634f;
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *(Shared*)raw;
   const uint32_t C = cluster_size(), me = cluster_rank();
@@ -185,21 +187,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const int k = a.top_k ? a.top_k[row_no * a.str[2]] : 0;
   const float p = a.top_p ? a.top_p[row_no * a.str[3]] : 1.f, least = a.min_p ? a.min_p[row_no * a.str[4]] : 0.f;
 
-  // ---- this block's share, and the row's largest ----
   Row<T> r;
   r.begin = (int)me * share < V ? (int)me * share : V;
   r.n = V - r.begin < share ? V - r.begin : share;
   r.x = (const T*)((const char*)a.logits + (int64_t)row_no * a.row_bytes) + r.begin;
   r.off = (int)((uintptr_t)r.x & (8 * sizeof(T) - 1)) / (int)sizeof(T);
   r.vecs = (r.n + r.off + 7) / 8;
+  r.held = nullptr;
+  const int parts = (r.vecs + 32 * DEEP - 1) / (32 * DEEP);
   unsigned char* const held = raw + sizeof(Shared);
   const bool greedy = !(temp > 0.f), by_k = k > 0 && k < V, by_p = p < 1.f;
-  // by temperature alone the row is read once, each warp's 256 elements at a time with a largest of their own
+  // by temperature alone the row is read once, its parts weighed relative to a largest of their own
   const bool once = !greedy && !by_k && !by_p && !(least > 0.f) && temp >= 1e-6f && temp <= 1e6f;
+  const bool hold = !greedy && !once && r.vecs * 8 * (int)sizeof(T) <= held_bytes;
   if (tid == 0) sh.listed = sh.staged = 0;
   if (tid < 32) sh.roots[tid] = kRoots[tid];
-  if (by_k || by_p)
-    for (int i = tid; i < kBins; i += kThreads) sh.hist[i] = 0;
+
   int turn = 0;
   // a value of every block, in all blocks
   auto gather = [&](uint64_t mine) {
@@ -216,19 +219,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     __syncthreads();
     return warp_sum(lane < kWarps ? sh.red[lane] : (uint64_t)0);
   };
+  auto block_sum_d = [&](double v) {
+    v = warp_sum(v);
+    __syncthreads();
+    if (lane == 0) sh.red_d[warp] = v;
+    __syncthreads();
+    return warp_sum(lane < kWarps ? sh.red_d[lane] : 0.0);
+  };
   auto total = [&](uint64_t v) {
     const uint64_t* const g = gather(block_sum(v));
     uint64_t s = 0;
     for (uint32_t c = 0; c < C; ++c) s += g[c];
     return s;
   };
-  constexpr int kAhead = sizeof(T) == 4 ? 4 : 8;   // loads of a thread in flight
-  constexpr float kLog2e = 1.4426950408889634f;
   const double per_t = 1.0 / (double)temp, c64 = 32.0 * 1.4426950408889634 * per_t, c_all = 1.4426950408889634 * per_t;
   const float ch = (float)c_all, cl = (float)(c_all - (double)ch);
-  const int strips = (r.vecs + kThreads - 1) / kThreads;
-  // Weights in fp32, relative to `largest`, from the approximate exponential (relative error 2^-22), whose argument is carried in two parts and
-  // whose product with the rest rounds twice (2^-23).
+  // Weights in fp32, relative to `largest`, from the approximate exponential (relative error 2^-22), whose argument is carried in two parts, and
+  // which is rounded once more with the second.
   auto weights32 = [&](const float (&f)[8], float largest, float (&w)[8]) {
     const float floor_d = -200.f / ch;           // (what lies further down weighs 0, as this does)
     const uint64_t ch2 = two(ch, ch), cl2 = two(cl, cl), top2 = two(-largest, -largest), ln2 = two(0.6931471805599453f, 0.6931471805599453f), minus = two(-1.f, -1.f);
@@ -244,50 +251,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
   };
   auto add8 = [](const float (&w)[8]) { return ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])); };
-  // How far a sum of such weights and u times their whole may lie from one another's true place: every weight is within e = 2^-20.7 (2^-22, 2^-23,
-  // three roundings of 2^-24 where eight are added) of itself, those before the place count 1 - u times and those behind it u times.
-  auto slack_of = [&](double all) { const double v = u > 0.f ? (u < 1.f ? (double)u : 1.0) : 0.0; return all * (2.0 * v * (1.0 - v) * 5.9e-7 + 1e-11); };
-  double lp_sum = 0.0;                           // of exp(x - this block's largest), for the log-probability
-  float top, mine_top;
-  int token = -1;
+  // How far a sum of such weights and u times their whole may lie from one another's true place: every weight is within e = 4.3e-7 (2^-22, and three
+  // roundings of 2^-24: one of its own, two where four are added; the rest is added in 64 bits) of itself, those before the place count 1 - u times
+  // and those behind it u times.
+  auto slack_of = [&](double all) { const double v = u > 0.f ? (u < 1.f ? (double)u : 1.0) : 0.0; return all * (2.0 * v * (1.0 - v) * 4.3e-7 + 1e-11); };
+  auto place_of = [&](double all) { return u > 0.f ? (u < 1.f ? (double)u * all : all) : 0.0; };
   double* const sums_d = (double*)sh.sums;
-  // The element of a warp's part q of a strip at which the sum passes t (all given relative to `largest` of that part), by a warp; -1: too near a border.
-  auto within = [&](int q, double before, double t, double slack, auto weights) -> int {
-    const int v = q / kWarps * kThreads + q % kWarps * 32 + lane;
-    float w[8];
-    if (v < r.vecs) weights(v, w);
-    else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = 0.f;
-    }
-    double s = 0.0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s += (double)w[e];
-    double upto = s;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double n = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += n;
-    }
-    double run = before + upto - s;
-    int at = -1;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (at < 0 && run + slack < t && t < run + (double)w[e] - slack) at = r.index(v, e);
-      run += (double)w[e];
-    }
-    const uint32_t hit = __ballot_sync(0xffffffffu, at >= 0);
-    return hit ? __shfl_sync(0xffffffffu, at, __ffs(hit) - 1) : -1;
-  };
-  // The part at which the running sum of sums_d passes t, by a warp; *before = the sum before it; -1: none.
-  auto part_of = [&](double t, double* before) -> int {
-    double b = *before;
-    for (int q0 = 0; q0 < strips * kWarps; q0 += 32) {
-      const double x = q0 + lane < strips * kWarps ? sums_d[q0 + lane] : 0.0;
-      double upto = x;
+  // The part at which the running sum of the parts' passes t, by a warp; *before = the sum before it; -1: none.
+  auto part_of = [&](auto* sums, auto t, auto* before) -> int {
+    auto b = *before;
+    for (int q0 = 0; q0 < parts; q0 += 32) {
+      auto upto = q0 + lane < parts ? sums[q0 + lane] : (decltype(b))0;
+      const auto x = upto;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const double n = __shfl_up_sync(0xffffffffu, upto, o);
+        const auto n = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += n;
       }
       const uint32_t hit = __ballot_sync(0xffffffffu, b + upto > t);
@@ -300,67 +278,145 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
     return -1;
   };
-  auto block_sum_d = [&](double v) {
-    v = warp_sum(v);
-    __syncthreads();
-    if (lane == 0) sh.red_d[warp] = v;
-    __syncthreads();
-    return warp_sum(lane < kWarps ? sh.red_d[lane] : 0.0);
-  };
-  {
-    // ---- the row's largest; where the row is read once, sums of the weights too ----
-    r.held = nullptr;
-    const bool hold = !greedy && !once && r.vecs * 8 * (int)sizeof(T) <= held_bytes;
-    uint64_t best = 0;                           // pattern, V - 1 - index
-    for (int v0 = tid; v0 < strips * kThreads; v0 += kAhead * kThreads) {   // (by whole warps)
-      typename Row<T>::Raw got[kAhead];
+  // The element of part q at which the running sum from `before` on passes t by more than `slack` and before which it stays as far below, by a warp;
+  // -1: none.
+  auto within = [&](int q, auto before, auto t, auto slack, auto weights) -> int {
+    using S = decltype(before);
+    S mine[DEEP];
+#pragma unroll 2
+    for (int s = 0; s < DEEP; ++s) {
+      const int v = (q * DEEP + s) * 32 + lane;
+      mine[s] = 0;
+      if (v < r.vecs) {
+        auto w = weights(v);
 #pragma unroll
-      for (int q = 0; q < kAhead; ++q)
-        if (v0 + q * kThreads < r.vecs) got[q] = r.load_raw(v0 + q * kThreads);
+        for (int e = 0; e < 8; ++e) mine[s] += (S)w.w[e];
+      }
+    }
+    int at = -1;
+    S run = before;
+#pragma unroll 1
+    for (int s = 0; s < DEEP; ++s) {
+      S m = 0;
 #pragma unroll
-      for (int q = 0; q < kAhead; ++q) {
-        const int v = v0 + q * kThreads;
-        if (v - lane >= r.vecs) continue;
-        float f[8];
-        if (v < r.vecs) {
-          Row<T>::unpack(got[q], f);
+      for (int x = 0; x < DEEP; ++x) m = x == s ? mine[x] : m;
+      const S all = warp_sum(m);
+      if (run + all > t || run + all + slack > t) {
+        S upto = m;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = clean(f[e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = -INFINITY;
+        for (int o = 1; o < 32; o <<= 1) {
+          const S n = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += n;
         }
-        float mx = f[0];
+        S b = run + upto - m;
+        const int v = (q * DEEP + s) * 32 + lane;
+        if (v < r.vecs && b <= t && b + m >= t) {
+          auto w = weights(v);
 #pragma unroll
-        for (int e = 1; e < 8; ++e) mx = fmaxf(mx, f[e]);
-        if (hold && v < r.vecs) {
+          for (int e = 0; e < 8; ++e) {
+            if (at < 0 && b + slack <= t && t + slack < b + (S)w.w[e]) at = r.index(v, e);
+            b += (S)w.w[e];
+          }
+        }
+        break;
+      }
+      run += all;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, at >= 0);
+    return hit ? __shfl_sync(0xffffffffu, at, __ffs(hit) - 1) : -1;
+  };
+  struct W8 { float w[8]; };
+  struct U8 { uint64_t w[8]; };
+
+  // ---- the row's largest; sums for the log-probability; where the row is read once, of the weights too ----
+  // Weights and the terms of the log-probability are relative to a reference of the warp's own: its first part's largest, moved where something lies
+  // more than 2^64 above it.  A part is asked for while the one before is worked on.
+  float top;
+  int token = -1;
+  {
+    uint64_t best = 0;                           // pattern, V - 1 - index (the index where the largest is all that is asked for)
+    float ref = -INFINITY, mx = -INFINITY;
+    const float steep = a.logprobs ? fmaxf(once ? ch : 0.f, kLog2e) : ch;
+    double lp = 0.0;
+    typename Row<T>::Raw next[DEEP];
+    auto ask = [&](int q) {
+#pragma unroll
+      for (int s = 0; s < DEEP; ++s) {
+        const int v = (q * DEEP + s) * 32 + lane;
+        if (v < r.vecs) next[s] = r.load_raw(v);
+        else {
+          alignas(16) T none[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) none[e] = (T)(-INFINITY);
+#pragma unroll
+          for (int x = 0; x < Row<T>::W; ++x) next[s].w[x] = ((const uint4*)none)[x];
+        }
+      }
+    };
+    ask(warp);
+#pragma unroll 1
+    for (int q = warp; q < parts; q += kWarps) {
+      float f[DEEP][8], m = -INFINITY;
+#pragma unroll
+      for (int s = 0; s < DEEP; ++s) {
+        Row<T>::unpack(next[s], f[s]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { f[s][e] = clean(f[s][e]); m = fmaxf(m, f[s][e]); }
+      }
+      ask(q + kWarps);
+      if (hold) {
+#pragma unroll
+        for (int s = 0; s < DEEP; ++s) {
+          const int v = (q * DEEP + s) * 32 + lane;
           alignas(16) T e8[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) e8[e] = (T)f[e];
+          for (int e = 0; e < 8; ++e) e8[e] = (T)f[s][e];
+          if (v < r.vecs)
 #pragma unroll
-          for (int x = 0; x < Row<T>::W; ++x) *(uint4*)(held + v * (16 * Row<T>::W) + 16 * x) = ((const uint4*)e8)[x];
+            for (int x = 0; x < Row<T>::W; ++x) *(uint4*)(held + v * (16 * Row<T>::W) + 16 * x) = ((const uint4*)e8)[x];
         }
-        if (once) {
-          const uint32_t key = __reduce_max_sync(0xffffffffu, pattern(mx));
-          const float largest = value_of(key);
-          double t = 0.0;
-          if (largest > -INFINITY && largest < INFINITY) {
-            float w[8];
-            weights32(f, largest, w);
-            t = warp_sum((double)add8(w));
-          }
-          const int part = v / kThreads * kWarps + warp;
-          if (lane == 0) { sums_d[part] = t; sh.refs[part] = largest; }
-          best = max(best, (uint64_t)key << 32);
-        } else {
+      }
+      mx = fmaxf(mx, m);
+      if (greedy) {
+        if (pattern(m) > (uint32_t)(best >> 32)) {           // (parts ascend: an equal one further back does not count)
           int at = 0;
 #pragma unroll
-          for (int e = 7; e >= 0; --e) at = f[e] == mx ? e : at;
-          const int index = r.index(v, at);
-          best = max(best, (uint64_t)pattern(mx) << 32 | (uint32_t)(index >= 0 && index < V ? V - 1 - index : 0));
+          for (int s = DEEP - 1; s >= 0; --s)
+#pragma unroll
+            for (int e = 7; e >= 0; --e) at = f[s][e] == m ? s * 256 + e : at;
+          if (m > -INFINITY) best = (uint64_t)pattern(m) << 32 | (uint32_t)(V - 1 - r.index(q * DEEP * 32 + lane, at));
+        }
+      }
+      if (!once && !a.logprobs) continue;
+      if (__any_sync(0xffffffffu, m > ref && !((m - ref) * steep < 64.f))) {
+        const float up = value_of(__reduce_max_sync(0xffffffffu, pattern(m)));
+        lp = ref > -INFINITY ? lp * exp2((double)(ref - up) * 1.4426950408889634) : 0.0;
+        ref = up;
+      }
+      if (once) {
+        double t = 0.0;
+        if (ref > -INFINITY && ref < INFINITY) {
+#pragma unroll
+          for (int s = 0; s < DEEP; ++s) {
+            float w[8];
+            weights32(f[s], ref, w);
+            t += (double)((w[0] + w[1]) + (w[2] + w[3])) + (double)((w[4] + w[5]) + (w[6] + w[7]));
+          }
+          t = warp_sum(t);
+        }
+        if (lane == 0) { sums_d[q] = t; sh.refs[q] = ref; }
+      }
+      if (a.logprobs && ref > -INFINITY) {
+#pragma unroll
+        for (int s = 0; s < DEEP; ++s) {
+          float w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = f[s][e] == ref ? 1.f : ex2((f[s][e] - ref) * kLog2e);
+          lp += (double)add8(w);
         }
       }
     }
+    if (!greedy && mx > -INFINITY) best = (uint64_t)pattern(mx) << 32;
     if (hold) r.held = held;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(0xffffffffu, best, o));
@@ -370,70 +426,61 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     best = lane < kWarps ? sh.red[lane] : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(0xffffffffu, best, o));
-    mine_top = r.vecs > 0 ? value_of((uint32_t)(best >> 32)) : -INFINITY;
+    const float mine_top = best ? value_of((uint32_t)(best >> 32)) : -INFINITY;
     double mine = 0.0;
     if (once) {
-      // parts relative to the block's largest (both below infinity, else the row is not decided here)
-      for (int q = tid; q < strips * kWarps; q += kThreads) {
-        const int v = q / kWarps * kThreads + q % kWarps * 32;
-        const float ref = v < r.vecs ? sh.refs[q] : -INFINITY;
-        const double w = ref > -INFINITY && mine_top < INFINITY ? sums_d[q] * exp2(((double)ref - (double)mine_top) * c_all) : 0.0;
+      // parts relative to the block's largest (where that is infinite the row is not decided here)
+      for (int q = tid; q < parts; q += kThreads) {
+        const float at = sh.refs[q];
+        const double w = at > -INFINITY && mine_top < INFINITY ? sums_d[q] * exp2(((double)at - (double)mine_top) * c_all) : 0.0;
         sums_d[q] = w;
         mine += w;
       }
       mine = block_sum_d(mine);
+      if (tid < (int)C) put64((uint64_t*)&sh.once_sum[me], (uint32_t)tid, (uint64_t)__double_as_longlong(mine));
     }
     if (a.logprobs) {
-      // (the row is in shared memory, or has just been read)
-      for (int v = tid; v < r.vecs; v += kThreads) {
-        float f[8], t = 0.f;
-        r.load8(v, f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) t += f[e] == mine_top ? 1.f : ex2((f[e] - mine_top) * kLog2e);
-        lp_sum += (double)t;
-      }
-      lp_sum = block_sum_d(lp_sum);
-      if (tid == 0) put64((uint64_t*)&sh.part[me], 0, (uint64_t)__double_as_longlong(lp_sum));
+      lp = block_sum_d(ref > -INFINITY ? (ref != mine_top ? lp * exp2((double)(ref - mine_top) * 1.4426950408889634) : lp) : 0.0);
+      if (tid == 0) put64((uint64_t*)&sh.part[me], 0, (uint64_t)__double_as_longlong(lp));
       if (tid == 32) put64((uint64_t*)&sh.part_top[me], 0, (uint64_t)__double_as_longlong((double)mine_top));
     }
-    if (once && tid < (int)C) put64((uint64_t*)&sh.once_sum[me], (uint32_t)tid, (uint64_t)__double_as_longlong(mine));
     const uint64_t* const g = gather(best);
     for (uint32_t c = 0; c < C; ++c) best = max(best, g[c]);
-    top = value_of((uint32_t)(best >> 32));
-    if (greedy && top > -INFINITY) token = V - 1 - (int)(uint32_t)best;
-    if (once && top > -INFINITY && top < INFINITY) {
+    top = best ? value_of((uint32_t)(best >> 32)) : -INFINITY;
+    if (greedy && best) token = V - 1 - (int)(uint32_t)best;
+    if (once && best && top < INFINITY) {
       double all = 0.0, part[kMaxCtas];
 #pragma unroll
       for (uint32_t c = 0; c < kMaxCtas; ++c) {
-        part[c] = 0.0;
-        if (c < C) {
-          const float ref = value_of((uint32_t)(g[c] >> 32));
-          part[c] = g[c] && ref > -INFINITY ? sh.once_sum[c] * exp2(((double)ref - (double)top) * c_all) : 0.0;
-          all += part[c];
-        }
+        part[c] = c < C && g[c] ? sh.once_sum[c] * exp2(((double)value_of((uint32_t)(g[c] >> 32)) - (double)top) * c_all) : 0.0;
+        all += part[c];
       }
-      const double slack = slack_of(all), t = u > 0.f ? (u < 1.f ? (double)u * all : all) : 0.0;
-      uint32_t who = C;
+      const double slack = slack_of(all), t = place_of(all);
+      uint32_t who = C - 1;
       double before = 0.0, run = 0.0;
+      bool found = false;
 #pragma unroll
       for (uint32_t c = 0; c < kMaxCtas; ++c) {
-        if (c < C && who == C && t < run + part[c]) { who = c; before = run; }
+        if (c < C && !found && t < run + part[c]) { who = c; before = run; found = true; }
         run += part[c];
       }
-      if (who == C) who = C - 1;
       if (who == me && warp == 0) {
-        // everything relative to this block's largest
-        const double up = exp2(((double)top - (double)mine_top) * c_all);
-        double b = before * up;
-        const int q = mine_top > -INFINITY ? part_of(t * up, &b) : -1;
+        // everything relative to this block's largest, then to the part's
         int at = -1;
-        if (q >= 0) {
-          const double there = exp2(((double)mine_top - (double)sh.refs[q]) * c_all);
-          at = within(q, b * there, t * up * there, slack * up * there, [&](int v, float (&w)[8]) {
-            float f[8];
-            r.load8(v, f);
-            weights32(f, sh.refs[q], w);
-          });
+        if (found) {
+          const double up = exp2(((double)top - (double)mine_top) * c_all);
+          double b = before * up;
+          const int q = part_of(sums_d, t * up, &b);
+          if (q >= 0) {
+            const double there = exp2(((double)mine_top - (double)sh.refs[q]) * c_all);
+            at = within(q, b * there, t * up * there, slack * up * there, [&](int v) {
+              float f[8];
+              W8 w;
+              r.load8(v, f);
+              weights32(f, sh.refs[q], w.w);
+              return w;
+            });
+          }
         }
         if (lane < (int)C) put32(&sh.answer[0], (uint32_t)lane, (uint32_t)at);
       }
@@ -450,74 +497,40 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   };
   auto enough = [&](float x) { return !(least > 0.f) || x == top || exp(((double)x - (double)top) * per_t) >= (double)least; };
 
-  // The first index at which the sum of `amount` passes `target(whole sum)`, all blocks' answer; *whole = the sum.
-  auto find = [&](auto amount, auto target, uint64_t* whole) -> int {
+  // The first index at which the sum of `amount` passes `target(whole sum)`, all blocks' answer.
+  auto find = [&](auto amount, auto target) -> int {
     uint64_t mine = 0;
-    for (int s = 0; s < strips; ++s) {
-      const int v = s * kThreads + tid;
+    for (int q = warp; q < parts; q += kWarps) {
       uint64_t t = 0;
-      if (v < r.vecs) {
+#pragma unroll 2
+      for (int s = 0; s < DEEP; ++s) {
+        const int v = (q * DEEP + s) * 32 + lane;
+        if (v >= r.vecs) continue;
         float f[8];
         r.load8(v, f);
 #pragma unroll
         for (int e = 0; e < 8; ++e) t += amount(f[e], r.index(v, e));
       }
       t = warp_sum(t);
-      if (lane == 0) sh.sums[s * kWarps + warp] = t;
-      mine += t;
+      if (lane == 0) { sh.sums[q] = t; mine += t; }
     }
-    __syncthreads();
-    if (lane == 0) sh.red[warp] = mine;
-    __syncthreads();
-    const uint64_t* const g = gather(warp_sum(lane < kWarps ? sh.red[lane] : (uint64_t)0));
+    const uint64_t* const g = gather(block_sum(mine));
     uint64_t all = 0;
     for (uint32_t c = 0; c < C; ++c) all += g[c];
-    *whole = all;
-    uint64_t t = target(all);
+    const uint64_t t = target(all);
+    uint64_t before = 0;
     uint32_t who = 0;
-    while (who + 1 < C && t >= g[who]) t -= g[who++];
-    if (who == me && warp == 0) {                            // the warp's part of a strip, the lane, the element
-      int q = 0;
-      uint64_t before = 0;
-      for (int q0 = 0; q0 < strips * kWarps; q0 += 32) {
-        const uint64_t x = q0 + lane < strips * kWarps ? sh.sums[q0 + lane] : 0;
-        uint64_t upto = x;
+    for (; who + 1 < C && before + g[who] <= t; ++who) before += g[who];
+    if (who == me && warp == 0) {
+      const int q = part_of(sh.sums, t, &before);
+      const int at = q < 0 ? V - 1 : within(q, before, t, (uint64_t)0, [&](int v) {
+        float f[8];
+        U8 w;
+        r.load8(v, f);
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint64_t n = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += n;
-        }
-        const uint32_t hit = __ballot_sync(0xffffffffu, before + upto > t);
-        if (hit) {
-          const int l = __ffs(hit) - 1;
-          q = q0 + l;
-          before += __shfl_sync(0xffffffffu, upto - x, l);
-          break;
-        }
-        before += __shfl_sync(0xffffffffu, upto, 31);
-        q = q0 + 31;
-      }
-      const int v = q / kWarps * kThreads + q % kWarps * 32 + lane;
-      float f[8];
-      uint64_t w[8], s = 0;
-      if (v < r.vecs) r.load8(v, f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { w[e] = v < r.vecs ? amount(f[e], r.index(v, e)) : 0; s += w[e]; }
-      uint64_t upto = s;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t n = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += n;
-      }
-      uint64_t run = before + upto - s;
-      int at = -1;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (at < 0 && run + w[e] > t) at = r.index(v, e);
-        run += w[e];
-      }
-      const uint32_t hit = __ballot_sync(0xffffffffu, at >= 0);
-      at = hit ? __shfl_sync(0xffffffffu, at, __ffs(hit) - 1) : V - 1;
+        for (int e = 0; e < 8; ++e) w.w[e] = amount(f[e], r.index(v, e));
+        return w;
+      });
       if (lane < (int)C) put32(&sh.answer[0], (uint32_t)lane, (uint32_t)at);
     }
     cluster_sync_all();
@@ -526,41 +539,40 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   // The token among those of which `stay(x, i)` says so, by weights in fp32.  -1 where the place to find lies too near an element's border (or a weight
   // too near min_p): then the whole numbers decide.
   auto find_fast = [&](auto stay) -> int {
-    auto weights = [&](int v, float (&w)[8]) {
+    auto weights = [&](int v) {
       float f[8];
+      W8 w;
       r.load8(v, f);
-      weights32(f, top, w);
+      weights32(f, top, w.w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if (least > 0.f) {
-          const float off = w[e] - least;
-          if (fabsf(off) <= least * 1.9073486328125e-6f && f[e] != top) w[e] = __uint_as_float(0x7fc00000u);    // 2^-19
-          else if (off < 0.f && f[e] != top) w[e] = 0.f;
+          const float off = w.w[e] - least;
+          if (fabsf(off) <= least * 1.9073486328125e-6f && f[e] != top) w.w[e] = __uint_as_float(0x7fc00000u);    // 2^-19
+          else if (off < 0.f && f[e] != top) w.w[e] = 0.f;
         }
-        if (!stay(f[e], r.index(v, e))) w[e] = 0.f;
+        if (!stay(f[e], r.index(v, e))) w.w[e] = 0.f;
       }
+      return w;
     };
     double mine = 0.0;
-    for (int s = 0; s < strips; ++s) {
-      const int v = s * kThreads + tid;
+    for (int q = warp; q < parts; q += kWarps) {
       double t = 0.0;
-      if (v < r.vecs) {
-        float w[8];
-        weights(v, w);
-        t = (double)add8(w);
+#pragma unroll 2
+      for (int s = 0; s < DEEP; ++s) {
+        const int v = (q * DEEP + s) * 32 + lane;
+        if (v < r.vecs) {
+          const W8 w = weights(v);
+          t += (double)((w.w[0] + w.w[1]) + (w.w[2] + w.w[3])) + (double)((w.w[4] + w.w[5]) + (w.w[6] + w.w[7]));
+        }
       }
       t = warp_sum(t);
-      if (lane == 0) sums_d[s * kWarps + warp] = t;
-      mine += t;
+      if (lane == 0) { sums_d[q] = t; mine += t; }
     }
-    __syncthreads();
-    if (lane == 0) sh.red_d[warp] = mine;
-    __syncthreads();
-    mine = warp_sum(lane < kWarps ? sh.red_d[lane] : 0.0);
-    const uint64_t* const g = gather((uint64_t)__double_as_longlong(mine));
+    const uint64_t* const g = gather((uint64_t)__double_as_longlong(block_sum_d(mine)));
     double all = 0.0;
     for (uint32_t c = 0; c < C; ++c) all += __longlong_as_double((long long)g[c]);
-    const double t = u > 0.f ? (u < 1.f ? (double)u * all : all) : 0.0;
+    const double t = place_of(all);
     uint32_t who = 0;
     double before = 0.0;
     for (; who + 1 < C; ++who) {
@@ -569,21 +581,25 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       before += n;
     }
     if (who == me && warp == 0) {
-      const int q = part_of(t, &before);
+      const int q = part_of(sums_d, t, &before);
       const int at = q >= 0 ? within(q, before, t, slack_of(all), weights) : -1;
       if (lane < (int)C) put32(&sh.answer[0], (uint32_t)lane, (uint32_t)at);
     }
     cluster_sync_all();
     return sh.answer[0];
   };
-  auto sum_of = [&](auto amount) {
-    uint64_t s = 0;
+  // a look at every element of the share
+  auto each = [&](auto look) {
     for (int v = tid; v < r.vecs; v += kThreads) {
       float f[8];
       r.load8(v, f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += amount(f[e], r.index(v, e));
+      for (int e = 0; e < 8; ++e) look(f[e], r.index(v, e));
     }
+  };
+  auto sum_of = [&](auto amount) {
+    uint64_t s = 0;
+    each([&](float x, int i) { s += amount(x, i); });
     return total(s);
   };
   auto stays = [&](const Border& b, float x, int i) { return pattern(x) > b.key || (pattern(x) == b.key && i <= b.index); };
@@ -595,12 +611,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       if (sum_of([&](float x, int i) { return pattern(x) >= mid && stays(from, x, i) ? amount(x) : 0ull; }) >= target) lo = mid; else hi = mid - 1;
     }
     const uint64_t above = sum_of([&](float x, int i) { return pattern(x) > lo && stays(from, x, i) ? amount(x) : 0ull; });
-    const uint64_t each = amount(value_of(lo));
+    const uint64_t one = amount(value_of(lo));
     Border b = {lo, V - 1};
-    if (each > 0) {                              // among equal ones, the first so many by index
-      const uint64_t n = (target - above + each - 1) / each;
-      uint64_t all;
-      b.index = find([&](float x, int i) { return (uint64_t)(pattern(x) == lo && stays(from, x, i)); }, [&](uint64_t) { return n - 1; }, &all);
+    if (one > 0) {                               // among equal ones, the first so many by index
+      const uint64_t n = (target - above + one - 1) / one;
+      b.index = find([&](float x, int i) { return (uint64_t)(pattern(x) == lo && stays(from, x, i)); }, [&](uint64_t) { return n - 1; });
     }
     return b;
   };
@@ -616,19 +631,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     Border b = {0u, V - 1};
     if (by_k || by_p) {
       // ---- how many logits in which step ----
-      for (int v = tid; v < r.vecs; v += kThreads) {
-        float f[8];
-        r.load8(v, f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int bin = bin_of(f[e]);
-          if (bin < kBins) atomicAdd(&sh.hist[bin], 1u);
-        }
-      }
+      for (int i = tid; i < kBins; i += kThreads) sh.hist[i] = 0;
+      __syncthreads();
+      each([&](float x, int) {
+        const int bin = bin_of(x);
+        if (bin < kBins) atomicAdd(&sh.hist[bin], 1u);
+      });
       cluster_sync_all();
-      const int each = kBins / (int)C;           // every block adds its part of the bins, for all
-      for (int i = tid; i < each; i += kThreads) {
-        const int bin = (int)me * each + i;
+      const int bins = kBins / (int)C;           // every block adds its part of the bins, for all
+      for (int i = tid; i < bins; i += kThreads) {
+        const int bin = (int)me * bins + i;
         uint32_t n = 0;
         for (uint32_t c = 0; c < C; ++c) n += get32(&sh.hist[bin], c);
         for (uint32_t c = 0; c < C; ++c) put32(&sh.merged[bin], c, n);
@@ -646,9 +658,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if (lane >= o) upto += n;
       }
       if (lane == 31) sh.scan[warp] = upto;
-      if (tid < 4) sh.answer[tid] = -1;
       __syncthreads();
       uint32_t before = upto - mine, in_range = 0;
+#pragma unroll
       for (int w = 0; w < kWarps; ++w) { if (w < warp) before += sh.scan[w]; in_range += sh.scan[w]; }
       const uint32_t want = by_k && (uint32_t)k < in_range ? (uint32_t)k : in_range;     // (what lies further has no weight)
       if (before < want && want <= before + mine) {
@@ -660,12 +672,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         }
       }
       __syncthreads();
-      int last_bin = sh.answer[0], list_n = sh.answer[1], first_bin = 0;                  // of the list
-      const int k_bin = last_bin, k_before = sh.answer[2];
-      const bool cut = want < in_range;                      // top-k leaves something out
-      bool few = list_n <= kList;                            // all that may stay fits the list
-      bool by_list = few;
-      uint64_t above = 0, whole = 0;
+      const int k_bin = sh.answer[0], k_upto = sh.answer[1], k_before = sh.answer[2];
+      const bool cut = want < in_range;          // top-k leaves something out
+      const bool few = k_upto <= kList;          // all that may stay fits the list
       // Entries are gathered in a block's own list, then put into the first block's, behind its own and one another.
       auto enlist = [&](float x, int index) {
         const uint32_t at = atomicAdd(&sh.staged, 1u);
@@ -682,20 +691,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           for (uint32_t i = tid; i < n; i += kThreads)
             if (sh.place + i < kList) put64(&sh.list[sh.place + i], 0, sh.list[i]);
         }
-        cluster_sync_all();
+        if (C > 1) cluster_sync_all();
         if (tid == 0) sh.staged = 0;
         __syncthreads();
       };
       auto into_list = [&](int lo, int hi) {
-        for (int v = tid; v < r.vecs; v += kThreads) {
-          float f[8];
-          r.load8(v, f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int bin = bin_of(f[e]);
-            if (bin >= lo && bin <= hi && bin < kBins) enlist(f[e], r.index(v, e));
-          }
-        }
+        each([&](float x, int i) {
+          const int bin = bin_of(x);
+          if (bin >= lo && bin <= hi && bin < kBins) enlist(x, i);
+        });
         deliver();
       };
       constexpr int LPT = kList / kThreads;      // neighbours of a thread
@@ -704,11 +708,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       auto sort_list = [&](int n) {
         int m = LPT * 32;
         while (m < n) m *= 2;
+        const bool live = LPT * 32 * warp < m;
         uint64_t x[LPT];
+        if (live)
 #pragma unroll
-        for (int q = 0; q < LPT; ++q) x[q] = LPT * tid + q < n ? sh.list[LPT * tid + q] : 0;
+          for (int q = 0; q < LPT; ++q) x[q] = LPT * tid + q < n ? sh.list[LPT * tid + q] : 0;
         for (int span = 2; span <= m; span *= 2)
           for (int d = span / 2; d > 0; d /= 2) {
+            if (d >= LPT * 32) {
+              __syncthreads();
+              if (live)
+#pragma unroll
+                for (int q = 0; q < LPT; ++q) sh.list[LPT * tid + q] = x[q];
+              __syncthreads();
+            }
+            if (!live) continue;
             if (d < LPT) {
 #pragma unroll
               for (int dd = 1; dd < LPT; dd *= 2)
@@ -720,31 +734,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
                       const uint64_t a0 = x[q], a1 = x[q + dd];
                       if ((a0 < a1) == down) { x[q] = a1; x[q + dd] = a0; }
                     }
-            } else if (d < LPT * 32) {
-              const bool first = (lane & (d / LPT)) == 0;
-#pragma unroll
-              for (int q = 0; q < LPT; ++q) {
-                const uint64_t y = __shfl_xor_sync(0xffffffffu, x[q], d / LPT);
-                const bool larger = (((LPT * tid + q) & span) == 0) == first;
-                x[q] = (x[q] < y) == larger ? y : x[q];
-              }
             } else {
-              __syncthreads();
-#pragma unroll
-              for (int q = 0; q < LPT; ++q) sh.list[LPT * tid + q] = x[q];
-              __syncthreads();
               const bool first = (LPT * tid & d) == 0;
 #pragma unroll
               for (int q = 0; q < LPT; ++q) {
-                const uint64_t y = sh.list[(LPT * tid + q) ^ d];
+                const uint64_t y = d < LPT * 32 ? (uint64_t)__shfl_xor_sync(0xffffffffu, x[q], d / LPT) : sh.list[(LPT * tid + q) ^ d];
                 const bool larger = (((LPT * tid + q) & span) == 0) == first;
                 x[q] = (x[q] < y) == larger ? y : x[q];
               }
             }
           }
         __syncthreads();
+        if (live)
 #pragma unroll
-        for (int q = 0; q < LPT; ++q) sh.list[LPT * tid + q] = x[q];
+          for (int q = 0; q < LPT; ++q) sh.list[LPT * tid + q] = x[q];
         __syncthreads();
       };
       // sums before each of a thread's entries, of amounts in order; *all = their sum
@@ -762,13 +765,25 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if (lane == 31) sh.red[warp] = upto;
         __syncthreads();
         uint64_t base = upto - mine, sum = 0;
+#pragma unroll
         for (int x = 0; x < kWarps; ++x) { if (x < warp) base += sh.red[x]; sum += sh.red[x]; }
 #pragma unroll
         for (int q = 0; q < LPT; ++q) before[q] += base;
         *all = sum;
       };
       auto list_value = [&](int i) { return value_of((uint32_t)(sh.list[i] >> 32)); };
-      auto list_index = [&](int i) { return V - 1 - (int)(uint32_t)sh.list[i]; };
+      auto nucleus = [&](uint64_t Z) {           // the sum that the weights in front of an element that stays are below
+        if (!by_p) return ~(uint64_t)0;
+        const uint64_t t = p > 0.f ? (uint64_t)ceil((double)p * (double)Z) : 1ull;
+        return t < 1 ? (uint64_t)1 : t;
+      };
+      auto place = [&](uint64_t Z) {
+        const uint64_t t = u > 0.f ? (u < 1.f ? (uint64_t)((double)u * (double)Z) : Z) : 0;
+        return t < Z ? t : Z - 1;
+      };
+      auto answer = [&](uint32_t index) {
+        for (uint32_t c = 0; c < C; ++c) put32(&sh.answer[0], c, index);
+      };
       // the element at which the sum of the list's amounts, in order, reaches `target`; by the first block, told to all
       auto in_list = [&](auto amount, uint64_t target) {
         if (me == 0) {
@@ -782,26 +797,60 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           for (int q = 0; q < LPT; ++q) {
             const int i = LPT * tid + q;
             if (i < n && before[q] < target && target <= before[q] + w[q])
-              for (uint32_t c = 0; c < C; ++c) { put32(&sh.answer[2], c, (uint32_t)(sh.list[i] >> 32)); put32(&sh.answer[3], c, (uint32_t)list_index(i)); }
+              for (uint32_t c = 0; c < C; ++c) { put32(&sh.answer[2], c, (uint32_t)(sh.list[i] >> 32)); put32(&sh.answer[3], c, (uint32_t)(V - 1 - (int)(uint32_t)sh.list[i])); }
           }
         }
         cluster_sync_all();
       };
       if (few) {
         // ---- all that may stay is in the list: the first block draws the token ----
-        into_list(0, last_bin);
-        if (me == 0) {
-          const int n = list_n;
+        into_list(0, k_bin);
+        if (me == 0 && k_upto <= kPairs) {
+          // every entry looks at all others: its rank and the sum in front of it, then the sum up to it by index
+          const int n = k_upto;
+          uint64_t x = 0, w = 0;
+          static_assert(kPairs == 128, "barriers");
+          auto some_sum = [&](uint64_t v) {      // over the first four warps
+            v = warp_sum(v);
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (lane == 0) sh.red[warp] = v;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            return warp_sum(lane < kPairs / 32 ? sh.red[lane] : (uint64_t)0);
+          };
+          if (warp < kPairs / 32) {
+            if (tid < n) {
+              x = sh.list[tid];
+              w = weigh(value_of((uint32_t)(x >> 32)));
+              sh.weight[tid] = w;
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            uint32_t rank = 0;
+            uint64_t before_w = 0, Zk = 0;
+            auto rank_of = [&](int i) {          // (every entry's rank is needed for the sum of the first k)
+              const uint64_t y = sh.list[i];
+              if (y > x) { ++rank; before_w += sh.weight[i]; }
+            };
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) rank_of(i);
+            const bool in_k = tid < n && rank < want;
+            Zk = some_sum(in_k ? w : 0);
+            const uint64_t target = nucleus(Zk);
+            const bool stay = in_k && w > 0 && before_w < target && enough(value_of((uint32_t)(x >> 32)));
+            if (tid < n) sh.weight[tid] = stay ? w : 0;
+            const uint64_t Z = some_sum(stay ? w : 0), t = place(Z);
+            uint64_t run = 0;
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) run += (uint32_t)sh.list[i] > (uint32_t)x ? sh.weight[i] : 0ull;
+            if (stay && run <= t && t < run + w) answer((uint32_t)(V - 1 - (int)(uint32_t)x));
+          }
+        } else if (me == 0) {
+          const int n = k_upto;
           sort_list(n);
           uint64_t w[LPT], before[LPT], Z;
 #pragma unroll
           for (int q = 0; q < LPT; ++q) w[q] = LPT * tid + q < n && (uint32_t)(LPT * tid + q) < want ? weigh(list_value(LPT * tid + q)) : 0;
           list_sums(w, before, &Z);
-          uint64_t target = ~0ull;
-          if (by_p) {
-            target = p > 0.f ? (uint64_t)ceil((double)p * (double)Z) : 1ull;
-            target = target < 1 ? 1 : target;
-          }
+          const uint64_t target = nucleus(Z);
           // what stays is a first part of the order: how long, and back by index
           int stay = 0;
 #pragma unroll
@@ -813,6 +862,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           __syncthreads();
           if (lane == 0) sh.red[warp] = (uint64_t)stay;
           __syncthreads();
+#pragma unroll
           for (int x = 0; x < kWarps; ++x) stay = max(stay, (int)sh.red[x]);
           uint64_t turned[LPT];
 #pragma unroll
@@ -821,36 +871,34 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 #pragma unroll
           for (int q = 0; q < LPT; ++q)
             if (LPT * tid + q < stay) sh.list[LPT * tid + q] = turned[q] << 32 | turned[q] >> 32;      // V - 1 - index, pattern
+          __syncthreads();
           sort_list(stay);
 #pragma unroll
           for (int q = 0; q < LPT; ++q) w[q] = LPT * tid + q < stay ? weigh(value_of((uint32_t)sh.list[LPT * tid + q])) : 0;
           list_sums(w, before, &Z);
-          uint64_t t = u > 0.f ? (u < 1.f ? (uint64_t)((double)u * (double)Z) : Z) : 0;
-          t = t < Z ? t : Z - 1;
+          const uint64_t t = place(Z);
 #pragma unroll
           for (int q = 0; q < LPT; ++q)
-            if (before[q] <= t && t < before[q] + w[q])
-              for (uint32_t c = 0; c < C; ++c) put32(&sh.answer[0], c, (uint32_t)(V - 1 - (int)(uint32_t)(sh.list[LPT * tid + q] >> 32)));
+            if (before[q] <= t && t < before[q] + w[q]) answer((uint32_t)(V - 1 - (int)(uint32_t)(sh.list[LPT * tid + q] >> 32)));
         }
         cluster_sync_all();
         token = sh.answer[0];
       } else {
         if (cut) {
-          if (list_n - k_before <= kList) {
+          if (k_upto - k_before <= kList) {
             into_list(k_bin, k_bin);
-            in_list([](float) { return 1ull; }, (uint64_t)(want - (uint32_t)k_before));
+            in_list([](float) { return (uint64_t)1; }, (uint64_t)(want - (uint32_t)k_before));
             b = {(uint32_t)sh.answer[2], sh.answer[3]};
-          } else b = border([](float) { return 1ull; }, (uint64_t)want, b);
+          } else b = border([](float) { return (uint64_t)1; }, (uint64_t)want, b);
         }
         if (by_p) {
           // where it should lie by the steps' mean weights
-          __syncthreads();
           double est[PER], sum = 0.0;
 #pragma unroll
           for (int i = 0; i < PER; ++i) {
             const int bin = tid * PER + i;
             const uint32_t n = bin < k_bin ? cnt[i] : (bin == k_bin ? want - (uint32_t)k_before : 0u);
-            est[i] = (double)n * (double)exp2f(-((float)bin + 0.5f) * (kRange / (float)kBins * 1.4426950408889634f));
+            est[i] = (double)n * (double)exp2f(-((float)bin + 0.5f) * (kRange / (float)kBins * kLog2e));
             sum += est[i];
           }
           double upto_d = sum;
@@ -859,10 +907,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             const double n = __shfl_up_sync(0xffffffffu, upto_d, o);
             if (lane >= o) upto_d += n;
           }
+          __syncthreads();
           if (lane == 31) sh.red_d[warp] = upto_d;
           if (tid == 0) sh.answer[0] = k_bin;
           __syncthreads();
           double run = upto_d - sum, all = 0.0;
+#pragma unroll
           for (int w = 0; w < kWarps; ++w) { if (w < warp) run += sh.red_d[w]; all += sh.red_d[w]; }
           const double t = (double)p * all;
 #pragma unroll
@@ -871,35 +921,27 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             run += est[i];
           }
           __syncthreads();
-          first_bin = sh.answer[0] > 0 ? sh.answer[0] - 1 : 0;
-          last_bin = sh.answer[0] + 1 < kBins ? sh.answer[0] + 1 : kBins - 1;
-          list_n = 0;
+          const int first_bin = sh.answer[0] > 0 ? sh.answer[0] - 1 : 0, last_bin = sh.answer[0] + 1 < kBins ? sh.answer[0] + 1 : kBins - 1;
+          int list_n = 0;
           for (int i = first_bin; i <= last_bin; ++i) list_n += (int)sh.merged[i];
-          // (the three sums and the list in one pass)
+          // the sums above, in and below these steps, and the list, in one pass
           uint64_t s_above = 0, s_list = 0, s_rest = 0;
-          by_list = list_n <= kList;
-          for (int v = tid; v < r.vecs; v += kThreads) {
-            float f[8];
-            r.load8(v, f);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              if (!stays(b, f[e], r.index(v, e))) continue;
-              const int bin = bin_of(f[e]);
-              const uint64_t w = weigh(f[e]);
-              if (bin < first_bin) s_above += w;
-              else if (bin > last_bin) s_rest += w;
-              else {
-                s_list += w;
-                if (by_list) enlist(f[e], r.index(v, e));
-              }
+          bool by_list = list_n <= kList;
+          each([&](float x, int i) {
+            if (cut && !stays(b, x, i)) return;
+            const int bin = bin_of(x);
+            const uint64_t w = weigh(x);
+            if (bin < first_bin) s_above += w;
+            else if (bin > last_bin) s_rest += w;
+            else {
+              s_list += w;
+              if (by_list) enlist(x, i);
             }
-          }
+          });
           if (by_list) deliver();
-          above = total(s_above);
-          const uint64_t inside = total(s_list);
-          whole = above + inside + total(s_rest);
-          uint64_t target = p > 0.f ? (uint64_t)ceil((double)p * (double)whole) : 1;
-          target = target < 1 ? 1 : (target > whole ? whole : target);
+          const uint64_t above = total(s_above), inside = total(s_list), whole = above + inside + total(s_rest);
+          uint64_t target = nucleus(whole);
+          target = target > whole ? whole : target;
           by_list = by_list && above < target && target <= above + inside;
           if (by_list) {
             in_list(weigh, target - above);
@@ -910,14 +952,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
     // (at temperatures like these -200 / c, which stands in for all that lies further down, weighs 0 and is itself exact enough)
     if (token < 0 && !once && top < INFINITY && temp >= 1e-6f && temp <= 1e6f) token = find_fast([&](float x, int i) { return !(by_k || by_p) || stays(b, x, i); });
-    if (token < 0) {
-      uint64_t Z;
-      token = find([&](float x, int i) { return stays(b, x, i) && enough(x) ? weigh(x) : 0ull; },
-                   [&](uint64_t whole) {
-                     const uint64_t t = u > 0.f ? (u < 1.f ? (uint64_t)((double)u * (double)whole) : whole) : 0;
-                     return t < whole ? t : whole - 1;
-                   }, &Z);
-    }
+    auto target = [&](uint64_t whole) {
+      const uint64_t t = u > 0.f ? (u < 1.f ? (uint64_t)((double)u * (double)whole) : whole) : 0;
+      return t < whole ? t : whole - 1;
+    };
+    if (token < 0 && once) token = find([&](float x, int) { return weigh(x); }, target);
+    if (token < 0) token = find([&](float x, int i) { return stays(b, x, i) && enough(x) ? weigh(x) : (uint64_t)0; }, target);
   }
   if (a.logprobs && me == 0 && tid == 0) {
     float y = 0.f;
@@ -954,7 +994,7 @@ template <typename T> cudaError_t launch_t(const SampleArgs& a, cudaStream_t st)
   // Blocks a row: enough that there are two for every SM, of at least 8192 elements each.  (What the blocks of a row say to one another takes 0.7 us
   // each time, so that many rows are better off with a block or two each; one row of 128256 takes 23 us by one, 13 by eight.)
   int ctas = 1;
-  while (ctas < kMaxCtas && (int64_t)a.N * ctas < 2 * sm_count() && a.V > ctas * 2 * kStrip) ctas *= 2;
+  while (ctas < kMaxCtas && ((int64_t)a.N * ctas < 2 * sm_count() || a.V > ctas * 65536) && a.V > ctas * 8192) ctas *= 2;
   for (;; ctas = 1) {
     const int share = ((a.V + ctas - 1) / ctas + 7) / 8 * 8;
     const int need = (share + 16) * (int)sizeof(T);
