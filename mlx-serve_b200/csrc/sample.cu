@@ -28,7 +28,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 4096;
 constexpr float kRange = 32.f;                 // temperatures below the largest that the bins cover: e^-32 < 2^-45
 constexpr int kList = 2048;
-constexpr int kPairs = 128;                    // entries of a list that are compared pair by pair rather than sorted
+constexpr int kSlots = 1024;                   // of a list's entries, by where they stand in an order
+constexpr int kPairs = 128;                    // entries of a slot that are compared pair by pair
 constexpr double kOne = 17592186044416.0;      // 2^44
 constexpr int kMaxCtas = 8;
 constexpr int kDeep = 2;                       // vectors of eight elements a lane has of a warp's part of a row
@@ -81,10 +82,9 @@ __constant__ double kRoots[32] = {
     1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
 // round(2^44 * 2^(d * c / 32)) for d <= 0, c > 0: d c = 32 n + i + f with |f| <= 1/2 (the nearest whole number by adding 1.5 * 2^52), 2^(f / 32)
 // as its series to f^5 (the next term is below 2.3e-15), 2^(i / 32) from a table, 2^n into the exponent, the whole number out of the low bits of a
-// sum with 2^52.  0 where the exponent is below -46.
+// sum with 2^52.  What lies below 2^-46.9, or is no number, counts as that, which rounds to 0.
 __device__ __forceinline__ uint64_t weight64(double d, double c, const double* roots) {
-  const double t = d * c;
-  if (!(t > -46.0 * 32.0)) return 0;
+  const double t = fmax(d * c, -46.9 * 32.0);
   const double shifted = t + 6755399441055744.0, f = t - (shifted - 6755399441055744.0);
   const int n = __double2loint(shifted);
   double y = fma(f, 3.973709984549416e-11, 9.172562701824643e-09);
@@ -114,12 +114,16 @@ struct alignas(16) Shared {
   };
   union {
     uint32_t merged[kBins];
-    uint64_t weight[kPairs];                   // of the list's entries
     float refs[kMaxParts];                     // of the parts: what their sums are relative to
   };
+  struct {
+    uint64_t mass[kSlots], order[kPairs], weight[kPairs], before;
+    uint32_t members;
+    int slot, found;
+  } slots;
   uint32_t scan[kWarps];
   uint32_t listed, staged, place;
-  int answer[4];
+  int answer[4], range[4];
 };
 static_assert(sizeof(Shared) % 16 == 0, "vectors behind it");
 
@@ -490,19 +494,37 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
   const bool nothing = top == -INFINITY;
   const double top64 = top;
-  auto weigh = [&](float x) -> uint64_t {        // (of an infinite temperature: all alike)
-    if (x == top) return (uint64_t)kOne;
-    if (x == -INFINITY || top == INFINITY) return 0;
-    return weight64((double)x - top64, c64, sh.roots);
-  };
+  double log_whole = 0.0;
+  if (a.logprobs && me == 0 && tid == kThreads - 1) {        // (while the others go on)
+    double all = 0.0;
+    for (uint32_t c = 0; c < C; ++c) {
+      const double ref = sh.part_top[c];
+      if (ref > -INFINITY) all += ref == top64 ? sh.part[c] : sh.part[c] * exp(ref - top64);
+    }
+    log_whole = log(all);
+  }
+  auto weigh = [&](float x) -> uint64_t { return weight64(x == top ? 0.0 : (double)x - top64, c64, sh.roots); };   // (of an infinite temperature: all alike)
   auto enough = [&](float x) { return !(least > 0.f) || x == top || exp(((double)x - (double)top) * per_t) >= (double)least; };
 
-  // The first index at which the sum of `amount` passes `target(whole sum)`, all blocks' answer.
-  auto find = [&](auto amount, auto target) -> int {
+  auto stays = [&](const Border& b, float x, int i) { return pattern(x) > b.key || (pattern(x) == b.key && i <= b.index); };
+  // What a logit counts: its weight, or 1; of those that stay at `b`, and with a key from `least_key` on, or that key alone.
+  struct What { bool weight, all, min_p, alone; uint32_t least_key; Border b; };
+  auto amount_of = [&](const What& h, float x, int i) -> uint64_t {
+    const uint32_t key = pattern(x);
+    const bool in = (h.all || stays(h.b, x, i)) && (h.alone ? key == h.least_key : key >= h.least_key) && (!h.min_p || enough(x));
+    const uint64_t w = h.weight ? weigh(x) : 1;
+    return in ? w : 0;
+  };
+  // The first index at which the sum passes a place (below 0: that of the random number), all blocks' answer.
+  auto find = [&](auto plain, const What& h, int64_t at_count) -> int {
+    auto amount = [&](float x, int i) -> uint64_t {
+      if constexpr (decltype(plain)::value) return weigh(x); else return amount_of(h, x, i);
+    };
     uint64_t mine = 0;
+#pragma unroll 1
     for (int q = warp; q < parts; q += kWarps) {
       uint64_t t = 0;
-#pragma unroll 2
+#pragma unroll 1
       for (int s = 0; s < DEEP; ++s) {
         const int v = (q * DEEP + s) * 32 + lane;
         if (v >= r.vecs) continue;
@@ -517,7 +539,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     const uint64_t* const g = gather(block_sum(mine));
     uint64_t all = 0;
     for (uint32_t c = 0; c < C; ++c) all += g[c];
-    const uint64_t t = target(all);
+    uint64_t t = (uint64_t)at_count;
+    if (at_count < 0) {
+      t = u > 0.f ? (u < 1.f ? (uint64_t)((double)u * (double)all) : all) : 0;
+      t = t < all ? t : all - 1;
+    }
     uint64_t before = 0;
     uint32_t who = 0;
     for (; who + 1 < C && before + g[who] <= t; ++who) before += g[who];
@@ -597,25 +623,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       for (int e = 0; e < 8; ++e) look(f[e], r.index(v, e));
     }
   };
-  auto sum_of = [&](auto amount) {
+  auto sum_of = [&](const What& h) {
     uint64_t s = 0;
-    each([&](float x, int i) { s += amount(x, i); });
+    each([&](float x, int i) { s += amount_of(h, x, i); });
     return total(s);
   };
-  auto stays = [&](const Border& b, float x, int i) { return pattern(x) > b.key || (pattern(x) == b.key && i <= b.index); };
-  // The border at which the amounts of what stays before it reach `target`, of what stays at `from`: by halving.
-  auto border = [&](auto amount, uint64_t target, const Border& from) {
+  // The border at which the counts (or weights) of what stays before it reach `target`, of what stays at `from`: by halving.
+  auto border = [&](bool weight, uint64_t target, const Border& from) {
+    What h = {weight, false, false, false, 0u, from};
     uint32_t lo = 0, hi = pattern(top);          // the largest key whose sum from there up reaches the target
+    uint64_t above = 0;                          // (of the smallest key that is known not to)
     while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2 + 1;
-      if (sum_of([&](float x, int i) { return pattern(x) >= mid && stays(from, x, i) ? amount(x) : 0ull; }) >= target) lo = mid; else hi = mid - 1;
+      h.least_key = lo + (hi - lo) / 2 + 1;
+      const uint64_t n = sum_of(h);
+      if (n >= target) lo = h.least_key; else { hi = h.least_key - 1; above = n; }
     }
-    const uint64_t above = sum_of([&](float x, int i) { return pattern(x) > lo && stays(from, x, i) ? amount(x) : 0ull; });
-    const uint64_t one = amount(value_of(lo));
     Border b = {lo, V - 1};
+    const uint64_t one = weight ? weigh(value_of(lo)) : 1;
     if (one > 0) {                               // among equal ones, the first so many by index
-      const uint64_t n = (target - above + one - 1) / one;
-      b.index = find([&](float x, int i) { return (uint64_t)(pattern(x) == lo && stays(from, x, i)); }, [&](uint64_t) { return n - 1; });
+      h.weight = false; h.alone = true; h.least_key = lo;
+      b.index = find(std::false_type{}, h, (int64_t)((target - above + one - 1) / one) - 1);
     }
     return b;
   };
@@ -771,7 +798,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         for (int q = 0; q < LPT; ++q) before[q] += base;
         *all = sum;
       };
-      auto list_value = [&](int i) { return value_of((uint32_t)(sh.list[i] >> 32)); };
       auto nucleus = [&](uint64_t Z) {           // the sum that the weights in front of an element that stays are below
         if (!by_p) return ~(uint64_t)0;
         const uint64_t t = p > 0.f ? (uint64_t)ceil((double)p * (double)Z) : 1ull;
@@ -781,23 +807,100 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         const uint64_t t = u > 0.f ? (u < 1.f ? (uint64_t)((double)u * (double)Z) : Z) : 0;
         return t < Z ? t : Z - 1;
       };
-      auto answer = [&](uint32_t index) {
-        for (uint32_t c = 0; c < C; ++c) put32(&sh.answer[0], c, index);
+      // Entry at which the amounts w of the entries [0, n) (LPT a thread, entry tid + q * kThreads), taken by descending `order`, reach `target`; by the first block.  An
+      // entry's slot (ascending where `order` descends) says roughly where; 1024 slots are added up, and the entries of the one that matters compared
+      // pair by pair.  -1: none, or too many in one slot.  (Sorting 600 entries by both orders took 42000 cycles, this takes 8000.)
+      auto locate = [&](int n, const int (&slot)[LPT], const uint64_t (&order)[LPT], const uint64_t (&w)[LPT], uint64_t target) -> int {
+        uint64_t* const mass = sh.slots.mass;
+        for (int i = tid; i < kSlots; i += kThreads) mass[i] = 0;
+        if (tid == 0) { sh.slots.members = 0; sh.slots.slot = -1; sh.slots.found = -1; }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < LPT; ++q)
+          if (w[q] > 0) atomicAdd((unsigned long long*)&mass[slot[q]], (unsigned long long)w[q]);
+        __syncthreads();
+        const uint64_t m0 = mass[2 * tid], m1 = mass[2 * tid + 1];
+        static_assert(kSlots == 2 * kThreads, "two a thread");
+        uint64_t upto = m0 + m1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += x;
+        }
+        if (lane == 31) sh.red[warp] = upto;
+        __syncthreads();
+        uint64_t before = upto - m0 - m1;
+#pragma unroll
+        for (int x = 0; x < kWarps; ++x) before += x < warp ? sh.red[x] : 0;
+        if (before < target && target <= before + m0) { sh.slots.slot = 2 * tid; sh.slots.before = before; }
+        else if (before + m0 < target && target <= before + m0 + m1) { sh.slots.slot = 2 * tid + 1; sh.slots.before = before + m0; }
+        __syncthreads();
+        const int in = sh.slots.slot;
+        int at[LPT];
+#pragma unroll
+        for (int q = 0; q < LPT; ++q) {
+          at[q] = -1;
+          if (w[q] > 0 && slot[q] == in) {
+            at[q] = (int)atomicAdd(&sh.slots.members, 1u);
+            if (at[q] < kPairs) { sh.slots.order[at[q]] = order[q]; sh.slots.weight[at[q]] = w[q]; }
+          }
+        }
+        __syncthreads();
+        const int members = (int)sh.slots.members;
+        if (in < 0 || members > kPairs) return -1;
+        const uint64_t base = sh.slots.before;
+#pragma unroll
+        for (int q = 0; q < LPT; ++q)
+          if (at[q] >= 0) {
+            uint64_t sum = base;
+            for (int i = 0; i < members; ++i) sum += sh.slots.order[i] > order[q] ? sh.slots.weight[i] : 0ull;
+            if (sum < target && target <= sum + w[q]) sh.slots.found = tid + q * kThreads;
+          }
+        __syncthreads();
+        return sh.slots.found;
       };
-      // the element at which the sum of the list's amounts, in order, reaches `target`; by the first block, told to all
-      auto in_list = [&](auto amount, uint64_t target) {
+      // the same by sorting (ties may fill a slot); the entries are in descending order afterwards
+      auto locate_sorted = [&](int n, bool weights, int limit, uint64_t target, bool by_index = false) -> int {
+        sort_list(n);
+        uint64_t w[LPT], before[LPT], all;
+#pragma unroll
+        for (int q = 0; q < LPT; ++q) {
+          const uint64_t x = LPT * tid + q < n && LPT * tid + q < limit ? sh.list[LPT * tid + q] : 0;
+          w[q] = x == 0 ? 0 : (weights ? weigh(value_of((uint32_t)(by_index ? x : x >> 32))) : 1);
+        }
+        list_sums(w, before, &all);
+        if (tid == 0) sh.slots.found = -1;
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < LPT; ++q)
+          if (before[q] < target && target <= before[q] + w[q]) sh.slots.found = LPT * tid + q;
+        __syncthreads();
+        return sh.slots.found;
+      };
+      auto slot_by_value = [&](float x, int lo, int hi) {    // of a logit in steps [lo, hi]
+        const float d = x == top ? 0.f : (top - x) * per_step;
+        const float sl = (d - (float)lo) * ((float)kSlots / (float)(hi + 1 - lo));
+        return sl < 0.f ? 0 : (sl < (float)(kSlots - 1) ? (int)sl : kSlots - 1);
+      };
+      // the element at which the sum of the list's counts (or weights), in order, reaches `target`; by the first block, told to all
+      auto in_list = [&](bool weights, int lo, int hi, uint64_t target) {
         if (me == 0) {
           const int n = (int)min(sh.listed, (uint32_t)kList);
-          sort_list(n);
-          uint64_t w[LPT], before[LPT], all;
-#pragma unroll
-          for (int q = 0; q < LPT; ++q) w[q] = LPT * tid + q < n ? amount(list_value(LPT * tid + q)) : 0;
-          list_sums(w, before, &all);
+          int slot[LPT];
+          uint64_t order[LPT], w[LPT];
 #pragma unroll
           for (int q = 0; q < LPT; ++q) {
-            const int i = LPT * tid + q;
-            if (i < n && before[q] < target && target <= before[q] + w[q])
-              for (uint32_t c = 0; c < C; ++c) { put32(&sh.answer[2], c, (uint32_t)(sh.list[i] >> 32)); put32(&sh.answer[3], c, (uint32_t)(V - 1 - (int)(uint32_t)sh.list[i])); }
+            const int i = tid + q * kThreads;
+            order[q] = i < n ? sh.list[i] : 0;
+            const float x = value_of((uint32_t)(order[q] >> 32));
+            w[q] = i < n ? (weights ? weigh(x) : 1) : 0;
+            slot[q] = i < n ? slot_by_value(x, lo, hi) : 0;
+          }
+          int at = locate(n, slot, order, w, target);
+          if (at < 0) at = locate_sorted(n, weights, n, target);
+          if (tid < (int)C && at >= 0) {
+            const uint64_t x = sh.list[at];
+            put32(&sh.answer[2], (uint32_t)tid, (uint32_t)(x >> 32)); put32(&sh.answer[3], (uint32_t)tid, (uint32_t)(V - 1 - (int)(uint32_t)x));
           }
         }
         cluster_sync_all();
@@ -808,78 +911,98 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if (me == 0 && k_upto <= kPairs) {
           // every entry looks at all others: its rank and the sum in front of it, then the sum up to it by index
           const int n = k_upto;
-          uint64_t x = 0, w = 0;
-          static_assert(kPairs == 128, "barriers");
-          auto some_sum = [&](uint64_t v) {      // over the first four warps
-            v = warp_sum(v);
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (lane == 0) sh.red[warp] = v;
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            return warp_sum(lane < kPairs / 32 ? sh.red[lane] : (uint64_t)0);
-          };
-          if (warp < kPairs / 32) {
-            if (tid < n) {
-              x = sh.list[tid];
-              w = weigh(value_of((uint32_t)(x >> 32)));
-              sh.weight[tid] = w;
-            }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            uint32_t rank = 0;
-            uint64_t before_w = 0, Zk = 0;
-            auto rank_of = [&](int i) {          // (every entry's rank is needed for the sum of the first k)
-              const uint64_t y = sh.list[i];
-              if (y > x) { ++rank; before_w += sh.weight[i]; }
-            };
+          uint64_t x = 0, w = 0, before_w = 0;
+          uint32_t rank = 0;
+          if (tid < n) {
+            x = sh.list[tid];
+            w = weigh(value_of((uint32_t)(x >> 32)));
+            sh.slots.weight[tid] = w;
+          }
+          __syncthreads();
+          if (tid < n)
 #pragma unroll 4
-            for (int i = 0; i < n; ++i) rank_of(i);
-            const bool in_k = tid < n && rank < want;
-            Zk = some_sum(in_k ? w : 0);
-            const uint64_t target = nucleus(Zk);
-            const bool stay = in_k && w > 0 && before_w < target && enough(value_of((uint32_t)(x >> 32)));
-            if (tid < n) sh.weight[tid] = stay ? w : 0;
-            const uint64_t Z = some_sum(stay ? w : 0), t = place(Z);
+            for (int i = 0; i < n; ++i)
+              if (sh.list[i] > x) { ++rank; before_w += sh.slots.weight[i]; }
+          const bool in_k = tid < n && rank < want;
+          const uint64_t target = nucleus(block_sum(in_k ? w : 0));
+          const bool stay = in_k && w > 0 && before_w < target && enough(value_of((uint32_t)(x >> 32)));
+          if (tid < n) sh.slots.weight[tid] = stay ? w : 0;
+          const uint64_t t = place(block_sum(stay ? w : 0));
+          if (stay) {
             uint64_t run = 0;
 #pragma unroll 4
-            for (int i = 0; i < n; ++i) run += (uint32_t)sh.list[i] > (uint32_t)x ? sh.weight[i] : 0ull;
-            if (stay && run <= t && t < run + w) answer((uint32_t)(V - 1 - (int)(uint32_t)x));
+            for (int i = 0; i < n; ++i) run += (uint32_t)sh.list[i] > (uint32_t)x ? sh.slots.weight[i] : 0ull;
+            if (run <= t && t < run + w)
+              for (uint32_t c = 0; c < C; ++c) put32(&sh.answer[0], c, (uint32_t)(V - 1 - (int)(uint32_t)x));
           }
         } else if (me == 0) {
           const int n = k_upto;
-          sort_list(n);
-          uint64_t w[LPT], before[LPT], Z;
+          int slot[LPT], at = 0;
+          uint64_t order[LPT], w[LPT], zero[LPT], mine = 0;
+          Border kb = {0u, V - 1};               // of top-k
+          auto fill = [&]() {
 #pragma unroll
-          for (int q = 0; q < LPT; ++q) w[q] = LPT * tid + q < n && (uint32_t)(LPT * tid + q) < want ? weigh(list_value(LPT * tid + q)) : 0;
-          list_sums(w, before, &Z);
-          const uint64_t target = nucleus(Z);
-          // what stays is a first part of the order: how long, and back by index
-          int stay = 0;
+            for (int q = 0; q < LPT; ++q) {
+              const int i = tid + q * kThreads;
+              order[q] = i < n ? sh.list[i] : 0;
+              const float x = value_of((uint32_t)(order[q] >> 32));
+              slot[q] = i < n ? slot_by_value(x, 0, k_bin) : 0;
+              zero[q] = i < n;
+              w[q] = i < n ? weigh(x) : 0;
+            }
+          };
+          fill();
+          // Where each border lies: the entry itself, so that an entry stays where its order is not below it.
+          uint64_t last = 0;
+          if (want < (uint32_t)n) {
+            at = locate(n, slot, order, zero, (uint64_t)want);
+            if (at < 0) { at = locate_sorted(n, false, n, (uint64_t)want); fill(); }
+            last = sh.list[at];
+          }
+#pragma unroll
+          for (int q = 0; q < LPT; ++q) { w[q] = order[q] >= last ? w[q] : 0; mine += w[q]; }
+          if (by_p) {
+            const uint64_t target = nucleus(block_sum(mine));
+            __syncthreads();
+            at = locate(n, slot, order, w, target);
+            if (at < 0) {
+              at = locate_sorted(n, true, (int)want, target);
+              fill();
+#pragma unroll
+              for (int q = 0; q < LPT; ++q) w[q] = order[q] >= last ? w[q] : 0;
+            }
+            last = at >= 0 ? sh.list[at] : last;             // (what has no weight may lie behind)
+          }
+          mine = 0;
 #pragma unroll
           for (int q = 0; q < LPT; ++q) {
-            const int i = LPT * tid + q;
-            if (w[q] > 0 && before[q] < target && enough(list_value(i))) stay = i + 1;
+            const int i = tid + q * kThreads;
+            if (w[q] > 0 && (order[q] < last || !enough(value_of((uint32_t)(order[q] >> 32))))) w[q] = 0;
+            slot[q] = i < n ? (int)((uint64_t)(uint32_t)(V - 1 - (int)(uint32_t)order[q]) * kSlots / (uint32_t)V) : 0;
+            order[q] = (uint64_t)(uint32_t)order[q];         // by index from here on
+            mine += w[q];
           }
-          stay = __reduce_max_sync(0xffffffffu, stay);
+          const uint64_t t = place(block_sum(mine));
           __syncthreads();
-          if (lane == 0) sh.red[warp] = (uint64_t)stay;
-          __syncthreads();
+          at = locate(n, slot, order, w, t + 1);
+          uint32_t back = at >= 0 ? (uint32_t)sh.list[at] : 0u;               // V - 1 - index
+          if (at < 0) {                          // (too many neighbours in a 1024th of the row: sorted by index)
+            __syncthreads();
+            uint64_t turned[LPT];
 #pragma unroll
-          for (int x = 0; x < kWarps; ++x) stay = max(stay, (int)sh.red[x]);
-          uint64_t turned[LPT];
+            for (int q = 0; q < LPT; ++q) {
+              const int i = tid + q * kThreads;
+              turned[q] = i < n && w[q] > 0 ? sh.list[i] << 32 | sh.list[i] >> 32 : 0;
+            }
+            __syncthreads();
 #pragma unroll
-          for (int q = 0; q < LPT; ++q) turned[q] = LPT * tid + q < stay ? sh.list[LPT * tid + q] : 0;
-          __syncthreads();
-#pragma unroll
-          for (int q = 0; q < LPT; ++q)
-            if (LPT * tid + q < stay) sh.list[LPT * tid + q] = turned[q] << 32 | turned[q] >> 32;      // V - 1 - index, pattern
-          __syncthreads();
-          sort_list(stay);
-#pragma unroll
-          for (int q = 0; q < LPT; ++q) w[q] = LPT * tid + q < stay ? weigh(value_of((uint32_t)sh.list[LPT * tid + q])) : 0;
-          list_sums(w, before, &Z);
-          const uint64_t t = place(Z);
-#pragma unroll
-          for (int q = 0; q < LPT; ++q)
-            if (before[q] <= t && t < before[q] + w[q]) answer((uint32_t)(V - 1 - (int)(uint32_t)(sh.list[LPT * tid + q] >> 32)));
+            for (int q = 0; q < LPT; ++q)
+              if (tid + q * kThreads < n) sh.list[tid + q * kThreads] = turned[q];
+            __syncthreads();
+            at = locate_sorted(n, true, n, t + 1, true);
+            back = at >= 0 ? (uint32_t)(sh.list[at] >> 32) : 0u;
+          }
+          if (tid < (int)C) put32(&sh.answer[0], (uint32_t)tid, (uint32_t)(V - 1 - (int)back));
         }
         cluster_sync_all();
         token = sh.answer[0];
@@ -887,9 +1010,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if (cut) {
           if (k_upto - k_before <= kList) {
             into_list(k_bin, k_bin);
-            in_list([](float) { return (uint64_t)1; }, (uint64_t)(want - (uint32_t)k_before));
+            in_list(false, k_bin, k_bin, (uint64_t)(want - (uint32_t)k_before));
             b = {(uint32_t)sh.answer[2], sh.answer[3]};
-          } else b = border([](float) { return (uint64_t)1; }, (uint64_t)want, b);
+          } else b = border(false, (uint64_t)want, b);
         }
         if (by_p) {
           // where it should lie by the steps' mean weights
@@ -909,34 +1032,41 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           }
           __syncthreads();
           if (lane == 31) sh.red_d[warp] = upto_d;
-          if (tid == 0) sh.answer[0] = k_bin;
+          if (tid == 0) { sh.answer[0] = k_bin; sh.range[0] = sh.range[2] = -1; }
           __syncthreads();
           double run = upto_d - sum, all = 0.0;
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) { if (w < warp) run += sh.red_d[w]; all += sh.red_d[w]; }
-          const double t = (double)p * all;
+          // a step's weights are within 2^-8 of their middle: the border is sought as far on both sides, where the list has room for that (it has where
+          // few heavy logits make the mean a poor one), else in three steps
+          const double t = (double)p * all, t_lo = t * 0.995, t_hi = fmin(t * 1.005, all);
 #pragma unroll
           for (int i = 0; i < PER; ++i) {
+            const uint32_t upto_n = before;
+            before += cnt[i];
             if (run < t && t <= run + est[i]) sh.answer[0] = tid * PER + i;
+            if (run < t_lo && t_lo <= run + est[i]) { sh.range[0] = tid * PER + i; sh.range[1] = (int)upto_n; }
+            if (run < t_hi && t_hi <= run + est[i]) { sh.range[2] = tid * PER + i; sh.range[3] = (int)before; }
             run += est[i];
           }
           __syncthreads();
-          const int first_bin = sh.answer[0] > 0 ? sh.answer[0] - 1 : 0, last_bin = sh.answer[0] + 1 < kBins ? sh.answer[0] + 1 : kBins - 1;
-          int list_n = 0;
-          for (int i = first_bin; i <= last_bin; ++i) list_n += (int)sh.merged[i];
+          const bool wide = sh.range[0] >= 0 && sh.range[2] >= 0 && sh.range[3] - sh.range[1] <= kList * 3 / 4;
+          const int from_bin = wide ? sh.range[0] : sh.answer[0], to_bin = wide ? sh.range[2] : sh.answer[0];
+          const int first_bin = from_bin > 0 ? from_bin - 1 : 0, last_bin = to_bin + 1 < kBins ? to_bin + 1 : kBins - 1;
+          int list_n = wide ? sh.range[3] - sh.range[1] + (int)sh.merged[first_bin] + (int)sh.merged[last_bin] : 0;
+          if (!wide)
+            for (int i = first_bin; i <= last_bin; ++i) list_n += (int)sh.merged[i];
           // the sums above, in and below these steps, and the list, in one pass
           uint64_t s_above = 0, s_list = 0, s_rest = 0;
           bool by_list = list_n <= kList;
           each([&](float x, int i) {
-            if (cut && !stays(b, x, i)) return;
             const int bin = bin_of(x);
             const uint64_t w = weigh(x);
-            if (bin < first_bin) s_above += w;
-            else if (bin > last_bin) s_rest += w;
-            else {
-              s_list += w;
-              if (by_list) enlist(x, i);
-            }
+            const bool in = !cut || stays(b, x, i), mine = in && bin >= first_bin && bin <= last_bin;
+            s_above += in && bin < first_bin ? w : 0;
+            s_list += mine ? w : 0;
+            s_rest += in && bin > last_bin ? w : 0;
+            if (mine && by_list) enlist(x, i);
           });
           if (by_list) deliver();
           const uint64_t above = total(s_above), inside = total(s_list), whole = above + inside + total(s_rest);
@@ -944,31 +1074,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           target = target > whole ? whole : target;
           by_list = by_list && above < target && target <= above + inside;
           if (by_list) {
-            in_list(weigh, target - above);
+            in_list(true, first_bin, last_bin, target - above);
             b = {(uint32_t)sh.answer[2], sh.answer[3]};
-          } else b = border(weigh, target, b);
+          } else b = border(true, target, b);
         }
       }
     }
     // (at temperatures like these -200 / c, which stands in for all that lies further down, weighs 0 and is itself exact enough)
     if (token < 0 && !once && top < INFINITY && temp >= 1e-6f && temp <= 1e6f) token = find_fast([&](float x, int i) { return !(by_k || by_p) || stays(b, x, i); });
-    auto target = [&](uint64_t whole) {
-      const uint64_t t = u > 0.f ? (u < 1.f ? (uint64_t)((double)u * (double)whole) : whole) : 0;
-      return t < whole ? t : whole - 1;
-    };
-    if (token < 0 && once) token = find([&](float x, int) { return weigh(x); }, target);
-    if (token < 0) token = find([&](float x, int i) { return stays(b, x, i) && enough(x) ? weigh(x) : (uint64_t)0; }, target);
+    const What all = {true, !(by_k || by_p), least > 0.f, false, 0u, b};
+    if (token < 0) token = once ? find(std::true_type{}, all, -1) : find(std::false_type{}, all, -1);
   }
-  if (a.logprobs && me == 0 && tid == 0) {
+  if (a.logprobs && me == 0 && tid == kThreads - 1) {
     float y = 0.f;
     if (!nothing) {
-      double all = 0.0;
-      for (uint32_t c = 0; c < C; ++c) {
-        const double ref = sh.part_top[c];
-        if (ref > -INFINITY) all += ref == top64 ? sh.part[c] : sh.part[c] * exp(ref - top64);
-      }
       const float x = clean(IO<T>::load((const char*)a.logits + (int64_t)row_no * a.row_bytes, token));
-      y = (float)((x == top ? 0.0 : (double)x - top64) - log(all));
+      y = (float)((x == top ? 0.0 : (double)x - top64) - log_whole);
     }
     a.logprobs[row_no] = y;
   }
