@@ -5,7 +5,7 @@
 // nodes before it on its line (with a window those at positions > p(t) - window or < sinks).
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c s_j - r),  s = q . k, c = scale * log2(e), r a running reference of the row.
 //
-// A tile is N (16, 32 or 64) query rows of one cache head: nodes times the heads of its group, node after node, so that a tree with few nodes
+// A tile is N (16, 32, 64 or 128) query rows of one cache head: nodes times the heads of its group, node after node, so that a tree with few nodes
 // fills few tiles.  The products are transposed, S^T = K Q^T and O^T = V^T P^T: the 128 tokens of a block are the rows (lanes), the queries the
 // columns, so that a product takes time in proportion to N, a thread of the softmax has one token, and what belongs to a token is a
 // register of its thread:
@@ -48,22 +48,25 @@ template <int BITS, int D, int N> struct Shape {
   static constexpr int WGS = N / NC, SW = 4 * WGS;           // groups of four softmax warps
   static constexpr int KW = QUANT ? 4 : 0;                   // warps that read keys
   static constexpr int V_AT = SW + KW, MMA_AT = V_AT + 4, COPY_AT = MMA_AT + 1;   // first warp of the values, of the products, of the copies
-  static constexpr bool SPLIT = QUANT && WGS == 2;           // registers dealt out by role
-  static constexpr int THREADS = SPLIT ? 640 : (COPY_AT + 1) * 32;
+  // registers dealt out by role, where the warps' even share is too little for the softmax; the warps fill up groups of four then
+  static constexpr bool SPLIT = WGS == 4 || (QUANT && WGS == 2);
+  static constexpr int THREADS = (SPLIT ? (COPY_AT + 4) / 4 * 4 : COPY_AT + 1) * 32;
+  static constexpr int R_SOFT = WGS == 4 ? (QUANT ? 88 : 96) : 128, R_READ = WGS == 4 ? 56 : 80, R_MISC = WGS == 4 ? 40 : 64;
   static constexpr int TILE = kBlk * 128 * HALVES;           // a block's keys or values as an operand
   static constexpr int SB = kBlk * G * 2;                    // bytes of a block's scales (or biases)
   static constexpr int VT = 2;                               // places for values as operands
-  static constexpr int PS = D == 128 && (BITS == 8 || (BITS == 16 && N == 64)) ? 1 : 2;   // places for P
-  static constexpr int PTILE = kBlk * 128;
+  static constexpr int PS = N == 128 || (D == 128 && (BITS == 8 || (BITS == 16 && N == 64))) ? 1 : 2;   // places for P
+  static constexpr int PTILE = kBlk * 128 * (N > 64 ? 2 : 1);
   // the rings: codes with scales and biases (the keys' with the values' too, for their units), or at 16 bits the operands themselves
-  static constexpr int KS = BITS == 4 ? 4 : (BITS == 8 ? 3 : (D == 64 ? 4 : 2)), VS = BITS == 4 ? 4 : (BITS == 8 ? 3 : (D == 64 ? 4 : 3));
+  static constexpr int KS = BITS == 4 ? 4 : (BITS == 8 ? (N == 128 && D == 128 ? 2 : 3) : (D == 64 ? 4 : 2)), VS = BITS == 4 ? 4 : (BITS == 8 ? (N == 128 && D == 128 ? 2 : 3) : (D == 64 ? 4 : (N == 128 ? 2 : 3)));
   static constexpr int K_STAGE = QUANT ? kBlk * ROWB + 4 * SB : TILE, V_STAGE = QUANT ? kBlk * ROWB + 2 * SB : TILE;
   static constexpr int V0 = 0, Q0 = QUANT ? VT * TILE : 0, P0 = Q0 + N * 128 * HALVES, KR = P0 + PS * PTILE, VR = KR + KS * K_STAGE;
   static constexpr int SMEM = VR + VS * V_STAGE + (QUANT || D == 128 ? 0 : TILE) + 1024;   // (a product of 128 rows reads a tile past the last one of 64)
   static constexpr int ATOM = QUANT && ROWB < 128 ? 512 : 1024;
   static_assert(KR % 1024 == 0 && K_STAGE % ATOM == 0 && V_STAGE % ATOM == 0, "places of boxes");
-  static_assert(SMEM + 2 * (kMaxPageSeqs + 1) * 4 + 11 * 1024 <= 227 * 1024, "shared memory");
-  static constexpr uint32_t S_AT = 0, O_AT = 128, K_AT = 192;   // columns of tensor memory: two of S, O, two of K
+  static_assert(SMEM + 2 * (kMaxPageSeqs + 1) * 4 + 13 * 1024 <= 227 * 1024, "shared memory");
+  static constexpr uint32_t SW_AT = N > 64 ? 128 : 64, S_AT = 0, O_AT = 2 * SW_AT, K_AT = 3 * SW_AT;   // columns of tensor memory: two of S, O, two of K
+  static_assert(K_AT + (QUANT ? 128 : 0) <= 512, "tensor memory");
 };
 
 // A pool's codes (or rows) as boxes of up to 128 tokens of one head in one page, and what a box takes along head and page (0: broadcast).
@@ -378,7 +381,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
 
   if (warp >= SW && warp < SH::MMA_AT) {
     // ---------------- keys, values ----------------
-    if constexpr (SH::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if constexpr (SH::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::R_READ));
     const bool V = warp >= SH::V_AT;
     const int wq = warp & 3, key = 32 * wq + lane;             // quarter of the block: 32 tokens, one a lane
     uint64_t* const full = V ? v_full : k_full;
@@ -502,7 +505,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
     }
   } else if (warp == SH::COPY_AT) {
     // ---------------- copies: a lane a piece of a block ----------------
-    if constexpr (SH::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if constexpr (SH::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::R_MISC));
     const int pieces_of = kBlk / maps.piece, groups = maps.piece / 16;
     int ks = 0, vs = 0;
     uint32_t kr = 0, vr = 0;
@@ -568,7 +571,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
       for (int i = 0; i < 1000; ++i) __nanosleep(1000);        // (copies may still be on their way)
   } else if (warp == SH::MMA_AT) {
     // ---------------- products ----------------
-    if constexpr (SH::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if constexpr (SH::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::R_MISC));
     constexpr uint32_t type = QUANT ? 0u : 1u;                 // fp16, bf16
     constexpr uint32_t idesc0 = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(N >> 3) << 17) | ((128u >> 4) << 24);
     constexpr uint32_t idesc_s = idesc0, idesc_o = idesc0 | (1u << 15) | (1u << 16);   // the values and P: columns contiguous
@@ -591,8 +594,8 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint64_t q = hi_k | (q_d + (k >> 2) * ((N * 128) >> 4) + (k & 3) * 2);
-          if constexpr (QUANT) umma_ts(tm + SH::S_AT + (J & 1) * 64, tm + SH::K_AT + (J & 1) * 64 + k * 8, q, idesc_s, k > 0);
-          else umma_ss(tm + SH::S_AT + (J & 1) * 64, hi_k | (k_d + ks * (SH::TILE >> 4) + (k >> 2) * ((kBlk * 128) >> 4) + (k & 3) * 2), q, idesc_s, k > 0);
+          if constexpr (QUANT) umma_ts(tm + SH::S_AT + (J & 1) * SH::SW_AT, tm + SH::K_AT + (J & 1) * 64 + k * 8, q, idesc_s, k > 0);
+          else umma_ss(tm + SH::S_AT + (J & 1) * SH::SW_AT, hi_k | (k_d + ks * (SH::TILE >> 4) + (k >> 2) * ((kBlk * 128) >> 4) + (k & 3) * 2), q, idesc_s, k > 0);
         }
         commit(&s_ready[J & 1]);
         if (!QUANT) commit(&k_empty[ks]);
@@ -631,7 +634,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
       for (int i = 0; i < 1000; ++i) __nanosleep(1000);        // (products may still be on their way)
   } else if (warp < SW) {
     // ---------------- softmax: a thread a token ----------------
-    if constexpr (SH::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+    if constexpr (SH::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH::R_SOFT));
     const int wg = warp >> 2, wq = warp & 3, key = tid & 127, col0 = wg * NC;
     const uint32_t lanes = tmem + ((uint32_t)wq << 21);
     constexpr int ALL = SW * 32;
@@ -655,7 +658,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
         }
         if (a.scale < 0.f) { raw[i][0] ^= 0x80008000u; raw[i][1] ^= 0x80008000u; }   // so that the largest score is the largest sum
       }
-      if (piece_no > 0) bar_sync(5, ALL);                      // (all are done with the last tile's lists)
+      if (piece_no > 0) bar_sync(1 + 2 * SH::WGS, ALL);                      // (all are done with the last tile's lists)
       if (tid < kMaxNodes && tid < s.n) {
         const int p = t.parents[(int64_t)pc.b * t.par_str + tid];
         s_par[tid] = p >= 0 && p < tid ? p : -1;
@@ -676,7 +679,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
           if (lane % LPR == 0) s_qe[(i * SW + warp) * RPW + lane / LPR] = mx > 0.f ? (e < -100 ? -100 : (e > 110 ? 110 : e)) : -1000;
         }
       }
-      bar_sync(5, ALL);
+      bar_sync(1 + 2 * SH::WGS, ALL);
       if (tid < s.n && tid < kMaxNodes) {
         uint64_t line = 0;
         int depth = -1;
@@ -711,7 +714,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
         *(uint2*)(smem + SH::Q0 + (d >> 6) * (N * 128) + n * 128 + ((c ^ (n & 7)) << 4) + (l & 1) * 8) = make_uint2(w0, w1);
       }
       fence_async();
-      bar_sync(5, ALL);
+      bar_sync(1 + 2 * SH::WGS, ALL);
       if (lane == 0) mbar_arrive(&q_ready);
       if (tid < N) {
         const int R = pc.rt * N + tid, node = R < live ? R / a.gqa : -1;
@@ -719,7 +722,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
         s_clo[tid] = node >= 0 ? s.base + s_depth[node] - a.window : 0;
       }
       if (tid == 0) note_count[(piece_no + 3) & 3] = 0;        // (read before, and not yet used again: the other roles are two blocks ahead at most)
-      bar_sync(5, ALL);
+      bar_sync(1 + 2 * SH::WGS, ALL);
       const float Cq = QUANT ? factor * pow2i(emax - 14) : factor;
 
       uint64_t l2[NC / 2];
@@ -739,7 +742,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
           w = pow2i(-e);
         }
         const bool masked = s_pages[J & 15] != 0xffu || !pc.whole(t, k0);
-        const uint32_t s_at = lanes + SH::S_AT + (J & 1) * 64 + col0;
+        const uint32_t s_at = lanes + SH::S_AT + (J & 1) * SH::SW_AT + col0;
         uint32_t z[NC];
         auto exponents = [&](bool with_reference) {            // of P' (or, without the reference, of P' 2^r)
           tmem_get<NC>(s_at, z);
@@ -793,7 +796,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
             }
           if constexpr (NC == 16) v[0] = fmaxf(v[0], __shfl_xor_sync(0xffffffffu, v[0], 16));
           if (lane < NC) s_wmax[wg][wq][lane] = v[0];
-          bar_sync(3 + wg, 128);
+          bar_sync(1 + SH::WGS + wg, 128);
           float f = 1.f, nr = 0.f;
           if (lane < NC) {
             nr = s_nr[col0 + lane];
@@ -803,7 +806,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
               nr = kAim - top;
             }
           }
-          bar_sync(3 + wg, 128);                               // (all have read the old ones)
+          bar_sync(1 + SH::WGS + wg, 128);                               // (all have read the old ones)
           if (wq == 0 && lane < NC) s_nr[col0 + lane] = nr;
           if (j > 0) {
             wait(&o_done[(J - 1) & 1], (uint32_t)((J - 1) >> 1), 610);
@@ -816,7 +819,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
 #pragma unroll
             for (int i = 0; i < NC / 2; ++i) l2[i] = mul2(l2[i], two(__shfl_sync(0xffffffffu, f, 2 * i), __shfl_sync(0xffffffffu, f, 2 * i + 1)));
           }
-          bar_sync(3 + wg, 128);
+          bar_sync(1 + SH::WGS + wg, 128);
           exponents(true);
         }
         uint32_t p[NC / 2];
@@ -828,10 +831,10 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
           else { l2[i] = add2(l2[i], two(x0, x1)); p[i] = pack2(x0, x1); }
         }
         if (J >= SH::PS) wait(&o_done[(J - SH::PS) & 1], (uint32_t)((J - SH::PS) >> 1), 611);
-        unsigned char* const prow = smem + SH::P0 + (J % SH::PS) * SH::PTILE + key * 128;
+        unsigned char* const prow = smem + SH::P0 + (J % SH::PS) * SH::PTILE + (col0 >> 6) * (kBlk * 128) + key * 128;
 #pragma unroll
         for (int c = 0; c < NC / 8; ++c)
-          *(uint4*)(prow + (((col0 / 8 + c) ^ (key & 7)) << 4)) = make_uint4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
+          *(uint4*)(prow + ((((col0 & 63) / 8 + c) ^ (key & 7)) << 4)) = make_uint4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
         fence_async();
         fence_before();
         __syncwarp();
@@ -857,7 +860,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
       uint32_t o[NC];
       tmem_get<NC>(lanes + SH::O_AT + col0, o);
       fence_before();
-      bar_sync(3 + wg, 128);
+      bar_sync(1 + SH::WGS + wg, 128);
       float L = 0.f, r = 0.f;
       if (lane < NC) {
         L = (s_wmax[wg][0][lane] + s_wmax[wg][1][lane]) + (s_wmax[wg][2][lane] + s_wmax[wg][3][lane]);
@@ -903,7 +906,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
       }
     }
   }
-  else if constexpr (SH::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");   // (two warps without a role complete the group of four)
+  else if constexpr (SH::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::R_MISC));   // (two warps without a role complete the group of four)
   __syncwarp();
   fence_before();
   __syncthreads();
@@ -983,8 +986,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const __grid
   }
 }
 
-// Columns of a tile: as many as the widest tree has rows of a cache head, up to 64.
-int columns(int64_t T, int64_t gqa) { return T * gqa <= 16 ? 16 : (T * gqa <= 32 ? 32 : 64); }
+// Columns of a tile: as many as the widest tree has rows of a cache head, up to 128.
+int columns(int64_t T, int64_t gqa) { return T * gqa <= 16 ? 16 : (T * gqa <= 32 ? 32 : (T * gqa <= 64 ? 64 : 128)); }
 
 // [pages, heads, page, cols] as boxes of `piece` tokens; axes that repeat one entry as one entry at coordinate 0.
 template <int BITS, int D> bool pool_map(CUtensorMap* m, const KvPagesAttnArgs& a, int side, int piece, int* mul) {
@@ -1031,7 +1034,8 @@ template <int BITS, int D> cudaError_t launch_d(const KvPagesTreeArgs& t, cudaSt
   switch (columns(t.T, t.a.gqa)) {
     case 16: return launch_n<BITS, D, 16>(t, st);
     case 32: return launch_n<BITS, D, 32>(t, st);
-    default: return launch_n<BITS, D, 64>(t, st);
+    case 64: return launch_n<BITS, D, 64>(t, st);
+    default: return launch_n<BITS, D, 128>(t, st);
   }
 }
 }  // namespace
