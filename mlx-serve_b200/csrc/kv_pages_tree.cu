@@ -47,10 +47,10 @@ template <int BITS, int D, int N> struct Shape {
   static constexpr int NC = N < 32 ? N : 32;                 // columns of a softmax warp
   static constexpr int WGS = N / NC, SW = 4 * WGS;           // groups of four softmax warps
   static constexpr int KW = QUANT ? 4 : 0;                   // warps that read keys
-  static constexpr int V_AT = SW + KW, MMA_AT = V_AT + 4, COPY_AT = MMA_AT + 1;   // first warp of the values, of the products, of the copies
+  static constexpr int V_AT = SW + KW, MMA_AT = V_AT + 4, COPY_AT = MMA_AT + 1;   // first warp of the values, of the products, of the copies (keys, values)
   // registers dealt out by role, where the warps' even share is too little for the softmax; the warps fill up groups of four then
   static constexpr bool SPLIT = WGS == 4 || (QUANT && WGS == 2);
-  static constexpr int THREADS = (SPLIT ? (COPY_AT + 4) / 4 * 4 : COPY_AT + 1) * 32;
+  static constexpr int THREADS = (SPLIT ? (COPY_AT + 5) / 4 * 4 : COPY_AT + 2) * 32;
   static constexpr int R_SOFT = WGS == 4 ? (QUANT ? 88 : 96) : 128, R_READ = WGS == 4 ? 56 : 80, R_MISC = WGS == 4 ? 40 : 64;
   static constexpr int TILE = kBlk * 128 * HALVES;           // a block's keys or values as an operand
   static constexpr int SB = kBlk * G * 2;                    // bytes of a block's scales (or biases)
@@ -137,6 +137,23 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool arrived(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(done) : "r"(bar), "r"(parity), "r"(kNap) : "memory");
+  return done != 0;
+}
+// The rest of a wait, for a warp whose barrier had not arrived at the first look: kPolls looks, each held by the hardware for kNap ns at most.  A wait
+// that runs out is noted once; the warp then goes on without waiting (on data that is not there yet, within its bounds), so that all warps
+// meet at every barrier and the CTA ends.
+__device__ __forceinline__ void wait_on(uint32_t bar, uint32_t parity, int code, int* fail) {
+  if (*(volatile int*)fail == 0) {
+    for (uint32_t it = 0; it < kPolls; ++it)
+      if (arrived(bar, parity)) return;
+    *(volatile int*)fail = code;
+    atomicCAS(&g_tree_error, 0, code);
+  }
 }
 // A bounded wait that polls without sleeping.
 __device__ __forceinline__ bool spin_cta(uint64_t* bar, uint32_t parity) {
@@ -368,13 +385,9 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
   const uint32_t tmem = tmem_slot;
   Pieces pieces(t, units, tiles, longest, N);
   Piece pc;
-  // A wait that runs out is noted once; the warp then goes on without waiting (on data that is not there yet, within its bounds), so that
-  // all warps meet at every barrier and the CTA ends.
-  bool dead = false;
   auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
-    if (dead) return;
-    dead = !__all_sync(0xffffffffu, wait_cta(bar, phase & 1, kPolls));
-    if (dead && lane == 0 && !s_fail) { s_fail = code; atomicCAS(&g_tree_error, 0, code); }
+    if (__builtin_expect(!arrived(smem_u32(bar), phase & 1), 0)) wait_on(smem_u32(bar), phase & 1, code, &s_fail);
+    __syncwarp();
   };
   const int pmask = (1 << a.page_shift) - 1;
   int J0 = 0;                        // blocks before this piece
@@ -394,12 +407,14 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
     while (pieces.next(pc)) {
 #pragma unroll 1
       for (int j = 0; j < pc.todo; ++j) {
-        const int J = J0 + j, tok = pc.first_token(j) + key;
+        const int J = J0 + j, k0 = pc.first_token(j), tok = k0 + key;
         wait(&full[st], round, 605);
-        const bool mine = pc.some_see(tok) && ((s_pages[J & 15] >> (key >> 4)) & 1u);
         // a value that some nodes see and others do not must not meet their 0 if it is not finite: it is zeroed and noted
-        const bool partly = V && mine && !pc.all_see(t, tok);
-        bool bad = false;
+        bool mine = true, partly = false, bad = false;
+        if (!pc.whole(t, k0) || s_pages[J & 15] != 0xffu) {
+          mine = pc.some_see(tok) && ((s_pages[J & 15] >> (key >> 4)) & 1u);
+          partly = V && mine && !pc.all_see(t, tok);
+        }
         if constexpr (QUANT) {
           const unsigned char* const codes = ring + st * stage_b;
           const unsigned char* const sb = codes + kBlk * SH::ROWB;
@@ -421,14 +436,11 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
             if constexpr (G == 2) x[G - 1] = bf16hi(v);
           };
           auto largest = [&]() {
-            float m = 0.f;
-            bad = false;
+            float m = 0.f;                                     // (what is not finite does not count)
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-              const float x = group_top<BITS>(s[g], b[g]);     // (a NaN where s or b is one or both are infinite)
-              const bool off = !(x < INFINITY) || !(fabsf(s[g]) < INFINITY);
-              bad |= off;
-              m = fmaxf(m, off ? 0.f : x);
+              const float x = group_top<BITS>(s[g], b[g]);
+              m = x < INFINITY ? fmaxf(m, x) : m;
             }
             return m;
           };
@@ -440,6 +452,9 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
           const int e = unit_exp(largest());
           const float up = pow2i(14 - e);
           if (!V) s_kunit[J & 3][key] = pow2i(e - 14);
+          if (partly)
+#pragma unroll
+            for (int g = 0; g < G; ++g) bad |= !(fabsf(s[g]) < INFINITY) || !(group_top<BITS>(s[g], b[g]) < INFINITY);
           const bool drop = partly && bad;
           __half2 s2[G], b2[G];
 #pragma unroll
@@ -503,12 +518,20 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
       J0 += pc.todo;
       ++piece_no;
     }
-  } else if (warp == SH::COPY_AT) {
-    // ---------------- copies: a lane a piece of a block ----------------
+  } else if (warp == SH::COPY_AT || warp == SH::COPY_AT + 1) {
+    // ---------------- copies: keys, values ----------------
+    // (one elected lane issues them all: 16 cycles each, where a lane of its own for every piece takes 70)
     if constexpr (SH::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::R_MISC));
-    const int pieces_of = kBlk / maps.piece, groups = maps.piece / 16;
-    int ks = 0, vs = 0;
-    uint32_t kr = 0, vr = 0;
+    const bool V = warp != SH::COPY_AT;
+    const int pieces_of = kBlk / maps.piece, groups = maps.piece / 16, stages = V ? VS : KS;
+    uint64_t* const full = V ? v_full : k_full;
+    uint64_t* const empty = V ? v_empty : k_empty;
+    const uint32_t ring = smem_u32(smem + (V ? SH::VR : SH::KR)), stage_b = V ? SH::V_STAGE : SH::K_STAGE;
+    const uint32_t codes_b = (uint32_t)maps.piece * SH::ROWB, box_b = QUANT ? codes_b : (uint32_t)maps.piece * 128u, sb_b = (uint32_t)maps.piece * G * 2;
+    const bool vec = QUANT && a.sb_vec;
+    const uint32_t piece_b = codes_b + (vec ? (V ? 2u : 4u) * sb_b : 0u);
+    int st = 0;
+    uint32_t round = 0;
     while (pieces.next(pc)) {
       const int32_t* const tab = a.table + (int64_t)pc.s.row * a.table_str;
       auto page_at = [&](int j) {
@@ -523,51 +546,54 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
       int pid_next = page_at(0);
 #pragma unroll 1
       for (int j = 0; j < pc.todo; ++j) {
-        const int J = J0 + j, pid = pid_next, tok = pc.first_token(j) + lane * maps.piece, row = tok & pmask;
+        const int pid = pid_next, row0 = pc.first_token(j) & pmask;      // (pieces of one page follow each other; else each begins its page)
         pid_next = page_at(j + 1);
         const uint32_t have = __ballot_sync(0xffffffffu, pid >= 0);
-        const int n = __popc(have);
-        uint32_t bits = 0;                                     // of 16 tokens each
-        for (int i = 0; i < pieces_of; ++i)
-          if ((have >> i) & 1u) bits |= ((1u << groups) - 1u) << (i * groups);
-        const uint32_t codes_b = (uint32_t)maps.piece * SH::ROWB, sb_b = (uint32_t)maps.piece * G * 2;
-        auto scales = [&](const KvPoolView& pl, unsigned char* to, uint64_t* bar) {
-          const int64_t at = (int64_t)pid * pl.sb_str[0] + (int64_t)pc.hk * pl.sb_str[1] + (int64_t)row * G;
-          bulk_load(smem_u32(to) + lane * sb_b, (const uint16_t*)pl.s + at, sb_b, bar);
-          bulk_load(smem_u32(to) + SH::SB + lane * sb_b, (const uint16_t*)pl.b + at, sb_b, bar);
-        };
-        const bool vec = QUANT && a.sb_vec;
-        if (kr > 0) wait(&k_empty[ks], kr - 1, 613);
-        unsigned char* const kst = smem + SH::KR + ks * SH::K_STAGE;
+        if (round > 0) wait(&empty[st], round - 1, V ? 614 : 613);
+        const uint32_t to = ring + st * stage_b;
         if (lane == 0) {
-          s_pages[J & 15] = bits;
-          mbar_expect_tx(&k_full[ks], (uint32_t)n * (codes_b + (vec ? 4 * sb_b : 0u)));
+          if (!V) {
+            uint32_t bits = 0xffu;                             // of 16 tokens each
+            if (have != (1u << pieces_of) - 1u) {
+              bits = 0;
+              for (int i = 0; i < pieces_of; ++i)
+                if ((have >> i) & 1u) bits |= ((1u << groups) - 1u) << (i * groups);
+            }
+            s_pages[(J0 + j) & 15] = bits;
+          }
+          mbar_expect_tx(&full[st], (uint32_t)__popc(have) * piece_b);
         }
         __syncwarp();
-        if (pid >= 0) {
+        for (int i = 0; i < pieces_of; ++i) {
+          const int page = __shfl_sync(0xffffffffu, pid, i);
+          if (page < 0) continue;
+          const int row = (row0 + i * maps.piece) & pmask;
+          if (elect_one()) {
 #pragma unroll
-          for (int h = 0; h < (QUANT ? 1 : SH::HALVES); ++h)
-            tma_load_4d(smem_u32(kst) + h * kBlk * 128 + lane * (QUANT ? codes_b : (uint32_t)maps.piece * 128u), &mk, &k_full[ks], 64 * h, row, pc.hk * maps.mul[0][0], pid * maps.mul[0][1]);
-          if (vec) { scales(a.pool[0], kst + kBlk * SH::ROWB, &k_full[ks]); scales(a.pool[1], kst + kBlk * SH::ROWB + 2 * SH::SB, &k_full[ks]); }
+            for (int h = 0; h < (QUANT ? 1 : SH::HALVES); ++h)
+              tma_load_4d(to + h * kBlk * 128 + i * box_b, V ? &mv : &mk, &full[st], 64 * h, row, pc.hk * maps.mul[V][0], page * maps.mul[V][1]);
+            if (vec) {
+              const uint32_t sb = to + kBlk * SH::ROWB + i * sb_b;
+              const int64_t at_v = (int64_t)page * a.pool[1].sb_str[0] + (int64_t)pc.hk * a.pool[1].sb_str[1] + (int64_t)row * G;
+              if (V) {
+                bulk_load(sb, (const uint16_t*)a.pool[1].s + at_v, sb_b, &full[st]);
+                bulk_load(sb + SH::SB, (const uint16_t*)a.pool[1].b + at_v, sb_b, &full[st]);
+              } else {
+                const int64_t at_k = (int64_t)page * a.pool[0].sb_str[0] + (int64_t)pc.hk * a.pool[0].sb_str[1] + (int64_t)row * G;
+                bulk_load(sb, (const uint16_t*)a.pool[0].s + at_k, sb_b, &full[st]);
+                bulk_load(sb + SH::SB, (const uint16_t*)a.pool[0].b + at_k, sb_b, &full[st]);
+                bulk_load(sb + 2 * SH::SB, (const uint16_t*)a.pool[1].s + at_v, sb_b, &full[st]);
+                bulk_load(sb + 3 * SH::SB, (const uint16_t*)a.pool[1].b + at_v, sb_b, &full[st]);
+              }
+            }
+          }
+          __syncwarp();
         }
-        __syncwarp();
-        if (vr > 0) wait(&v_empty[vs], vr - 1, 614);
-        unsigned char* const vst = smem + SH::VR + vs * SH::V_STAGE;
-        if (lane == 0) mbar_expect_tx(&v_full[vs], (uint32_t)n * (codes_b + (vec ? 2 * sb_b : 0u)));
-        __syncwarp();
-        if (pid >= 0) {
-#pragma unroll
-          for (int h = 0; h < (QUANT ? 1 : SH::HALVES); ++h)
-            tma_load_4d(smem_u32(vst) + h * kBlk * 128 + lane * (QUANT ? codes_b : (uint32_t)maps.piece * 128u), &mv, &v_full[vs], 64 * h, row, pc.hk * maps.mul[1][0], pid * maps.mul[1][1]);
-          if (vec) scales(a.pool[1], vst + kBlk * SH::ROWB, &v_full[vs]);
-        }
-        __syncwarp();
-        if (++ks == KS) { ks = 0; ++kr; }
-        if (++vs == VS) { vs = 0; ++vr; }
+        if (++st == stages) { st = 0; ++round; }
       }
       J0 += pc.todo;
     }
-    if (dead)
+    if (*(volatile int*)&s_fail)
       for (int i = 0; i < 1000; ++i) __nanosleep(1000);        // (copies may still be on their way)
   } else if (warp == SH::MMA_AT) {
     // ---------------- products ----------------
@@ -580,9 +606,9 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
     const uint64_t hi_k = make_desc(0) & 0xFFFFFFFF00000000ull, hi_v = make_desc_mn(0) & 0xFFFFFFFF00000000ull;
     const uint32_t q_d = (uint32_t)make_desc(sm + SH::Q0), k_d = (uint32_t)make_desc(sm + SH::KR), v_d = (uint32_t)make_desc_mn(sm + (QUANT ? SH::V0 : SH::VR)), p_d = (uint32_t)make_desc_mn(sm + SH::P0);
     auto spin = [&](uint64_t* bar, uint32_t phase, int code) {
-      if (dead) return;
-      dead = !__all_sync(0xffffffffu, spin_cta(bar, phase & 1));
-      if (dead && lane == 0 && !s_fail) { s_fail = code; atomicCAS(&g_tree_error, 0, code); }
+      if (*(volatile int*)&s_fail) return;
+      if (!__all_sync(0xffffffffu, spin_cta(bar, phase & 1)) && lane == 0) { *(volatile int*)&s_fail = code; atomicCAS(&g_tree_error, 0, code); }
+      __syncwarp();
     };
     int piece_no = 0, ks = 0, vs = 0;                          // (at 16 bits the operands are the rings' places)
     uint32_t kr = 0;
@@ -630,7 +656,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
     }
     // every product is complete before tensor memory and shared memory go
     if (J0 > 0) spin(&o_done[(J0 - 1) & 1], (uint32_t)((J0 - 1) >> 1), 608);
-    if (s_fail)
+    if (*(volatile int*)&s_fail)
       for (int i = 0; i < 1000; ++i) __nanosleep(1000);        // (products may still be on their way)
   } else if (warp < SW) {
     // ---------------- softmax: a thread a token ----------------
@@ -733,7 +759,6 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
         const int J = J0 + j, k0 = pc.first_token(j), tok = k0 + key;
         wait(&s_ready[J & 1], (uint32_t)(J >> 1), 609);
         fence_after();
-        const bool mine = pc.some_see(tok) && ((s_pages[J & 15] >> (key >> 4)) & 1u);
         float ck = Cq, w = 1.f, ev = 0.f;
         if constexpr (QUANT) {
           const int e = s_vexp[J & 3][key];
@@ -766,7 +791,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
             z[4 * i] = __float_as_uint(f0); z[4 * i + 1] = __float_as_uint(f1); z[4 * i + 2] = __float_as_uint(f2); z[4 * i + 3] = __float_as_uint(f3);
           }
           if (masked) {
-            const bool drafted = tok >= s.base;
+            const bool mine = pc.some_see(tok) && ((s_pages[J & 15] >> (key >> 4)) & 1u), drafted = tok >= s.base;
             const int m = drafted ? tok - s.base : 0, at = drafted ? s.base + (mine ? s_depth[m] : 0) : tok;
             const bool inside = a.window == 0 || at < a.sinks;
 #pragma unroll
