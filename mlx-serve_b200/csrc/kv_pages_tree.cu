@@ -14,10 +14,18 @@
 //    row's sum takes P' / unit.  Tokens and groups 2^28 apart in size keep fp16's 11 bits.  At 16 bits the operands are the cache's bf16.
 //  * r moves only where some P' would pass 2^15: then it is placed 2^8 below the block's maximum, and O is rescaled.
 //  * Roles of a CTA's warps: four a 32 columns of the softmax; four read keys and dequantise them into tensor memory (the A operand of S^T); four
-//    read values and dequantise them into shared memory; one issues the products, S^T two blocks ahead of O^T.  A warp's codes come through a cp.async
-//    ring of its own, page numbers a block ahead; at 16 bits the ring's slots are the operands themselves.
+//    read values and dequantise them into shared memory; one issues the products, S^T two blocks ahead of O^T; two issue the copies: codes by
+//    TMA in boxes of up to a page, scales and biases as bulk copies where a page's are one run, into rings of whole blocks.  At 16 bits the
+//    rings' places are the operands themselves.
 //  * The grid is one CTA an SM; every CTA works out all sequences' blocks from `lens` and takes an even share of them, or every tile is cut in the
 //    same number of parts.  Parts of a tile go to the workspace and are joined by a second kernel.
+//
+// Measured: 16 sequences of 32k tokens, 4 bits, 32 query heads over 8, 515 us with 32 nodes (128 rows of a cache head; the codes alone take 101 us at
+// the rate of a copy, the products 45), 382 with 16, 322 with 8, 274 with 4; 4 sequences of 8k, 8 bits, 64 nodes 126 us; 32 sequences of a window of 1024 over
+// bf16 98 us; one of 700 tokens 22.5.  What bounds a long one is neither the bytes (20 to 37 %) nor the products but the work a block of 128 tokens takes,
+// handed from warp to warp: with copies, products and barriers alone 260 us (128 rows) and 177 (16); without the readers' arithmetic 407 and 189,
+// without the softmax's 347 and 231.  Rings by cp.async in every reader took 695 instead of 527 us; two groups of readers that
+// take turns, a sleeping instead of a polling issuer, and operands made uniform for it changed nothing.
 #include <mutex>
 #include <type_traits>
 
@@ -1014,8 +1022,17 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const __grid
   }
 }
 
-// Columns of a tile: as many as the widest tree has rows of a cache head, up to 128.
+// Columns of a tile: as many as the widest tree has rows of a cache head, up to 128.  More than 64 rows take 128 columns where there is much to
+// read (128 rows over 16 sequences of 32k tokens 515 us, as two tiles of 64 723), but 64 where the tables hold at most four blocks an SM, since
+// the wide tile takes longer to begin and to end (135 rows over 3 sequences of 2k tokens 31.9 us, 37.5 with 128; one of 2k with 128 rows 30.9 and 36.5;
+// with seven blocks an SM 36.0 and 34.9).
 int columns(int64_t T, int64_t gqa) { return T * gqa <= 16 ? 16 : (T * gqa <= 32 ? 32 : (T * gqa <= 64 ? 64 : 128)); }
+int columns_of(const KvPagesTreeArgs& t) {
+  const int n = columns(t.T, t.a.gqa);
+  if (n < 128) return n;
+  const int64_t blocks = (((int64_t)t.a.M << t.a.page_shift) + kBlk - 1) / kBlk, tiles = (int64_t)t.a.B * t.a.Hkv * (((int64_t)t.T * t.a.gqa + 63) / 64);
+  return blocks * tiles <= 4 * (int64_t)sm_count() ? 64 : 128;
+}
 
 // [pages, heads, page, cols] as boxes of `piece` tokens; axes that repeat one entry as one entry at coordinate 0.
 template <int BITS, int D> bool pool_map(CUtensorMap* m, const KvPagesAttnArgs& a, int side, int piece, int* mul) {
@@ -1059,7 +1076,7 @@ template <int BITS, int D, int N> cudaError_t launch_n(const KvPagesTreeArgs& t,
   return launch_behind(tree_join_kernel<BITS, D>, dim3(grid, (N + kJoinRows - 1) / kJoinRows), dim3(kJoinWarps * 32), 0, st, t, N);
 }
 template <int BITS, int D> cudaError_t launch_d(const KvPagesTreeArgs& t, cudaStream_t st) {
-  switch (columns(t.T, t.a.gqa)) {
+  switch (columns_of(t)) {
     case 16: return launch_n<BITS, D, 16>(t, st);
     case 32: return launch_n<BITS, D, 32>(t, st);
     case 64: return launch_n<BITS, D, 64>(t, st);
@@ -1075,7 +1092,7 @@ size_t kv_pages_tree_workspace_bytes(int64_t, int64_t Hq, int64_t Hkv, int64_t T
 }
 
 cudaError_t launch_kv_pages_tree(KvPagesTreeArgs t, int D, void* workspace, cudaStream_t st) {
-  const size_t ctas = (size_t)sm_count(), rows = (size_t)columns(t.T, t.a.gqa);
+  const size_t ctas = (size_t)sm_count(), rows = (size_t)columns_of(t);
   t.a.joins = (int4*)workspace;
   t.a.part_ml = (float2*)((char*)workspace + ctas * 16);
   t.a.part_o = (float*)((char*)workspace + ctas * 16 + ctas * 2 * rows * 8);
