@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
   __shared__ int s_fail, s_longest[32], warp_sums[2][32];
   __shared__ __align__(16) float s_nr[N], s_kunit[4][kBlk];     // -r of the columns; of a block's tokens
   __shared__ int s_vexp[4][kBlk];
-  __shared__ uint32_t s_pages[16];       // of a block: which of its 16 tokens have a page
+  __shared__ uint32_t s_pages[2][16];    // of a block, from the keys' and from the values' copies: which of its 16 tokens have a page
   __shared__ float s_wmax[SH::WGS][4][NC];
   __shared__ int s_par[kMaxNodes], s_depth[kMaxNodes], s_clo[N], s_qe[N];
   __shared__ uint64_t s_line[kMaxNodes], s_cline[N];
@@ -419,8 +419,9 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
         wait(&full[st], round, 605);
         // a value that some nodes see and others do not must not meet their 0 if it is not finite: it is zeroed and noted
         bool mine = true, partly = false, bad = false;
-        if (!pc.whole(t, k0) || s_pages[J & 15] != 0xffu) {
-          mine = pc.some_see(tok) && ((s_pages[J & 15] >> (key >> 4)) & 1u);
+        const uint32_t have = s_pages[V][J & 15];              // (their own copies' word: the other's may be ahead or behind)
+        if (!pc.whole(t, k0) || have != 0xffu) {
+          mine = pc.some_see(tok) && ((have >> (key >> 4)) & 1u);
           partly = V && mine && !pc.all_see(t, tok);
         }
         if constexpr (QUANT) {
@@ -452,14 +453,14 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
             }
             return m;
           };
+          int ev = 0;
           if (!V) {
             params(2, s); params(3, b);
-            s_vexp[J & 3][key] = unit_exp(largest()) - 14;
+            ev = unit_exp(largest()) - 14;
           }
           params(0, s); params(1, b);
           const int e = unit_exp(largest());
           const float up = pow2i(14 - e);
-          if (!V) s_kunit[J & 3][key] = pow2i(e - 14);
           if (partly)
 #pragma unroll
             for (int g = 0; g < G; ++g) bad |= !(fabsf(s[g]) < INFINITY) || !(group_top<BITS>(s[g], b[g]) < INFINITY);
@@ -468,6 +469,10 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
 #pragma unroll
           for (int g = 0; g < G; ++g) { s2[g] = __float2half2_rn(drop ? 0.f : s[g] * up); b2[g] = __float2half2_rn(drop ? 0.f : b[g] * up); }
           if (J >= 2) wait((V ? o_done : s_ready) + (J & 1), (uint32_t)((J >> 1) - 1), V ? 602 : 601);
+          if (!V) {                                            // (S two blocks back is complete, so the softmax has left the block four back: its place is free)
+            s_kunit[J & 3][key] = pow2i(e - 14);
+            s_vexp[J & 3][key] = ev;
+          }
           unsigned char* const vrow = smem + SH::V0 + (J & 1) * SH::TILE + key * 128;
           constexpr int CG = CH / G;                           // chunks of a group
           // (Rolled, the code is shorter: 16 sequences of 32k tokens, 64 rows 424 -> 382 us, 16 rows 302 -> 274.  With 128 rows the readers' registers
@@ -531,7 +536,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
     }
   } else if (warp == SH::COPY_AT || warp == SH::COPY_AT + 1) {
     // ---------------- copies: keys, values ----------------
-    // (one elected lane issues them all: 16 cycles each, where a lane of its own for every piece takes 70)
+    // (one elected lane issues them all; a lane of its own for every piece was no faster)
     if constexpr (SH::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::R_MISC));
     const bool V = warp != SH::COPY_AT;
     const int pieces_of = kBlk / maps.piece, groups = maps.piece / 16, stages = V ? VS : KS;
@@ -563,15 +568,13 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
         if (round > 0) wait(&empty[st], round - 1, V ? 614 : 613);
         const uint32_t to = ring + st * stage_b;
         if (lane == 0) {
-          if (!V) {
-            uint32_t bits = 0xffu;                             // of 16 tokens each
-            if (have != (1u << pieces_of) - 1u) {
-              bits = 0;
-              for (int i = 0; i < pieces_of; ++i)
-                if ((have >> i) & 1u) bits |= ((1u << groups) - 1u) << (i * groups);
-            }
-            s_pages[(J0 + j) & 15] = bits;
+          uint32_t bits = 0xffu;                               // of 16 tokens each
+          if (have != (1u << pieces_of) - 1u) {
+            bits = 0;
+            for (int i = 0; i < pieces_of; ++i)
+              if ((have >> i) & 1u) bits |= ((1u << groups) - 1u) << (i * groups);
           }
+          s_pages[V][(J0 + j) & 15] = bits;
           mbar_expect_tx(&full[st], (uint32_t)__popc(have) * piece_b);
         }
         __syncwarp();
@@ -777,7 +780,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
           ev = (float)e;
           w = pow2i(-e);
         }
-        const bool masked = s_pages[J & 15] != 0xffu || !pc.whole(t, k0);
+        const bool masked = s_pages[0][J & 15] != 0xffu || !pc.whole(t, k0);
         const uint32_t s_at = lanes + SH::S_AT + (J & 1) * SH::SW_AT + col0;
         uint32_t z[NC];
         auto exponents = [&](bool with_reference) {            // of P' (or, without the reference, of P' 2^r)
@@ -802,7 +805,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
             z[4 * i] = __float_as_uint(f0); z[4 * i + 1] = __float_as_uint(f1); z[4 * i + 2] = __float_as_uint(f2); z[4 * i + 3] = __float_as_uint(f3);
           }
           if (masked) {
-            const bool mine = pc.some_see(tok) && ((s_pages[J & 15] >> (key >> 4)) & 1u), drafted = tok >= s.base;
+            const bool mine = pc.some_see(tok) && ((s_pages[0][J & 15] >> (key >> 4)) & 1u), drafted = tok >= s.base;
             const int m = drafted ? tok - s.base : 0, at = drafted ? s.base + (mine ? s_depth[m] : 0) : tok;
             const bool inside = a.window == 0 || at < a.sinks;
 #pragma unroll

@@ -52,3 +52,30 @@ def test_one_call_by_both_widths(bits):
         table = make_table(lens, page, M, P)
         o = qb200.kv_pages_tree_attention(q, kp, vp, ints(table), ints(lens), ints(trees), bits, 64, 0.1, counts=ints(counts))
         check(o, q, kp, vp, table, lens, trees, counts, page, bits, 0.1)
+
+
+@pytest.mark.parametrize("bits", [4, 8, 16])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("T,gqa", [(16, 7), (8, 7), (4, 7), (4, 4)])
+def test_units_and_pages_of_long_ragged_batches_do_not_mix(bits, page, T, gqa):
+    """Tokens of very different sizes over many blocks, pages missing here and there: every run gives the same, and the right rows."""
+    torch.manual_seed(9)
+    H, D, B = 2, 128, 9
+    lens = [2500 - 217 * b for b in range(B)]
+    counts = [max(1, T - b) for b in range(B)]
+    P = sum(-(-n // page) for n in lens) + 3
+    pools = []
+    for _ in range(2):
+        x = torch.randn(P, H, page, D, device="cuda") * torch.exp2(torch.randint(-3, 4, (P, H, page, 1), device="cuda").float())
+        pools.append((x.to(BF16), None, None) if bits == 16 else qb200.quantize(x.to(BF16), 64, bits))
+    M = 160 * 1024 // page
+    table = make_table(lens, page, M, P)
+    for b in range(B):
+        table[b][3 * b + 1] = -1
+    trees = [make_tree(n, T, b) for b, n in enumerate(counts)]
+    q = torch.randn(B, H * gqa, T, D, device="cuda").to(BF16)
+    args = (q, *pools, ints(table), ints(lens), ints(trees), bits, 64, 0.02)
+    out = qb200.kv_pages_tree_attention(*args, counts=ints(counts))
+    check(out, q, *pools, table, lens, trees, counts, page, bits, 0.02)
+    for _ in range(20):
+        assert torch.equal(out, qb200.kv_pages_tree_attention(*args, counts=ints(counts)))
