@@ -9,10 +9,17 @@
 //    2^-45 of the largest counts as 0.
 //  * A row is a cluster of up to eight blocks, each with a share of the row in shared memory (read from memory again where it is too
 //    large); sums and histograms meet through distributed shared memory.
-//  * The border of top-k and top-p in the order: a histogram of how far the logits lie below the largest, in steps of 2^-7 of the temperature, says in which step it lies
-//    (top-k exactly; top-p by the steps' mean weights, and the sums of the next pass say whether that was right).  The logits of
-//    these steps go to a list in the first block, where each looks at all others.  Few that stay are drawn from that list alone.  Where the list
+//  * By temperature alone a row is read once, in parts of 512 elements that a warp weighs relative to its own largest logit in 32 bits, with a bound on how far
+//    such a sum may be off; the part where the token lies, and the parts beside it that the bound leaves open, are summed exactly.  Where the bound
+//    leaves too much open, all of the row is.
+//  * The border of top-k and top-p in the order: a histogram of how far the logits lie below the largest, 4096 steps over 32 temperatures, says in which step it
+//    lies (top-k exactly; top-p by the steps' mean weights, and the sums of the next pass say whether that was right).  The logits of
+//    these steps go to a list in the first block, by 1024 slots along the order, and those of one slot look at one another.  Few that stay are drawn from that list alone.  Where the list
 //    would be too long (equal logits, flat rows) the border is found by halving the range of the logits' patterns, a sum over the row each time.
+//
+// Measured: one row of 128256 with top-k 50 and top-p 0.95 18.5 us (meetings of its eight blocks and the work on a list, one after the other); 256 rows of
+// 32001 (fp32) with filters of all kinds 66 us, where reading them once takes 5; 24 rows with a nucleus of flat logits 66; 256 rows of 262144 by temperature alone
+// 109 us, 1.2 TB/s: instructions bound it (30 a warp for 32 logits), not the memory.
 #include <cstddef>
 #include <mutex>
 #include <type_traits>
@@ -809,7 +816,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       };
       // Entry at which the amounts w of the entries [0, n) (LPT a thread, entry tid + q * kThreads), taken by descending `order`, reach `target`; by the first block.  An
       // entry's slot (ascending where `order` descends) says roughly where; 1024 slots are added up, and the entries of the one that matters compared
-      // pair by pair.  -1: none, or too many in one slot.  (Sorting 600 entries by both orders took 42000 cycles, this takes 8000.)
+      // pair by pair.  -1: none, or too many in one slot.  (256 rows with top-k 500 and top-p 0.9: 88 us by
+      // sorting, 62 by slots.)
       auto locate = [&](int n, const int (&slot)[LPT], const uint64_t (&order)[LPT], const uint64_t (&w)[LPT], uint64_t target) -> int {
         uint64_t* const mass = sh.slots.mass;
         for (int i = tid; i < kSlots; i += kThreads) mass[i] = 0;
@@ -1112,10 +1120,11 @@ template <typename T> cudaError_t launch_t(const SampleArgs& a, cudaStream_t st)
       if (dev >= 0 && dev < 64) done[dev] = true;
     }
   }
-  // Blocks a row: enough that there are two for every SM, of at least 8192 elements each.  (What the blocks of a row say to one another takes 0.7 us
-  // each time, so that many rows are better off with a block or two each; one row of 128256 takes 23 us by one, 13 by eight.)
+  // Blocks a row: enough that there is one for every SM (two a row up to two rows an SM), of at least 8192 elements each, and so many that a share stays in
+  // shared memory.  (128256 logits, the 50 largest, by 1, 2, 4, 8 blocks a row: one row 68, 42, 24, 19 us; 64 rows 74, 45, 32, 47; 128 rows -, 57, 62, 90.  256
+  // rows of 32001 with filters of all kinds 78, 66, 87, 151.  A nucleus over flat rows pays for more: 48 rows by 4 blocks 120, by 8 102.)
   int ctas = 1;
-  while (ctas < kMaxCtas && ((int64_t)a.N * ctas < 2 * sm_count() || a.V > ctas * 65536) && a.V > ctas * 8192) ctas *= 2;
+  while (ctas < kMaxCtas && ((int64_t)a.N * ctas < (ctas == 1 ? 2 : 1) * sm_count() || a.V > ctas * 65536) && a.V > ctas * 8192) ctas *= 2;
   for (;; ctas = 1) {
     const int share = ((a.V + ctas - 1) / ctas + 7) / 8 * 8;
     const int need = (share + 16) * (int)sizeof(T);
