@@ -116,5 +116,10 @@ pub extern "c" fn qb200_kv_pages_compact(remap: *Tensor, moves: *Tensor, count: 
 pub extern "c" fn qb200_kv_pages_copy(pools: [*]const *Tensor, num_pools: c_int, pairs: *const Tensor, count: ?*const Tensor, s: Stream) c_int;
 pub extern "c" fn qb200_kv_pages_decode_attention(res: *Tensor, q: *const Tensor, k_q: *const Tensor, k_scales: ?*const Tensor, k_biases: ?*const Tensor, v_q: *const Tensor, v_scales: ?*const Tensor, v_biases: ?*const Tensor, table: *const Tensor, rows: ?*const Tensor, lens: *const Tensor, bits: c_int, group_size: c_int, scale: f32, window: i64, sinks: i64, workspace: ?*anyopaque, workspace_bytes: usize, s: Stream) c_int;
 pub extern "c" fn qb200_kv_pages_decode_attention_workspace_size(B: i64, Hq: i64, Hkv: i64, D: i64) usize;
+pub extern "c" fn qb200_kv_pages_tree_attention(res: *Tensor, q: *const Tensor, k_q: *const Tensor, k_scales: ?*const Tensor, k_biases: ?*const Tensor, v_q: *const Tensor, v_scales: ?*const Tensor, v_biases: ?*const Tensor, table: *const Tensor, rows: ?*const Tensor, lens: *const Tensor, parents: *const Tensor, counts: ?*const Tensor, bits: c_int, group_size: c_int, scale: f32, window: i64, sinks: i64, workspace: ?*anyopaque, workspace_bytes: usize, s: Stream) c_int;
+pub extern "c" fn qb200_kv_pages_tree_attention_workspace_size(B: i64, Hq: i64, Hkv: i64, T: i64, D: i64) usize;
+pub extern "c" fn qb200_kv_pages_accept(path: *Tensor, next: *Tensor, accepted: *Tensor, ends: *Tensor, pools: [*]const *Tensor, num_pools: c_int, table: *const Tensor, lens: *const Tensor, page: c_int, rows: ?*const Tensor, parents: *const Tensor, tokens: *const Tensor, sampled: *const Tensor, counts: ?*const Tensor, s: Stream) c_int;
+// sampleTokenLazy (src/generate.zig:6929) for a batch of rows with parameters of their own
+pub extern "c" fn qb200_sample(tokens: *Tensor, logprobs: ?*Tensor, logits: *const Tensor, random: *const Tensor, temperature: ?*const Tensor, top_k: ?*const Tensor, top_p: ?*const Tensor, min_p: ?*const Tensor, s: Stream) c_int;
 // mlx_fast_scaled_dot_product_attention of a prompt (src/mlx.zig:325) with a sliding window and sinks
 pub extern "c" fn qb200_window_attention(res: *Tensor, q: *const Tensor, k: *const Tensor, v: *const Tensor, scale: f32, window: i64, sinks: i64, kv_lens: ?*const Tensor, s: Stream) c_int;

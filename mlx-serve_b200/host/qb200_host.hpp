@@ -315,6 +315,39 @@ inline void quantAttentionPaged(Array& out, const Array& q, const PagedCache& c,
                                         &c.table.t, rows ? &rows->t : nullptr, &c.lens.t, l.keys.bits, l.keys.group_size, scale, window, sinks, workspace,
                                         workspace_bytes, s));
 }
+// A tree of drafted tokens a sequence, appended behind its cached ones: attention of all nodes, sampling, and what of it stays.
+struct DraftTree {
+  Array parents, tokens;     // [B, T]: int32
+  const Array* counts = nullptr;   // [B]: nodes of each tree (null: T)
+};
+inline size_t quantAttentionTreeWorkspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D) {
+  return qb200_kv_pages_tree_attention_workspace_size(B, Hq, Hkv, T, D);
+}
+inline void quantAttentionTree(Array& out, const Array& q, const PagedCache& c, int layer, const Array* rows, const DraftTree& tree, float scale, int64_t window,
+                               int64_t sinks, void* workspace, size_t workspace_bytes, qb200_stream s) {
+  const PagePool& l = c.layers[(size_t)layer];
+  check(qb200_kv_pages_tree_attention(&out.t, &q.t, &l.keys.q.t, &l.keys.scales.t, &l.keys.biases.t, &l.values.q.t, &l.values.scales.t, &l.values.biases.t,
+                                      &c.table.t, rows ? &rows->t : nullptr, &c.lens.t, &tree.parents.t, tree.counts ? &tree.counts->t : nullptr, l.keys.bits,
+                                      l.keys.group_size, scale, window, sinks, workspace, workspace_bytes, s));
+}
+// sampleTokenLazy (src/generate.zig:6929) for rows with parameters of their own; null parameters: 1, 0, 1, 0.
+inline void sampleTokens(Array& tokens, Array* logprobs, const Array& logits, const Array& random, const Array* temperature, const Array* top_k, const Array* top_p,
+                         const Array* min_p, qb200_stream s) {
+  check(qb200_sample(&tokens.t, logprobs ? &logprobs->t : nullptr, &logits.t, &random.t, temperature ? &temperature->t : nullptr, top_k ? &top_k->t : nullptr,
+                     top_p ? &top_p->t : nullptr, min_p ? &min_p->t : nullptr, s));
+}
+// The nodes that the samples confirm, their rows moved together in every layer, and the other nodes' pages given back.
+inline void pagesAccept(PagedCache& c, Array& path, Array& next, Array& accepted, Array& ends, const DraftTree& tree, const Array& sampled, const Array& rows,
+                        qb200_stream s) {
+  std::vector<qb200_tensor*> pools;
+  for (PagePool& l : c.layers)
+    for (QuantizedKV* kv : {&l.keys, &l.values})
+      for (Array* a : {&kv->q, &kv->scales, &kv->biases})
+        if (a->t.data) pools.push_back(&a->t);
+  check(qb200_kv_pages_accept(&path.t, &next.t, &accepted.t, &ends.t, pools.data(), (int)pools.size(), &c.table.t, &c.lens.t, c.page, &rows.t, &tree.parents.t,
+                              &tree.tokens.t, &sampled.t, tree.counts ? &tree.counts->t : nullptr, s));
+  pagesFree(c, rows, &ends, nullptr, s);
+}
 // Causal attention of a prompt (or a chunk behind cached tokens) with a sliding window and a few first tokens that stay visible.
 inline void windowAttention(Array& out, const Array& q, const Array& k, const Array& v, float scale, int64_t window, int64_t sinks, const Array* kv_lens,
                             qb200_stream s) {

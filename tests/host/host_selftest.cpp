@@ -280,6 +280,29 @@ int main(int argc, char** argv) {
       cudaDeviceSynchronize();
       ok = gate(f32_of(to_host((uint16_t*)out.t.data, (size_t)(2 * Hq * D))), ref, 1e-2, "paged cache: reserve, append, fork, attention") && ok;
 
+      // a drafted round of one node: the same attention; its sample from one open token; and the node stays
+      {
+        DraftTree tree;
+        tree.parents = Array(to_dev(std::vector<int32_t>{-1, -1}), QB200_INT32, {2, 1});
+        tree.tokens = Array(to_dev(std::vector<int32_t>{7, 9}), QB200_INT32, {2, 1});
+        const size_t tneed = quantAttentionTreeWorkspace(2, Hq, H, 1, D);
+        void* tws = dev_alloc<char>(tneed);
+        Array tout(dev_alloc<uint16_t>((size_t)(2 * Hq * D)), QB200_BFLOAT16, {2, Hq, 1, D});
+        quantAttentionTree(tout, dq, c, 0, &both, tree, scale, 0, 0, tws, tneed, stream);
+        std::vector<float> lg(2 * 100, -1e30f);
+        lg[42] = 3.0f; lg[100 + 17] = -2.0f;
+        Array logits(to_dev(lg), QB200_FLOAT32, {2, 100}), random(to_dev(std::vector<float>{0.25f, 0.75f}), QB200_FLOAT32, {2}), sampled = list({0, 0});
+        sampleTokens(sampled, nullptr, logits, random, nullptr, nullptr, nullptr, nullptr, stream);
+        Array s2((int32_t*)sampled.t.data, QB200_INT32, {2, 1}), path(dev_alloc<int32_t>(2), QB200_INT32, {2, 1}), next(dev_alloc<int32_t>(2), QB200_INT32, {2, 1}), accepted = list({0, 0}), ends = list({0, 0});
+        pagesAccept(c, path, next, accepted, ends, tree, s2, both, stream);
+        cudaDeviceSynchronize();
+        ok = gate(f32_of(to_host((uint16_t*)tout.t.data, (size_t)(2 * Hq * D))), ref, 1e-2, "drafted tree of one node: attention") && ok;
+        const std::vector<int32_t> nx = to_host((int32_t*)next.t.data, 2), ac = to_host((int32_t*)accepted.t.data, 2), en = to_host((int32_t*)ends.t.data, 2);
+        const bool good = nx[0] == 42 && nx[1] == 17 && ac[0] == 1 && ac[1] == 1 && en[0] == (int32_t)T && en[1] == (int32_t)T + 1;
+        std::printf("%s drafted round: sample, accept, free\n", good ? "ok  " : "FAIL");
+        ok = good && ok;
+      }
+
       // a prompt of 32 tokens whose every query sees itself alone: its values come back
       const int64_t n = 32;
       Array pq(to_dev(bf16_of(rand_bf16((size_t)(Hq * n * D), 1.0f))), QB200_BFLOAT16, {1, Hq, n, D}), po(dev_alloc<uint16_t>((size_t)(Hq * n * D)), QB200_BFLOAT16, {1, Hq, n, D});
