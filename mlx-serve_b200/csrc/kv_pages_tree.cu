@@ -20,9 +20,9 @@
 //  * The grid is one CTA an SM; every CTA works out all sequences' blocks from `lens` and takes an even share of them, or every tile is cut in the
 //    same number of parts.  Parts of a tile go to the workspace and are joined by a second kernel.
 //
-// Measured: 16 sequences of 32k tokens, 4 bits, 32 query heads over 8, 515 us with 32 nodes (128 rows of a cache head; the codes alone take 101 us at
-// the rate of a copy, the products 45), 382 with 16, 322 with 8, 274 with 4; 4 sequences of 8k, 8 bits, 64 nodes 126 us; 32 sequences of a window of 1024 over
-// bf16 98 us; one of 700 tokens 22.5.  What bounds a long one is neither the bytes (20 to 37 %) nor the products but the work a block of 128 tokens takes,
+// Measured: 16 sequences of 32k tokens, 4 bits, 32 query heads over 8, 515 us with 32 nodes (128 rows of a cache head; the products alone take 102 us at
+// the rate of a library's, the codes 72 at that of a copy), 371 with 16, 324 with 8, 277 with 4; 4 sequences of 8k, 8 bits, 64 nodes 133 us; 32 sequences of a
+// window of 1024 over bf16 98 us; one of 700 tokens 22.5.  What bounds a long one is neither the bytes nor the products but the work a block of 128 tokens takes,
 // handed from warp to warp: with copies, products and barriers alone 260 us (128 rows) and 177 (16); without the readers' arithmetic 407 and 189,
 // without the softmax's 347 and 231.  Rings by cp.async in every reader took 695 instead of 527 us; two groups of readers that
 // take turns, a sleeping instead of a polling issuer, and operands made uniform for it changed nothing.
