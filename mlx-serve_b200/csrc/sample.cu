@@ -60,6 +60,8 @@ __device__ __forceinline__ double warp_sum(double v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void put64(uint64_t* p, uint32_t rank, uint64_t v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(map_to_rank(smem_u32(p), rank)), "l"(v) : "memory");
 }
@@ -192,6 +194,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& sh = *(Shared*)raw;
   const uint32_t C = cluster_size(), me = cluster_rank();
+  // A block's shared memory may be written by the others once it runs: all say so here, and wait for it before the first value that goes to another
+  // block, behind the reading of the row (every block and thread does both, whatever its row asks for).
+  cluster_arrive();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int row_no = (int)(blockIdx.x / C), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
   const float temp = a.temperature ? a.temperature[row_no * a.str[1]] : 1.f, u = a.random[row_no * a.str[0]];
@@ -438,6 +443,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(0xffffffffu, best, o));
     const float mine_top = best ? value_of((uint32_t)(best >> 32)) : -INFINITY;
+    cluster_wait();                              // all blocks of the cluster run
     double mine = 0.0;
     if (once) {
       // parts relative to the block's largest (where that is infinite the row is not decided here)
