@@ -1029,42 +1029,47 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
           } else b = border(false, (uint64_t)want, b);
         }
         if (by_p) {
-          // where it should lie by the steps' mean weights
-          double est[PER], sum = 0.0;
+          // Where it should lie by the steps' mean weights, as whole numbers like the weights: their sums are the same in whatever order they are added, so
+          // that every place in (0, all] lies in one step of one thread, and in the same one in all blocks, which go on by it alike.
+          uint64_t est[PER], sum = 0;
 #pragma unroll
           for (int i = 0; i < PER; ++i) {
             const int bin = tid * PER + i;
             const uint32_t n = bin < k_bin ? cnt[i] : (bin == k_bin ? want - (uint32_t)k_before : 0u);
-            est[i] = (double)n * (double)exp2f(-((float)bin + 0.5f) * (kRange / (float)kBins * kLog2e));
+            est[i] = n * (uint64_t)(exp2f(-((float)bin + 0.5f) * (kRange / (float)kBins * kLog2e)) * (float)kOne);
             sum += est[i];
           }
-          double upto_d = sum;
+          uint64_t upto_e = sum;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
-            const double n = __shfl_up_sync(0xffffffffu, upto_d, o);
-            if (lane >= o) upto_d += n;
+            const uint64_t n = __shfl_up_sync(0xffffffffu, upto_e, o);
+            if (lane >= o) upto_e += n;
           }
           __syncthreads();
-          if (lane == 31) sh.red_d[warp] = upto_d;
-          if (tid == 0) { sh.answer[0] = k_bin; sh.range[0] = sh.range[2] = -1; }
+          if (lane == 31) sh.red[warp] = upto_e;
           __syncthreads();
-          double run = upto_d - sum, all = 0.0;
+          uint64_t run = upto_e - sum, all = 0;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) { if (w < warp) run += sh.red_d[w]; all += sh.red_d[w]; }
+          for (int w = 0; w < kWarps; ++w) { if (w < warp) run += sh.red[w]; all += sh.red[w]; }
           // a step's weights are within 2^-8 of their middle: the border is sought as far on both sides, where the list has room for that (it has where
           // few heavy logits make the mean a poor one), else in three steps
-          const double t = (double)p * all, t_lo = t * 0.995, t_hi = fmin(t * 1.005, all);
+          auto inside_of = [&](double x) {           // (the largest logit's step alone makes `all` more than 1)
+            const uint64_t v = x > 1.0 ? (uint64_t)x : 1;
+            return v < all ? v : all;
+          };
+          const double t = (double)p * (double)all;
+          const uint64_t t_mid = inside_of(t), t_lo = inside_of(t * 0.995), t_hi = inside_of(t * 1.005);
 #pragma unroll
           for (int i = 0; i < PER; ++i) {
             const uint32_t upto_n = before;
             before += cnt[i];
-            if (run < t && t <= run + est[i]) sh.answer[0] = tid * PER + i;
+            if (run < t_mid && t_mid <= run + est[i]) sh.answer[0] = tid * PER + i;
             if (run < t_lo && t_lo <= run + est[i]) { sh.range[0] = tid * PER + i; sh.range[1] = (int)upto_n; }
             if (run < t_hi && t_hi <= run + est[i]) { sh.range[2] = tid * PER + i; sh.range[3] = (int)before; }
             run += est[i];
           }
           __syncthreads();
-          const bool wide = sh.range[0] >= 0 && sh.range[2] >= 0 && sh.range[3] - sh.range[1] <= kList * 3 / 4;
+          const bool wide = sh.range[3] - sh.range[1] <= kList * 3 / 4;
           const int from_bin = wide ? sh.range[0] : sh.answer[0], to_bin = wide ? sh.range[2] : sh.answer[0];
           const int first_bin = from_bin > 0 ? from_bin - 1 : 0, last_bin = to_bin + 1 < kBins ? to_bin + 1 : kBins - 1;
           int list_n = wide ? sh.range[3] - sh.range[1] + (int)sh.merged[first_bin] + (int)sh.merged[last_bin] : 0;
