@@ -454,7 +454,7 @@ QB200_API size_t qb200_kv_pages_tree_attention_workspace_size(int64_t B, int64_t
  * top_k of the order stay (0 or less: all), of these the fewest whose weights reach top_p of their sum (at least one; 1 or more: all),
  * of these the ones with w_i >= min_p (and the first); the token is the first, by index, at which the running sum of what stays passes
  * random times the whole.  A temperature that is not above 0 takes the first of the order.  Sums and borders are those of 64-bit
- * arithmetic to 2^-45 of the largest weight.  temperature, random, top_p, min_p f32 and top_k int32, [N] on the device, of any stride
+ * arithmetic with weights rounded to 2^-45 of the largest.  temperature, random, top_p, min_p f32 and top_k int32, [N] on the device, of any stride
  * (0: one for all); all but random may be empty (1, 0, 1, 0).  tokens [N] int32, -1 for a row of -inf alone (a NaN counts as -inf); logprobs
  * [N] f32 (or empty): log softmax of the row at the token, before temperature and filters (0 beside -1).  V up to 2^19. */
 QB200_API int qb200_sample(qb200_tensor* tokens, qb200_tensor* logprobs, const qb200_tensor* logits, const qb200_tensor* random,

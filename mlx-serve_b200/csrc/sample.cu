@@ -5,8 +5,8 @@
 // first one in index order at which the running sum of the weights that stay passes u times their sum.
 //
 //  * Weights are whole numbers, round(w_i * 2^44), of a 64-bit exponential: sums of them do not depend on the order in which threads
-//    or atomics run, and borders (the nucleus, the token) are met as 64-bit sums meet them.  2^19 of them fit 63 bits; a token below
-//    2^-45 of the largest counts as 0.
+//    or atomics run, and borders (the nucleus, the token) are met as 64-bit sums meet them, but for the rounding: 2^-45 of the largest for each
+//    weight.  2^19 of them fit 63 bits; a token below 2^-45 of the largest counts as 0.
 //  * A row is a cluster of up to eight blocks, each with a share of the row in shared memory (read from memory again where it is too
 //    large); sums and histograms meet through distributed shared memory.
 //  * By temperature alone a row is read once, in parts of 512 elements that a warp weighs relative to its own largest logit in 32 bits, with a bound on how far
@@ -115,6 +115,7 @@ struct alignas(16) Shared {
   double red_d[kWarps];
   double part[kMaxCtas], part_top[kMaxCtas];   // of the sum for the log-probability: a block's sum and its largest
   double once_sum[kMaxCtas];
+  double far[kMaxCtas];                        // a block's sum of weights times how far their logits lie from the reference, or a bound of it
   double roots[32];
   union {                                      // (never of use at the same time)
     uint32_t hist[kBins];
@@ -242,6 +243,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     __syncthreads();
     return warp_sum(lane < kWarps ? sh.red_d[lane] : 0.0);
   };
+  // of a sum, and of how far its terms may be off, for all blocks behind the next meeting
+  auto block_sums_d = [&](double v, double off) {
+    v = warp_sum(v);
+    off = warp_sum(off);
+    __syncthreads();
+    if (lane == 0) { sh.red_d[warp] = v; sh.red[warp] = (uint64_t)__double_as_longlong(off); }
+    __syncthreads();
+    off = warp_sum(lane < kWarps ? __longlong_as_double((long long)sh.red[lane]) : 0.0);
+    if (tid < (int)C) put64((uint64_t*)&sh.far[me], (uint32_t)tid, (uint64_t)__double_as_longlong(off));
+    return warp_sum(lane < kWarps ? sh.red_d[lane] : 0.0);
+  };
   auto total = [&](uint64_t v) {
     const uint64_t* const g = gather(block_sum(v));
     uint64_t s = 0;
@@ -250,17 +262,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   };
   const double per_t = 1.0 / (double)temp, c64 = 32.0 * 1.4426950408889634 * per_t, c_all = 1.4426950408889634 * per_t;
   const float ch = (float)c_all, cl = (float)(c_all - (double)ch);
-  // Weights in fp32, relative to `largest`, from the approximate exponential (relative error 2^-22), whose argument is carried in two parts, and
-  // which is rounded once more with the second.
-  auto weights32 = [&](const float (&f)[8], float largest, float (&w)[8]) {
-    const float floor_d = -200.f / ch;           // (what lies further down weighs 0, as this does)
+  // Weights in fp32, relative to `largest`, from the approximate exponential (relative error 2^-22), whose argument, difference times factor, is carried
+  // in two parts, and which is rounded once more with the second.  `exact`: with the rounding of the difference to fp32 in the second part too.
+  auto weights32 = [&](auto exact, const float (&f)[8], float largest, float (&w)[8]) {
+    // what lies further down weighs 0, as this does (several steps of fp32 below the largest, so that it is below it, however large that is)
+    const float floor_f = largest - (200.f / ch + fabsf(largest) * 4.76837158203125e-7f);
     const uint64_t ch2 = two(ch, ch), cl2 = two(cl, cl), top2 = two(-largest, -largest), ln2 = two(0.6931471805599453f, 0.6931471805599453f), minus = two(-1.f, -1.f);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      float d0, d1, y0, y1;
-      untwo(add2(two(f[2 * q], f[2 * q + 1]), top2), d0, d1);
-      const uint64_t d = two(fmaxf(d0, floor_d), fmaxf(d1, floor_d)), y = mul2(d, ch2);
-      const uint64_t rest = fma2(d, cl2, fma2(d, ch2, mul2(y, minus)));
+      float y0, y1;
+      const uint64_t x = two(fmaxf(f[2 * q], floor_f), fmaxf(f[2 * q + 1], floor_f)), d = add2(x, top2), y = mul2(d, ch2);
+      uint64_t rest = fma2(d, cl2, fma2(d, ch2, mul2(y, minus)));
+      if constexpr (decltype(exact)::value) {
+        const uint64_t b = fma2(x, minus, d);    // (what the sum has of -largest; Knuth's exact sum of two)
+        rest = fma2(add2(fma2(fma2(b, minus, d), minus, x), fma2(b, minus, top2)), ch2, rest);
+      }
       untwo(y, y0, y1);
       const uint64_t e = two(ex2(y0), ex2(y1));
       untwo(fma2(e, mul2(rest, ln2), e), w[2 * q], w[2 * q + 1]);
@@ -270,7 +286,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   // How far a sum of such weights and u times their whole may lie from one another's true place: every weight is within e = 4.3e-7 (2^-22, and three
   // roundings of 2^-24: one of its own, two where four are added; the rest is added in 64 bits) of itself, those before the place count 1 - u times
   // and those behind it u times.
-  auto slack_of = [&](double all) { const double v = u > 0.f ? (u < 1.f ? (double)u : 1.0) : 0.0; return all * (2.0 * v * (1.0 - v) * 4.3e-7 + 1e-11); };
+  const double u64 = u > 0.f ? (u < 1.f ? (double)u : 1.0) : 0.0;
+  auto slack_of = [&](double all) { return all * (2.0 * u64 * (1.0 - u64) * 4.3e-7 + 1e-11); };
   auto place_of = [&](double all) { return u > 0.f ? (u < 1.f ? (double)u * all : all) : 0.0; };
   double* const sums_d = (double*)sh.sums;
   // The part at which the running sum of the parts' passes t, by a warp; *before = the sum before it; -1: none.
@@ -345,8 +362,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   struct U8 { uint64_t w[8]; };
 
   // ---- the row's largest; sums for the log-probability; where the row is read once, of the weights too ----
-  // Weights and the terms of the log-probability are relative to a reference of the warp's own: its first part's largest, moved where something lies
-  // more than 2^64 above it.  A part is asked for while the one before is worked on.
+  // Weights and the terms of the log-probability are relative to a reference of the warp's own: the largest of its parts so far, to a factor of
+  // 2^(1/4) of a weight.  A part is asked for while the one before is worked on.
   float top;
   int token = -1;
   {
@@ -404,9 +421,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         }
       }
       if (!once && !a.logprobs) continue;
-      if (__any_sync(0xffffffffu, m > ref && !((m - ref) * steep < 64.f))) {
+      if (__any_sync(0xffffffffu, m > ref && !((m - ref) * steep < 0.25f))) {
         const float up = value_of(__reduce_max_sync(0xffffffffu, pattern(m)));
-        lp = ref > -INFINITY ? lp * exp2((double)(ref - up) * 1.4426950408889634) : 0.0;
+        if (a.logprobs) lp = ref > -INFINITY ? lp * exp2((double)(ref - up) * 1.4426950408889634) : 0.0;
         ref = up;
       }
       if (once) {
@@ -415,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 #pragma unroll
           for (int s = 0; s < DEEP; ++s) {
             float w[8];
-            weights32(f[s], ref, w);
+            weights32(std::false_type{}, f[s], ref, w);
             t += (double)((w[0] + w[1]) + (w[2] + w[3])) + (double)((w[4] + w[5]) + (w[6] + w[7]));
           }
           t = warp_sum(t);
@@ -446,14 +463,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     cluster_wait();                              // all blocks of the cluster run
     double mine = 0.0;
     if (once) {
-      // parts relative to the block's largest (where that is infinite the row is not decided here)
+      // Parts relative to the block's largest (where that is infinite the row is not decided here).  The differences were rounded to fp32, which puts a
+      // weight e^-x off by 2^-24 x of itself.  With x weighted by the weights, its mean over a part's n = 512 and ln(sum) make the weights' entropy,
+      // at most ln(n): their x add up to no more than sum * ln(n / sum).  (A logit may lie above its reference, by a factor of 2^(1/4) of its
+      // weight, which takes up to 0.18 of the sum from that and may be off by as much.)
+      double far = 0.0;
       for (int q = tid; q < parts; q += kThreads) {
         const float at = sh.refs[q];
-        const double w = at > -INFINITY && mine_top < INFINITY ? sums_d[q] * exp2(((double)at - (double)mine_top) * c_all) : 0.0;
+        double w = 0.0;
+        if (at > -INFINITY && mine_top < INFINITY) {
+          const double sum = sums_d[q], down = exp2(((double)at - (double)mine_top) * c_all);
+          w = sum * down;
+          far += w * (double)(0.37f + fmaxf(logf(32.f * 8.f * DEEP / fmaxf((float)sum, 1e-30f)), 0.f));
+        }
         sums_d[q] = w;
         mine += w;
       }
-      mine = block_sum_d(mine);
+      mine = block_sums_d(mine, far);
       if (tid < (int)C) put64((uint64_t*)&sh.once_sum[me], (uint32_t)tid, (uint64_t)__double_as_longlong(mine));
     }
     if (a.logprobs) {
@@ -466,21 +492,30 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     top = best ? value_of((uint32_t)(best >> 32)) : -INFINITY;
     if (greedy && best) token = V - 1 - (int)(uint32_t)best;
     if (once && best && top < INFINITY) {
-      double all = 0.0, part[kMaxCtas];
+      double all = 0.0, far_all = 0.0, part[kMaxCtas], far_of[kMaxCtas];
 #pragma unroll
       for (uint32_t c = 0; c < kMaxCtas; ++c) {
-        part[c] = c < C && g[c] ? sh.once_sum[c] * exp2(((double)value_of((uint32_t)(g[c] >> 32)) - (double)top) * c_all) : 0.0;
+        const double down = c < C && g[c] ? exp2(((double)value_of((uint32_t)(g[c] >> 32)) - (double)top) * c_all) : 0.0;
+        part[c] = down > 0.0 ? sh.once_sum[c] * down : 0.0;
+        far_of[c] = down > 0.0 ? sh.far[c] * down : 0.0;
+        far_all += far_of[c];
         all += part[c];
       }
-      const double slack = slack_of(all), t = place_of(all);
+      const double t = place_of(all);
       uint32_t who = C - 1;
-      double before = 0.0, run = 0.0;
+      double before = 0.0, run = 0.0, far_run = 0.0, off = 0.0;
       bool found = false;
 #pragma unroll
       for (uint32_t c = 0; c < kMaxCtas; ++c) {
-        if (c < C && !found && t < run + part[c]) { who = c; before = run; found = true; }
+        if (c < C && !found && t < run + part[c]) {
+          who = c; before = run; found = true;
+          // (2^-24 and 1 % for what it is made of in fp32)
+          off = 6.02e-8 * ((1.0 - u64) * far_run + u64 * (far_all - far_run - far_of[c]) + fmax(u64, 1.0 - u64) * far_of[c]);
+        }
         run += part[c];
+        far_run += far_of[c];
       }
+      const double slack = slack_of(all) + off;
       if (who == me && warp == 0) {
         // everything relative to this block's largest, then to the part's
         int at = -1;
@@ -494,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
               float f[8];
               W8 w;
               r.load8(v, f);
-              weights32(f, sh.refs[q], w.w);
+              weights32(std::false_type{}, f, sh.refs[q], w.w);
               return w;
             });
           }
@@ -582,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       float f[8];
       W8 w;
       r.load8(v, f);
-      weights32(f, top, w.w);
+      weights32(std::true_type{}, f, top, w.w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if (least > 0.f) {

@@ -68,3 +68,53 @@ def test_nuclei_whose_last_steps_hold_the_most():
             x[i, 1 + far:1 + far + other] = 9.0 - d - 1.0 - torch.rand(other, device="cuda") * 0.004
         x = x[:, torch.randperm(V, device="cuda")]
         check(x, [rng.random() for _ in range(N)], [1.0] * N, [0] * N, [rng.uniform(0.996, 0.9999) for _ in range(N)], [0.0] * N, runs=10)
+
+
+def beside_borders(row, t, near, count, rng):
+    """Random numbers in fp32 whose place lies within `near` (of a token's own weight) of that token's border, on either side."""
+    w = np.exp((row.astype(np.float64) - float(row.max())) / t)
+    run = np.cumsum(w.astype(np.longdouble))
+    found = []
+    while len(found) < count:
+        u = f32(rng.uniform(0.3, 0.7))
+        place = np.longdouble(u) * run[-1]
+        i = int(np.searchsorted(run, place, side="right"))
+        part = float((run[i] - place) / w[i])
+        if w[i] < 1 and min(part, 1 - part) < near:
+            found.append(u)
+    return found
+
+
+@pytest.mark.parametrize("top,t", [(16.5, 1.5), (16.5, 1.3), (17.9, 1.6), (9.1, 0.8)])
+def test_places_beside_a_border_where_logits_lie_far_below_the_largest(top, t):
+    """Half of the row at a logit whose distance from the largest is rounded up in fp32, half at one where it is rounded down, by nearly half a step: sums of
+    fp32 weights lie a part of a token beside those of 64 bits, and the token may not be the neighbour for that."""
+    V, N = 2 ** 19, 32
+    top = f32(top)
+    near = [np.float32(0.3)]
+    for _ in range(200):
+        near.append(np.nextafter(near[-1], np.float32(1)))
+    off = [float(np.float32(v - np.float32(top))) - (float(v) - top) for v in near]
+    row = np.empty(V, np.float32)
+    row[: V // 2], row[V // 2:], row[0] = near[int(np.argmax(off))], near[int(np.argmin(off))], top
+    # (the weights' rounding decides up to 2^-25 of the largest weight, the token's own is e^(-16.2 / 1.3) and more: a quarter of the 3 % around a border)
+    some = N // 2
+    u = beside_borders(row, t, 0.03, N, random.Random(int(top * 10)))
+    x = torch.from_numpy(row).cuda()[None].expand(N, V)
+    check(x, u, [t] * N, [0] * N, [1.0] * N, [1e-6] * N, undecided=some)
+    check(x, u, [t] * N, [0] * N, [1.0] * N, [0.0] * N, undecided=some)
+    check(torch.cat([x[:1, :1].expand(1, 1), x[:1, 1:].flip(1)], 1).expand(N, V), u, [t] * N, [0] * N, [1.0] * N, [1e-6] * N, undecided=some)
+
+
+@pytest.mark.parametrize("size,steps", [(1e10, 1024.0), (-1e10, 1024.0), (3e37, 2.0 ** 101), (100.0, 2.0 ** -17)])
+def test_logits_of_any_size(size, steps):
+    """Logits a few steps of fp32 beside one another, at temperatures under, around and over a step."""
+    N, V = 24, 5000
+    torch.manual_seed(8)
+    x = (torch.randint(-20, 21, (N, V), device="cuda", dtype=torch.float64) * steps + size).float()
+    rng = random.Random(9)
+    t = [min(steps * (0.01, 0.7, 5.0)[i % 3], 3e37) for i in range(N)]
+    u = [rng.random() for _ in range(N)]
+    check(x, u, t, [0] * N, [1.0] * N, [0.0] * N)
+    check(x, u, t, [0] * N, [1.0] * N, [(0.0, 1e-4, 0.3)[i // 3 % 3] for i in range(N)])
+    check(x, u, t, [0, 200] * (N // 2), [0.9, 0.99, 1.0] * (N // 3), [0.0] * N)
