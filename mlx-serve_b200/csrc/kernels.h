@@ -367,6 +367,7 @@ struct KvPagesTreeArgs {
   const int32_t* parents; int64_t par_str;
   const int32_t* counts;                 // may be null
   int T;
+  int polls;                             // wait_polls(), set by the launcher
 };
 size_t kv_pages_tree_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D);
 cudaError_t launch_kv_pages_tree(KvPagesTreeArgs a, int D, void* workspace, cudaStream_t st);

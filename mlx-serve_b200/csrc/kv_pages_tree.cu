@@ -152,21 +152,21 @@ __device__ __forceinline__ bool arrived(uint32_t bar, uint32_t parity) {
                : "=r"(done) : "r"(bar), "r"(parity), "r"(kNap) : "memory");
   return done != 0;
 }
-// The rest of a wait, for a warp whose barrier had not arrived at the first look: kPolls looks, each held by the hardware for kNap ns at most.  A wait
-// that runs out is noted once; the warp then goes on without waiting (on data that is not there yet, within its bounds), so that all warps
-// meet at every barrier and the CTA ends.
-__device__ __forceinline__ void wait_on(uint32_t bar, uint32_t parity, int code, int* fail) {
+// The rest of a wait, for a warp whose barrier had not arrived at the first look: `most` looks, each held by the hardware for kNap ns at most.  A wait
+// that runs out is noted once.  From then on nothing is copied and no product is issued any more; the readers and the softmax go on without waiting, on
+// data that is not there and within their bounds, so that all warps meet at every barrier and the CTA ends; and its results are NaN.
+__device__ __forceinline__ void wait_on(uint32_t bar, uint32_t parity, int code, int* fail, uint32_t most) {
   if (*(volatile int*)fail == 0) {
-    for (uint32_t it = 0; it < kPolls; ++it)
+    for (uint32_t it = 0; it < most; ++it)
       if (arrived(bar, parity)) return;
     *(volatile int*)fail = code;
     atomicCAS(&g_tree_error, 0, code);
   }
 }
 // A bounded wait that polls without sleeping.
-__device__ __forceinline__ bool spin_cta(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool spin_cta(uint64_t* bar, uint32_t parity, uint32_t most) {
   const uint32_t addr = smem_u32(bar);
-  for (uint32_t it = 0; it < kSpins; ++it) {
+  for (uint32_t it = 0; it < most; ++it) {
     uint32_t done;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(done) : "r"(addr), "r"(parity) : "memory");
@@ -365,7 +365,8 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
     longest = __reduce_max_sync(0xffffffffu, longest);
     if (lane == 31) { warp_sums[0][warp] = upto; warp_sums[1][warp] = upto_t; s_longest[warp] = longest; }
     if (tid == 0) {
-      s_fail = 0;
+      s_fail = t.polls < 0 ? 600 : 0;
+      if (t.polls < 0) atomicCAS(&g_tree_error, 0, 600);
       mbar_init(&q_ready, SW);
       for (int i = 0; i < 2; ++i) { mbar_init(&k_ready[i], 4); mbar_init(&v_ready[i], 4); mbar_init(&s_ready[i], 1); mbar_init(&p_ready[i], SW); mbar_init(&o_done[i], 1); }
       for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], QUANT ? 4 : 1); }
@@ -394,9 +395,10 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
   Pieces pieces(t, units, tiles, longest, N);
   Piece pc;
   auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
-    if (__builtin_expect(!arrived(smem_u32(bar), phase & 1), 0)) wait_on(smem_u32(bar), phase & 1, code, &s_fail);
+    if (__builtin_expect(!arrived(smem_u32(bar), phase & 1), 0)) wait_on(smem_u32(bar), phase & 1, code, &s_fail, t.polls > 0 ? (uint32_t)t.polls : kPolls);
     __syncwarp();
   };
+  auto failed = [&]() { return __any_sync(0xffffffffu, *(volatile int*)&s_fail != 0); };   // (the same for the warp, whoever notes it when)
   const int pmask = (1 << a.page_shift) - 1;
   int J0 = 0;                        // blocks before this piece
 
@@ -437,8 +439,10 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
               const KvPoolView& pl = a.pool[V || arr >= 2];
               const int pid = a.table[(int64_t)pc.s.row * a.table_str + (tok >> a.page_shift)];
               const uint16_t* const src = (const uint16_t*)((arr & 1) ? pl.b : pl.s) + (int64_t)pid * pl.sb_str[0] + (int64_t)pc.hk * pl.sb_str[1] + (int64_t)(tok & pmask) * pl.sb_str[2];
-              v = src[0];
-              if constexpr (G == 2) v |= (uint32_t)src[1] << 16;
+              if (pid >= 0 && pid < a.P) {                     // (behind a wait that ran out `mine` may not be true)
+                v = src[0];
+                if constexpr (G == 2) v |= (uint32_t)src[1] << 16;
+              }
             }
             v = mine ? v : 0u;
             x[0] = bf16lo(v);
@@ -548,7 +552,8 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
     const uint32_t piece_b = codes_b + (vec ? (V ? 2u : 4u) * sb_b : 0u);
     int st = 0;
     uint32_t round = 0;
-    while (pieces.next(pc)) {
+    bool stop = false;
+    while (!stop && pieces.next(pc)) {
       const int32_t* const tab = a.table + (int64_t)pc.s.row * a.table_str;
       auto page_at = [&](int j) {
         int pid = -1;
@@ -566,6 +571,8 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
         pid_next = page_at(j + 1);
         const uint32_t have = __ballot_sync(0xffffffffu, pid >= 0);
         if (round > 0) wait(&empty[st], round - 1, V ? 614 : 613);
+        stop = failed();                                       // (a place whose copies may not have come is not armed again)
+        if (stop) break;
         const uint32_t to = ring + st * stage_b;
         if (lane == 0) {
           uint32_t bits = 0xffu;                               // of 16 tokens each
@@ -607,8 +614,6 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
       }
       J0 += pc.todo;
     }
-    if (*(volatile int*)&s_fail)
-      for (int i = 0; i < 1000; ++i) __nanosleep(1000);        // (copies may still be on their way)
   } else if (warp == SH::MMA_AT) {
     // ---------------- products ----------------
     if constexpr (SH::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::R_MISC));
@@ -619,18 +624,22 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
     const uint32_t tm = (uint32_t)U((int)tmem), sm = (uint32_t)U((int)smem_u32(smem));
     const uint64_t hi_k = make_desc(0) & 0xFFFFFFFF00000000ull, hi_v = make_desc_mn(0) & 0xFFFFFFFF00000000ull;
     const uint32_t q_d = (uint32_t)make_desc(sm + SH::Q0), k_d = (uint32_t)make_desc(sm + SH::KR), v_d = (uint32_t)make_desc_mn(sm + (QUANT ? SH::V0 : SH::VR)), p_d = (uint32_t)make_desc_mn(sm + SH::P0);
+    const uint32_t most = t.polls > 0 ? (uint32_t)t.polls : kSpins;
     auto spin = [&](uint64_t* bar, uint32_t phase, int code) {
-      if (*(volatile int*)&s_fail) return;
-      if (!__all_sync(0xffffffffu, spin_cta(bar, phase & 1)) && lane == 0) { *(volatile int*)&s_fail = code; atomicCAS(&g_tree_error, 0, code); }
+      if (failed()) return false;
+      const bool ok = __all_sync(0xffffffffu, spin_cta(bar, phase & 1, most));
+      if (!ok && lane == 0) { *(volatile int*)&s_fail = code; atomicCAS(&g_tree_error, 0, code); }
       __syncwarp();
+      return ok;
     };
     int piece_no = 0, ks = 0, vs = 0;                          // (at 16 bits the operands are the rings' places)
     uint32_t kr = 0;
     auto scores = [&](int J) {
-      if constexpr (QUANT) spin(&k_ready[J & 1], (uint32_t)(J >> 1), 603);
-      else spin(&k_full[ks], kr, 603);
+      bool ok;
+      if constexpr (QUANT) ok = spin(&k_ready[J & 1], (uint32_t)(J >> 1), 603);
+      else ok = spin(&k_full[ks], kr, 603);
       fence_after();
-      if (elect_one()) {
+      if (ok && elect_one()) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint64_t q = hi_k | (q_d + (k >> 2) * ((N * 128) >> 4) + (k & 3) * 2);
@@ -649,10 +658,9 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
       for (int j = -2; j < todo; ++j) {
         if (j >= 0) {
           const int J = J0 + j;
-          spin(&v_ready[J & 1], (uint32_t)(J >> 1), 606);
-          spin(&p_ready[J & 1], (uint32_t)(J >> 1), 607);
+          const bool ok = spin(&v_ready[J & 1], (uint32_t)(J >> 1), 606) && spin(&p_ready[J & 1], (uint32_t)(J >> 1), 607);
           fence_after();
-          if (elect_one()) {
+          if (ok && elect_one()) {
 #pragma unroll
             for (int k = 0; k < kBlk / 16; ++k)
               umma_ss(tm + SH::O_AT, hi_v | (v_d + (QUANT ? J & 1 : vs) * (SH::TILE >> 4) + k * (2048 >> 4)), hi_v | (p_d + (J % SH::PS) * (SH::PTILE >> 4) + k * (2048 >> 4)), idesc_o,
@@ -670,8 +678,6 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
     }
     // every product is complete before tensor memory and shared memory go
     if (J0 > 0) spin(&o_done[(J0 - 1) & 1], (uint32_t)((J0 - 1) >> 1), 608);
-    if (*(volatile int*)&s_fail)
-      for (int i = 0; i < 1000; ++i) __nanosleep(1000);        // (products may still be on their way)
   } else if (warp < SW) {
     // ---------------- softmax: a thread a token ----------------
     if constexpr (SH::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH::R_SOFT));
@@ -904,12 +910,14 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
       if (lane < NC) {
         L = (s_wmax[wg][0][lane] + s_wmax[wg][1][lane]) + (s_wmax[wg][2][lane] + s_wmax[wg][3][lane]);
         r = -s_nr[col0 + lane];
+        if (*(volatile int*)&s_fail) L = __uint_as_float(0x7fc00000u);
         const int notes = note_count[piece_no & 3];
         for (int i = 0; i < notes && i < kNotes; ++i) {
           const int k = note_key[piece_no & 3][i];
           const bool drafted = k >= s.base;
-          const int at = drafted ? s.base + s_depth[k - s.base] : k;
-          if ((!drafted || ((s_cline[col0 + lane] >> (k - s.base)) & 1ull)) && (a.window == 0 || at < a.sinks || at > s_clo[col0 + lane])) L = __uint_as_float(0x7fc00000u);
+          const int m = drafted ? (k - s.base) & (kMaxNodes - 1) : 0;        // (behind a wait that ran out, k may be anything)
+          const int at = drafted ? s.base + s_depth[m] : k;
+          if ((!drafted || ((s_cline[col0 + lane] >> m) & 1ull)) && (a.window == 0 || at < a.sinks || at > s_clo[col0 + lane])) L = __uint_as_float(0x7fc00000u);
         }
       }
       const bool all = pc.blk0 == 0 && pc.todo == s.blocks;
@@ -949,6 +957,8 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
   __syncwarp();
   fence_before();
   __syncthreads();
+  if (*(volatile int*)&s_fail)
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);          // (copies and products may still be on their way: a millisecond for them)
   if (warp == SH::MMA_AT) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
 }
 
@@ -1096,6 +1106,7 @@ size_t kv_pages_tree_workspace_bytes(int64_t, int64_t Hq, int64_t Hkv, int64_t T
 
 cudaError_t launch_kv_pages_tree(KvPagesTreeArgs t, int D, void* workspace, cudaStream_t st) {
   const size_t ctas = (size_t)sm_count(), rows = (size_t)columns_of(t);
+  t.polls = wait_polls();
   t.a.joins = (int4*)workspace;
   t.a.part_ml = (float2*)((char*)workspace + ctas * 16);
   t.a.part_o = (float*)((char*)workspace + ctas * 16 + ctas * 2 * rows * 8);
