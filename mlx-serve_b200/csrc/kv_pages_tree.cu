@@ -11,7 +11,9 @@
 // register of its thread:
 //  * Codes are dequantised to fp16, rounded once, in a unit of the token's own (a power of two, its largest |q s + b| in [2^14, 2^15)), so that the
 //    range of fp16 holds for each token by itself; a key's unit is a factor of its thread's scores, a value's goes to its probabilities: P' = p * unit, and the
-//    row's sum takes P' / unit.  Tokens and groups 2^28 apart in size keep fp16's 11 bits.  At 16 bits the operands are the cache's bf16.
+//    row's sum takes P' / unit.  Tokens and groups 2^28 apart in size keep fp16's 11 bits.  At 16 bits the operands are the cache's bf16 and
+//    P is a sum of two bf16 (16 bits, as where one token is decoded), each multiplied with the values: rounded to one its errors were as large as
+//    the result's own rounding.
 //  * r moves only where some P' would pass 2^15: then it is placed 2^8 below the block's maximum, and O is rescaled.
 //  * Roles of a CTA's warps: four a 32 columns of the softmax; four read keys and dequantise them into tensor memory (the A operand of S^T); four
 //    read values and dequantise them into shared memory; one issues the products, S^T two blocks ahead of O^T; two issue the copies: codes by
@@ -64,9 +66,10 @@ template <int BITS, int D, int N> struct Shape {
   static constexpr int SB = kBlk * G * 2;                    // bytes of a block's scales (or biases)
   static constexpr int VT = 2;                               // places for values as operands
   static constexpr int PS = N == 128 || (D == 128 && (BITS == 8 || (BITS == 16 && N == 64))) ? 1 : 2;   // places for P
-  static constexpr int PTILE = kBlk * 128 * (N > 64 ? 2 : 1);
+  // P of a block, 128 bytes of columns a token; at 16 bits what bf16 leaves of it stands behind it: in the other half of the 128 bytes, or in a tile of its own
+  static constexpr int PP = QUANT ? 1 : 2, PCOLS = kBlk * 128 * (N > 64 ? 2 : 1), LOW = N <= 32 ? 64 : PCOLS, PTILE = PP == 2 && N > 32 ? 2 * PCOLS : PCOLS;
   // the rings: codes with scales and biases (the keys' with the values' too, for their units), or at 16 bits the operands themselves
-  static constexpr int KS = BITS == 4 ? 4 : (BITS == 8 ? (N == 128 && D == 128 ? 2 : 3) : (D == 64 ? 4 : 2)), VS = BITS == 4 ? 4 : (BITS == 8 ? (N == 128 && D == 128 ? 2 : 3) : (D == 64 ? 4 : (N == 128 ? 2 : 3)));
+  static constexpr int KS = BITS == 4 ? 4 : (BITS == 8 ? (N == 128 && D == 128 ? 2 : 3) : (D == 64 ? (N >= 64 ? 3 : 4) : 2)), VS = BITS == 4 ? 4 : (BITS == 8 ? (N == 128 && D == 128 ? 2 : 3) : (D == 64 ? (N >= 64 ? 3 : 4) : (N == 64 ? 2 : 3)));
   static constexpr int K_STAGE = QUANT ? kBlk * ROWB + 4 * SB : TILE, V_STAGE = QUANT ? kBlk * ROWB + 2 * SB : TILE;
   static constexpr int V0 = 0, Q0 = QUANT ? VT * TILE : 0, P0 = Q0 + N * 128 * HALVES, KR = P0 + PS * PTILE, VR = KR + KS * K_STAGE;
   static constexpr int SMEM = VR + VS * V_STAGE + (QUANT || D == 128 ? 0 : TILE) + 1024;   // (a product of 128 rows reads a tile past the last one of 64)
@@ -662,9 +665,11 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
           fence_after();
           if (ok && elect_one()) {
 #pragma unroll
-            for (int k = 0; k < kBlk / 16; ++k)
-              umma_ss(tm + SH::O_AT, hi_v | (v_d + (QUANT ? J & 1 : vs) * (SH::TILE >> 4) + k * (2048 >> 4)), hi_v | (p_d + (J % SH::PS) * (SH::PTILE >> 4) + k * (2048 >> 4)), idesc_o,
-                      k > 0 ? 1u : (j > 0 ? 1u : 0u));
+            for (int part = 0; part < SH::PP; ++part)
+#pragma unroll
+              for (int k = 0; k < kBlk / 16; ++k)
+                umma_ss(tm + SH::O_AT, hi_v | (v_d + (QUANT ? J & 1 : vs) * (SH::TILE >> 4) + k * (2048 >> 4)),
+                        hi_v | (p_d + (J % SH::PS) * (SH::PTILE >> 4) + part * (SH::LOW >> 4) + k * (2048 >> 4)), idesc_o, part + k > 0 ? 1u : (j > 0 ? 1u : 0u));
             commit(&o_done[J & 1]);
             if (!QUANT) commit(&v_empty[vs]);
           }
@@ -873,13 +878,21 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
         for (int i = 0; i < NC / 2; ++i) {
           const float x0 = ex2(__uint_as_float(z[2 * i])), x1 = ex2(__uint_as_float(z[2 * i + 1]));
           if constexpr (QUANT) { l2[i] = fma2(two(x0, x1), w2, l2[i]); p[i] = pack_f16x2(x0, x1); }
-          else { l2[i] = add2(l2[i], two(x0, x1)); p[i] = pack2(x0, x1); }
+          else {
+            l2[i] = add2(l2[i], two(x0, x1));
+            p[i] = pack2(x0, x1);
+            z[i] = pack2(x0 - bf16lo(p[i]), x1 - bf16hi(p[i]));
+          }
         }
         if (J >= SH::PS) wait(&o_done[(J - SH::PS) & 1], (uint32_t)((J - SH::PS) >> 1), 611);
         unsigned char* const prow = smem + SH::P0 + (J % SH::PS) * SH::PTILE + (col0 >> 6) * (kBlk * 128) + key * 128;
 #pragma unroll
         for (int c = 0; c < NC / 8; ++c)
           *(uint4*)(prow + ((((col0 & 63) / 8 + c) ^ (key & 7)) << 4)) = make_uint4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
+        if constexpr (SH::PP == 2)
+#pragma unroll
+          for (int c = 0; c < NC / 8; ++c)
+            *(uint4*)(prow + (N > 32 ? SH::LOW : 0) + ((((col0 & 63) / 8 + c + (N > 32 ? 0 : 4)) ^ (key & 7)) << 4)) = make_uint4(z[4 * c], z[4 * c + 1], z[4 * c + 2], z[4 * c + 3]);
         fence_async();
         fence_before();
         __syncwarp();
@@ -1040,9 +1053,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const __grid
 // the wide tile takes longer to begin and to end (135 rows over 3 sequences of 2k tokens 31.9 us, 37.5 with 128; one of 2k with 128 rows 30.9 and 36.5;
 // with seven blocks an SM 36.0 and 34.9).
 int columns(int64_t T, int64_t gqa) { return T * gqa <= 16 ? 16 : (T * gqa <= 32 ? 32 : (T * gqa <= 64 ? 64 : 128)); }
-int columns_of(const KvPagesTreeArgs& t) {
+// Over 16-bit rows of 128 dims there is no room for 128 columns of P in two parts: 64 (4 sequences of 8k tokens with 64 nodes 159 us, 128 rows over 4 of 32k
+// 196; 108 and 147 with 128 columns and P rounded to 8 bits).
+int columns_of(const KvPagesTreeArgs& t, int D) {
   const int n = columns(t.T, t.a.gqa);
   if (n < 128) return n;
+  if (t.a.bits == 16 && D == 128) return 64;
   const int64_t blocks = (((int64_t)t.a.M << t.a.page_shift) + kBlk - 1) / kBlk, tiles = (int64_t)t.a.B * t.a.Hkv * (((int64_t)t.T * t.a.gqa + 63) / 64);
   return blocks * tiles <= 4 * (int64_t)sm_count() ? 64 : 128;
 }
@@ -1089,11 +1105,13 @@ template <int BITS, int D, int N> cudaError_t launch_n(const KvPagesTreeArgs& t,
   return launch_behind(tree_join_kernel<BITS, D>, dim3(grid, (N + kJoinRows - 1) / kJoinRows), dim3(kJoinWarps * 32), 0, st, t, N);
 }
 template <int BITS, int D> cudaError_t launch_d(const KvPagesTreeArgs& t, cudaStream_t st) {
-  switch (columns_of(t)) {
+  switch (columns_of(t, D)) {
     case 16: return launch_n<BITS, D, 16>(t, st);
     case 32: return launch_n<BITS, D, 32>(t, st);
     case 64: return launch_n<BITS, D, 64>(t, st);
-    default: return launch_n<BITS, D, 128>(t, st);
+    default:
+      if constexpr (BITS == 16 && D == 128) return cudaErrorInvalidValue;   // (columns_of does not ask for it)
+      else return launch_n<BITS, D, 128>(t, st);
   }
 }
 }  // namespace
@@ -1105,7 +1123,7 @@ size_t kv_pages_tree_workspace_bytes(int64_t, int64_t Hq, int64_t Hkv, int64_t T
 }
 
 cudaError_t launch_kv_pages_tree(KvPagesTreeArgs t, int D, void* workspace, cudaStream_t st) {
-  const size_t ctas = (size_t)sm_count(), rows = (size_t)columns_of(t);
+  const size_t ctas = (size_t)sm_count(), rows = (size_t)columns_of(t, D);
   t.polls = wait_polls();
   t.a.joins = (int4*)workspace;
   t.a.part_ml = (float2*)((char*)workspace + ctas * 16);
