@@ -69,7 +69,7 @@ template <int BITS, int D, int N> struct Shape {
   // P of a block, 128 bytes of columns a token; at 16 bits what bf16 leaves of it stands behind it: in the other half of the 128 bytes, or in a tile of its own
   static constexpr int PP = QUANT ? 1 : 2, PCOLS = kBlk * 128 * (N > 64 ? 2 : 1), LOW = N <= 32 ? 64 : PCOLS, PTILE = PP == 2 && N > 32 ? 2 * PCOLS : PCOLS;
   // the rings: codes with scales and biases (the keys' with the values' too, for their units), or at 16 bits the operands themselves
-  static constexpr int KS = BITS == 4 ? 4 : (BITS == 8 ? (N == 128 && D == 128 ? 2 : 3) : (D == 64 ? (N >= 64 ? 3 : 4) : 2)), VS = BITS == 4 ? 4 : (BITS == 8 ? (N == 128 && D == 128 ? 2 : 3) : (D == 64 ? (N >= 64 ? 3 : 4) : (N == 64 ? 2 : 3)));
+  static constexpr int KS = BITS == 4 ? 4 : (BITS == 8 ? (N == 128 && D == 128 ? 2 : 3) : (D == 64 ? (N >= 64 ? 3 : 4) : (N == 128 ? 1 : 2))), VS = BITS == 4 ? 4 : (BITS == 8 ? (N == 128 && D == 128 ? 2 : 3) : (D == 64 ? (N >= 64 ? 3 : 4) : (N >= 64 ? 2 : 3)));
   static constexpr int K_STAGE = QUANT ? kBlk * ROWB + 4 * SB : TILE, V_STAGE = QUANT ? kBlk * ROWB + 2 * SB : TILE;
   static constexpr int V0 = 0, Q0 = QUANT ? VT * TILE : 0, P0 = Q0 + N * 128 * HALVES, KR = P0 + PS * PTILE, VR = KR + KS * K_STAGE;
   static constexpr int SMEM = VR + VS * V_STAGE + (QUANT || D == 128 ? 0 : TILE) + 1024;   // (a product of 128 rows reads a tile past the last one of 64)
@@ -1053,12 +1053,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const __grid
 // the wide tile takes longer to begin and to end (135 rows over 3 sequences of 2k tokens 31.9 us, 37.5 with 128; one of 2k with 128 rows 30.9 and 36.5;
 // with seven blocks an SM 36.0 and 34.9).
 int columns(int64_t T, int64_t gqa) { return T * gqa <= 16 ? 16 : (T * gqa <= 32 ? 32 : (T * gqa <= 64 ? 64 : 128)); }
-// Over 16-bit rows of 128 dims there is no room for 128 columns of P in two parts: 64 (4 sequences of 8k tokens with 64 nodes 159 us, 128 rows over 4 of 32k
-// 196; 108 and 147 with 128 columns and P rounded to 8 bits).
-int columns_of(const KvPagesTreeArgs& t, int D) {
+int columns_of(const KvPagesTreeArgs& t) {
   const int n = columns(t.T, t.a.gqa);
   if (n < 128) return n;
-  if (t.a.bits == 16 && D == 128) return 64;
   const int64_t blocks = (((int64_t)t.a.M << t.a.page_shift) + kBlk - 1) / kBlk, tiles = (int64_t)t.a.B * t.a.Hkv * (((int64_t)t.T * t.a.gqa + 63) / 64);
   return blocks * tiles <= 4 * (int64_t)sm_count() ? 64 : 128;
 }
@@ -1105,13 +1102,11 @@ template <int BITS, int D, int N> cudaError_t launch_n(const KvPagesTreeArgs& t,
   return launch_behind(tree_join_kernel<BITS, D>, dim3(grid, (N + kJoinRows - 1) / kJoinRows), dim3(kJoinWarps * 32), 0, st, t, N);
 }
 template <int BITS, int D> cudaError_t launch_d(const KvPagesTreeArgs& t, cudaStream_t st) {
-  switch (columns_of(t, D)) {
+  switch (columns_of(t)) {
     case 16: return launch_n<BITS, D, 16>(t, st);
     case 32: return launch_n<BITS, D, 32>(t, st);
     case 64: return launch_n<BITS, D, 64>(t, st);
-    default:
-      if constexpr (BITS == 16 && D == 128) return cudaErrorInvalidValue;   // (columns_of does not ask for it)
-      else return launch_n<BITS, D, 128>(t, st);
+    default: return launch_n<BITS, D, 128>(t, st);
   }
 }
 }  // namespace
@@ -1123,7 +1118,7 @@ size_t kv_pages_tree_workspace_bytes(int64_t, int64_t Hq, int64_t Hkv, int64_t T
 }
 
 cudaError_t launch_kv_pages_tree(KvPagesTreeArgs t, int D, void* workspace, cudaStream_t st) {
-  const size_t ctas = (size_t)sm_count(), rows = (size_t)columns_of(t, D);
+  const size_t ctas = (size_t)sm_count(), rows = (size_t)columns_of(t);
   t.polls = wait_polls();
   t.a.joins = (int4*)workspace;
   t.a.part_ml = (float2*)((char*)workspace + ctas * 16);
