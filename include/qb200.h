@@ -467,7 +467,7 @@ QB200_API int qb200_sample(qb200_tensor* tokens, qb200_tensor* logprobs, const q
  * scales and biases of all layers) the rows of the path's nodes move to the places behind the cached tokens, in the path's order; lens
  * stays, and qb200_kv_pages_free(begin = ends) gives back the rest.  A sequence that does not exist, or is listed again, has accepted 0
  * (and ends at 0, or its length).  At most 1024 trees.  No page of the drafted tokens may be another sequence's too, which
- * qb200_kv_pages_reserve sees to. */
+ * qb200_kv_pages_reserve sees to, and no two pools may share memory (one listed twice is refused). */
 QB200_API int qb200_kv_pages_accept(qb200_tensor* path, qb200_tensor* next, qb200_tensor* accepted, qb200_tensor* ends, qb200_tensor* const* pools, int num_pools,
                                     const qb200_tensor* table, const qb200_tensor* lens, int page, const qb200_tensor* rows, const qb200_tensor* parents,
                                     const qb200_tensor* tokens, const qb200_tensor* sampled, const qb200_tensor* counts, qb200_stream s);

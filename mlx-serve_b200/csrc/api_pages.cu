@@ -1,9 +1,12 @@
 // C ABI of the paged key-value cache, of drafted trees over it and of windowed prompt attention: argument validation and dispatch (include/qb200.h).
 // As in the other entries everything is checked on the host before any CUDA call; what only the device knows (page numbers,
 // lengths, listed sequences) is checked by the kernels, which skip what lies outside the tensors.
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <memory>
+#include <new>
 
 #include "kernels.h"
 
@@ -82,6 +85,26 @@ bool distinct(const qb200_tensor* t) {
     span += str * ext;
   }
   return true;
+}
+// Whether two tensors of a list start at the same place (those with no elements aside).
+bool listed_twice(qb200_tensor* const* ts, int n, bool* no_memory) {
+  const void* few[256];
+  std::unique_ptr<const void*[]> many;
+  const void** at = few;
+  if (n > 256) {
+    many.reset(new (std::nothrow) const void*[(size_t)n]);
+    at = many.get();
+    *no_memory = at == nullptr;
+    if (*no_memory) return false;
+  }
+  int k = 0;
+  for (int i = 0; i < n; ++i) {
+    bool none = false;
+    for (int d = 0; d < ts[i]->ndim; ++d) none = none || ts[i]->shape[d] == 0;
+    if (!none) at[k++] = ts[i]->data;
+  }
+  std::sort(at, at + k);
+  return std::adjacent_find(at, at + k) != at + k;
 }
 int page_shift_of(int64_t page) {
   for (int k = 4; k <= 16; ++k)
@@ -524,6 +547,11 @@ QB200_API int qb200_kv_pages_accept(qb200_tensor* path, qb200_tensor* next, qb20
   a.seqs = ps.S; a.M = ps.M; a.page_shift = ps.page_shift; a.B = (int)B; a.T = (int)T;
   const int launches = num_pools > kMaxCopyPools ? (num_pools + kMaxCopyPools - 1) / kMaxCopyPools : 1;
   for (int pass = 0; pass < 2; ++pass) {                       // every pool is checked before the first launch
+    if (pass == 1 && B > 0) {                                  // (rows that have moved would move again)
+      bool no_memory = false;
+      if (listed_twice(pools, num_pools, &no_memory)) return pg_fail(QB200_ERR_BAD_ARG, "%s: a pool is listed twice", who);
+      if (no_memory) return pg_fail(QB200_ERR_BAD_ARG, "%s: %d pools are too many", who, num_pools);
+    }
     for (int l = 0; l < launches; ++l) {
       const int p0 = l * kMaxCopyPools, p1 = p0 + kMaxCopyPools < num_pools ? p0 + kMaxCopyPools : num_pools;
       uint64_t bits = 0;                                       // every address, stride and row, or-ed: what they are all multiples of

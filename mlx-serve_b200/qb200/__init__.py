@@ -417,7 +417,7 @@ def kv_pages_tree_attention(q, k_pool, v_pool, table, lens, parents, bits, group
 
 def kv_pages_accept(pools, table, lens, page, parents, tokens, sampled, rows=None, counts=None):
     """The nodes of drafted trees that the samples confirm (from node 0 on, each the lowest child that carries the token sampled behind its
-    parent), and their rows moved together in every tensor of the list ``pools`` [pages, heads, page, cols].  Returns (path, next, accepted,
+    parent), and their rows moved together in every tensor of the list ``pools`` [pages, heads, page, cols], each listed once.  Returns (path, next, accepted,
     ends): the nodes, the tokens sampled behind them, how many, and the length for ``kv_pages_free(..., begin=ends)``."""
     return _native.kv_pages_accept(pools, table, lens, page, parents, tokens, sampled, rows, counts)
 
