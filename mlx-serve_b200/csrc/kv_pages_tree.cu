@@ -156,8 +156,8 @@ __device__ __forceinline__ bool arrived(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 // The rest of a wait, for a warp whose barrier had not arrived at the first look: `most` looks, each held by the hardware for kNap ns at most.  A wait
-// that runs out is noted once.  From then on nothing is copied and no product is issued any more; the readers and the softmax go on without waiting, on
-// data that is not there and within their bounds, so that all warps meet at every barrier and the CTA ends; and its results are NaN.
+// that runs out is noted once.  From then on nothing is copied any more and the issuer does not wait for what has not come; the readers and the softmax go
+// on without waiting, on data that is not there and within their bounds, so that all warps meet at every barrier and the CTA ends; and its results are NaN.
 __device__ __forceinline__ void wait_on(uint32_t bar, uint32_t parity, int code, int* fail, uint32_t most) {
   if (*(volatile int*)fail == 0) {
     for (uint32_t it = 0; it < most; ++it)
@@ -166,10 +166,10 @@ __device__ __forceinline__ void wait_on(uint32_t bar, uint32_t parity, int code,
     atomicCAS(&g_tree_error, 0, code);
   }
 }
-// A bounded wait that polls without sleeping.
-__device__ __forceinline__ bool spin_cta(uint64_t* bar, uint32_t parity, uint32_t most) {
+// A bounded wait that polls without sleeping, and ends too where another has run out.
+__device__ __forceinline__ bool spin_cta(uint64_t* bar, uint32_t parity, uint32_t most, const int* fail) {
   const uint32_t addr = smem_u32(bar);
-  for (uint32_t it = 0; it < most; ++it) {
+  for (uint32_t it = 0; it < most && ((it & 15) != 8 || *(volatile const int*)fail == 0); ++it) {
     uint32_t done;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(done) : "r"(addr), "r"(parity) : "memory");
@@ -629,8 +629,7 @@ __global__ void __launch_bounds__(Shape<BITS, D, N>::THREADS, 1) tree_kernel(con
     const uint32_t q_d = (uint32_t)make_desc(sm + SH::Q0), k_d = (uint32_t)make_desc(sm + SH::KR), v_d = (uint32_t)make_desc_mn(sm + (QUANT ? SH::V0 : SH::VR)), p_d = (uint32_t)make_desc_mn(sm + SH::P0);
     const uint32_t most = t.polls > 0 ? (uint32_t)t.polls : kSpins;
     auto spin = [&](uint64_t* bar, uint32_t phase, int code) {
-      if (failed()) return false;
-      const bool ok = __all_sync(0xffffffffu, spin_cta(bar, phase & 1, most));
+      const bool ok = __all_sync(0xffffffffu, spin_cta(bar, phase & 1, most, &s_fail));
       if (!ok && lane == 0) { *(volatile int*)&s_fail = code; atomicCAS(&g_tree_error, 0, code); }
       __syncwarp();
       return ok;
