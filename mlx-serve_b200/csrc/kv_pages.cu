@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(256) pages_copy_kernel(const __grid_constant__
 // a lane, and finds a child with two ballots; every block walks again, so that one launch does it all.  A path's nodes ascend and stand
 // at or behind the places they go to, path[i] >= i: taken in ascending order, no row is overwritten that is still to be read, and a
 // thread's column of a row (16 bytes of one head in one pool) needs no other thread.  Eight rows are asked for at a time.
-// Bound by the launch and two dependent reads: 4 trees of eight over two layers 10 us a call, 16 trees over more layers 14 (their rows alone 0.5).
+// Bound by the launch and two dependent reads: 4 trees of eight over two layers 10 us a call, 16 trees over more layers 15 (their rows alone 0.5).
 template <typename V, int N>
 __global__ void __launch_bounds__(256) pages_accept_kernel(const __grid_constant__ PagesAcceptList<N> a) {
   __shared__ int s_path[kMaxNodes], s_pid[kMaxNodes + 1][2], s_n;   // of a place: its page and the page of the node that goes there

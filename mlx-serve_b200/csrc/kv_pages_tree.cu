@@ -22,12 +22,16 @@
 //  * The grid is one CTA an SM; every CTA works out all sequences' blocks from `lens` and takes an even share of them, or every tile is cut in the
 //    same number of parts.  Parts of a tile go to the workspace and are joined by a second kernel.
 //
-// Measured: 16 sequences of 32k tokens, 4 bits, 32 query heads over 8, 515 us with 32 nodes (128 rows of a cache head; the products alone take 102 us at
-// the rate of a library's, the codes 72 at that of a copy), 371 with 16, 324 with 8, 277 with 4; 4 sequences of 8k, 8 bits, 64 nodes 133 us; 32 sequences of a
-// window of 1024 over bf16 98 us; one of 700 tokens 22.5.  What bounds a long one is neither the bytes nor the products but the work a block of 128 tokens takes,
-// handed from warp to warp: with copies, products and barriers alone 260 us (128 rows) and 177 (16); without the readers' arithmetic 407 and 189,
-// without the softmax's 347 and 231.  Rings by cp.async in every reader took 695 instead of 527 us; two groups of readers that
+// Measured: 16 sequences of 32k tokens, 4 bits, 32 query heads over 8, 518 us with 32 nodes (128 rows of a cache head; the products alone take 102 us at
+// the rate of a library's, the codes 72 at that of a copy), 371 with 16, 324 with 8, 277 with 4; 4 sequences of 8k, 8 bits, 64 nodes 128 to 133 us; 32
+// sequences of a window of 1024 over bf16 99 us; one of 700 tokens 22.  What bounds a long one is neither the bytes nor the products but the work a block of 128
+// tokens takes, handed from warp to warp: 3.0 us a block with 128 rows, 1.5 of them copies, products and barriers alone (260 of 515 us; 177 of 277 with 16
+// rows; without the readers' arithmetic 407 and 189, without the softmax's 347 and 231).  A short one is bound by what a call and a piece take beside their
+// blocks: 2, 8, 32 and 128 blocks a CTA of 128 rows take 61, 78, 149 and 399 us behind a write of 256 MB, 16 rows 31, 39, 80 and 213, that is about 56 and 28 us
+// and 2.7 and 1.4 for a block.  Rings by cp.async in every reader took 695 instead of 527 us; two groups of readers that
 // take turns, a sleeping instead of a polling issuer, and operands made uniform for it changed nothing.
+// With 128 columns the softmax's 88 registers (the readers' 56) do not hold everything: -Xptxas -v reports 272 to 324 bytes of spill stores and 392 to 456 of
+// loads a thread for codes, 88 and 216 of stores for bf16 rows; narrower tiles have 64 and 132 at most.  What fewer registers' worth would give is not measured.
 #include <mutex>
 #include <type_traits>
 

@@ -17,9 +17,11 @@
 //    these steps go to a list in the first block, by 1024 slots along the order, and those of one slot look at one another.  Few that stay are drawn from that list alone.  Where the list
 //    would be too long (equal logits, flat rows) the border is found by halving the range of the logits' patterns, a sum over the row each time.
 //
-// Measured: one row of 128256 with top-k 50 and top-p 0.95 18.5 us (meetings of its eight blocks and the work on a list, one after the other); 256 rows of
-// 32001 (fp32) with filters of all kinds 66 us, where reading them once takes 5; 24 rows with a nucleus of flat logits 66; 256 rows of 262144 by temperature alone
-// 109 us, 1.2 TB/s: instructions bound it (30 a warp for 32 logits), not the memory.
+// Measured: one row of 128256 with top-k 50 and top-p 0.95 18.6 us (meetings of its eight blocks and the work on a list, one after the other); 256 rows of
+// 32001 (fp32) with filters of all kinds 70 us, where reading them once takes 5; 24 rows with a nucleus of flat logits 57, or 69 to 78 where one of them is left
+// open by the fp32 weights; 256 rows of 262144 by temperature alone 111 us, 1.2 TB/s: instructions bound it (30 a warp for 32 logits), not the memory.  256 rows
+// of 128256 in bf16, behind a write of 256 MB: 115 us with top-k 50 and top-p 0.95, 289 with top-p alone, 33 greedy.
+// The 64 registers that two blocks an SM leave a thread do not hold everything: -Xptxas -v reports 128 to 144 bytes of spill stores, 128 to 140 of loads.
 #include <cstddef>
 #include <mutex>
 #include <type_traits>
@@ -1154,7 +1156,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 template <typename T> cudaError_t launch_t(const SampleArgs& a, cudaStream_t st) {
   auto kern = sample_kernel<T>;
   static bool done[64] = {};
-  constexpr int kHeld = 96 * 1024;               // of a row's share at most: two blocks an SM
+  constexpr int kHeld = 96 * 1024;               // of a row's share at most (beside 43 KB of Shared: two blocks an SM up to 70 KB of it, one above)
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -1166,9 +1168,11 @@ template <typename T> cudaError_t launch_t(const SampleArgs& a, cudaStream_t st)
       if (dev >= 0 && dev < 64) done[dev] = true;
     }
   }
-  // Blocks a row: enough that there is one for every SM (two a row up to two rows an SM), of at least 8192 elements each, and so many that a share stays in
-  // shared memory.  (128256 logits, the 50 largest, by 1, 2, 4, 8 blocks a row: one row 68, 42, 24, 19 us; 64 rows 74, 45, 32, 47; 128 rows -, 57, 62, 90.  256
-  // rows of 32001 with filters of all kinds 78, 66, 87, 151.  A nucleus over flat rows pays for more: 48 rows by 4 blocks 120, by 8 102.)
+  // Blocks a row: enough that there is one for every SM (two a row up to two rows an SM), of at least 8192 and, up to eight blocks, at most 65536 elements
+  // each.  A share of up to 96 KB stays in shared memory (49152 elements of 16 bits, 24576 of 32); a larger one is read again in every pass, as those of 74
+  // and more rows of 128256 logits in bf16 are, or of 296 and more rows of 32001 in fp32.  (128256 logits, the 50 largest, by 1, 2, 4, 8 blocks a row: one row 68, 42, 24, 19 us;
+  // 64 rows 74, 45, 32, 47; 128 rows -, 57, 62, 90.  256 rows of 32001 with filters of all kinds 78, 66, 87, 151.  A nucleus over flat rows pays for more: 48
+  // rows by 4 blocks 120, by 8 102.  Not measured: more blocks where a share does not stay.)
   int ctas = 1;
   while (ctas < kMaxCtas && ((int64_t)a.N * ctas < (ctas == 1 ? 2 : 1) * sm_count() || a.V > ctas * 65536) && a.V > ctas * 8192) ctas *= 2;
   for (;; ctas = 1) {
